@@ -78,8 +78,8 @@ def draw(rng):
         longest = min(16384, (1 << 25) // (b * q * hkv * group))
         return dict(kind="attention", B=b, Q=q, L=q + _log(rng, 16, longest), **common, type=rng.choice(["bfloat16", "half", "float"]))
     t = rng.choice(["bfloat16", "half", "half", "bfloat16", "float"])
-    b, q = _log(rng, 1, 8), _log(rng, 32, 4096 if t != "float" else 500)
-    longest = min(8192, (1 << 30) // (b * q * hkv * group))
+    b, q = _log(rng, 1, 8), _log(rng, 32, 2048 if t != "float" else 500)
+    longest = min(8192, (1 << 37) // (b * q * hkv * group * max(d, 128)))
     return dict(kind="attention", B=b, Q=q, L=max(q, _log(rng, 32, max(32, longest))), **common, type=t)
 
 
