@@ -501,6 +501,105 @@ int itexhip_mfma_probe(int workgroups, int iters, const void* operands, int32_t*
  * which the bandwidth-bound kernels (the decode MatMul above all) are to be read. */
 int itexhip_read_probe(const void* src, size_t bytes, int32_t* sink, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Between a decoder's qkv linear and its output linear: norm and rotation of queries and keys, a paged cache of keys and
+ * values held in 4 bits, attention over it.  The reference has no such ops (its graphs hold the unfused element-wise ops
+ * and two BatchMatMuls, itexhip_qbatch_matmul); they complete a served decoder around the quantized linears above.
+ *
+ * One rule for all of them: positions, slots, lengths and page tables are device arrays that a captured graph reads anew at
+ * every replay; nothing is read back to the host.  What they say is bounds-checked in the kernels as described below.
+ * ---------------------------------------------------------------------------------------- */
+
+/* Rows of heads: `type` (FLOAT | BFLOAT16 | HALF) is that of queries, keys, values and outputs.  Strides are in elements,
+ * [0] between tokens, [1] between heads; the dimensions of a head are contiguous.  Tensors may be slices of packed qkv rows. */
+typedef struct {
+  int type;
+  int head_dim;           /* even, 2 .. 256; a multiple of 8 where a cache is involved */
+  int q_heads, kv_heads;  /* 0 .. 65535 */
+  int rotary_dim;         /* dimensions that are rotated: even, 0 .. head_dim */
+  int interleaved;        /* 0: pairs (i, i + rotary_dim / 2), 1: pairs (2 i, 2 i + 1) */
+  double eps;              /* of the norms, >= 0 */
+  double attention_factor; /* on cosine and sine; 1 unless the frequencies' scaling says otherwise */
+  int64_t q_strides[2], k_strides[2], v_strides[2], q_out_strides[2], k_out_strides[2];
+} itexhip_heads_params;
+
+/* Host only: the rotation frequency of each pair i < rotary_dim / 2 in TURNS a position, base^(-2 i / rotary_dim) / (2 pi),
+ * in 64 bits (at position 10^6 a 32-bit angle is off by 0.06), after the scaling for longer contexts:
+ * NONE; LINEAR: divided by factor; NTK: base times factor^(rotary_dim / (rotary_dim - 2)); LLAMA3: divided by factor where
+ * a pair makes fewer than low_freq turns within original_context positions, kept over high_freq, a linear ramp in the turns
+ * between; YARN: divided by factor below beta_slow turns, kept over beta_fast, a linear ramp over the pair's index between
+ * (the ends rounded outwards to whole indices), and *attention_factor = 0.1 ln(factor) + 1 (1 in all other cases).
+ * low / high: LLAMA3's low_freq and high_freq (1 and 4 usually), YARN's beta_slow and beta_fast (1 and 32); else unread. */
+enum { ITEXHIP_ROPE_NONE = 0, ITEXHIP_ROPE_LINEAR = 1, ITEXHIP_ROPE_NTK = 2, ITEXHIP_ROPE_LLAMA3 = 3, ITEXHIP_ROPE_YARN = 4 };
+int itexhip_rope_frequencies(int scaling, int rotary_dim, double base, double factor, double original_context, double low,
+                             double high, double* freqs, double* attention_factor);
+
+/* q_out, k_out = rotate(norm(q)), rotate(norm(k)), one launch:
+ *   norm    x * rsqrt(mean(x^2) + eps) * weight over a head's dimensions, where a weight (head_dim floats) is given
+ *   rotate  pair (a, b) at angle 2 pi position freqs[i] -> (a c - b s, b c + a s), c and s times attention_factor
+ * in fp32 (angles in 64 bits), rounded once.  freqs (device, rotary_dim / 2 doubles) and positions (device, one int32 a
+ * token, any sign) are not read if rotary_dim is 0.  Either tensor may be NULL.  An output may be its input (same strides);
+ * any other overlap is not allowed. */
+int itexhip_qk_norm_rope(const itexhip_heads_params* p, int64_t tokens, const void* q, const void* k, const float* q_weight,
+                         const float* k_weight, const int32_t* positions, const double* freqs, void* q_out, void* k_out,
+                         void* stream);
+
+/* A layer's cache: num_pages rows of itexhip_kv4_page_bytes bytes (16-byte aligned), page_size tokens each.  A token's key
+ * (or value) of one head is held as scale * (code - 8) + offset: codes of 0 .. 15, scale and offset in half precision,
+ *   scale = half((max - min) / 15), offset = half(min + 8 scale), code = 8 + clamp(rne((x - offset) / scale), -8, 7)
+ * of the dimensions after norm and rotation, clamped to +-65504, evaluated as in 64 bits (codes do not depend on the
+ * call that made them); scale 0: all codes are 8; a NaN among the dimensions makes scale and offset NaN, and so all of the head's.
+ * A page holds, for each kv head, [page_size][DP / 2] bytes of key codes (lower dimension in the low bits), [page_size / 4]
+ * [DP / 8][4 tokens][4] bytes of value codes, [page_size / 4][4 scales, 4 offsets] of the keys and the same of the values;
+ * DP is head_dim rounded up to 64, 128 or 256.  (Four tokens' value codes of eight dimensions are one 16-byte load.) */
+typedef struct {
+  int head_dim;   /* a multiple of 8, 8 .. 256 */
+  int kv_heads;   /* 1 .. 65535 */
+  int page_size;  /* 16, 32, 64, 128 or 256 tokens */
+  int64_t num_pages;
+} itexhip_kv4_cache;
+int64_t itexhip_kv4_page_bytes(const itexhip_kv4_cache* c); /* 0: not a valid geometry */
+
+/* Norm, rotation and quantization of new keys, quantization of new values, into the cache, with the queries' norm and
+ * rotation in the same launch (q may be NULL, then q_out is not written).  slots[t] (device) = page * page_size + place in
+ * the page; a slot below 0 or beyond the cache writes nothing (padded rows).  A slot occurs once in a call: which of two
+ * rows' codes, scales and offsets a slot given twice holds is not defined. */
+int itexhip_kv4_append(const itexhip_heads_params* p, const itexhip_kv4_cache* c, int64_t tokens, const void* q, const void* k,
+                       const void* v, const float* q_weight, const float* k_weight, const int32_t* positions,
+                       const double* freqs, const int64_t* slots, void* q_out, void* cache, void* stream);
+
+/* The values that slots hold, [tokens, kv_heads, head_dim] of `type`; zeros for a slot outside the cache.  Either output may
+ * be NULL. */
+int itexhip_kv4_gather(const itexhip_kv4_cache* c, int type, int64_t tokens, const void* cache, const int64_t* slots, void* k_out,
+                       void* v_out, void* stream);
+
+/* Attention of new tokens over their sequences' caches, which hold them already.  Sequence b has the rows cu_q[b] ..
+ * cu_q[b + 1] - 1 of q and out, and kv_len[b] tokens in the pages block_table[b * table_stride + token / page_size]; row i of
+ * n sits at position kv_len - n + i and sees the tokens up to there (all of them if not causal), of these the last `window`
+ * if window > 0.  q_heads is a multiple of kv_heads; consecutive query heads share a kv head.
+ *   out = softmax(scale q k) v, rounded once; lse (NULL: not wanted; [total_q, q_heads] floats) the log of the sum of exponents
+ * A row that sees nothing is 0 with lse -inf.  Rows outside every sequence are left as they are.  Keys and values a row does
+ * not see do not reach it, whatever they hold.  A page outside the cache counts as tokens that no row sees; kv_len beyond the
+ * table is cut to it, a sequence's rows beyond max_q_len or total_q are not computed.
+ * workspace: itexhip_kv4_attention_workspace bytes of device memory (16-byte aligned), contents irrelevant; calls that may
+ * overlap in time need one each.  Results do not depend on timing: equal calls give equal bits. */
+typedef struct {
+  int type;             /* FLOAT | BFLOAT16 | HALF of q and out */
+  int q_heads;
+  int num_seqs;         /* 0 .. 65535 */
+  int max_q_len;        /* most rows of a sequence: decides, with the heads, which kernel runs */
+  int64_t total_q;      /* rows of q and out, below 2^31 */
+  float scale;          /* > 0 */
+  int causal;
+  int window;           /* 0: none */
+  int64_t table_stride; /* entries of block_table between sequences: the most pages of one */
+  int64_t q_strides[2], out_strides[2];
+} itexhip_kv4_attention_params;
+int64_t itexhip_kv4_attention_workspace(const itexhip_kv4_attention_params* p, const itexhip_kv4_cache* c); /* 0: not valid */
+int itexhip_kv4_attention(const itexhip_kv4_attention_params* p, const itexhip_kv4_cache* c, const void* q, const void* cache,
+                          const int32_t* block_table, const int32_t* cu_q, const int32_t* kv_len, void* workspace, void* out,
+                          float* lse, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

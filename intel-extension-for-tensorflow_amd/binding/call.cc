@@ -27,13 +27,17 @@ namespace {
   X(quantize) X(quantize_bf16) X(dequantize) X(dequantize16) X(requantize) X(requantize_per_channel)                  \
   X(minmax_i32_per_channel) X(minmax_f32) X(qgemm) X(qgemm_tile) X(qgemv) X(qgemm_sum) X(qmatmul) X(qmatmul_per_row)  \
   X(qmatmul_device_range) X(qmatmul_unpacked) X(quantize_dynamic) X(quantize_dynamic_static) X(quantize_dynamic_rows) \
-  X(qbatch_matmul) X(pad_nhwc8) X(qconv2d) X(qconv2d_sum) X(qdepthwise_conv2d)
+  X(qbatch_matmul) X(pad_nhwc8) X(qconv2d) X(qconv2d_sum) X(qdepthwise_conv2d)                                        \
+  X(qk_norm_rope) X(kv4_append) X(kv4_gather) X(kv4_attention)
+
+// MatmulParams, Epilogue, BmmParams, ConvGeometry, HeadsParams, Kv4Cache, Kv4AttentionParams
+constexpr int kStructs = 7;
 
 // All zero until init
 struct State {
   PyObject* check;           // the binding's _check(status): raises unless it is 0
   PyObject* data_ptr;        // "data_ptr"
-  PyTypeObject* structs[4];  // MatmulParams, Epilogue, BmmParams, ConvGeometry
+  PyTypeObject* structs[kStructs];
 #define POINTER(NAME) decltype(&itexhip_##NAME) NAME;
   ENTRY_POINTS(POINTER) POINTER(transpose)
 #undef POINTER
@@ -55,6 +59,9 @@ template <class T> constexpr int struct_index() {
   if (std::is_same_v<T, itexhip_epilogue>) return 1;
   if (std::is_same_v<T, itexhip_bmm_params>) return 2;
   if (std::is_same_v<T, itexhip_conv_geometry>) return 3;
+  if (std::is_same_v<T, itexhip_heads_params>) return 4;
+  if (std::is_same_v<T, itexhip_kv4_cache>) return 5;
+  if (std::is_same_v<T, itexhip_kv4_attention_params>) return 6;
   return -1;
 }
 
@@ -193,8 +200,8 @@ PyObject* f_transpose(PyObject* self, PyObject* const* args, Py_ssize_t n) {
 // init(address, check, structures): address(name) gives an entry point's address in the loaded library
 PyObject* init(PyObject* self, PyObject* args) {
   State& st = *state_of(self);
-  PyObject *addresses, *check, *s[4];
-  if (!PyArg_ParseTuple(args, "OO(OOOO)", &addresses, &check, &s[0], &s[1], &s[2], &s[3])) return nullptr;
+  PyObject *addresses, *check, *s[kStructs];
+  if (!PyArg_ParseTuple(args, "OO(OOOOOOO)", &addresses, &check, &s[0], &s[1], &s[2], &s[3], &s[4], &s[5], &s[6])) return nullptr;
   for (PyObject* t : s)
     if (!PyType_Check(t)) { PyErr_SetString(PyExc_TypeError, "structures are types"); return nullptr; }
   bool ok = true;
@@ -210,7 +217,7 @@ PyObject* init(PyObject* self, PyObject* args) {
   if (!ok) return nullptr;
   Py_INCREF(check);
   Py_XSETREF(st.check, check);
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kStructs; ++i) {
     Py_INCREF(s[i]);
     PyTypeObject* old = st.structs[i];
     st.structs[i] = reinterpret_cast<PyTypeObject*>(s[i]);

@@ -21,6 +21,7 @@ ACT_NONE, ACT_RELU, ACT_RELU6, ACT_LEAKYRELU, ACT_GELU_APPROX, ACT_GELU_EXACT = 
 ACT_ELU, ACT_SIGMOID, ACT_TANH, ACT_SWISH, ACT_MISH = 6, 7, 8, 9, 10
 ELT_RELU, ELT_CLIP, ELT_LINEAR, ELT_GELU_TANH, ELT_GELU_ERF, ELT_SUM = 1, 2, 3, 4, 5, 6
 ELT_ELU, ELT_LOGISTIC, ELT_TANH, ELT_SWISH, ELT_MISH = 7, 8, 9, 10, 11
+ROPE_NONE, ROPE_LINEAR, ROPE_NTK, ROPE_LLAMA3, ROPE_YARN = 0, 1, 2, 3, 4
 
 EXPORTS = [
     "itexhip_device_count", "itexhip_device_info", "itexhip_mem_info", "itexhip_malloc", "itexhip_free",
@@ -36,6 +37,8 @@ EXPORTS = [
     "itexhip_qgemm_prepack_b", "itexhip_qgemm", "itexhip_qgemm_tile", "itexhip_qgemv", "itexhip_qmatmul", "itexhip_qmatmul_per_row", "itexhip_qmatmul_device_range", "itexhip_quantize_dynamic", "itexhip_quantize_dynamic_static", "itexhip_quantize_dynamic_rows", "itexhip_qmatmul_unpacked", "itexhip_mfma_probe", "itexhip_read_probe",
     "itexhip_qgemm_naive", "itexhip_qbatch_matmul", "itexhip_transpose", "itexhip_im2col8", "itexhip_pad_nhwc8", "itexhip_scale_vector",
     "itexhip_qconv2d_implicit_ok", "itexhip_qconv2d", "itexhip_qgemm_sum", "itexhip_qconv2d_sum", "itexhip_qdepthwise_conv2d",
+    "itexhip_rope_frequencies", "itexhip_qk_norm_rope", "itexhip_kv4_page_bytes", "itexhip_kv4_append", "itexhip_kv4_gather",
+    "itexhip_kv4_attention_workspace", "itexhip_kv4_attention",
 ]
 
 
@@ -562,4 +565,102 @@ def scale_vector(bias, bias_type, factors, n_factors, n, out, stream=0):
     _check(_lib.itexhip_scale_vector(_ptr(bias), int(bias_type), _ptr(factors), _i64(n_factors), _i64(n), _ptr(out), _ptr(stream)))
 
 
-_call.init(lambda name: C.cast(getattr(_lib, name), C.c_void_p).value, _check, (MatmulParams, Epilogue, BmmParams, ConvGeometry))
+# ---- between a decoder's qkv linear and its output linear -------------------------------------------
+class HeadsParams(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("type", "head_dim", "q_heads", "kv_heads", "rotary_dim", "interleaved")] + \
+               [("eps", C.c_double), ("attention_factor", C.c_double)] + \
+               [(n, C.c_int64 * 2) for n in ("q_strides", "k_strides", "v_strides", "q_out_strides", "k_out_strides")]
+
+
+class Kv4Cache(C.Structure):
+    _fields_ = [("head_dim", C.c_int), ("kv_heads", C.c_int), ("page_size", C.c_int), ("num_pages", C.c_int64)]
+
+
+class Kv4AttentionParams(C.Structure):
+    _fields_ = [("type", C.c_int), ("q_heads", C.c_int), ("num_seqs", C.c_int), ("max_q_len", C.c_int), ("total_q", C.c_int64),
+                ("scale", C.c_float), ("causal", C.c_int), ("window", C.c_int), ("table_stride", C.c_int64),
+                ("q_strides", C.c_int64 * 2), ("out_strides", C.c_int64 * 2)]
+
+
+# Prototypes of these entry points, for what the C extension does not take
+_SERVING = {name: _bind("itexhip_" + name, signature) for name, signature in (
+    ("qk_norm_rope", "plppppppppp"), ("kv4_append", "pplppppppppppp"), ("kv4_gather", "pilppppp"), ("kv4_attention", "ppppppppppp"))}
+
+
+def heads_params(type, head_dim, q_heads, kv_heads, rotary_dim=0, interleaved=False, eps=0.0, attention_factor=1.0, q_strides=None,
+                 k_strides=None, v_strides=None, q_out_strides=None, k_out_strides=None):
+    """Rows of heads; strides (between tokens, between heads) in elements, dense [tokens, heads, head_dim] where not given."""
+    p = HeadsParams(type, head_dim, q_heads, kv_heads, rotary_dim, int(bool(interleaved)), eps, attention_factor)
+    for name, given, heads in (("q_strides", q_strides, q_heads), ("k_strides", k_strides, kv_heads), ("v_strides", v_strides, kv_heads),
+                               ("q_out_strides", q_out_strides, q_heads), ("k_out_strides", k_out_strides, kv_heads)):
+        setattr(p, name, (C.c_int64 * 2)(*(given or (heads * head_dim, head_dim))))
+    return p
+
+
+def rope_frequencies(rotary_dim, base=10000.0, scaling=ROPE_NONE, factor=1.0, original_context=0.0, low=0.0, high=0.0):
+    """(frequencies in turns a position, a list of rotary_dim / 2 floats to be put on the device as doubles; attention factor)"""
+    freqs, attention = (C.c_double * max(1, int(rotary_dim) // 2))(), C.c_double()
+    _check(_lib.itexhip_rope_frequencies(C.c_int(scaling), C.c_int(int(rotary_dim)), C.c_double(base), C.c_double(factor),
+                                         C.c_double(original_context), C.c_double(low), C.c_double(high), freqs, C.byref(attention)))
+    return list(freqs), attention.value
+
+
+def qk_norm_rope(p, tokens, q, k, q_weight, k_weight, positions, freqs, q_out, k_out, stream=0):
+    if not _call.qk_norm_rope(p, tokens, q, k, q_weight, k_weight, positions, freqs, q_out, k_out, stream):
+        _check(_SERVING["qk_norm_rope"](C.byref(p), int(tokens), _addr(q), _addr(k), _addr(q_weight), _addr(k_weight), _addr(positions),
+                                        _addr(freqs), _addr(q_out), _addr(k_out), _addr(stream)))
+
+
+def kv4_cache(head_dim, kv_heads, page_size, num_pages):
+    return Kv4Cache(int(head_dim), int(kv_heads), int(page_size), int(num_pages))
+
+
+_lib.itexhip_kv4_page_bytes.restype = C.c_int64
+_lib.itexhip_kv4_attention_workspace.restype = C.c_int64
+
+
+def _size(n):
+    if n == 0:
+        _check(INVALID_ARGUMENT)
+    return int(n)
+
+
+def kv4_page_bytes(c):
+    return _size(_lib.itexhip_kv4_page_bytes(C.byref(c)))
+
+
+def kv4_append(p, c, tokens, q, k, v, q_weight, k_weight, positions, freqs, slots, q_out, cache, stream=0):
+    if not _call.kv4_append(p, c, tokens, q, k, v, q_weight, k_weight, positions, freqs, slots, q_out, cache, stream):
+        _check(_SERVING["kv4_append"](C.byref(p), C.byref(c), int(tokens), _addr(q), _addr(k), _addr(v), _addr(q_weight), _addr(k_weight),
+                                      _addr(positions), _addr(freqs), _addr(slots), _addr(q_out), _addr(cache), _addr(stream)))
+
+
+def kv4_gather(c, type, tokens, cache, slots, k_out, v_out, stream=0):
+    if not _call.kv4_gather(c, type, tokens, cache, slots, k_out, v_out, stream):
+        _check(_SERVING["kv4_gather"](C.byref(c), int(type), int(tokens), _addr(cache), _addr(slots), _addr(k_out), _addr(v_out),
+                                      _addr(stream)))
+
+
+def kv4_attention_params(type, q_heads, head_dim, num_seqs, max_q_len, total_q, scale, table_stride, causal=True, window=0,
+                         q_strides=None, out_strides=None):
+    """A ragged batch; strides (between tokens, between heads) in elements, dense [total_q, q_heads, head_dim] where not given."""
+    p = Kv4AttentionParams(type, q_heads, int(num_seqs), int(max_q_len), int(total_q), scale, int(bool(causal)), int(window),
+                           int(table_stride))
+    for name, given in (("q_strides", q_strides), ("out_strides", out_strides)):
+        setattr(p, name, (C.c_int64 * 2)(*(given or (q_heads * head_dim, head_dim))))
+    return p
+
+
+def kv4_attention_workspace(p, c):
+    """Bytes of device memory that kv4_attention needs besides its arguments."""
+    return _size(_lib.itexhip_kv4_attention_workspace(C.byref(p), C.byref(c)))
+
+
+def kv4_attention(p, c, q, cache, block_table, cu_q, kv_len, workspace, out, lse=None, stream=0):
+    if not _call.kv4_attention(p, c, q, cache, block_table, cu_q, kv_len, workspace, out, lse, stream):
+        _check(_SERVING["kv4_attention"](C.byref(p), C.byref(c), _addr(q), _addr(cache), _addr(block_table), _addr(cu_q), _addr(kv_len),
+                                         _addr(workspace), _addr(out), _addr(lse), _addr(stream)))
+
+
+_call.init(lambda name: C.cast(getattr(_lib, name), C.c_void_p).value, _check,
+           (MatmulParams, Epilogue, BmmParams, ConvGeometry, HeadsParams, Kv4Cache, Kv4AttentionParams))
