@@ -11,9 +11,10 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 
+constexpr int kMostGroups = 1024;      // workgroups of a split kernel
 constexpr int kStep = 128;             // tokens a workgroup takes at a time, 32 a wavefront
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kProbExponent = 14.0f; // probabilities are held as 2^14 p: half keeps 11 bits of them down to 2^-28
+constexpr float kProbExponent = 9.0f;  // probabilities are held as 2^9 p, up to 2^14 p above the maximum so far: half keeps 11 bits down to 2^-23
 
 struct AttArgs {
   const void* q;
@@ -51,7 +52,14 @@ __device__ __forceinline__ Seq sequence(const AttArgs& A, int b) {
   return s;
 }
 
-__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t a, uint32_t o) { return (x & a) | o; }
+// One instruction takes one scalar register and no literals: the masks stay in scalar registers, what is or-ed in a vector register
+struct CodeBits {
+  uint32_t low = 0x000f000fu, high = 0x00f000f0u;        // the codes
+  uint32_t low_one = 0x64006400u, high_one = 0x54005400u; // halves of 1024 and 64
+  __device__ __forceinline__ void pin() { asm("" : "+s"(low), "+s"(high), "+v"(low_one), "+v"(high_one)); }
+  __device__ __forceinline__ uint32_t at_64(uint32_t x) const { return (x & high) | high_one; }
+  __device__ __forceinline__ uint32_t at_1024(uint32_t x) const { return (x & low) | low_one; }
+};
 __device__ __forceinline__ half2v as_half2(uint32_t u) { half2v h; __builtin_memcpy(&h, &u, 4); return h; }
 __device__ __forceinline__ uint32_t as_bits(half2v h) { uint32_t u; __builtin_memcpy(&u, &h, 4); return u; }
 __device__ __forceinline__ float low_half(uint32_t u) { return static_cast<float>(as_half2(u)[0]); }
@@ -64,17 +72,13 @@ __device__ __forceinline__ float load_q(const void* q, int64_t i) {
   else return f16_bits_to_f32(static_cast<const uint16_t*>(q)[i]);
 }
 
-// What a lane loads of 32 tokens (two tiles of 16, each in one page): lane = 16 g + c.
-//   keys      token c of a tile, dwords g NKK .. g NKK + NKK - 1 of its row
-//   values    tokens 4 g .. 4 g + 3 of a tile, dword c (and c + 16; a half of dword c / 2 if a head has 8 of them)
-//   params    of tokens 4 g .. 4 g + 3: four scales, four offsets
-template <int DP>
-struct Raw {
-  static constexpr int NKK = DP / 32, NV = DP <= 128 ? 1 : 2;
-  uint32_t k[2][NKK];
-  u4v v[2][NV], kp[2], vp[2];
-  bool ok[2];
-};
+#ifndef PWAVES
+#define PWAVES 8
+#endif
+#ifndef OCC1
+#define OCC1 3
+#endif
+template <int T, int DP, int NB> constexpr int kOccupancy = NB == 1 && DP < 256 ? OCC1 : 1;
 
 // A wavefront's 16 NB rows against 32 tokens at a time, everything in registers.
 //
@@ -82,25 +86,42 @@ struct Raw {
 // of each tile, which is the layout that the second product O^T = V^T P^T takes as its operand, so probabilities never
 // leave the lane.  (The order of the 32 tokens within that product is the same on both sides and otherwise free.)
 //
-// Codes become operands without conversions.  A code c in the low bits of a half whose exponent is that of 1024 is the
-// number 1024 + c, four bits further up with the exponent of 64 it is 64 + c: one and-or for two codes.  For keys the excess is
-// taken back once a column (corr, the product's initial value) and scale and offset of a token are applied to its score:
-// q . k = scale (q . code) + offset sum(q).  For values the excess is subtracted (exactly) and scale and offset applied in
-// packed half arithmetic: long averages of values would otherwise cancel against the excess.
+// Codes become operands without conversions.  A code c four bits up in a half whose exponent is that of 64 is the number
+// 64 + c, in its lowest bits with the exponent of 1024 it is 1024 + c: an and-or for two codes.  For keys the excess of 72 (64
+// and the 8 that the codes are held over) is taken back once a column (corr, the product's initial value), and scale and
+// offset of a token are applied to its score: q . k = scale (q . code) + offset sum(q).  An excess of 1032 would save two shifts
+// of seven instructions for eight codes, but costs four bits of the score.  For values the excess is subtracted (exactly:
+// averages of many values would cancel against it), the scale is multiplied into the probability before that is
+// rounded to half, and offset times probability is summed apart in fp32: codes and products of 11 bits are exact, the one
+// rounding is that of the probability.
+//
+// Probabilities times scales have to fit a half: they are held relative to a power of two that bounds the scales seen so far,
+// which grows like the maximum of the scores does; both are in `ref`, p = 2^(score log2(e) + ref).
 //
 // Queries are multiplied by a power of two of their row so that half holds what bfloat16 does.  In fp32 the products are
 // fp32 MFMAs on fp32 operands.
 template <int T, int DP, int NB>
 struct Engine {
   static constexpr bool F32 = T == ITEXHIP_FLOAT;
-  static constexpr int NKK = DP / 32, E = DP / 16, NV = Raw<DP>::NV;
+  static constexpr int NKK = DP / 32, E = DP / 16, NV = DP <= 128 ? 1 : 2;
+  static constexpr float kSlack = F32 ? 0.0f : 5.0f;  // log2 of how far a score may exceed the maximum that sums are relative to
   half8v q16[F32 ? 1 : NB][NKK];
   float q32[F32 ? NB : 1][NKK][8];
-  float corr[NB], sumq[NB], qs[NB], m[NB], l[NB];
+  float corr[NB], sumq[NB], qs[NB], m[NB], raise_at[NB], ref[NB], l[NB], po[NB];
+  uint32_t scale_bound;  // half bits that no value's scale so far exceeds: an exponent with all ones below
   int limit[NB], start[NB];  // the tokens that column c of block nb sees: start <= t < limit
   f4 o[NB][E];
   int min_limit, max_start;  // over the wavefront's rows
+  int seq_len;               // tokens of the sequence
   int lane, c, g;
+  CodeBits bits;
+  uint32_t kraw[2][NKK];
+  u4v vraw[2][NV], kp[2], vp[2];
+  const __attribute__((address_space(4))) int32_t* table;
+  const uint8_t* head_base;
+  int64_t page_bytes;
+  int last_tile, shift, num_pages;
+  uint32_t k_lane, v_lane, p_lane, vp_more;
 
   __device__ __forceinline__ void init(const AttArgs& A, const Seq& s, int kv_head, int row0) {
     lane = threadIdx.x & 63;
@@ -154,9 +175,9 @@ struct Engine {
             q16[nb][kk][(j & 3) * 2 + (j >> 2)] = h;
             const float f = static_cast<float>(h);
             sum += f;
-            excess += f * ((j & 1) ? 72.0f : 1032.0f);
           }
         }
+        excess = 72.0f * sum;
       } else {
 #pragma unroll
         for (int kk = 0; kk < NKK; ++kk) {
@@ -175,104 +196,129 @@ struct Engine {
       sumq[nb] = sum;
       corr[nb] = -excess;
       qs[nb] = fmaxf(A.scale * kLog2e * back, 1.2e-38f);
-      m[nb] = -INFINITY;
-      l[nb] = 0.0f;
+      m[nb] = raise_at[nb] = -INFINITY;
+      ref[nb] = kProbExponent + (F32 ? 0.0f : 15.0f);
+      l[nb] = po[nb] = 0.0f;
 #pragma unroll
       for (int e = 0; e < E; ++e) o[nb][e] = f4{0, 0, 0, 0};
     }
+    scale_bound = 0x03ffu;  // exponent 2^-15 (subnormals): scales below 2^-14
   }
 
-  // Loads of the tiles at t0 and t0 + 16; a tile that ends before `from` or starts at `to` or beyond, or has no page, is not ok and holds zeros
-  __device__ __forceinline__ void load(const AttArgs& A, const int32_t* table, int kv_head, int t0, int to, Raw<DP>& r) const {
+  // The tokens from .. to - 1 of a sequence; `table` may be read at the pages of those only.
+  __device__ __forceinline__ void open(const AttArgs& A, const int32_t* pages, int kv_head, int to) {
+    table = (const __attribute__((address_space(4))) int32_t*)(pages);
+    last_tile = (to - 1) & ~15;
+    shift = A.page_shift;
+    num_pages = static_cast<int>(A.num_pages);
+    page_bytes = A.page_bytes;
     const Kv4Block block{A.page_size, DP};
+    head_base = A.cache + static_cast<int64_t>(kv_head) * block.bytes();
+    k_lane = c * (DP / 2) + g * (DP / 8);
+    v_lane = block.value_codes(4 * g, DP == 64 ? c / 2 : c);
+    p_lane = block.key_params(4 * g);
+    vp_more = block.value_params(0) - block.key_params(0);
+  }
+  // Pages of the tiles at t and t + 16 (beyond the last tile: that one's again, masked by its tokens)
+  __device__ __forceinline__ void fetch_pages(int t, int (&pages)[2]) const {
+    pages[0] = table[min(t, last_tile) >> shift];
+    pages[1] = table[min(t + 16, last_tile) >> shift];
+  }
+  // Where tile i of the step at t is; a page that is none: page 0 (masked)
+  __device__ __forceinline__ const uint8_t* tile(int page, int t, int i, int* place) const {
+    *place = min(t + 16 * i, last_tile) & ((1 << shift) - 1);
+    return head_base + (page >= 0 && page < num_pages ? page : 0) * page_bytes;
+  }
+  __device__ __forceinline__ bool valid(int page) const { return page >= 0 && page < num_pages; }
+
+  // What a lane (16 g + c) loads of a step's two tiles of 16 tokens:
+  //   keys      token c of a tile, dwords g NKK .. g NKK + NKK - 1 of its row
+  //   values    tokens 4 g .. 4 g + 3 of a tile, dword c (and c + 16; a half of dword c / 2 if a head has 8 of them)
+  //   params    of tokens 4 g .. 4 g + 3: four scales, four offsets
+  __device__ __forceinline__ void load_keys(const int (&pages)[2], int t) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int t = t0 + 16 * i;
-      int page = t < to ? table[t >> A.page_shift] : -1;
-      page = __builtin_amdgcn_readfirstlane(page);
-      r.ok[i] = page >= 0 && page < A.num_pages;
+      int place;
+      const uint8_t* base = tile(pages[i], t, i, &place);
+      const uint8_t* kr = base + place * (DP / 2);
+      if constexpr (NKK == 2) {
+        const uint2 w = *reinterpret_cast<const uint2*>(kr + k_lane);
+        kraw[i][0] = w.x;
+        kraw[i][1] = w.y;
+      } else {
 #pragma unroll
-      for (int kk = 0; kk < NKK; ++kk) r.k[i][kk] = 0;
+        for (int j = 0; j < NKK / 4; ++j) {
+          const u4v w = *reinterpret_cast<const u4v*>(kr + k_lane + 16 * j);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) r.v[i][j] = u4v{0, 0, 0, 0};
-      r.kp[i] = r.vp[i] = u4v{0, 0, 0, 0};
-      if (r.ok[i]) {
-        const uint8_t* base = A.cache + page * A.page_bytes + static_cast<int64_t>(kv_head) * block.bytes();
-        const int place = t & (A.page_size - 1);
-        const uint8_t* kr = base + block.key_codes(place + c) + g * (DP / 8);
-        if constexpr (NKK == 2) {
-          const uint2 w = *reinterpret_cast<const uint2*>(kr);
-          r.k[i][0] = w.x;
-          r.k[i][1] = w.y;
-        } else {
-#pragma unroll
-          for (int j = 0; j < NKK / 4; ++j) {
-            const u4v w = *reinterpret_cast<const u4v*>(kr + 16 * j);
-#pragma unroll
-            for (int n = 0; n < 4; ++n) r.k[i][4 * j + n] = w[n];
-          }
+          for (int n = 0; n < 4; ++n) kraw[i][4 * j + n] = w[n];
         }
-        const uint8_t* vr = base + block.value_codes(place + 4 * g, DP == 64 ? c / 2 : c);
-#pragma unroll
-        for (int j = 0; j < NV; ++j) r.v[i][j] = *reinterpret_cast<const u4v*>(vr + 256 * j);
-        r.kp[i] = *reinterpret_cast<const u4v*>(base + block.key_params(place + 4 * g));
-        r.vp[i] = *reinterpret_cast<const u4v*>(base + block.value_params(place + 4 * g));
       }
+      kp[i] = *reinterpret_cast<const u4v*>(base + place * 4 + p_lane);
+    }
+  }
+  __device__ __forceinline__ void load_values(const int (&pages)[2], int t) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      int place;
+      const uint8_t* base = tile(pages[i], t, i, &place);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) vraw[i][j] = *reinterpret_cast<const u4v*>(base + place * (DP / 2) + v_lane + 256 * j);
+      vp[i] = *reinterpret_cast<const u4v*>(base + place * 4 + vp_more + p_lane);
     }
   }
 
   __device__ __forceinline__ half8v key_operand(uint32_t w) const {
-    const uint32_t v = w >> 8;
-    const u4v u = {and_or(w, 0x000f000fu, 0x64006400u), and_or(w, 0x00f000f0u, 0x54005400u), and_or(v, 0x000f000fu, 0x64006400u),
-                   and_or(v, 0x00f000f0u, 0x54005400u)};
+    const u4v u = {bits.at_64(w << 4), bits.at_64(w), bits.at_64(w >> 4), bits.at_64(w >> 8)};
     half8v h;
     __builtin_memcpy(&h, &u, 16);
     return h;
   }
 
-  // The scores of a column become probabilities (times 2^14), the sums so far are rescaled where the maximum has grown
-  __device__ __forceinline__ void softmax(int nb, float (&x)[8]) {
-    float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    if (__any(top > m[nb])) {
-      const float now = fmaxf(m[nb], top);
-      const float a = now == m[nb] ? 1.0f : __builtin_amdgcn_exp2f((m[nb] - now) * qs[nb]);
-      m[nb] = now;
-      l[nb] *= a;
+  __device__ __forceinline__ void rescale(int nb, float a) {
+    l[nb] *= a;
+    po[nb] *= a;
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[nb][e] *= a;
-    }
-    const float ref = kProbExponent - (m[nb] == -INFINITY ? 0.0f : m[nb] * qs[nb]);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], qs[nb], ref));
-      l[nb] += x[j];
-    }
+    for (int e = 0; e < E; ++e) o[nb][e] *= a;
   }
 
-  __device__ __forceinline__ void step(const Raw<DP>& r, int t0) {
-    const bool mask = !(r.ok[0] && r.ok[1] && t0 + 32 <= min_limit && t0 >= max_start);
-    u4v vp[2] = {r.vp[0], r.vp[1]};
-    uint32_t nan = 0;  // bit 4 i + j: the value of token 4 g + j of tile i is NaN and only some rows may see it
-    if (mask) {
-      // tokens beyond the last one hold whatever memory held: their values must not reach a product, not even times zero
-      const int last = limit_of_wave();
+  // The sums are held relative to a maximum of the scores and a power of two over the values' scales: either has grown
+  __device__ __forceinline__ void raise(const float (&p)[NB][8], uint32_t most) {
+    if constexpr (!F32) {
+      most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 16)));
+      most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 32)));
+      most = (most > 0x7bffu ? 0x7bffu : most) | 0x3ffu;  // NaN comes through the products
+      if (most > scale_bound) {
+        const float by = static_cast<float>(static_cast<int>((most >> 10) - (scale_bound >> 10)));
+        scale_bound = most;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t keep = (j & 1) ? 0x0000ffffu : 0xffff0000u;
-          const uint32_t sc = (vp[i][j / 2] >> (16 * (j & 1))) & 0x7fffu, of = (vp[i][2 + j / 2] >> (16 * (j & 1))) & 0x7fffu;
-          const bool beyond = t0 + 16 * i + 4 * g + j >= last;
-          if (beyond || sc >= 0x7c00u || of >= 0x7c00u) {
-            if (!beyond) nan |= 1u << (4 * i + j);
-            vp[i][j / 2] &= keep;
-            vp[i][2 + j / 2] &= keep;
-          }
+        for (int nb = 0; nb < NB; ++nb) {
+          ref[nb] -= by;
+          rescale(nb, __builtin_amdgcn_exp2f(-by));
         }
       }
     }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      float top = p[nb][0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) top = fmaxf(top, p[nb][j]);
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float was = m[nb];
+      if (top > was) {
+        m[nb] = top;
+        const float by = was == -INFINITY ? top * qs[nb] : (top - was) * qs[nb];
+        ref[nb] -= by;
+        rescale(nb, was == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(-by));
+        raise_at[nb] = top + kSlack / qs[nb];
+      }
+    }
+  }
+
+  // One step: `pages` are its own, `next` (at `tn`) those of the step to load behind it
+  __device__ __forceinline__ void step(bool mask, const int (&pages)[2], int t0, const int (&next)[2], int tn) {
+    bool ok[2] = {true, true};
+    uint32_t nan = 0;  // bit 4 i + j: the value of token 4 g + j of tile i is NaN and only some rows may see it
     float p[NB][8];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
@@ -282,35 +328,87 @@ struct Engine {
 #pragma unroll
         for (int kk = 0; kk < NKK; ++kk) {
           if constexpr (!F32) {
-            s = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_operand(r.k[i][kk]), q16[nb][kk], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_operand(kraw[i][kk]), q16[nb][kk], s, 0, 0, 0);
           } else {
 #pragma unroll
             for (int n = 0; n < 8; ++n)
-              s = __builtin_amdgcn_mfma_f32_16x16x4f32(static_cast<float>((r.k[i][kk] >> (4 * n)) & 15u), q32[nb][kk][n], s, 0, 0, 0);
+              s = __builtin_amdgcn_mfma_f32_16x16x4f32(static_cast<float>((kraw[i][kk] >> (4 * n)) & 15u), q32[nb][kk][n], s, 0, 0, 0);
           }
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t sc = r.kp[i][j / 2], of = r.kp[i][2 + j / 2];
+          const uint32_t sc = kp[i][j / 2], of = kp[i][2 + j / 2];
           const float ks = (j & 1) ? high_half(sc) : low_half(sc), ko = (j & 1) ? high_half(of) : low_half(of);
-          float x = fmaf(ks, s[j], ko * sumq[nb]);
-          if (mask) {
-            const int t = t0 + 16 * i + 4 * g + j;
-            const bool seen = r.ok[i] && t < limit[nb] && t >= start[nb];
-            x = seen ? x : -INFINITY;
-            if (seen && (nan >> (4 * i + j) & 1)) l[nb] = NAN;
-          }
-          p[nb][4 * i + j] = x;
+          p[nb][4 * i + j] = fmaf(ks, s[j], ko * sumq[nb]);
         }
       }
-      softmax(nb, p[nb]);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    load_keys(next, tn);
+    __builtin_amdgcn_sched_barrier(0);
+    if (mask) {
+      ok[0] = valid(pages[0]);
+      ok[1] = valid(pages[1]);
+      // tokens beyond the last one hold whatever memory held: their values must not reach a product, not even times zero
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t keep = (j & 1) ? 0x0000ffffu : 0xffff0000u;
+          const uint32_t sc = (vp[i][j / 2] >> (16 * (j & 1))) & 0x7fffu, of = (vp[i][2 + j / 2] >> (16 * (j & 1))) & 0x7fffu;
+          const bool beyond = t0 + 16 * i + 4 * g + j >= seq_len || !ok[i];
+          if (beyond || sc >= 0x7c00u || of >= 0x7c00u) {
+            if (!beyond) nan |= 1u << (4 * i + j);
+            vp[i][j / 2] &= keep;
+            vp[i][2 + j / 2] &= keep;
+          }
+        }
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int t = t0 + 16 * (k / 4) + 4 * g + k % 4;
+          const bool seen = ok[k / 4] && t < limit[nb] && t >= start[nb];
+          p[nb][k] = seen ? p[nb][k] : -INFINITY;
+          if (seen && (nan >> k & 1)) l[nb] = NAN;
+        }
+      }
+    }
+    uint32_t most = 0;
+    bool over = false;
+    if constexpr (!F32) {
+      typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+      auto v = [](uint32_t x) { us2 r; __builtin_memcpy(&r, &x, 4); return r; };
+      const us2 two = __builtin_elementwise_max(__builtin_elementwise_max(v(vp[0][0]), v(vp[0][1])), __builtin_elementwise_max(v(vp[1][0]), v(vp[1][1])));
+      most = two[0] > two[1] ? two[0] : two[1];
+      over = most > scale_bound;
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const float top = fmaxf(fmaxf(fmaxf(p[nb][0], p[nb][1]), fmaxf(p[nb][2], p[nb][3])), fmaxf(fmaxf(p[nb][4], p[nb][5]), fmaxf(p[nb][6], p[nb][7])));
+      over = over || top > raise_at[nb];
+    }
+    if (__any(over)) raise(p, most);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        p[nb][j] = __builtin_amdgcn_exp2f(fmaf(p[nb][j], qs[nb], ref[nb]));
+        l[nb] += p[nb][j];
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
     if constexpr (!F32) {
       half8v pb[NB];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) pb[nb][j] = static_cast<_Float16>(p[nb][j]);
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t sc = vp[j / 4][j % 4 / 2], of = vp[j / 4][2 + j % 4 / 2];
+          po[nb] = fmaf(p[nb][j], (j & 1) ? high_half(of) : low_half(of), po[nb]);
+          pb[nb][j] = static_cast<_Float16>(p[nb][j] * ((j & 1) ? high_half(sc) : low_half(sc)));
+        }
       }
       // a lane's eight tokens of one dimension, two a register: first the halves of two tokens' dwords that hold its code
 #pragma unroll
@@ -320,7 +418,7 @@ struct Engine {
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const u4v& d = r.v[i][part / 2 % NV];
+            const u4v& d = vraw[i][part / 2 % NV];
             if constexpr (DP == 64) w[2 * i + j] = __builtin_amdgcn_perm(d[2 * j + 1], d[2 * j], (c & 1) ? 0x07060302u : 0x05040100u);
             else w[2 * i + j] = __builtin_amdgcn_perm(d[2 * j + 1], d[2 * j], (part & 1) ? 0x07060302u : 0x05040100u);
           }
@@ -331,9 +429,8 @@ struct Engine {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t x = n < 2 ? w[k] : w[k] >> 8;
-            half2v h = (n & 1) ? as_half2(and_or(x, 0x00f000f0u, 0x54005400u)) + half2v{-72, -72}
-                               : as_half2(and_or(x, 0x000f000fu, 0x64006400u)) + half2v{-1032, -1032};
-            h = __builtin_elementwise_fma(h, as_half2(vp[k / 2][k & 1]), as_half2(vp[k / 2][2 + (k & 1)]));
+            const half2v h = (n & 1) ? as_half2(bits.at_64(x)) + half2v{-72, -72}
+                               : as_half2(bits.at_1024(x)) + half2v{-1032, -1032};
             a[k] = as_bits(h);
           }
           half8v v;
@@ -353,7 +450,7 @@ struct Engine {
           const float low = fmaf(-8.0f, vs, vo);
 #pragma unroll
           for (int e = 0; e < E; ++e) {
-            const uint32_t d = r.v[i][e / 8][j];
+            const uint32_t d = vraw[i][e / 8][j];
             const uint32_t code = DP == 64 ? (d >> (16 * (c & 1) + 4 * e)) & 15u : (d >> (4 * (e & 7))) & 15u;
             const float v = fmaf(static_cast<float>(code), vs, low);
 #pragma unroll
@@ -362,23 +459,51 @@ struct Engine {
         }
       }
     }
+    __builtin_amdgcn_sched_barrier(0);
+    load_values(next, tn);
+    __builtin_amdgcn_sched_barrier(0);
   }
 
-  int seq_len;  // tokens of the sequence
-  __device__ __forceinline__ int limit_of_wave() const { return seq_len; }
+  // Tokens from, from + stride, ..., 32 each, up to `to`
+  __device__ __forceinline__ void run(const AttArgs& A, const int32_t* pages, int kv_head, int from, int to, int stride, int len) {
+    if (from >= to) return;
+    seq_len = len;
+    bits.pin();
+    open(A, pages, kv_head, to);
+    int now[2], next[2], later[2];
+    fetch_pages(from, now);
+    fetch_pages(from + stride, next);
+    load_keys(now, from);
+    load_values(now, from);
+    for (int t = from; t < to; t += stride) {
+      fetch_pages(t + 2 * stride, later);
+      step(!(valid(now[0]) && valid(now[1]) && t + 32 <= min_limit && t >= max_start), now, t, next, t + stride);
+      now[0] = next[0]; now[1] = next[1];
+      next[0] = later[0]; next[1] = later[1];
+    }
+  }
 
   // the first of the four or eight dimensions that o[..][e][r], e = 0 .. 3 (+ 4), belong to
   __device__ __forceinline__ int dim_of(int e, int r) const {
     return DP == 64 ? 4 * (4 * g + r) + e : 8 * (4 * g + r) + (e & 7) + 128 * (e >> 3);
   }
 
-  __device__ __forceinline__ void sum_l() {
+  // The parts of a column's sums that its four lanes hold apart
+  __device__ __forceinline__ void close() {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       l[nb] += __shfl_xor(l[nb], 16);
       l[nb] += __shfl_xor(l[nb], 32);
+      if constexpr (!F32) {
+        po[nb] += __shfl_xor(po[nb], 16);
+        po[nb] += __shfl_xor(po[nb], 32);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[nb][e] += po[nb];
+      }
     }
   }
+  // What the sums are relative to, in units of log2
+  __device__ __forceinline__ float top_of(int nb) const { return m[nb] == -INFINITY ? -INFINITY : -ref[nb]; }
 
   // o / l and the log-sum-exp of the rows; `top` in units of log2
   __device__ __forceinline__ void finish(const AttArgs& A, const Seq& s, int kv_head, int row0, const float (&top)[NB], const float (&sum)[NB]) const {
@@ -391,7 +516,7 @@ struct Engine {
       const bool empty = sum[nb] == 0.0f;
       const float inv = empty ? 0.0f : 1.0f / sum[nb];
       if (g == 0 && A.lse != nullptr)
-        A.lse[q_row * A.q_heads + head] = empty ? -INFINITY : kLn2 * (top[nb] - kProbExponent + log2f(sum[nb]));
+        A.lse[q_row * A.q_heads + head] = empty ? -INFINITY : kLn2 * (top[nb] + log2f(sum[nb]));
       const int64_t at = q_row * A.o_st + head * A.o_sh;
 #pragma unroll
       for (int e = 0; e < E; e += 4) {
@@ -420,12 +545,12 @@ struct Engine {
 // knowing them.  A share may end one (sequence, head), hold several whole ones and begin another: whole ones are written out,
 // the two at its ends leave their sums in the workspace for combine_kernel.
 template <int T, int DP, int NB>
-__global__ __launch_bounds__(256) void split_kernel(const AttArgs A) {
+__global__ __launch_bounds__(256, (kOccupancy<T, DP, NB>)) void split_kernel(const AttArgs A) {
   __shared__ int64_t scan[5];
   __shared__ int64_t found[2];
   __shared__ float lds_ml[4][2][16 * NB];
   __shared__ float lds_o[2][NB * (DP / 16) * 4][64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   // steps of all sequences, then the sequence in which this workgroup's share begins
   auto prefix_of = [&](int base, int64_t& inclusive, int64_t& all) {
@@ -485,26 +610,16 @@ __global__ __launch_bounds__(256) void split_kernel(const AttArgs A) {
 
     Engine<T, DP, NB> eng;
     eng.init(A, s, head, 0);
-    eng.seq_len = s.len;
-    const int32_t* table = A.table + b * A.table_stride;
-    const int t_begin = s.lo + static_cast<int>(s0) * kStep + 32 * wave;
-    Raw<DP> now, next;
-    eng.load(A, table, head, t_begin, s.len, now);
-    for (int i = 0; i < static_cast<int>(n); ++i) {
-      const int t = t_begin + i * kStep;
-      if (t >= s.len) break;
-      if (i + 1 < n) eng.load(A, table, head, t + kStep, s.len, next);
-      eng.step(now, t);
-      now = next;
-    }
-    eng.sum_l();
+    const int first = s.lo + static_cast<int>(s0) * kStep, last = first + static_cast<int>(n) * kStep;
+    eng.run(A, A.table + b * A.table_stride, head, first + 32 * wave, last < s.len ? last : s.len, kStep, s.len);
+    eng.close();
 
     // the four wavefronts' sums into those of the first
     float top[NB], sum[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       if (eng.g == 0) {
-        lds_ml[wave][0][nb * 16 + eng.c] = eng.m[nb] == -INFINITY ? -INFINITY : eng.m[nb] * eng.qs[nb];
+        lds_ml[wave][0][nb * 16 + eng.c] = eng.top_of(nb);
         lds_ml[wave][1][nb * 16 + eng.c] = eng.l[nb];
       }
     }
@@ -574,43 +689,63 @@ __global__ __launch_bounds__(256) void split_kernel(const AttArgs A) {
 // One row of a (sequence, kv head) that several workgroups shared: their sums, in the order of the tokens
 template <int T, int DP, int NB>
 __global__ __launch_bounds__(256) void combine_kernel(const AttArgs A) {
-  __shared__ float lds_o[256 / (DP / 4)][DP];
-  __shared__ float lds_l[256 / (DP / 4)];
-  const int b = blockIdx.z, head = blockIdx.y, row = blockIdx.x;
+  constexpr int LANES = DP / 4, PARTS = 256 / LANES, CHUNK = kMostGroups;
+  __shared__ float lds_o[PARTS][DP];
+  __shared__ float lds_l[4], lds_top[4], weight[CHUNK];
+  const int b = blockIdx.z, head = blockIdx.y, row = blockIdx.x, tid = threadIdx.x;
   const Seq s = sequence(A, b);
   if (row >= s.n * A.group) return;
   const int64_t share = A.prefix[A.num_seqs], i0 = A.prefix[b] + head * s.steps;
   const int64_t w0 = i0 / share, w1 = (i0 + s.steps - 1) / share;
   if (w0 == w1) return;
-  const int count = static_cast<int>(w1 - w0 + 1);
+  const int count = static_cast<int>(w1 - w0 + 1);  // at most the workgroups of the split kernel, kMostGroups
   auto at = [&](int i) { return (2 * (w0 + i) + (i == 0 ? 1 : 0)) * 16 * NB + row; };
-  constexpr int LANES = DP / 4, PARTS = 256 / LANES;
-  const int lane = threadIdx.x % LANES, part = threadIdx.x / LANES;
-  float top = -INFINITY;
-  for (int i = 0; i < count; ++i) top = fmaxf(top, A.part_ml[at(i) * 2]);
+  const int lane = tid % LANES, part = tid / LANES;
+  // every thread takes the maxima and sums of up to CHUNK / 256 parts
+  float tops[CHUNK / 256], sums[CHUNK / 256], top = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < CHUNK / 256; ++k) {
+    const int i = tid + 256 * k;
+    tops[k] = -INFINITY;
+    sums[k] = 0.0f;
+    if (i < count) {
+      const float2 v = *reinterpret_cast<const float2*>(A.part_ml + at(i) * 2);
+      tops[k] = v.x;
+      sums[k] = v.y;
+    }
+    top = fmaxf(top, tops[k]);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+  if (tid % 64 == 0) lds_top[tid / 64] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(lds_top[0], lds_top[1]), fmaxf(lds_top[2], lds_top[3]));
   const float ref = top == -INFINITY ? 0.0f : top;
   float sum = 0.0f;
-  f4 o = {0, 0, 0, 0};
-  for (int i = part; i < count; i += PARTS) {
-    const int64_t k = at(i);
-    const float w = __builtin_amdgcn_exp2f(A.part_ml[k * 2] - ref);
-    sum += A.part_ml[k * 2 + 1] * w;
-    o += *reinterpret_cast<const f4*>(A.part_o + k * DP + 4 * lane) * w;
+#pragma unroll
+  for (int k = 0; k < CHUNK / 256; ++k) {
+    const float w = __builtin_amdgcn_exp2f(tops[k] - ref);
+    weight[tid + 256 * k] = w;
+    sum += sums[k] * w;
   }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+  if (tid % 64 == 0) lds_l[tid / 64] = sum;
+  __syncthreads();
+  sum = lds_l[0] + lds_l[1] + lds_l[2] + lds_l[3];
+  f4 o = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int i = part; i < count; i += PARTS) o += *reinterpret_cast<const f4*>(A.part_o + at(i) * DP + 4 * lane) * weight[i];
   *reinterpret_cast<f4*>(&lds_o[part][4 * lane]) = o;
-  if (lane == 0) lds_l[part] = sum;
   __syncthreads();
   if (part != 0) return;
 #pragma unroll
-  for (int i = 1; i < PARTS; ++i) {
-    o += *reinterpret_cast<const f4*>(&lds_o[i][4 * lane]);
-    sum += lds_l[i];
-  }
+  for (int i = 1; i < PARTS; ++i) o += *reinterpret_cast<const f4*>(&lds_o[i][4 * lane]);
   const int q_head = head * A.group + row % A.group;
   const int64_t q_row = s.first + row / A.group;
   const bool empty = sum == 0.0f;
   const float inv = empty ? 0.0f : 1.0f / sum;
-  if (lane == 0 && A.lse != nullptr) A.lse[q_row * A.q_heads + q_head] = empty ? -INFINITY : kLn2 * (top - kProbExponent + log2f(sum));
+  if (lane == 0 && A.lse != nullptr) A.lse[q_row * A.q_heads + q_head] = empty ? -INFINITY : kLn2 * (top + log2f(sum));
   if (4 * lane >= A.head_dim) return;
   const int64_t to = q_row * A.o_st + q_head * A.o_sh + 4 * lane;
 #pragma unroll
@@ -620,13 +755,12 @@ __global__ __launch_bounds__(256) void combine_kernel(const AttArgs A) {
 // Sequences of more rows: a wavefront takes 16 NB rows through all the tokens that they see
 template <int T, int DP, int NB>
 __global__ __launch_bounds__(256) void rows_kernel(const AttArgs A) {
-  const int wave = threadIdx.x >> 6, b = blockIdx.z, head = blockIdx.y;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), b = blockIdx.z, head = blockIdx.y;
   const Seq s = sequence(A, b);
   const int rows = s.n * A.group, row0 = (static_cast<int>(blockIdx.x) * 4 + wave) * 16 * NB;
   if (row0 >= rows) return;
   Engine<T, DP, NB> eng;
   eng.init(A, s, head, row0);
-  eng.seq_len = s.len;
   const int first = row0 / A.group, last = (row0 + 16 * NB < rows ? row0 + 16 * NB - 1 : rows - 1) / A.group;
   int to = s.len, from = s.lo;
   if (A.causal) {
@@ -637,19 +771,330 @@ __global__ __launch_bounds__(256) void rows_kernel(const AttArgs A) {
     from = s.len - s.n + first - A.window + 1;
     from = (from < 0 ? 0 : from) & ~31;
   }
-  const int32_t* table = A.table + b * A.table_stride;
-  Raw<DP> now, next;
-  if (from < to) eng.load(A, table, head, from, to, now);
-  for (int t = from; t < to; t += 32) {
-    if (t + 32 < to) eng.load(A, table, head, t + 32, to, next);
-    eng.step(now, t);
-    now = next;
-  }
-  eng.sum_l();
+  eng.run(A, A.table + b * A.table_stride, head, from, to, 32, s.len);
+  eng.close();
   float top[NB];
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) top[nb] = eng.m[nb] == -INFINITY ? -INFINITY : eng.m[nb] * eng.qs[nb];
+  for (int nb = 0; nb < NB; ++nb) top[nb] = eng.top_of(nb);
   eng.finish(A, s, head, row0, top, eng.l);
+}
+
+// Sequences of many rows on half MFMAs.  A workgroup takes 32 rows a wavefront through the tokens that they see, TT tokens at a
+// time: all its threads turn a tile's codes into operands in LDS, once for all rows, while the tile before is worked on; the
+// wavefronts read them as whole fragments.  32 x 32 x 16 products with the same transposition as in Engine: S^T = K Q^T gives
+// lane 32 h + c the scores of column c for tokens 8 i + 4 h + 0 .. 3, which O^T = V^T P^T takes as they are.
+//
+// LDS holds a fragment as 64 lanes of 16 bytes.  Keys: [32 tokens][16 dimensions], lane 32 h + token: dimensions 8 h .. 8 h + 7 in the
+// order of key_operand.  Values: [16 tokens][32 dimensions], lane 32 h + dimension: tokens 4 h .. 4 h + 3 and 8 + 4 h .. + 3.
+template <int DP> constexpr int kTile = DP == 256 ? 32 : 64;
+template <int T, int DP, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, (DP == 256 ? 1 : 2)) void prompt_kernel(const AttArgs A) {
+  constexpr int TT = kTile<DP>, TB = TT / 32, KK = DP / 16, DB = DP / 32, U = TT / 16, THREADS = WAVES * 64, DW = DP / 8;
+  constexpr bool FOLD = T == ITEXHIP_HALF;  // see below
+  __shared__ u4v lds_k[2][TB * KK * 64], lds_v[2][U * DB * 64];
+  __shared__ u4v lds_kp[2][TT / 4], lds_vp[2][TT / 4];
+  __shared__ unsigned long long lds_valid[2], lds_nan[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, hi = lane >> 5;
+  const int head = blockIdx.x % A.kv_heads, b = blockIdx.z;  // neighbouring workgroups, on different dies, take different heads
+  const Seq s = sequence(A, b);
+  const int rows = s.n * A.group, tile_rows = 32 * WAVES;
+  const int tiles = (rows + tile_rows - 1) / tile_rows;
+  const int at_tile = tiles - 1 - static_cast<int>(blockIdx.x / A.kv_heads);  // the longest first
+  if (at_tile < 0) return;
+  const int row0 = at_tile * tile_rows + 32 * wave, row = row0 + c;
+  const int before = s.len - s.n;  // position of the first row
+  auto limit_of = [&](int r) { const int to = A.causal ? before + r / A.group + 1 : s.len; return to < 0 ? 0 : to; };
+  auto start_of = [&](int r) { const int from = A.window > 0 ? before + r / A.group - A.window + 1 : 0; return from < 0 ? 0 : from; };
+  // of the workgroup, the wavefront and the lane's column
+  const int first_row = at_tile * tile_rows, last_row = min(first_row + tile_rows, rows) - 1;
+  const int from = start_of(first_row) & ~(TT - 1), to = min(limit_of(last_row), s.len);
+  const bool there = row0 < rows;
+  const int w_last = min(row0 + 31, rows - 1);
+  const int w_to = there ? limit_of(w_last) : 0, w_from = start_of(row0), w_all_to = limit_of(row0), w_all_from = there ? start_of(w_last) : 0;
+  const int limit = row < rows ? limit_of(row) : 0, start = row < rows ? start_of(row) : 0;
+
+  // queries, as in Engine::init
+  half8v q[KK];
+  float sumq = 0.0f, qs;
+  {
+    float most = 0.0f;
+    const int64_t at = row < rows ? (s.first + row / A.group) * A.q_st + static_cast<int64_t>(head * A.group + row % A.group) * A.q_sh : 0;
+    float x[KK][8];
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      const int d0 = kk * 16 + hi * 8;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[kk][j] = row < rows && d0 < A.head_dim ? load_q<T>(A.q, at + d0 + j) : 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[kk][j]));
+    }
+    most = fmaxf(most, __shfl_xor(most, 32));
+    int ex = 0;
+    if (most > 1e-30f && most < 3e38f) ex = static_cast<int>((__float_as_uint(most) >> 23) & 255) - 127;
+    const float by = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
+    qs = fmaxf(A.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + ex) << 23), 1.2e-38f);
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const _Float16 h = static_cast<_Float16>(x[kk][j] * by);
+        q[kk][(j & 3) * 2 + (j >> 2)] = h;
+        sumq += static_cast<float>(h);
+      }
+    }
+    sumq += __shfl_xor(sumq, 32);
+  }
+  const float corr = -72.0f * sumq;
+  float m = -INFINITY, raise_at = -INFINITY, l = 0.0f, po = 0.0f, ref = kProbExponent + (FOLD ? 15.0f : 0.0f);
+  uint32_t scale_bound = 0x03ffu;
+  typedef float f16v __attribute__((ext_vector_type(16)));
+  f16v o[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+
+  CodeBits bits;
+  bits.pin();
+  const Kv4Block block{A.page_size, DP};
+  const uint8_t* head_base = A.cache + static_cast<int64_t>(head) * block.bytes();
+  const int32_t* table = A.table + b * A.table_stride;
+  // tasks of a tile: keys (token, pair of dwords); values (16 tokens, half, dword, pair of codes)
+  constexpr int KT = TT * DW / 2, VT = U * 2 * DW * 4, KN = (KT + THREADS - 1) / THREADS, VN = (VT + THREADS - 1) / THREADS;
+  uint2 kraw[KN];
+  u4v vraw[VN][2], vpar[VN][2], kpar;
+  bool v_ok[VN];
+  uint32_t token_vs = 0, token_vo = 0;
+  bool token_ok = false;
+  auto page_of = [&](int t) { return table[min(t, to - 1) >> A.page_shift]; };
+  auto good = [&](int page) { return page >= 0 && page < A.num_pages; };
+  auto base_of = [&](int page) { return head_base + (good(page) ? page : 0) * A.page_bytes; };
+  auto fetch = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < KN; ++i) {
+      const int task = tid + i * THREADS;
+      if (KT % THREADS != 0 && task >= KT) break;
+      const int t = t0 + task % TT, j = task / TT;
+      kraw[i] = *reinterpret_cast<const uint2*>(base_of(page_of(t)) + block.key_codes(t & (A.page_size - 1)) + 8 * j);
+    }
+#pragma unroll
+    for (int i = 0; i < VN; ++i) {
+      const int task = tid + i * THREADS;
+      if (VT % THREADS != 0 && task >= VT) break;
+      const int w = (task >> 2) % DW, h = (task >> 2) / DW & 1, u = (task >> 2) / DW >> 1, t = t0 + 16 * u;
+      const int page = page_of(t), place = (t & (A.page_size - 1)) + 4 * h;
+      const uint8_t* base = base_of(page);
+      v_ok[i] = good(page);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        vraw[i][k] = *reinterpret_cast<const u4v*>(base + block.value_codes(place + 8 * k, w));
+        if (!FOLD) vpar[i][k] = *reinterpret_cast<const u4v*>(base + block.value_params(place + 8 * k));
+      }
+    }
+    if (tid < TT) {  // one token each: what holds for it
+      const int t = t0 + tid, page = page_of(t);
+      const uint8_t* base = base_of(page) + block.value_params(t & (A.page_size - 1));
+      token_ok = good(page) && t < s.len;
+      token_vs = *reinterpret_cast<const uint16_t*>(base);
+      token_vo = *reinterpret_cast<const uint16_t*>(base + 8);
+      if (tid < TT / 4) {
+        const int t4 = t0 + 4 * tid;
+        kpar = *reinterpret_cast<const u4v*>(base_of(page_of(t4)) + block.key_params(t4 & (A.page_size - 1)));
+      }
+    }
+  };
+  auto stage = [&](int t0, int buf) {
+#pragma unroll
+    for (int i = 0; i < KN; ++i) {
+      const int task = tid + i * THREADS;
+      if (KT % THREADS != 0 && task >= KT) break;
+      const int t = task % TT, j = task / TT;
+      u4v* to_k = &lds_k[buf][((t / 32) * KK + j) * 64 + t % 32];
+      to_k[0] = u4v{bits.at_64(kraw[i].x << 4), bits.at_64(kraw[i].x), bits.at_64(kraw[i].x >> 4), bits.at_64(kraw[i].x >> 8)};
+      to_k[32] = u4v{bits.at_64(kraw[i].y << 4), bits.at_64(kraw[i].y), bits.at_64(kraw[i].y >> 4), bits.at_64(kraw[i].y >> 8)};
+    }
+#pragma unroll
+    for (int i = 0; i < VN; ++i) {
+      const int task = tid + i * THREADS;
+      if (VT % THREADS != 0 && task >= VT) break;
+      const int n2 = task & 3, w = (task >> 2) % DW, h = (task >> 2) / DW & 1, u = (task >> 2) / DW >> 1;
+      const uint32_t pick = (n2 & 2) ? 0x07060302u : 0x05040100u;
+      const int shift = (n2 & 1) * 8;
+      u4v a, z;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t x = __builtin_amdgcn_perm(vraw[i][k / 2][2 * (k & 1) + 1], vraw[i][k / 2][2 * (k & 1)], pick) >> shift;
+        half2v first = as_half2(bits.at_1024(x)) + half2v{-1032, -1032}, second = as_half2(bits.at_64(x)) + half2v{-72, -72};
+        if constexpr (!FOLD) {
+          // a token that nothing may read becomes zeros: beyond the sequence, without a page, NaN (which `lds_nan` tells of)
+          uint32_t vs = vpar[i][k / 2][k & 1], vo = vpar[i][k / 2][2 + (k & 1)];
+          const int t = t0 + 16 * u + 8 * (k / 2) + 4 * h + 2 * (k & 1);
+          const uint32_t keep = (v_ok[i] && t < s.len && (vs & 0x7c00u) != 0x7c00u && (vo & 0x7c00u) != 0x7c00u ? 0xffffu : 0u) |
+                                (v_ok[i] && t + 1 < s.len && (vs & 0x7c000000u) != 0x7c000000u && (vo & 0x7c000000u) != 0x7c000000u ? 0xffff0000u : 0u);
+          vs &= keep;
+          vo &= keep;
+          first = __builtin_elementwise_fma(first, as_half2(vs), as_half2(vo));
+          second = __builtin_elementwise_fma(second, as_half2(vs), as_half2(vo));
+        }
+        a[k] = as_bits(first);
+        z[k] = as_bits(second);
+      }
+      u4v* to_v = &lds_v[buf][(u * DB + w / 4) * 64 + h * 32 + (w & 3) * 8 + 2 * n2];
+      to_v[0] = a;
+      to_v[1] = z;
+    }
+    if (tid < TT) {
+      const bool nan = token_ok && ((token_vs & 0x7c00u) == 0x7c00u || (token_vo & 0x7c00u) == 0x7c00u);
+      const unsigned long long valid = __ballot(token_ok), nans = __ballot(nan);
+      if (tid == 0) {
+        lds_valid[buf] = valid;
+        lds_nan[buf] = nans;
+      }
+      if (FOLD) {
+        const bool keep = token_ok && !nan;
+        uint16_t* par = reinterpret_cast<uint16_t*>(&lds_vp[buf][tid / 4]) + (tid & 3);
+        par[0] = static_cast<uint16_t>(keep ? token_vs : 0);
+        par[4] = static_cast<uint16_t>(keep ? token_vo : 0);
+      }
+      if (tid < TT / 4) lds_kp[buf][tid] = kpar;
+    }
+  };
+  auto rescale = [&](float a) {
+    l *= a;
+    po *= a;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] *= a;
+  };
+
+  if (from < to) {
+    fetch(from);
+    stage(from, 0);
+  }
+  __syncthreads();
+  constexpr unsigned long long kAll = TT == 64 ? ~0ull : (1ull << (TT & 63)) - 1;
+  for (int t0 = from, buf = 0; t0 < to; t0 += TT, buf ^= 1) {
+    const bool more = t0 + TT < to;
+    if (more) fetch(t0 + TT);
+    if (t0 < w_to && t0 + TT > w_from) {
+      const unsigned long long valid = lds_valid[buf], nans = lds_nan[buf];
+      const bool mask = valid != kAll || nans != 0 || t0 + TT > w_all_to || t0 < w_all_from;
+#pragma unroll
+      for (int tb = 0; tb < TB; ++tb) {
+        f16v sc;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[r] = corr;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          half8v a;
+          __builtin_memcpy(&a, &lds_k[buf][(tb * KK + kk) * 64 + lane], 16);
+          sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q[kk], sc, 0, 0, 0);
+        }
+        float p[16], top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const u4v par = lds_kp[buf][tb * 8 + 2 * i + hi];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float ks = (j & 1) ? high_half(par[j / 2]) : low_half(par[j / 2]), ko = (j & 1) ? high_half(par[2 + j / 2]) : low_half(par[2 + j / 2]);
+            p[4 * i + j] = fmaf(ks, sc[4 * i + j], ko * sumq);
+          }
+        }
+        if (mask) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int at = 32 * tb + 8 * (r / 4) + 4 * hi + r % 4, t = t0 + at;
+            const bool seen = (valid >> at & 1) && t < limit && t >= start;
+            p[r] = seen ? p[r] : -INFINITY;
+            if (seen && (nans >> at & 1)) l = NAN;
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, p[r]);
+        uint32_t most = 0;
+        u4v vp[4];
+        if constexpr (FOLD) {
+          typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+          us2 two = {0, 0};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            vp[i] = lds_vp[buf][tb * 8 + 2 * i + hi];
+            us2 x[2];
+            __builtin_memcpy(x, &vp[i], 8);
+            two = __builtin_elementwise_max(two, __builtin_elementwise_max(x[0], x[1]));
+          }
+          most = two[0] > two[1] ? two[0] : two[1];
+        }
+        if (__any(top > raise_at || (FOLD && most > scale_bound))) {
+          if constexpr (FOLD) {
+            most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 32))) | 0x3ffu;
+            if (most > scale_bound) {
+              const float by = static_cast<float>(static_cast<int>((most >> 10) - (scale_bound >> 10)));
+              scale_bound = most;
+              ref -= by;
+              rescale(__builtin_amdgcn_exp2f(-by));
+            }
+          }
+          top = fmaxf(top, __shfl_xor(top, 32));
+          if (top > m) {
+            const float by = m == -INFINITY ? top * qs : (top - m) * qs;
+            ref -= by;
+            rescale(m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(-by));
+            m = top;
+            raise_at = top + 5.0f / qs;
+          }
+        }
+        half8v pb[2];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float x = __builtin_amdgcn_exp2f(fmaf(p[r], qs, ref));
+          l += x;
+          if constexpr (FOLD) {
+            const uint32_t vs = vp[r / 4][r % 4 / 2], vo = vp[r / 4][2 + r % 4 / 2];
+            po = fmaf(x, (r & 1) ? high_half(vo) : low_half(vo), po);
+            x *= (r & 1) ? high_half(vs) : low_half(vs);
+          }
+          pb[r / 8][r % 8] = static_cast<_Float16>(x);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {
+            half8v a;
+            __builtin_memcpy(&a, &lds_v[buf][((2 * tb + u) * DB + d) * 64 + lane], 16);
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pb[u], o[d], 0, 0, 0);
+          }
+        }
+      }
+    }
+    if (more) stage(t0 + TT, buf ^ 1);
+    __syncthreads();
+  }
+
+  l += __shfl_xor(l, 32);
+  if constexpr (FOLD) po += __shfl_xor(po, 32);
+  if (row >= rows) return;
+  const int q_head = head * A.group + row % A.group;
+  const int64_t q_row = s.first + row / A.group, at = q_row * A.o_st + q_head * A.o_sh;
+  const bool empty = l == 0.0f;
+  const float inv = empty ? 0.0f : 1.0f / l;
+  if (hi == 0 && A.lse != nullptr) A.lse[q_row * A.q_heads + q_head] = empty ? -INFINITY : kLn2 * (log2f(l) - ref);
+#pragma unroll
+  for (int d = 0; d < DB; ++d) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int dim = 32 * d + 8 * i + 4 * hi;
+      if (dim >= A.head_dim) continue;
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = (o[d][4 * i + j] + (FOLD ? po : 0.0f)) * inv;
+      if (A.vec) {
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(A.out) + at + dim) = uint2{f32x2_to_bits16<T>(v[0], v[1]), f32x2_to_bits16<T>(v[2], v[3])};
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) store_output<T>(A.out, at + dim + j, v[j]);
+      }
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -669,7 +1114,7 @@ Plan plan_of(const itexhip_kv4_attention_params* p, const itexhip_kv4_cache* c) 
   plan.split = rows <= 16 * plan.blocks;
   if (plan.split) {
     const int64_t bound = static_cast<int64_t>(p->num_seqs) * c->kv_heads * ((p->table_stride * c->page_size + kStep - 1) / kStep);
-    const int64_t full = plan.blocks == 1 ? 1024 : 512;
+    const int64_t full = plan.blocks == 1 && dp < 256 ? OCC1 * 256 : 256;
     plan.groups = bound < 1 ? 1 : bound < full ? bound : full;
     plan.prefix = (static_cast<size_t>(p->num_seqs) + 1) * 8 + 15 & ~size_t{15};
     plan.ml = static_cast<size_t>(plan.groups) * 2 * 16 * plan.blocks * 2 * 4;
@@ -688,8 +1133,8 @@ int check(const char* who, const itexhip_kv4_attention_params* p, const itexhip_
   ITEXHIP_REQUIRE(p->type == ITEXHIP_FLOAT || is_float16_type(p->type), "%s: type is float, bfloat16 or half", who);
   ITEXHIP_REQUIRE(p->q_heads >= 1 && p->q_heads <= 65535 && p->q_heads % c->kv_heads == 0, "%s: q_heads is a multiple of kv_heads, at most 65535", who);
   ITEXHIP_REQUIRE(p->num_seqs >= 0 && p->num_seqs <= 65535, "%s: num_seqs is 0 to 65535", who);
-  ITEXHIP_REQUIRE(p->max_q_len >= 0 && static_cast<int64_t>(p->max_q_len) * (p->q_heads / c->kv_heads) < (1ll << 30),
-                  "%s: max_q_len times the heads of a kv head is 0 to 2^30", who);
+  ITEXHIP_REQUIRE(p->max_q_len >= 0 && static_cast<int64_t>(p->max_q_len) * p->q_heads < (1ll << 30),
+                  "%s: max_q_len times q_heads is 0 to 2^30 - 1", who);
   ITEXHIP_REQUIRE(p->total_q >= 0 && p->total_q < (1ll << 31), "%s: total_q is 0 to 2^31 - 1", who);
   ITEXHIP_REQUIRE(p->scale > 0.0f && isfinite(p->scale), "%s: scale is finite and positive", who);
   ITEXHIP_REQUIRE(p->window >= 0, "%s: window is not negative", who);
@@ -708,7 +1153,12 @@ void launch(const AttArgs& A, const Plan& plan, hipStream_t stream) {
     split_kernel<T, DP, NB><<<dim3(static_cast<unsigned>(plan.groups)), dim3(256), 0, stream>>>(A);
     if (plan.groups > 1) combine_kernel<T, DP, NB><<<dim3(rows, A.kv_heads, A.num_seqs), dim3(256), 0, stream>>>(A);
   } else {
-    rows_kernel<T, DP, NB><<<dim3((rows + 64 * NB - 1) / (64 * NB), A.kv_heads, A.num_seqs), dim3(256), 0, stream>>>(A);
+    if constexpr (T == ITEXHIP_FLOAT) {
+      rows_kernel<T, DP, NB><<<dim3((rows + 64 * NB - 1) / (64 * NB), A.kv_heads, A.num_seqs), dim3(256), 0, stream>>>(A);
+    } else {
+      constexpr int WAVES = DP == 256 ? 4 : PWAVES;
+      prompt_kernel<T, DP, WAVES><<<dim3(A.kv_heads * ((rows + 32 * WAVES - 1) / (32 * WAVES)), 1, A.num_seqs), dim3(64 * WAVES), 0, stream>>>(A);
+    }
   }
 }
 template <int T, int DP>
