@@ -861,45 +861,51 @@ __global__ __launch_bounds__(WAVES * 64, (DP == 256 ? 1 : 2)) void prompt_kernel
   const int32_t* table = A.table + b * A.table_stride;
   // tasks of a tile: keys (token, pair of dwords); values (16 tokens, half, dword, pair of codes)
   constexpr int KT = TT * DW / 2, VT = U * 2 * DW * 4, KN = (KT + THREADS - 1) / THREADS, VN = (VT + THREADS - 1) / THREADS;
+  static_assert(THREADS % TT == 0, "a thread's key tasks are one token's");
   uint2 kraw[KN];
-  u4v vraw[VN][2], vpar[VN][2], kpar;
-  bool v_ok[VN];
-  uint32_t token_vs = 0, token_vo = 0;
-  bool token_ok = false;
-  auto page_of = [&](int t) { return table[min(t, to - 1) >> A.page_shift]; };
+  u4v vraw[VN][2], vpar[VN][2];
+  uint32_t token_ks = 0, token_ko = 0, token_vs = 0, token_vo = 0;
+  // pages of a thread's tasks, read a tile ahead of the loads that need them
+  int page_k = -1, page_v[VN], next_k = -1, next_v[VN];
+  auto v_tokens = [&](int i) { return 16 * ((tid + i * THREADS) / (8 * DW)); };
+  auto look_up = [&](int t0) {
+    next_k = table[min(t0 + tid % TT, to - 1) >> A.page_shift];
+#pragma unroll
+    for (int i = 0; i < VN; ++i) next_v[i] = table[min(t0 + v_tokens(i), to - 1) >> A.page_shift];
+  };
   auto good = [&](int page) { return page >= 0 && page < A.num_pages; };
   auto base_of = [&](int page) { return head_base + (good(page) ? page : 0) * A.page_bytes; };
   auto fetch = [&](int t0) {
+    page_k = next_k;
+#pragma unroll
+    for (int i = 0; i < VN; ++i) page_v[i] = next_v[i];
+    look_up(t0 + TT);
+    const int place_k = (t0 + tid % TT) & (A.page_size - 1);
+    const uint8_t* base = base_of(page_k);
 #pragma unroll
     for (int i = 0; i < KN; ++i) {
       const int task = tid + i * THREADS;
       if (KT % THREADS != 0 && task >= KT) break;
-      const int t = t0 + task % TT, j = task / TT;
-      kraw[i] = *reinterpret_cast<const uint2*>(base_of(page_of(t)) + block.key_codes(t & (A.page_size - 1)) + 8 * j);
+      kraw[i] = *reinterpret_cast<const uint2*>(base + block.key_codes(place_k) + 8 * (task / TT));
+    }
+    if (tid < TT) {  // one token each: its parameters
+      const uint8_t *kp = base + block.key_params(place_k), *vp = base + block.value_params(place_k);
+      token_ks = *reinterpret_cast<const uint16_t*>(kp);
+      token_ko = *reinterpret_cast<const uint16_t*>(kp + 8);
+      token_vs = *reinterpret_cast<const uint16_t*>(vp);
+      token_vo = *reinterpret_cast<const uint16_t*>(vp + 8);
     }
 #pragma unroll
     for (int i = 0; i < VN; ++i) {
       const int task = tid + i * THREADS;
       if (VT % THREADS != 0 && task >= VT) break;
-      const int w = (task >> 2) % DW, h = (task >> 2) / DW & 1, u = (task >> 2) / DW >> 1, t = t0 + 16 * u;
-      const int page = page_of(t), place = (t & (A.page_size - 1)) + 4 * h;
-      const uint8_t* base = base_of(page);
-      v_ok[i] = good(page);
+      const int w = (task >> 2) % DW, h = (task >> 2) / DW & 1;
+      const int place = ((t0 + v_tokens(i)) & (A.page_size - 1)) + 4 * h;
+      const uint8_t* base = base_of(page_v[i]);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         vraw[i][k] = *reinterpret_cast<const u4v*>(base + block.value_codes(place + 8 * k, w));
         if (!FOLD) vpar[i][k] = *reinterpret_cast<const u4v*>(base + block.value_params(place + 8 * k));
-      }
-    }
-    if (tid < TT) {  // one token each: what holds for it
-      const int t = t0 + tid, page = page_of(t);
-      const uint8_t* base = base_of(page) + block.value_params(t & (A.page_size - 1));
-      token_ok = good(page) && t < s.len;
-      token_vs = *reinterpret_cast<const uint16_t*>(base);
-      token_vo = *reinterpret_cast<const uint16_t*>(base + 8);
-      if (tid < TT / 4) {
-        const int t4 = t0 + 4 * tid;
-        kpar = *reinterpret_cast<const u4v*>(base_of(page_of(t4)) + block.key_params(t4 & (A.page_size - 1)));
       }
     }
   };
@@ -920,19 +926,22 @@ __global__ __launch_bounds__(WAVES * 64, (DP == 256 ? 1 : 2)) void prompt_kernel
       const int n2 = task & 3, w = (task >> 2) % DW, h = (task >> 2) / DW & 1, u = (task >> 2) / DW >> 1;
       const uint32_t pick = (n2 & 2) ? 0x07060302u : 0x05040100u;
       const int shift = (n2 & 1) * 8;
+      if (!FOLD && (!good(page_v[i]) || t0 + TT > s.len)) {  // tokens beyond the last one or without a page become zeros
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int t = t0 + 16 * u + 8 * (k / 2) + 4 * h + 2 * (k & 1);
+          const uint32_t keep = !good(page_v[i]) ? 0 : (t < s.len ? 0xffffu : 0u) | (t + 1 < s.len ? 0xffff0000u : 0u);
+          vpar[i][k / 2][k & 1] &= keep;
+          vpar[i][k / 2][2 + (k & 1)] &= keep;
+        }
+      }
       u4v a, z;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const uint32_t x = __builtin_amdgcn_perm(vraw[i][k / 2][2 * (k & 1) + 1], vraw[i][k / 2][2 * (k & 1)], pick) >> shift;
         half2v first = as_half2(bits.at_1024(x)) + half2v{-1032, -1032}, second = as_half2(bits.at_64(x)) + half2v{-72, -72};
         if constexpr (!FOLD) {
-          // a token that nothing may read becomes zeros: beyond the sequence, without a page, NaN (which `lds_nan` tells of)
-          uint32_t vs = vpar[i][k / 2][k & 1], vo = vpar[i][k / 2][2 + (k & 1)];
-          const int t = t0 + 16 * u + 8 * (k / 2) + 4 * h + 2 * (k & 1);
-          const uint32_t keep = (v_ok[i] && t < s.len && (vs & 0x7c00u) != 0x7c00u && (vo & 0x7c00u) != 0x7c00u ? 0xffffu : 0u) |
-                                (v_ok[i] && t + 1 < s.len && (vs & 0x7c000000u) != 0x7c000000u && (vo & 0x7c000000u) != 0x7c000000u ? 0xffff0000u : 0u);
-          vs &= keep;
-          vo &= keep;
+          const uint32_t vs = vpar[i][k / 2][k & 1], vo = vpar[i][k / 2][2 + (k & 1)];
           first = __builtin_elementwise_fma(first, as_half2(vs), as_half2(vo));
           second = __builtin_elementwise_fma(second, as_half2(vs), as_half2(vo));
         }
@@ -944,19 +953,22 @@ __global__ __launch_bounds__(WAVES * 64, (DP == 256 ? 1 : 2)) void prompt_kernel
       to_v[1] = z;
     }
     if (tid < TT) {
-      const bool nan = token_ok && ((token_vs & 0x7c00u) == 0x7c00u || (token_vo & 0x7c00u) == 0x7c00u);
-      const unsigned long long valid = __ballot(token_ok), nans = __ballot(nan);
+      const bool ok = good(page_k) && t0 + tid < s.len;
+      const bool nan = ok && ((token_vs & 0x7c00u) == 0x7c00u || (token_vo & 0x7c00u) == 0x7c00u);
+      const unsigned long long valid = __ballot(ok), nans = __ballot(nan);
       if (tid == 0) {
         lds_valid[buf] = valid;
         lds_nan[buf] = nans;
       }
+      uint16_t* par = reinterpret_cast<uint16_t*>(&lds_kp[buf][tid / 4]) + (tid & 3);
+      par[0] = static_cast<uint16_t>(token_ks);
+      par[4] = static_cast<uint16_t>(token_ko);
       if (FOLD) {
-        const bool keep = token_ok && !nan;
-        uint16_t* par = reinterpret_cast<uint16_t*>(&lds_vp[buf][tid / 4]) + (tid & 3);
+        const bool keep = ok && !nan;
+        par = reinterpret_cast<uint16_t*>(&lds_vp[buf][tid / 4]) + (tid & 3);
         par[0] = static_cast<uint16_t>(keep ? token_vs : 0);
         par[4] = static_cast<uint16_t>(keep ? token_vo : 0);
       }
-      if (tid < TT / 4) lds_kp[buf][tid] = kpar;
     }
   };
   auto rescale = [&](float a) {
@@ -967,6 +979,7 @@ __global__ __launch_bounds__(WAVES * 64, (DP == 256 ? 1 : 2)) void prompt_kernel
   };
 
   if (from < to) {
+    look_up(from);
     fetch(from);
     stage(from, 0);
   }
@@ -975,20 +988,32 @@ __global__ __launch_bounds__(WAVES * 64, (DP == 256 ? 1 : 2)) void prompt_kernel
   for (int t0 = from, buf = 0; t0 < to; t0 += TT, buf ^= 1) {
     const bool more = t0 + TT < to;
     if (more) fetch(t0 + TT);
+    if (!FOLD && lds_nan[buf] != 0) {  // values that are NaN reach the rows that see them through l, the products as zeros
+      half8v* all = reinterpret_cast<half8v*>(lds_v[buf]);
+      for (int i = tid; i < U * DB * 64; i += THREADS) {
+        half8v a = all[i];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a[j] = a[j] == a[j] ? a[j] : static_cast<_Float16>(0);
+        all[i] = a;
+      }
+      __syncthreads();
+    }
     if (t0 < w_to && t0 + TT > w_from) {
       const unsigned long long valid = lds_valid[buf], nans = lds_nan[buf];
       const bool mask = valid != kAll || nans != 0 || t0 + TT > w_all_to || t0 < w_all_from;
 #pragma unroll
       for (int tb = 0; tb < TB; ++tb) {
+        // fragments are asked for ahead of the products that take them: the keys' at once, the values' before the softmax
+        half8v kf[KK], vf[2][DB];
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) __builtin_memcpy(&kf[kk], &lds_k[buf][(tb * KK + kk) * 64 + lane], 16);
         f16v sc;
 #pragma unroll
         for (int r = 0; r < 16; ++r) sc[r] = corr;
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          half8v a;
-          __builtin_memcpy(&a, &lds_k[buf][(tb * KK + kk) * 64 + lane], 16);
-          sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q[kk], sc, 0, 0, 0);
-        }
+        for (int kk = 0; kk < KK; ++kk) sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[kk], q[kk], sc, 0, 0, 0);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) __builtin_memcpy(&vf[0][d], &lds_v[buf][(2 * tb * DB + d) * 64 + lane], 16);
         float p[16], top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -1000,12 +1025,14 @@ __global__ __launch_bounds__(WAVES * 64, (DP == 256 ? 1 : 2)) void prompt_kernel
           }
         }
         if (mask) {
+          const uint32_t here = static_cast<uint32_t>(valid >> (32 * tb)) >> (4 * hi), nan_here = static_cast<uint32_t>(nans >> (32 * tb)) >> (4 * hi);
+          const int first = t0 + 32 * tb + 4 * hi, below = limit - first, above = start - first;
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const int at = 32 * tb + 8 * (r / 4) + 4 * hi + r % 4, t = t0 + at;
-            const bool seen = (valid >> at & 1) && t < limit && t >= start;
+            const int at = 8 * (r / 4) + r % 4;  // from the lane's first token of the block
+            const bool seen = (here >> at & 1) && at < below && at >= above;
             p[r] = seen ? p[r] : -INFINITY;
-            if (seen && (nans >> at & 1)) l = NAN;
+            if (seen && (nan_here >> at & 1)) l = NAN;
           }
         }
 #pragma unroll
@@ -1056,13 +1083,11 @@ __global__ __launch_bounds__(WAVES * 64, (DP == 256 ? 1 : 2)) void prompt_kernel
           pb[r / 8][r % 8] = static_cast<_Float16>(x);
         }
 #pragma unroll
+        for (int d = 0; d < DB; ++d) __builtin_memcpy(&vf[1][d], &lds_v[buf][((2 * tb + 1) * DB + d) * 64 + lane], 16);
+#pragma unroll
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
-          for (int d = 0; d < DB; ++d) {
-            half8v a;
-            __builtin_memcpy(&a, &lds_v[buf][((2 * tb + u) * DB + d) * 64 + lane], 16);
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pb[u], o[d], 0, 0, 0);
-          }
+          for (int d = 0; d < DB; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[u][d], pb[u], o[d], 0, 0, 0);
         }
       }
     }
