@@ -1,6 +1,8 @@
 // Rows of heads: norm and rotation of queries and keys, appending to the 4-bit cache, reading its rows back.
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.hpp"
 #include "kv4.hpp"
 
@@ -18,7 +20,8 @@ struct HeadsArgs {
   uint8_t* cache;
   int64_t tokens, num_slots, page_bytes;
   int page_shift, page_size, dp;
-  int passes_q, passes_k, passes, parts;  // passes: groups of 64 / LPH heads of one tensor; a wavefront takes every parts-th
+  int passes_k, passes_v, passes;  // groups of 64 / LPH heads of a token's keys, values, all with the queries
+  int64_t share;                   // passes a wavefront
 };
 
 template <int T>
@@ -26,20 +29,6 @@ __device__ __forceinline__ float load1(const void* base, int64_t i) {
   if constexpr (T == ITEXHIP_FLOAT) return static_cast<const float*>(base)[i];
   else if constexpr (T == ITEXHIP_BFLOAT16) return bf16_bits_to_f32(static_cast<const uint16_t*>(base)[i]);
   else return f16_bits_to_f32(static_cast<const uint16_t*>(base)[i]);
-}
-template <int T>
-__device__ __forceinline__ void load4(const void* base, int64_t i, float (&x)[4]) {
-  if constexpr (T == ITEXHIP_FLOAT) {
-    const f4 v = *reinterpret_cast<const f4*>(static_cast<const float*>(base) + i);
-    for (int j = 0; j < 4; ++j) x[j] = v[j];
-  } else {
-    const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + i);
-    const uint32_t w[2] = {v.x, v.y};
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t h = (w[j / 2] >> (16 * (j % 2))) & 0xffffu;
-      x[j] = T == ITEXHIP_BFLOAT16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
-    }
-  }
 }
 template <int T>
 __device__ __forceinline__ void store4(void* base, int64_t i, const float (&x)[4]) {
@@ -51,287 +40,387 @@ __device__ __forceinline__ void store4(void* base, int64_t i, const float (&x)[4
   }
 }
 
-template <int LPH, class V>
-__device__ __forceinline__ V head_sum(V x) {
+// Over the LPH lanes of a head.  Lanes 1, 2, 4 and 8 apart meet within the vector unit; of a mirrored row any lane of the
+// other half will do, since its half agrees by then.
+template <int CTRL, class V>
+__device__ __forceinline__ V from_lane(V x) {
+  static_assert(sizeof(V) == 4 || sizeof(V) == 8, "one or two registers");
+  int w[sizeof(V) / 4];
+  __builtin_memcpy(w, &x, sizeof(V));
 #pragma unroll
-  for (int m = 1; m < LPH; m *= 2) x += __shfl_xor(x, m);
+  for (unsigned i = 0; i < sizeof(V) / 4; ++i) w[i] = __builtin_amdgcn_update_dpp(w[i], w[i], CTRL, 0xf, 0xf, false);
+  __builtin_memcpy(&x, w, sizeof(V));
   return x;
 }
-template <int LPH, class V>
-__device__ __forceinline__ V head_max(V x) {
-#pragma unroll
-  for (int m = 1; m < LPH; m *= 2) {
-    const V y = __shfl_xor(x, m);
-    x = x > y ? x : y;
-  }
+template <int LPH, class V, class F>
+__device__ __forceinline__ V over_head(V x, F&& f) {
+  if constexpr (LPH > 1) x = f(x, from_lane<0xb1>(x));    // quad_perm 1 0 3 2
+  if constexpr (LPH > 2) x = f(x, from_lane<0x4e>(x));    // quad_perm 2 3 0 1
+  if constexpr (LPH > 4) x = f(x, from_lane<0x141>(x));   // row_half_mirror
+  if constexpr (LPH > 8) x = f(x, from_lane<0x140>(x));   // row_mirror
+  if constexpr (LPH > 16) x = f(x, __shfl_xor(x, 16));
   return x;
 }
 
-// cosine and sine of 2 pi t, |t| <= 1/2, times the factor
-__device__ __forceinline__ void turn(float t, double factor, float* c, float* s) {
-  sincospif(2.0f * t, s, c);
-  const float f = static_cast<float>(factor);
-  *c *= f;
-  *s *= f;
-}
+// cosine and sine of 2 pi t for |t| <= 1/2, to about 1e-15: sine and cosine of the angle to the nearest quarter turn, |y| <= pi / 4,
+// by their Taylor sums (the first terms left out are y^17 / 17! < 5e-17 and y^16 / 16! < 2e-15), put back by the quarter
 __device__ __forceinline__ void turn(double t, double factor, double* c, double* s) {
-  sincospi(2.0 * t, s, c);
-  *c *= factor;
-  *s *= factor;
+  const double quarter = rint(4.0 * t);
+  const double y = fma(quarter, -0.25, t) * 6.283185307179586, z = y * y;
+  double a = fma(z, -1.0 / 1307674368000.0, 1.0 / 6227020800.0);
+  a = fma(z, a, -1.0 / 39916800.0);
+  a = fma(z, a, 1.0 / 362880.0);
+  a = fma(z, a, -1.0 / 5040.0);
+  a = fma(z, a, 1.0 / 120.0);
+  a = fma(z, a, -1.0 / 6.0);
+  a = fma(z * y, a, y);
+  double b = fma(z, -1.0 / 87178291200.0, 1.0 / 479001600.0);
+  b = fma(z, b, -1.0 / 3628800.0);
+  b = fma(z, b, 1.0 / 40320.0);
+  b = fma(z, b, -1.0 / 720.0);
+  b = fma(z, b, 1.0 / 24.0);
+  b = fma(z, b, -0.5);
+  b = fma(z, b, 1.0);
+  const int n = static_cast<int>(quarter);
+  const double cs = (n & 1) ? a : b, sn = (n & 1) ? b : a;
+  *c = ((n + 1) & 2) ? -cs * factor : cs * factor;
+  *s = (n & 2) ? -sn * factor : sn * factor;
 }
 
-// A lane's four pairs of a head, the pairs 4 chunk .. 4 chunk + 3 of head_dim / 2: those below rotary_dim / 2 are rotated.
-template <class Real>
-struct Pairs {
-  Real a[4], b[4];
-};
-
-// Norm and rotation in fp32 or fp64; lanes without pairs hold zeros and keep them.
-template <int LPH, class Real>
-__device__ __forceinline__ void norm_rotate(const HeadsArgs& A, Pairs<Real>& x, bool norm, const float (&wa)[4], const float (&wb)[4],
-                                            int rotated, const Real (&c)[4], const Real (&s)[4]) {
-  if (norm) {
-    Real sum = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sum += x.a[j] * x.a[j] + x.b[j] * x.b[j];
-    sum = head_sum<LPH>(sum);
-    const Real r = Real(1) / sqrt(sum / static_cast<Real>(A.p.head_dim) + static_cast<Real>(A.p.eps));
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      x.a[j] = x.a[j] * r * static_cast<Real>(wa[j]);
-      x.b[j] = x.b[j] * r * static_cast<Real>(wb[j]);
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (j < rotated) {
-      const Real a = x.a[j], b = x.b[j];
-      x.a[j] = a * c[j] - b * s[j];
-      x.b[j] = b * c[j] + a * s[j];
-    }
-  }
+// The same in fp32, to about 1e-7 (y^11 / 11!, y^10 / 10! left out), from t in 64 bits
+__device__ __forceinline__ void turn(double t, float factor, float* c, float* s) {
+  const double quarter = rint(4.0 * t);
+  const float y = static_cast<float>(fma(quarter, -0.25, t)) * 6.2831855f, z = y * y;
+  float a = fmaf(z, 1.0f / 362880.0f, -1.0f / 5040.0f);
+  a = fmaf(z, a, 1.0f / 120.0f);
+  a = fmaf(z, a, -1.0f / 6.0f);
+  a = fmaf(z * y, a, y);
+  float b = fmaf(z, 1.0f / 40320.0f, -1.0f / 720.0f);
+  b = fmaf(z, b, 1.0f / 24.0f);
+  b = fmaf(z, b, -0.5f);
+  b = fmaf(z, b, 1.0f);
+  const int n = static_cast<int>(quarter);
+  const float cs = (n & 1) ? a : b, sn = (n & 1) ? b : a;
+  *c = ((n + 1) & 2) ? -cs * factor : cs * factor;
+  *s = (n & 2) ? -sn * factor : sn * factor;
 }
 
 __device__ __forceinline__ uint32_t half_of(double x) { return f32_to_f16_bits(static_cast<float>(x)); }
-template <class Real> __device__ __forceinline__ Real saturate(Real x) { return x > Real(65504) ? Real(65504) : x < Real(-65504) ? Real(-65504) : x; }
 
-// Parameters and codes of a head whose pairs are spread over LPH lanes.  `error` bounds how far the pairs are off, relative to
-// the largest of them.  Returns whether a rounding (of scale, offset or a code) is closer to its border than that.
-template <int LPH, class Real>
-__device__ __forceinline__ bool quantize_head(Pairs<Real>& x, bool active, Real error, uint32_t* scale_bits, uint32_t* offset_bits,
-                                              uint32_t (&code)[8]) {
-  bool nan = false;
-  Real hi = Real(-65504), lo = Real(65504);
+// Two runs of NPL dimensions of a head, held by one lane
+template <class Real, int NPL>
+struct Runs {
+  Real x[2][NPL];
+};
+
+template <int LPH, int NPL, class Real>
+__device__ __forceinline__ void norm(const HeadsArgs& A, Runs<Real, NPL>& v, const float (&weight)[2][NPL]) {
+  Real sum = 0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    nan = nan || x.a[j] != x.a[j] || x.b[j] != x.b[j];
-    x.a[j] = saturate(x.a[j]);
-    x.b[j] = saturate(x.b[j]);
-    if (active) {
-      hi = x.a[j] > hi ? x.a[j] : hi;
-      hi = x.b[j] > hi ? x.b[j] : hi;
-      lo = x.a[j] < lo ? x.a[j] : lo;
-      lo = x.b[j] < lo ? x.b[j] : lo;
-    }
-  }
-  hi = head_max<LPH>(hi);
-  lo = -head_max<LPH>(-lo);
-  const int lane = __lane_id();
-  nan = ((__ballot(nan && active) >> (lane & ~(LPH - 1))) & (LPH == 64 ? ~0ull : (1ull << (LPH & 63)) - 1)) != 0;
-  const double largest = hi > -lo ? hi : -lo, e = static_cast<double>(error) * largest;
-  const double step = (static_cast<double>(hi) - static_cast<double>(lo)) / 15.0;
-  const uint32_t sb = half_of(step);
-  const double scale = f16_bits_to_f32(sb);
-  const double middle = static_cast<double>(lo) + 8.0 * scale;
-  const uint32_t ob = half_of(middle);
-  const Real offset = f16_bits_to_f32(ob), sc = f16_bits_to_f32(sb);
-  bool close = error > 0 && (half_of(step - e) != half_of(step + e) || half_of(middle - e) != half_of(middle + e));
-  const Real near = static_cast<Real>(0.5) - static_cast<Real>(e / scale + 2e-6);  // never reached in fp64 (error is 0 there)
-  auto one = [&](Real v) -> uint32_t {
-    if (sc == 0) return 8;
-    const Real t = (v - offset) / sc, r = rint(t);
-    if (sizeof(Real) == 4) close = close || !(fabs(t - r) < near);
-    return static_cast<uint32_t>(static_cast<int>(r < -8 ? Real(-8) : r > 7 ? Real(7) : r) + 8);
-  };
+  for (int j = 0; j < 2 * NPL; ++j) sum = fma(v.x[j / NPL][j % NPL], v.x[j / NPL][j % NPL], sum);
+  sum = over_head<LPH>(sum, [](Real a, Real b) { return a + b; });
+  const Real r = Real(1) / sqrt(sum / static_cast<Real>(A.p.head_dim) + static_cast<Real>(A.p.eps));
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    code[j] = one(x.a[j]);
-    code[4 + j] = one(x.b[j]);
-  }
-  if (nan) {
-    *scale_bits = *offset_bits = 0x7e00;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) code[j] = 8;
-    return false;
-  }
-  *scale_bits = sb;
-  *offset_bits = ob;
-  return close && active;
+  for (int j = 0; j < 2 * NPL; ++j) v.x[j / NPL][j % NPL] = v.x[j / NPL][j % NPL] * r * static_cast<Real>(weight[j / NPL][j % NPL]);
 }
 
-// One wavefront takes one token: its cosines and sines once, then groups of 64 / LPH heads, LPH lanes a head, four pairs a
-// lane.  In the half layout the two ends of a rotated pair lie rotary_dim / 2 apart, so a lane's eight dimensions are two
-// runs of four, otherwise one of eight.
+// The lane's pairs, each turned by what turn_of(pair) gives: the first `rotated` of them, with WHOLE all or none.  `across`: a pair's
+// ends are in the two runs, otherwise neighbours in one
+template <bool WHOLE, int NPL, class Real, class F>
+__device__ __forceinline__ void rotate(Runs<Real, NPL>& v, bool across, int rotated, F&& turn_of) {
+  auto pair = [&](int j, Real& a, Real& b) {
+    Real c, s;
+    turn_of(j, &c, &s);
+    const Real u = a, w = b;
+    a = fma(u, c, -(w * s));
+    b = fma(w, c, u * s);
+  };
+  if (rotated == 0) return;
+  if (across) {
+#pragma unroll
+    for (int j = 0; j < NPL; ++j)
+      if (WHOLE || j < rotated) pair(j, v.x[0][j], v.x[1][j]);
+    asm volatile("; ends of pairs in two runs");  // (two branches that end alike would be merged, with the runs in memory)
+  } else {
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) pair(j, v.x[2 * j / NPL][2 * j % NPL], v.x[2 * j / NPL][2 * j % NPL + 1]);
+  }
+}
+
+// Parameters and codes of a head whose dimensions are spread over LPH lanes (`mine`: this lane has some).
+template <int LPH, int NPL>
+__device__ __forceinline__ void quantize_head(Runs<double, NPL>& v, bool mine, uint32_t* scale_bits, uint32_t* offset_bits, uint32_t (&code)[2][NPL]) {
+  bool nan = false;
+  double hi = -65504.0, lo = 65504.0;
+#pragma unroll
+  for (int j = 0; j < 2 * NPL; ++j) {
+    double& x = v.x[j / NPL][j % NPL];
+    nan = nan || x != x;
+    x = fmin(fmax(x, -65504.0), 65504.0);
+    if (mine) {
+      hi = fmax(hi, x);
+      lo = fmin(lo, x);
+    }
+  }
+  hi = over_head<LPH>(hi, [](double a, double b) { return fmax(a, b); });
+  lo = over_head<LPH>(lo, [](double a, double b) { return fmin(a, b); });
+  const int lane = __lane_id();
+  nan = ((__ballot(nan && mine) >> (lane & ~(LPH - 1))) & ((1ull << LPH) - 1)) != 0;
+  const uint32_t sb = half_of((hi - lo) / 15.0);
+  const double scale = f16_bits_to_f32(sb);
+  const uint32_t ob = half_of(fma(8.0, scale, lo));
+  const double offset = f16_bits_to_f32(ob), inv = scale == 0.0 ? 0.0 : 1.0 / scale;
+  // A quotient that is a half exactly has to come out as one: the product with the reciprocal is off by 2^-52 of it, and adding
+  // and subtracting 3 2^11 rounds it to a multiple of 2^-40.
+#pragma unroll
+  for (int j = 0; j < 2 * NPL; ++j) {
+    double t = (v.x[j / NPL][j % NPL] - offset) * inv;
+    t = (t + 6144.0) - 6144.0;
+    const int r = static_cast<int>(rint(t));
+    code[j / NPL][j % NPL] = static_cast<uint32_t>((r < -8 ? -8 : r > 7 ? 7 : r) + 8);
+  }
+  *scale_bits = nan ? 0x7e00u : sb;
+  *offset_bits = nan ? 0x7e00u : ob;
+}
+
+// A pass is 64 / LPH heads of one token's keys, values or queries, in this order: LPH lanes a head, NPL pairs a lane.  In the half
+// layout the two ends of a rotated pair lie rotary_dim / 2 apart, so a lane's dimensions are two runs of NPL, otherwise one of
+// 2 NPL; runs are 16-byte loads where alignment and sizes allow (VEC; NPL = 8 of 16-bit types).  The passes of all tokens in
+// a row are cut into equal shares for as many wavefronts as the device holds; a share's next pass is being loaded while one
+// is worked on, and a token's cosines and sines are computed once for its passes in a share.
 //
-// The codes of the cache are those of the 64-bit formulas: a key computed again by another call (a shared prefix, a resumed
-// sequence) has the same codes.  The fp32 pass knows how far it may be off and tells when a rounding is closer to its border
-// than that, for about one head in a hundred; those are done again in fp64.
-template <int T, int LPH, bool VEC, bool APPEND>
-__global__ __launch_bounds__(256) void heads_kernel(const HeadsArgs A) {
-  __shared__ __align__(8) uint8_t lds_codes[APPEND ? 4 * 64 * 8 : 8];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + wave;
-  const int64_t token = unit / A.parts;
-  if (token >= A.tokens) return;
-  const int part = static_cast<int>(unit - token * A.parts);
+// Queries are normed and rotated in fp32.  Keys go through 64 bits all the way to their codes: a key computed by another call (a
+// shared prefix, a resumed sequence) has the same codes then, whichever way the arithmetic is ordered, and with eight kv heads to a
+// token it is a tenth of the vector instructions' time that the memory takes.
+#ifndef SPLIT_FROM
+#define SPLIT_FROM 512
+#endif
+#ifndef HA8
+#define HA8 2
+#define HA4 3
+#define HN8 4
+#endif
+template <int NPL, bool APPEND> constexpr int kHeadsOccupancy = APPEND ? (NPL == 8 ? HA8 : HA4) : NPL == 8 ? HN8 : 6;
+template <int T, int NPL, int LPH, bool VEC, bool APPEND>
+__global__ __launch_bounds__(256, (kHeadsOccupancy<NPL, APPEND>)) void heads_kernel(const HeadsArgs A) {
+  constexpr bool DWORDS = VEC && NPL == 8;  // a run is a dword of codes
+  constexpr int WORDS = VEC ? NPL * (T == ITEXHIP_FLOAT ? 4 : 2) / 4 : NPL;
+  using Angle = std::conditional_t<APPEND, double, float>;
+  __shared__ __align__(16) Angle lds_turns[4][128][2];  // a wavefront's token: cosine and sine of each pair
+  __shared__ __align__(8) uint8_t lds_codes[APPEND && !DWORDS ? 4 * 64 * 2 * NPL : 8];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t begin = (static_cast<int64_t>(blockIdx.x) * 4 + wave) * A.share;
+  const int64_t end = begin + A.share < A.tokens * A.passes ? begin + A.share : A.tokens * A.passes;
+  if (begin >= end) return;
   const int sub = lane & (LPH - 1), group = lane / LPH;
-  const int D = A.p.head_dim, half_rot = A.p.rotary_dim / 2, pair0 = 4 * sub;
-  const bool active = pair0 < D / 2;
-  const int rotated = active ? (half_rot - pair0 < 0 ? 0 : half_rot - pair0 > 4 ? 4 : half_rot - pair0) : 0;
-  const bool split = !A.p.interleaved && pair0 < half_rot;  // VEC: the whole chunk is rotated or none of it
-  const int run0 = split ? pair0 : 2 * pair0, run1 = split ? pair0 + half_rot : 2 * pair0 + 4;
-  auto dim_a = [&](int j) { return !A.p.interleaved && pair0 + j < half_rot ? pair0 + j : 2 * (pair0 + j); };
-  auto dim_b = [&](int j) { return !A.p.interleaved && pair0 + j < half_rot ? pair0 + j + half_rot : 2 * (pair0 + j) + 1; };
-
-  auto load = [&](const void* src, int64_t at, Pairs<float>& x) {
-    if constexpr (VEC) {
-      float u[4] = {}, w[4] = {};
-      if (active) {
-        load4<T>(src, at + run0, u);
-        load4<T>(src, at + run1, w);
-      }
-      x.a[0] = u[0]; x.a[1] = split ? u[1] : u[2]; x.a[2] = split ? u[2] : w[0]; x.a[3] = split ? u[3] : w[2];
-      x.b[0] = split ? w[0] : u[1]; x.b[1] = split ? w[1] : u[3]; x.b[2] = split ? w[2] : w[1]; x.b[3] = w[3];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool in = pair0 + j < D / 2;
-        x.a[j] = in ? load1<T>(src, at + dim_a(j)) : 0.0f;
-        x.b[j] = in ? load1<T>(src, at + dim_b(j)) : 0.0f;
-      }
-    }
+  const int D = A.p.head_dim, half_rot = A.p.rotary_dim / 2, pair0 = NPL * sub;
+  const bool mine = pair0 < D / 2;
+  const int rotated = mine ? (half_rot - pair0 < 0 ? 0 : half_rot - pair0 > NPL ? NPL : half_rot - pair0) : 0;
+  const bool split = !A.p.interleaved && pair0 < half_rot;  // VEC: all the lane's pairs are rotated or none
+  const int run0 = split ? pair0 : 2 * pair0, run1 = split ? pair0 + half_rot : 2 * pair0 + NPL;
+  // without VEC: run 0 holds the pairs' first ends, run 1 the second ones, wherever they are
+  auto dim_of = [&](int r, int j) {
+    if constexpr (VEC) return (r == 0 ? run0 : run1) + j;
+    else return !A.p.interleaved && pair0 + j < half_rot ? pair0 + j + r * half_rot : 2 * (pair0 + j) + r;
   };
-  auto store = [&](void* dst, int64_t at, const Pairs<float>& x) {
-    if constexpr (VEC) {
-      if (!active) return;
-      const float u[4] = {x.a[0], split ? x.a[1] : x.b[0], split ? x.a[2] : x.a[1], split ? x.a[3] : x.b[1]};
-      const float w[4] = {split ? x.b[0] : x.a[2], split ? x.b[1] : x.b[2], split ? x.b[2] : x.a[3], x.b[3]};
-      store4<T>(dst, at + run0, u);
-      store4<T>(dst, at + run1, w);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (pair0 + j >= D / 2) continue;
-        store_output<T>(dst, at + dim_a(j), x.a[j]);
-        store_output<T>(dst, at + dim_b(j), x.b[j]);
-      }
-    }
-  };
+  auto in_head = [&](int j) { return VEC ? mine : pair0 + j < D / 2; };
 
-  double phase[4] = {};
-  float c[4] = {}, s[4] = {};
+  struct Raw { uint32_t w[2][WORDS]; };
+  auto load = [&](const void* src, int64_t at, Raw& raw) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (j < rotated) {
-      const double t = static_cast<double>(A.positions[token]) * A.freqs[pair0 + j];
-      phase[j] = t - rint(t);
-      turn(static_cast<float>(phase[j]), A.p.attention_factor, &c[j], &s[j]);
-    }
-  }
-  int64_t slot = -1, page_at = 0;
-  if constexpr (APPEND) {
-    slot = A.slots[token];
-    if (slot >= 0 && slot < A.num_slots) page_at = (slot >> A.page_shift) * A.page_bytes;
-    else slot = -1;
-  }
-  float wa[4] = {1, 1, 1, 1}, wb[4] = {1, 1, 1, 1};
-  int loaded = -1;
-  for (int pass = part; pass < A.passes; pass += A.parts) {
-    const int role = pass < A.passes_q ? 0 : pass < A.passes_q + A.passes_k ? 1 : 2;
-    if (APPEND && role > 0 && slot < 0) break;
-    const int first = role == 0 ? 0 : role == 1 ? A.passes_q : A.passes_q + A.passes_k;
-    const int head = (pass - first) * (64 / LPH) + group, heads = role == 0 ? A.p.q_heads : A.p.kv_heads;
-    const void* src = role == 0 ? A.q : role == 1 ? A.k : A.v;
-    const int64_t* st = role == 0 ? A.p.q_strides : role == 1 ? A.p.k_strides : A.p.v_strides;
-    const float* weight = role == 0 ? A.q_weight : role == 1 ? A.k_weight : nullptr;
-    const bool there = head < heads;  // lanes beyond the last head run along on its values and store nothing
-    const int64_t at = token * st[0] + (there ? head : heads - 1) * st[1];
-    Pairs<float> x;
-    load(src, at, x);
-    if (weight != nullptr && loaded != role) {
-      loaded = role;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (pair0 + j < D / 2) {
-          wa[j] = weight[dim_a(j)];
-          wb[j] = weight[dim_b(j)];
+    for (int r = 0; r < 2; ++r) {
+      if constexpr (VEC) {
+        const char* from = static_cast<const char*>(src) + (at + (r == 0 ? run0 : run1)) * (T == ITEXHIP_FLOAT ? 4 : 2);
+        if (mine) {
+          if constexpr (WORDS == 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(from);
+            raw.w[r][0] = v.x; raw.w[r][1] = v.y; raw.w[r][2] = v.z; raw.w[r][3] = v.w;
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(from);
+            raw.w[r][0] = v.x; raw.w[r][1] = v.y;
+          }
         }
-      }
-    }
-    if (role == 0 || !APPEND) {
-      norm_rotate<LPH, float>(A, x, weight != nullptr, wa, wb, rotated, c, s);
-      const int64_t* so = role == 0 ? A.p.q_out_strides : A.p.k_out_strides;
-      if (there) store(role == 0 ? A.q_out : A.k_out, token * so[0] + head * so[1], x);
-      continue;
-    }
-    if constexpr (APPEND) {
-      const Pairs<float> raw = x;
-      uint32_t code[8], scale_bits, offset_bits;
-      bool close;
-      if (role == 1) {
-        norm_rotate<LPH, float>(A, x, weight != nullptr, wa, wb, rotated, c, s);
-        close = quantize_head<LPH, float>(x, active, 2e-6f, &scale_bits, &offset_bits, code);
       } else {
-        close = quantize_head<LPH, float>(x, active, 0.0f, &scale_bits, &offset_bits, code);
-      }
-      if (__any(close)) {
-        Pairs<double> y;
-        double cd[4] = {}, sd[4] = {};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          y.a[j] = raw.a[j];
-          y.b[j] = raw.b[j];
-          if (role == 1 && j < rotated) turn(phase[j], A.p.attention_factor, &cd[j], &sd[j]);
-        }
-        if (role == 1) norm_rotate<LPH, double>(A, y, weight != nullptr, wa, wb, rotated, cd, sd);
-        quantize_head<LPH, double>(y, active, 0.0, &scale_bits, &offset_bits, code);
-      }
-      // to the order of the dimensions through LDS, eight codes a lane
-      uint8_t* mine = lds_codes + wave * 512 + group * (LPH * 8);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (!active) continue;
-
-
-        mine[dim_a(j)] = static_cast<uint8_t>(code[j]);
-        mine[dim_b(j)] = static_cast<uint8_t>(code[4 + j]);
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      uint32_t packed = 0x88888888u;  // the padding of a head: codes that stand for the offset, never used
-      if (active) {
-        const uint2 w = *reinterpret_cast<const uint2*>(mine + 8 * sub);
-        packed = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          packed |= ((w.x >> (8 * j)) & 15u) << (4 * j);
-          packed |= ((w.y >> (8 * j)) & 15u) << (16 + 4 * j);
-        }
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      const Kv4Block block{A.page_size, A.dp};
-      if (there && 8 * sub < A.dp) {
-        uint8_t* to = A.cache + page_at + static_cast<int64_t>(head) * block.bytes();
-        const int in_page = static_cast<int>(slot & (A.page_size - 1));
-        *reinterpret_cast<uint32_t*>(to + (role == 1 ? block.key_codes(in_page) + 4 * sub : block.value_codes(in_page, sub))) = packed;
-        if (sub == 0) {
-          uint8_t* par = to + (role == 1 ? block.key_params(in_page) : block.value_params(in_page));
-          *reinterpret_cast<uint16_t*>(par) = static_cast<uint16_t>(scale_bits);
-          *reinterpret_cast<uint16_t*>(par + 8) = static_cast<uint16_t>(offset_bits);
-        }
+        for (int j = 0; j < NPL; ++j)
+          if (in_head(j)) raw.w[r][j] = __float_as_uint(load1<T>(src, at + dim_of(r, j)));
       }
     }
+  };
+  auto widen = [&](const Raw& raw, auto& v) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+#pragma unroll
+      for (int j = 0; j < NPL; ++j) {
+        float x;
+        if constexpr (!VEC || T == ITEXHIP_FLOAT) {
+          x = __uint_as_float(raw.w[r][j]);
+        } else {
+          const uint32_t h = (raw.w[r][j / 2] >> (16 * (j % 2))) & 0xffffu;
+          x = T == ITEXHIP_BFLOAT16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
+        }
+        v.x[r][j] = in_head(j) ? x : 0.0f;
+      }
+    }
+  };
+  auto store = [&](void* dst, int64_t at, const Runs<float, NPL>& v) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      if constexpr (VEC) {
+        if (!mine) continue;
+        char* to = static_cast<char*>(dst) + (at + (r == 0 ? run0 : run1)) * (T == ITEXHIP_FLOAT ? 4 : 2);
+        if constexpr (T == ITEXHIP_FLOAT) {
+          *reinterpret_cast<f4*>(to) = f4{v.x[r][0], v.x[r][1], v.x[r][2], v.x[r][3]};
+        } else {
+          uint32_t w[WORDS];
+#pragma unroll
+          for (int j = 0; j < WORDS; ++j) w[j] = f32x2_to_bits16<T>(v.x[r][2 * j], v.x[r][2 * j + 1]);
+          if constexpr (WORDS == 4) *reinterpret_cast<uint4*>(to) = uint4{w[0], w[1], w[2], w[3]};
+          else *reinterpret_cast<uint2*>(to) = uint2{w[0], w[1]};
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < NPL; ++j)
+          if (in_head(j)) store_output<T>(dst, at + dim_of(r, j), v.x[r][j]);
+      }
+    }
+  };
+
+  enum { kKeys, kValues, kQueries };
+  struct Pass { int64_t token, slot; int position, role, head, there; };  // no padding: its copy would be an array in memory
+  auto pass_of = [&](int64_t token, int pass, Raw& to) {
+    Pass q;
+    q.token = token;
+    q.role = pass < A.passes_k ? kKeys : pass < A.passes_k + A.passes_v ? kValues : kQueries;
+    const int first = q.role == kKeys ? 0 : q.role == kValues ? A.passes_k : A.passes_k + A.passes_v;
+    const int heads = q.role == kQueries ? A.p.q_heads : A.p.kv_heads;
+    const int64_t st = q.role == kQueries ? A.p.q_strides[0] : q.role == kKeys ? A.p.k_strides[0] : A.p.v_strides[0];
+    const int64_t sh = q.role == kQueries ? A.p.q_strides[1] : q.role == kKeys ? A.p.k_strides[1] : A.p.v_strides[1];
+    q.head = (pass - first) * (64 / LPH) + group;
+    q.there = q.head < heads;  // lanes beyond the last head run along on its values and store nothing
+    q.position = half_rot > 0 ? A.positions[token] : 0;
+    q.slot = 0;
+    if constexpr (APPEND) q.slot = A.slots[token];
+    load(q.role == kQueries ? A.q : q.role == kKeys ? A.k : A.v, token * st + (q.there ? q.head : heads - 1) * sh, to);
+    return q;
+  };
+  Raw raw, next;
+  int64_t token = begin / A.passes;
+  int pass = static_cast<int>(begin - token * A.passes);
+  Pass now = pass_of(token, pass, raw);
+  float weight[2][NPL];
+  int64_t turned = -1;  // the token that lds_turns is for
+  int weights_of = -1;
+  for (int64_t i = begin; i < end; ++i) {
+    Pass then = now;
+    if (++pass == A.passes) {
+      pass = 0;
+      ++token;
+    }
+    if (i + 1 < end) then = pass_of(token, pass, next);
+    const float* w = now.role == kQueries ? A.q_weight : now.role == kKeys ? A.k_weight : nullptr;
+    if (w != nullptr && weights_of != now.role) {
+      weights_of = now.role;
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) weight[r][j] = in_head(j) ? w[dim_of(r, j)] : 0.0f;
+    }
+    if (half_rot > 0 && turned != now.token && now.role != kValues) {
+      turned = now.token;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      for (int pair = lane; pair < half_rot; pair += 64) {
+        const double t = static_cast<double>(now.position) * A.freqs[pair];
+        turn(t - rint(t), static_cast<Angle>(A.p.attention_factor), &lds_turns[wave][pair][0], &lds_turns[wave][pair][1]);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+    auto turn_of = [&](int j, auto* c, auto* s) {
+      const Angle* at = lds_turns[wave][VEC ? pair0 + j : min(pair0 + j, half_rot - 1)];
+      *c = static_cast<std::remove_reference_t<decltype(*c)>>(at[0]);
+      *s = static_cast<std::remove_reference_t<decltype(*s)>>(at[1]);
+    };
+    if (now.role == kQueries || !APPEND) {
+      Runs<float, NPL> v;
+      widen(raw, v);
+      if (w != nullptr) norm<LPH>(A, v, weight);
+      rotate<VEC, NPL, float>(v, !VEC || split, rotated, turn_of);
+      const int64_t st = now.role == kQueries ? A.p.q_out_strides[0] : A.p.k_out_strides[0], sh = now.role == kQueries ? A.p.q_out_strides[1] : A.p.k_out_strides[1];
+      if (now.there) store(now.role == kQueries ? A.q_out : A.k_out, now.token * st + now.head * sh, v);
+    } else if constexpr (APPEND) {
+      Runs<double, NPL> v;
+      widen(raw, v);
+      if (now.role == kKeys) {
+        if (w != nullptr) norm<LPH>(A, v, weight);
+        rotate<VEC, NPL, double>(v, !VEC || split, rotated, turn_of);
+      }
+      const bool placed = now.slot >= 0 && now.slot < A.num_slots;
+      const int64_t slot = placed ? now.slot : 0, page_at = (slot >> A.page_shift) * A.page_bytes;
+      now.there = now.there && placed;
+      uint32_t code[2][NPL], scale_bits, offset_bits;
+      quantize_head<LPH, NPL>(v, mine, &scale_bits, &offset_bits, code);
+      const Kv4Block block{A.page_size, A.dp};
+      uint8_t* to = A.cache + page_at + static_cast<int64_t>(now.head) * block.bytes();
+      const int place = static_cast<int>(slot & (A.page_size - 1));
+      auto put = [&](int dword, uint32_t packed) {
+        *reinterpret_cast<uint32_t*>(to + (now.role == kKeys ? block.key_codes(place) + 4 * dword : block.value_codes(place, dword))) = packed;
+      };
+      // the padding of a head: codes that stand for the offset; nothing uses them
+      if constexpr (DWORDS) {
+        uint32_t packed[2] = {0, 0};
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) packed[r] |= code[r][j] << (4 * j);
+        if (now.there) {
+          if (mine) {
+            put(run0 / 8, packed[0]);
+            put(run1 / 8, packed[1]);
+          } else if (16 * sub < A.dp) {
+            put(2 * sub, 0x88888888u);
+            put(2 * sub + 1, 0x88888888u);
+          }
+        }
+      } else {
+        // to the order of the dimensions through LDS; the lane then has 2 NPL consecutive ones
+        uint8_t* codes = lds_codes + (wave * 64 + group * LPH) * 2 * NPL;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          if constexpr (VEC) {
+            if (mine) *reinterpret_cast<uint32_t*>(codes + dim_of(r, 0)) = code[r][0] | code[r][1] << 8 | code[r][2] << 16 | code[r][3] << 24;
+          } else {
+#pragma unroll
+            for (int j = 0; j < NPL; ++j)
+              if (in_head(j)) codes[dim_of(r, j)] = static_cast<uint8_t>(code[r][j]);
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        static_assert(NPL == 4 || DWORDS, "a dword a lane");
+        uint32_t packed = 0x88888888u;
+        if (mine) {
+          const uint2 u = *reinterpret_cast<const uint2*>(codes + 8 * sub);
+          packed = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            packed |= ((u.x >> (8 * j)) & 15u) << (4 * j);
+            packed |= ((u.y >> (8 * j)) & 15u) << (16 + 4 * j);
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (now.there && 8 * sub < A.dp) put(sub, packed);
+      }
+      if (now.there && sub == 0) {
+        uint8_t* par = to + (now.role == kKeys ? block.key_params(place) : block.value_params(place));
+        *reinterpret_cast<uint16_t*>(par) = static_cast<uint16_t>(scale_bits);
+        *reinterpret_cast<uint16_t*>(par + 8) = static_cast<uint16_t>(offset_bits);
+      }
+    }
+    raw = next;
+    now = then;
   }
 }
 
@@ -388,37 +477,50 @@ int check_heads(const char* who, const itexhip_heads_params* p, int64_t tokens) 
   return ITEXHIP_OK;
 }
 
+template <int T, int NPL, int LPH, bool VEC, bool APPEND>
+void launch(HeadsArgs& A, hipStream_t stream) {
+  // as many wavefronts as the device holds at once, or one a pass
+  const int64_t all = A.tokens * A.passes, held = 1024 * kHeadsOccupancy<NPL, APPEND>;
+  A.share = (all + held - 1) / held;
+  const int64_t waves = (all + A.share - 1) / A.share;
+  heads_kernel<T, NPL, LPH, VEC, APPEND><<<dim3(static_cast<unsigned>((waves + 3) / 4)), dim3(256), 0, stream>>>(A);
+}
 template <int T, bool APPEND>
-void launch(const HeadsArgs& A, int lph, bool vec, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>((A.tokens * A.parts + 3) / 4)), block(256);
-  if (!vec) heads_kernel<T, 32, false, APPEND><<<grid, block, 0, stream>>>(A);
-  else if (lph == 8) heads_kernel<T, 8, true, APPEND><<<grid, block, 0, stream>>>(A);
-  else if (lph == 16) heads_kernel<T, 16, true, APPEND><<<grid, block, 0, stream>>>(A);
-  else heads_kernel<T, 32, true, APPEND><<<grid, block, 0, stream>>>(A);
+void launch_runs(HeadsArgs& A, int npl, int lph, bool vec, hipStream_t stream) {
+  if constexpr (T != ITEXHIP_FLOAT) {
+    if (npl == 8) {
+      if (lph == 4) launch<T, 8, 4, true, APPEND>(A, stream);
+      else if (lph == 8) launch<T, 8, 8, true, APPEND>(A, stream);
+      else launch<T, 8, 16, true, APPEND>(A, stream);
+      return;
+    }
+  }
+  if (!vec) launch<T, 4, 32, false, APPEND>(A, stream);
+  else if (lph == 8) launch<T, 4, 8, true, APPEND>(A, stream);
+  else if (lph == 16) launch<T, 4, 16, true, APPEND>(A, stream);
+  else launch<T, 4, 32, true, APPEND>(A, stream);
 }
 
 template <bool APPEND>
 int run(HeadsArgs& A, hipStream_t stream, const char* who) {
   const itexhip_heads_params& p = A.p;
-  const size_t esize = p.type == ITEXHIP_FLOAT ? 4 : 2, vector = 4 * esize;
-  bool vec = p.head_dim % 8 == 0 && (p.rotary_dim % 8 == 0);
-  auto ok = [&](const void* x, const int64_t* s) { vec = vec && (x == nullptr || (aligned(x, vector) && s[0] % 4 == 0 && s[1] % 4 == 0)); };
-  ok(A.q, p.q_strides);
-  ok(A.k, p.k_strides);
-  ok(A.v, p.v_strides);
-  ok(A.q_out, p.q_out_strides);
-  ok(A.k_out, p.k_out_strides);
-  const int lph = !vec ? 32 : p.head_dim <= 64 ? 8 : p.head_dim <= 128 ? 16 : 32, group = 64 / lph;
-  A.passes_q = A.q != nullptr ? (p.q_heads + group - 1) / group : 0;
+  const size_t esize = p.type == ITEXHIP_FLOAT ? 4 : 2;
+  // runs of `n` elements as one load: sizes, strides and addresses are multiples of it
+  auto runs_of = [&](int n) {
+    auto ok = [&](const void* x, const int64_t* s) { return x == nullptr || (aligned(x, n * esize) && s[0] % n == 0 && s[1] % n == 0); };
+    return p.head_dim % (2 * n) == 0 && p.rotary_dim % (2 * n) == 0 && ok(A.q, p.q_strides) && ok(A.k, p.k_strides) && ok(A.v, p.v_strides) &&
+           ok(A.q_out, p.q_out_strides) && ok(A.k_out, p.k_out_strides);
+  };
+  const int npl = p.type != ITEXHIP_FLOAT && runs_of(8) ? 8 : 4;
+  const bool vec = npl == 8 || runs_of(4);
+  const int lph = !vec ? 32 : (p.head_dim <= 64 ? 32 : p.head_dim <= 128 ? 64 : 128) / npl, group = 64 / lph;
   A.passes_k = A.k != nullptr ? (p.kv_heads + group - 1) / group : 0;
-  A.passes = A.passes_q + A.passes_k * (APPEND ? 2 : 1);
+  A.passes_v = APPEND ? A.passes_k : 0;
+  A.passes = A.passes_k + A.passes_v + (A.q != nullptr ? (p.q_heads + group - 1) / group : 0);
   if (A.passes == 0 || A.tokens == 0) return ITEXHIP_OK;
-  // few tokens: a token's groups of heads go to several wavefronts, each with its own cosines and sines
-  const int64_t waves = 8192;
-  A.parts = static_cast<int>(A.tokens >= waves ? 1 : (waves + A.tokens - 1) / A.tokens < A.passes ? (waves + A.tokens - 1) / A.tokens : A.passes);
-  if (p.type == ITEXHIP_FLOAT) launch<ITEXHIP_FLOAT, APPEND>(A, lph, vec, stream);
-  else if (p.type == ITEXHIP_BFLOAT16) launch<ITEXHIP_BFLOAT16, APPEND>(A, lph, vec, stream);
-  else launch<ITEXHIP_HALF, APPEND>(A, lph, vec, stream);
+  if (p.type == ITEXHIP_FLOAT) launch_runs<ITEXHIP_FLOAT, APPEND>(A, npl, lph, vec, stream);
+  else if (p.type == ITEXHIP_BFLOAT16) launch_runs<ITEXHIP_BFLOAT16, APPEND>(A, npl, lph, vec, stream);
+  else launch_runs<ITEXHIP_HALF, APPEND>(A, npl, lph, vec, stream);
   ITEXHIP_CHECK_LAUNCH(who);
   return ITEXHIP_OK;
 }
@@ -516,6 +618,12 @@ extern "C" int itexhip_kv4_append(const itexhip_heads_params* p, const itexhip_k
   A.p = *p;
   A.q = q; A.k = k; A.v = v; A.q_weight = q_weight; A.k_weight = k_weight; A.positions = positions; A.freqs = freqs; A.slots = slots;
   A.q_out = q_out; A.cache = static_cast<uint8_t*>(cache); A.tokens = tokens;
+  if (q != nullptr && tokens >= SPLIT_FROM) {
+    HeadsArgs Q = A;
+    Q.k = Q.v = nullptr;
+    if (const int st = run<false>(Q, as_stream(stream), who)) return st;
+    A.q = nullptr;
+  }
   A.page_size = c->page_size;
   A.page_shift = log2_of(c->page_size);
   A.num_slots = c->num_pages * c->page_size;
