@@ -11,6 +11,7 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 
+constexpr int kMostSplitRows = 64;     // rows of a sequence, times heads of a kv head, that split kernels take
 constexpr int kMostGroups = 1024;      // workgroups of a split kernel
 constexpr int kStep = 128;             // tokens a workgroup takes at a time, 32 a wavefront
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -77,8 +78,9 @@ __device__ __forceinline__ float load_q(const void* q, int64_t i) {
 #endif
 #ifndef OCC1
 #define OCC1 3
+#define OCC2 2
 #endif
-template <int T, int DP, int NB> constexpr int kOccupancy = NB == 1 && DP < 256 ? OCC1 : 1;
+constexpr int occupancy_of(int nb, int dp) { return dp == 256 ? 1 : nb == 1 ? OCC1 : OCC2; }  // wavefronts a SIMD of a split kernel
 
 // A wavefront's 16 NB rows against 32 tokens at a time, everything in registers.
 //
@@ -107,7 +109,8 @@ struct Engine {
   static constexpr float kSlack = F32 ? 0.0f : 5.0f;  // log2 of how far a score may exceed the maximum that sums are relative to
   half8v q16[F32 ? 1 : NB][NKK];
   float q32[F32 ? NB : 1][NKK][8];
-  float corr[NB], sumq[NB], qs[NB], m[NB], raise_at[NB], ref[NB], l[NB], po[NB];
+  f4 corr[NB];  // what a product starts from: minus the excess of the codes
+  float sumq[NB], qs[NB], m[NB], raise_at[NB], ref[NB], l[NB], po[NB];
   uint32_t scale_bound;  // half bits that no value's scale so far exceeds: an exponent with all ones below
   int limit[NB], start[NB];  // the tokens that column c of block nb sees: start <= t < limit
   f4 o[NB][E];
@@ -128,21 +131,17 @@ struct Engine {
     c = lane & 15;
     g = lane >> 4;
     const int rows = s.n * A.group;
-    auto sees = [&](int row, int* from, int* to) {
-      const int pos = s.len - s.n + row / A.group;
-      *to = A.causal ? (pos + 1 < 0 ? 0 : pos + 1) : s.len;
-      *from = A.window > 0 && pos - A.window + 1 > 0 ? pos - A.window + 1 : 0;
-    };
-    int unused;
-    sees(row0, &unused, &min_limit);
-    const int last = row0 + 16 * NB - 1;
-    sees(last < rows ? last : rows - 1, &max_start, &unused);
+    const int before = s.len - s.n;  // position of the first row
+    auto limit_of = [&](int row) { return A.causal ? max(before + row / A.group + 1, 0) : s.len; };
+    auto start_of = [&](int row) { return A.window > 0 ? max(before + row / A.group - A.window + 1, 0) : 0; };
+    min_limit = limit_of(row0);
+    max_start = start_of(min(row0 + 16 * NB, rows) - 1);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       const int row = row0 + nb * 16 + c;
       const bool in = row < rows;
-      limit[nb] = start[nb] = 0;
-      if (in) sees(row, &start[nb], &limit[nb]);
+      limit[nb] = in ? limit_of(row) : 0;
+      start[nb] = in ? start_of(row) : 0;
       const int64_t at = in ? (s.first + row / A.group) * A.q_st + static_cast<int64_t>(kv_head * A.group + row % A.group) * A.q_sh : 0;
       float x[NKK][8], most = 0.0f, sum = 0.0f;
 #pragma unroll
@@ -194,7 +193,7 @@ struct Engine {
       excess += __shfl_xor(excess, 16);
       excess += __shfl_xor(excess, 32);
       sumq[nb] = sum;
-      corr[nb] = -excess;
+      corr[nb] = f4{-excess, -excess, -excess, -excess};
       qs[nb] = fmaxf(A.scale * kLog2e * back, 1.2e-38f);
       m[nb] = raise_at[nb] = -INFINITY;
       ref[nb] = kProbExponent + (F32 ? 0.0f : 15.0f);
@@ -324,7 +323,7 @@ struct Engine {
     for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        f4 s = f4{corr[nb], corr[nb], corr[nb], corr[nb]};
+        f4 s = corr[nb];
 #pragma unroll
         for (int kk = 0; kk < NKK; ++kk) {
           if constexpr (!F32) {
@@ -540,12 +539,14 @@ struct Engine {
   }
 };
 
-// Rows of every sequence fit one tile of 16 NB: the tokens are what is divided.  The steps of all sequences and kv heads in a
-// row, [sequence][kv head][step], are cut into equal shares, one a workgroup, whatever the lengths are and without the host
+// Sequences of few rows, in tiles of 16 NB: the tokens are what is divided.  The steps of all sequences, kv heads and tiles in a
+// row, [sequence][kv head][tile][step], are cut into equal shares, one a workgroup, whatever the lengths are and without the host
 // knowing them.  A share may end one (sequence, head), hold several whole ones and begin another: whole ones are written out,
 // the two at its ends leave their sums in the workspace for combine_kernel.
+template <int NB>
+__device__ __forceinline__ int tiles_of(const AttArgs& A, const Seq& s) { return (s.n * A.group + 16 * NB - 1) / (16 * NB); }
 template <int T, int DP, int NB>
-__global__ __launch_bounds__(256, (kOccupancy<T, DP, NB>)) void split_kernel(const AttArgs A) {
+__global__ __launch_bounds__(256, occupancy_of(NB, DP)) void split_kernel(const AttArgs A) {
   __shared__ int64_t scan[5];
   __shared__ int64_t found[2];
   __shared__ float lds_ml[4][2][16 * NB];
@@ -555,7 +556,11 @@ __global__ __launch_bounds__(256, (kOccupancy<T, DP, NB>)) void split_kernel(con
   // steps of all sequences, then the sequence in which this workgroup's share begins
   auto prefix_of = [&](int base, int64_t& inclusive, int64_t& all) {
     const int b = base + tid;
-    int64_t x = b < A.num_seqs ? sequence(A, b).steps * A.kv_heads : 0;
+    int64_t x = 0;
+    if (b < A.num_seqs) {
+      const Seq s = sequence(A, b);
+      x = s.steps * A.kv_heads * tiles_of<NB>(A, s);
+    }
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
       const int64_t y = __shfl_up(x, d);
@@ -582,7 +587,8 @@ __global__ __launch_bounds__(256, (kOccupancy<T, DP, NB>)) void split_kernel(con
     const int b = base + tid;
     __syncthreads();
     if (b < A.num_seqs) {
-      const int64_t mine = sequence(A, b).steps * A.kv_heads, from = before + inclusive - mine;
+      const Seq s = sequence(A, b);
+      const int64_t mine = s.steps * A.kv_heads * tiles_of<NB>(A, s), from = before + inclusive - mine;
       if (begin >= from && begin < from + mine) {
         found[0] = b;
         found[1] = from;
@@ -604,12 +610,12 @@ __global__ __launch_bounds__(256, (kOccupancy<T, DP, NB>)) void split_kernel(con
       continue;
     }
     const int64_t rel = at - from;
-    const int head = static_cast<int>(rel / s.steps);
-    const int64_t s0 = rel - head * s.steps, left = s.steps - s0, n = left < end - at ? left : end - at;
+    const int tiles = tiles_of<NB>(A, s), item = static_cast<int>(rel / s.steps), head = item / tiles, row0 = (item - head * tiles) * 16 * NB;
+    const int64_t s0 = rel - item * s.steps, left = s.steps - s0, n = left < end - at ? left : end - at;
     const bool whole = n == s.steps;
 
     Engine<T, DP, NB> eng;
-    eng.init(A, s, head, 0);
+    eng.init(A, s, head, row0);
     const int first = s.lo + static_cast<int>(s0) * kStep, last = first + static_cast<int>(n) * kStep;
     eng.run(A, A.table + b * A.table_stride, head, first + 32 * wave, last < s.len ? last : s.len, kStep, s.len);
     eng.close();
@@ -658,13 +664,13 @@ __global__ __launch_bounds__(256, (kOccupancy<T, DP, NB>)) void split_kernel(con
     }
     if (wave == 0) {
       if (whole) {
-        eng.finish(A, s, head, 0, top, sum);
+        eng.finish(A, s, head, row0, top, sum);
       } else {
         const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (s0 == 0 ? 1 : 0);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           const int row = nb * 16 + eng.c;
-          if (row >= s.n * A.group) continue;
+          if (row0 + row >= s.n * A.group) continue;
           if (eng.g == 0) {
             A.part_ml[(slot * 16 * NB + row) * 2] = top[nb];
             A.part_ml[(slot * 16 * NB + row) * 2 + 1] = sum[nb];
@@ -679,7 +685,7 @@ __global__ __launch_bounds__(256, (kOccupancy<T, DP, NB>)) void split_kernel(con
       }
     }
     at += n;
-    if (rel + n == s.steps * A.kv_heads) {
+    if (rel + n == s.steps * A.kv_heads * tiles) {
       ++b;
       from = at;
     }
@@ -695,11 +701,12 @@ __global__ __launch_bounds__(256) void combine_kernel(const AttArgs A) {
   const int b = blockIdx.z, head = blockIdx.y, row = blockIdx.x, tid = threadIdx.x;
   const Seq s = sequence(A, b);
   if (row >= s.n * A.group) return;
-  const int64_t share = A.prefix[A.num_seqs], i0 = A.prefix[b] + head * s.steps;
+  const int item = head * tiles_of<NB>(A, s) + row / (16 * NB);
+  const int64_t share = A.prefix[A.num_seqs], i0 = A.prefix[b] + item * s.steps;
   const int64_t w0 = i0 / share, w1 = (i0 + s.steps - 1) / share;
   if (w0 == w1) return;
   const int count = static_cast<int>(w1 - w0 + 1);  // at most the workgroups of the split kernel, kMostGroups
-  auto at = [&](int i) { return (2 * (w0 + i) + (i == 0 ? 1 : 0)) * 16 * NB + row; };
+  auto at = [&](int i) { return (2 * (w0 + i) + (i == 0 ? 1 : 0)) * 16 * NB + row % (16 * NB); };
   const int lane = tid % LANES, part = tid / LANES;
   // every thread takes the maxima and sums of up to CHUNK / 256 parts
   float tops[CHUNK / 256], sums[CHUNK / 256], top = -INFINITY;
@@ -1134,12 +1141,11 @@ Plan plan_of(const itexhip_kv4_attention_params* p, const itexhip_kv4_cache* c) 
   Plan plan = {};
   const int dp = kv4_padded(c->head_dim);
   const int64_t rows = static_cast<int64_t>(p->max_q_len) * (p->q_heads / c->kv_heads);
-  const int most = dp == 256 ? 1 : p->type == ITEXHIP_FLOAT ? 2 : 4;
-  plan.blocks = rows <= 16 || most == 1 ? 1 : rows <= 32 || most == 2 ? 2 : 4;
-  plan.split = rows <= 16 * plan.blocks;
+  plan.blocks = rows <= 16 || dp == 256 ? 1 : 2;
+  plan.split = rows <= kMostSplitRows;
   if (plan.split) {
-    const int64_t bound = static_cast<int64_t>(p->num_seqs) * c->kv_heads * ((p->table_stride * c->page_size + kStep - 1) / kStep);
-    const int64_t full = plan.blocks == 1 && dp < 256 ? OCC1 * 256 : 256;
+    const int64_t bound = static_cast<int64_t>(p->num_seqs) * c->kv_heads * ((p->table_stride * c->page_size + kStep - 1) / kStep) * ((rows + 16 * plan.blocks - 1) / (16 * plan.blocks));
+    const int64_t full = 256 * occupancy_of(plan.blocks, dp);
     plan.groups = bound < 1 ? 1 : bound < full ? bound : full;
     plan.prefix = (static_cast<size_t>(p->num_seqs) + 1) * 8 + 15 & ~size_t{15};
     plan.ml = static_cast<size_t>(plan.groups) * 2 * 16 * plan.blocks * 2 * 4;
@@ -1189,8 +1195,7 @@ void launch(const AttArgs& A, const Plan& plan, hipStream_t stream) {
 template <int T, int DP>
 void launch_blocks(const AttArgs& A, const Plan& plan, hipStream_t stream) {
   if (plan.blocks == 1) launch<T, DP, 1>(A, plan, stream);
-  else if (plan.blocks == 2) { if constexpr (DP != 256) launch<T, DP, 2>(A, plan, stream); }
-  else if constexpr (T != ITEXHIP_FLOAT && DP != 256) launch<T, DP, 4>(A, plan, stream);
+  else if constexpr (DP != 256) launch<T, DP, 2>(A, plan, stream);
 }
 template <int T>
 void launch_dims(const AttArgs& A, const Plan& plan, hipStream_t stream) {
