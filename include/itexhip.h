@@ -547,8 +547,8 @@ int itexhip_qk_norm_rope(const itexhip_heads_params* p, int64_t tokens, const vo
 /* A layer's cache: num_pages rows of itexhip_kv4_page_bytes bytes (16-byte aligned), page_size tokens each.  A token's key
  * (or value) of one head is held as scale * (code - 8) + offset: codes of 0 .. 15, scale and offset in half precision,
  *   scale = half((max - min) / 15), offset = half(min + 8 scale), code = 8 + clamp(rne((x - offset) / scale), -8, 7)
- * of the dimensions after norm and rotation, clamped to +-65504, evaluated as in 64 bits (codes do not depend on the
- * call that made them); scale 0: all codes are 8; a NaN among the dimensions makes scale and offset NaN, and so all of the head's.
+ * of the dimensions after norm and rotation, clamped to +-65504, evaluated in 64 bits (codes do not depend on the
+ * call that made them); scale 0: all codes are 8; a NaN among the dimensions: scale and offset are NaN, all codes 8.
  * A page holds, for each kv head, [page_size][DP / 2] bytes of key codes (lower dimension in the low bits), [page_size / 4]
  * [DP / 8][4 tokens][4] bytes of value codes, [page_size / 4][4 scales, 4 offsets] of the keys and the same of the values;
  * DP is head_dim rounded up to 64, 128 or 256.  (Four tokens' value codes of eight dimensions are one 16-byte load.) */

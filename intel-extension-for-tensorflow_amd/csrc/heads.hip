@@ -87,24 +87,6 @@ __device__ __forceinline__ void turn(double t, double factor, double* c, double*
   *s = (n & 2) ? -sn * factor : sn * factor;
 }
 
-// The same in fp32, to about 1e-7 (y^11 / 11!, y^10 / 10! left out), from t in 64 bits
-__device__ __forceinline__ void turn(double t, float factor, float* c, float* s) {
-  const double quarter = rint(4.0 * t);
-  const float y = static_cast<float>(fma(quarter, -0.25, t)) * 6.2831855f, z = y * y;
-  float a = fmaf(z, 1.0f / 362880.0f, -1.0f / 5040.0f);
-  a = fmaf(z, a, 1.0f / 120.0f);
-  a = fmaf(z, a, -1.0f / 6.0f);
-  a = fmaf(z * y, a, y);
-  float b = fmaf(z, 1.0f / 40320.0f, -1.0f / 720.0f);
-  b = fmaf(z, b, 1.0f / 24.0f);
-  b = fmaf(z, b, -0.5f);
-  b = fmaf(z, b, 1.0f);
-  const int n = static_cast<int>(quarter);
-  const float cs = (n & 1) ? a : b, sn = (n & 1) ? b : a;
-  *c = ((n + 1) & 2) ? -cs * factor : cs * factor;
-  *s = (n & 2) ? -sn * factor : sn * factor;
-}
-
 __device__ __forceinline__ uint32_t half_of(double x) { return f32_to_f16_bits(static_cast<float>(x)); }
 
 // Two runs of NPL dimensions of a head, held by one lane
@@ -169,7 +151,7 @@ __device__ __forceinline__ void quantize_head(Runs<double, NPL>& v, bool mine, u
   const uint32_t sb = half_of((hi - lo) / 15.0);
   const double scale = f16_bits_to_f32(sb);
   const uint32_t ob = half_of(fma(8.0, scale, lo));
-  const double offset = f16_bits_to_f32(ob), inv = scale == 0.0 ? 0.0 : 1.0 / scale;
+  const double offset = f16_bits_to_f32(ob), inv = scale == 0.0 || nan ? 0.0 : 1.0 / scale;
   // A quotient that is a half exactly has to come out as one: the product with the reciprocal is off by 2^-52 of it, and adding
   // and subtracting 3 2^11 rounds it to a multiple of 2^-40.
 #pragma unroll
@@ -332,7 +314,10 @@ __global__ __launch_bounds__(256, (kHeadsOccupancy<NPL, APPEND>)) void heads_ker
       __builtin_amdgcn_wave_barrier();
       for (int pair = lane; pair < half_rot; pair += 64) {
         const double t = static_cast<double>(now.position) * A.freqs[pair];
-        turn(t - rint(t), static_cast<Angle>(A.p.attention_factor), &lds_turns[wave][pair][0], &lds_turns[wave][pair][1]);
+        double c, s;
+        turn(t - rint(t), A.p.attention_factor, &c, &s);
+        lds_turns[wave][pair][0] = static_cast<Angle>(c);
+        lds_turns[wave][pair][1] = static_cast<Angle>(s);
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
