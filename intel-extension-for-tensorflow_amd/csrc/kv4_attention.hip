@@ -1,6 +1,8 @@
 // Attention over the paged 4-bit cache.
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.hpp"
 #include "kv4.hpp"
 
@@ -73,9 +75,6 @@ __device__ __forceinline__ float load_q(const void* q, int64_t i) {
   else return f16_bits_to_f32(static_cast<const uint16_t*>(q)[i]);
 }
 
-#ifndef PWAVES
-#define PWAVES 8
-#endif
 #ifndef OCC1
 #define OCC1 3
 #define OCC2 2
@@ -406,7 +405,9 @@ struct Engine {
         for (int j = 0; j < 8; ++j) {
           const uint32_t sc = vp[j / 4][j % 4 / 2], of = vp[j / 4][2 + j % 4 / 2];
           po[nb] = fmaf(p[nb][j], (j & 1) ? high_half(of) : low_half(of), po[nb]);
-          pb[nb][j] = static_cast<_Float16>(p[nb][j] * ((j & 1) ? high_half(sc) : low_half(sc)));
+          float x = fmaf(p[nb][j], (j & 1) ? high_half(sc) : low_half(sc), 0.0f);
+          asm("" : "+v"(x));  // (merged with the conversion it would be an instruction that writes half a register, at twice the time)
+          pb[nb][j] = static_cast<_Float16>(x);
         }
       }
       // a lane's eight tokens of one dimension, two a register: first the halves of two tokens' dwords that hold its code
@@ -786,21 +787,24 @@ __global__ __launch_bounds__(256) void rows_kernel(const AttArgs A) {
   eng.finish(A, s, head, row0, top, eng.l);
 }
 
-// Sequences of many rows on half MFMAs.  A workgroup takes 32 rows a wavefront through the tokens that they see, TT tokens at a
-// time: all its threads turn a tile's codes into operands in LDS, once for all rows, while the tile before is worked on; the
-// wavefronts read them as whole fragments.  32 x 32 x 16 products with the same transposition as in Engine: S^T = K Q^T gives
-// lane 32 h + c the scores of column c for tokens 8 i + 4 h + 0 .. 3, which O^T = V^T P^T takes as they are.
+// Sequences of many rows on half MFMAs.  A workgroup goes through the tokens that its rows see, TT at a time, 32 rows a wavefront: all
+// its threads turn a tile's codes into operands in LDS, once for all rows, and the wavefronts read them as whole fragments.
+// 32 x 32 x 16 products with the same transposition as in Engine: S^T = K Q^T gives lane 32 h + c the scores of column c for tokens
+// 8 i + 4 h + 0 .. 3, which O^T = V^T P^T takes as they are.
 //
 // LDS holds a fragment as 64 lanes of 16 bytes.  Keys: [32 tokens][16 dimensions], lane 32 h + token: dimensions 8 h .. 8 h + 7 in the
 // order of key_operand.  Values: [16 tokens][32 dimensions], lane 32 h + dimension: tokens 4 h .. 4 h + 3 and 8 + 4 h .. + 3.
+//
+// A wavefront stages tokens of one group of 16 at a time, which lie in one page: page and addresses are scalar.
 template <int DP> constexpr int kTile = DP == 256 ? 32 : 64;
-template <int T, int DP, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, (DP == 256 ? 1 : 2)) void prompt_kernel(const AttArgs A) {
-  constexpr int TT = kTile<DP>, TB = TT / 32, KK = DP / 16, DB = DP / 32, U = TT / 16, THREADS = WAVES * 64, DW = DP / 8;
-  constexpr bool FOLD = T == ITEXHIP_HALF;  // see below
-  __shared__ u4v lds_k[2][TB * KK * 64], lds_v[2][U * DB * 64];
-  __shared__ u4v lds_kp[2][TT / 4], lds_vp[2][TT / 4];
-  __shared__ unsigned long long lds_valid[2], lds_nan[2];
+template <int DP> constexpr int kWaves = DP == 256 ? 4 : 8;
+template <int T, int DP>
+__global__ __launch_bounds__(64 * kWaves<DP>, kWaves<DP> / 4) void prompt_kernel(const AttArgs A) {
+  constexpr int WAVES = kWaves<DP>, TT = kTile<DP>, TB = TT / 32, KK = DP / 16, DB = DP / 32, U = TT / 16, THREADS = 64 * WAVES, DW = DP / 8;
+  constexpr bool FOLD = T == ITEXHIP_HALF;  // scales of values go into the probabilities, as in Engine; else into the operands, a rounding to half
+  typedef float f16v __attribute__((ext_vector_type(16)));
+  __shared__ u4v lds_k[2][TB * KK * 64], lds_v[2][U * DB * 64], lds_kp[2][TT / 4], lds_vp[2][TT / 4];
+  __shared__ uint64_t lds_valid[2], lds_nan[2];  // a bit a token
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, hi = lane >> 5;
   const int head = blockIdx.x % A.kv_heads, b = blockIdx.z;  // neighbouring workgroups, on different dies, take different heads
   const Seq s = sequence(A, b);
@@ -810,28 +814,28 @@ __global__ __launch_bounds__(WAVES * 64, (DP == 256 ? 1 : 2)) void prompt_kernel
   if (at_tile < 0) return;
   const int row0 = at_tile * tile_rows + 32 * wave, row = row0 + c;
   const int before = s.len - s.n;  // position of the first row
-  auto limit_of = [&](int r) { const int to = A.causal ? before + r / A.group + 1 : s.len; return to < 0 ? 0 : to; };
-  auto start_of = [&](int r) { const int from = A.window > 0 ? before + r / A.group - A.window + 1 : 0; return from < 0 ? 0 : from; };
-  // of the workgroup, the wavefront and the lane's column
+  auto limit_of = [&](int r) { return A.causal ? max(before + r / A.group + 1, 0) : s.len; };
+  auto start_of = [&](int r) { return A.window > 0 ? max(before + r / A.group - A.window + 1, 0) : 0; };
+  // of the workgroup and the wavefront
   const int first_row = at_tile * tile_rows, last_row = min(first_row + tile_rows, rows) - 1;
   const int from = start_of(first_row) & ~(TT - 1), to = min(limit_of(last_row), s.len);
   const bool there = row0 < rows;
-  const int w_last = min(row0 + 31, rows - 1);
+  const int w_last = min(row0 + 32, rows) - 1;
   const int w_to = there ? limit_of(w_last) : 0, w_from = start_of(row0), w_all_to = limit_of(row0), w_all_from = there ? start_of(w_last) : 0;
-  const int limit = row < rows ? limit_of(row) : 0, start = row < rows ? start_of(row) : 0;
 
   // queries, as in Engine::init
   half8v q[KK];
   float sumq = 0.0f, qs;
+  const bool in = row < rows;
+  const int limit = in ? limit_of(row) : 0, start = in ? start_of(row) : 0;
   {
-    float most = 0.0f;
-    const int64_t at = row < rows ? (s.first + row / A.group) * A.q_st + static_cast<int64_t>(head * A.group + row % A.group) * A.q_sh : 0;
-    float x[KK][8];
+    float x[KK][8], most = 0.0f;
+    const int64_t at = in ? (s.first + row / A.group) * A.q_st + static_cast<int64_t>(head * A.group + row % A.group) * A.q_sh : 0;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
       const int d0 = kk * 16 + hi * 8;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[kk][j] = row < rows && d0 < A.head_dim ? load_q<T>(A.q, at + d0 + j) : 0.0f;
+      for (int j = 0; j < 8; ++j) x[kk][j] = in && d0 < A.head_dim ? load_q<T>(A.q, at + d0 + j) : 0.0f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[kk][j]));
     }
@@ -851,97 +855,85 @@ __global__ __launch_bounds__(WAVES * 64, (DP == 256 ? 1 : 2)) void prompt_kernel
     }
     sumq += __shfl_xor(sumq, 32);
   }
-  const float corr = -72.0f * sumq;
   float m = -INFINITY, raise_at = -INFINITY, l = 0.0f, po = 0.0f, ref = kProbExponent + (FOLD ? 15.0f : 0.0f);
-  uint32_t scale_bound = 0x03ffu;
-  typedef float f16v __attribute__((ext_vector_type(16)));
+  const float corr = -72.0f * sumq;
   f16v o[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+  uint32_t scale_bound = 0x03ffu;
 
   CodeBits bits;
   bits.pin();
   const Kv4Block block{A.page_size, DP};
   const uint8_t* head_base = A.cache + static_cast<int64_t>(head) * block.bytes();
-  const int32_t* table = A.table + b * A.table_stride;
-  // tasks of a tile: keys (token, pair of dwords); values (16 tokens, half, dword, pair of codes)
-  constexpr int KT = TT * DW / 2, VT = U * 2 * DW * 4, KN = (KT + THREADS - 1) / THREADS, VN = (VT + THREADS - 1) / THREADS;
-  static_assert(THREADS % TT == 0, "a thread's key tasks are one token's");
-  uint2 kraw[KN];
-  u4v vraw[VN][2], vpar[VN][2];
-  uint32_t token_ks = 0, token_ko = 0, token_vs = 0, token_vo = 0;
-  // pages of a thread's tasks, read a tile ahead of the loads that need them
-  int page_k = -1, page_v[VN], next_k = -1, next_v[VN];
-  auto v_tokens = [&](int i) { return 16 * ((tid + i * THREADS) / (8 * DW)); };
+  const auto* table = (const __attribute__((address_space(4))) int32_t*)(A.table + b * A.table_stride);
+  // Tasks of a group of 16 tokens: keys (token, pair of dwords), values (half, dword, pair of codes).  A wavefront has its tasks in one
+  // group, or (DP = 256) in both one after the other.
+  constexpr int KG = 16 * DW / 2, VG = 2 * DW * 4, N = (U * VG + THREADS - 1) / THREADS;
+  static_assert(KG == VG && VG % 64 == 0 && (N == 1 || VG == THREADS), "the wavefronts of a group");
+  const bool stages = N > 1 || wave < U * VG / 64;
+  const int in_group = tid % VG;
+  auto group_of = [&](int i) { return N > 1 ? i : wave / (VG / 64); };
+  const int k_token = in_group & 15, k_pair = in_group >> 4, v_pair = in_group & 3, v_dword = (in_group >> 2) % DW, v_half = (in_group >> 2) / DW;
+  const uint32_t k_lane = k_token * (DP / 2) + 8 * k_pair, v_lane = block.value_codes(4 * v_half, v_dword), vp_lane = block.value_params(4 * v_half),
+                 par_lane = block.key_params(k_token);
+  const bool has_token = in_group < 16;
+  uint2 kraw[N];
+  u4v vraw[N][2], vpar[N][2];
+  uint32_t tok_k[N][2], tok_v[N][2];
+  int page[N];
+  auto good = [&](int p) { return p >= 0 && p < A.num_pages; };
+  int next[N];  // pages, read a tile ahead of the loads that need them
   auto look_up = [&](int t0) {
-    next_k = table[min(t0 + tid % TT, to - 1) >> A.page_shift];
 #pragma unroll
-    for (int i = 0; i < VN; ++i) next_v[i] = table[min(t0 + v_tokens(i), to - 1) >> A.page_shift];
+    for (int i = 0; i < N; ++i) next[i] = table[min(t0 + 16 * group_of(i), to - 1) >> A.page_shift];
   };
-  auto good = [&](int page) { return page >= 0 && page < A.num_pages; };
-  auto base_of = [&](int page) { return head_base + (good(page) ? page : 0) * A.page_bytes; };
   auto fetch = [&](int t0) {
-    page_k = next_k;
+    if (!stages) return;
 #pragma unroll
-    for (int i = 0; i < VN; ++i) page_v[i] = next_v[i];
+    for (int i = 0; i < N; ++i) page[i] = next[i];
     look_up(t0 + TT);
-    const int place_k = (t0 + tid % TT) & (A.page_size - 1);
-    const uint8_t* base = base_of(page_k);
 #pragma unroll
-    for (int i = 0; i < KN; ++i) {
-      const int task = tid + i * THREADS;
-      if (KT % THREADS != 0 && task >= KT) break;
-      kraw[i] = *reinterpret_cast<const uint2*>(base + block.key_codes(place_k) + 8 * (task / TT));
-    }
-    if (tid < TT) {  // one token each: its parameters
-      const uint8_t *kp = base + block.key_params(place_k), *vp = base + block.value_params(place_k);
-      token_ks = *reinterpret_cast<const uint16_t*>(kp);
-      token_ko = *reinterpret_cast<const uint16_t*>(kp + 8);
-      token_vs = *reinterpret_cast<const uint16_t*>(vp);
-      token_vo = *reinterpret_cast<const uint16_t*>(vp + 8);
-    }
-#pragma unroll
-    for (int i = 0; i < VN; ++i) {
-      const int task = tid + i * THREADS;
-      if (VT % THREADS != 0 && task >= VT) break;
-      const int w = (task >> 2) % DW, h = (task >> 2) / DW & 1;
-      const int place = ((t0 + v_tokens(i)) & (A.page_size - 1)) + 4 * h;
-      const uint8_t* base = base_of(page_v[i]);
+    for (int i = 0; i < N; ++i) {
+      const int place = (t0 + 16 * group_of(i)) & (A.page_size - 1);
+      const uint8_t* base = head_base + (good(page[i]) ? page[i] : 0) * A.page_bytes;
+      const uint8_t *codes = base + place * (DP / 2), *params = base + place * 4;
+      kraw[i] = *reinterpret_cast<const uint2*>(codes + k_lane);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        vraw[i][k] = *reinterpret_cast<const u4v*>(base + block.value_codes(place + 8 * k, w));
-        if (!FOLD) vpar[i][k] = *reinterpret_cast<const u4v*>(base + block.value_params(place + 8 * k));
+        vraw[i][k] = *reinterpret_cast<const u4v*>(codes + v_lane + k * (8 * DP / 2));
+        if (!FOLD) vpar[i][k] = *reinterpret_cast<const u4v*>(params + vp_lane + k * 32);
+      }
+      if (has_token) {
+        const uint8_t *kp = params + par_lane, *vp = kp + A.page_size * 4;
+        tok_k[i][0] = *reinterpret_cast<const uint16_t*>(kp);
+        tok_k[i][1] = *reinterpret_cast<const uint16_t*>(kp + 8);
+        tok_v[i][0] = *reinterpret_cast<const uint16_t*>(vp);
+        tok_v[i][1] = *reinterpret_cast<const uint16_t*>(vp + 8);
       }
     }
   };
   auto stage = [&](int t0, int buf) {
+    if (!stages) return;
 #pragma unroll
-    for (int i = 0; i < KN; ++i) {
-      const int task = tid + i * THREADS;
-      if (KT % THREADS != 0 && task >= KT) break;
-      const int t = task % TT, j = task / TT;
-      u4v* to_k = &lds_k[buf][((t / 32) * KK + j) * 64 + t % 32];
+    for (int i = 0; i < N; ++i) {
+      const int u = group_of(i), tg = t0 + 16 * u, t = 16 * u + k_token;
+      u4v* to_k = &lds_k[buf][((t / 32) * KK + k_pair) * 64 + t % 32];
       to_k[0] = u4v{bits.at_64(kraw[i].x << 4), bits.at_64(kraw[i].x), bits.at_64(kraw[i].x >> 4), bits.at_64(kraw[i].x >> 8)};
       to_k[32] = u4v{bits.at_64(kraw[i].y << 4), bits.at_64(kraw[i].y), bits.at_64(kraw[i].y >> 4), bits.at_64(kraw[i].y >> 8)};
-    }
-#pragma unroll
-    for (int i = 0; i < VN; ++i) {
-      const int task = tid + i * THREADS;
-      if (VT % THREADS != 0 && task >= VT) break;
-      const int n2 = task & 3, w = (task >> 2) % DW, h = (task >> 2) / DW & 1, u = (task >> 2) / DW >> 1;
-      const uint32_t pick = (n2 & 2) ? 0x07060302u : 0x05040100u;
-      const int shift = (n2 & 1) * 8;
-      if (!FOLD && (!good(page_v[i]) || t0 + TT > s.len)) {  // tokens beyond the last one or without a page become zeros
+      if (!FOLD && (!good(page[i]) || tg + 16 > s.len)) {  // tokens beyond the last one or without a page become zeros
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const int t = t0 + 16 * u + 8 * (k / 2) + 4 * h + 2 * (k & 1);
-          const uint32_t keep = !good(page_v[i]) ? 0 : (t < s.len ? 0xffffu : 0u) | (t + 1 < s.len ? 0xffff0000u : 0u);
+          const int t2 = tg + 8 * (k / 2) + 4 * v_half + 2 * (k & 1);
+          const uint32_t keep = !good(page[i]) ? 0 : (t2 < s.len ? 0xffffu : 0u) | (t2 + 1 < s.len ? 0xffff0000u : 0u);
           vpar[i][k / 2][k & 1] &= keep;
           vpar[i][k / 2][2 + (k & 1)] &= keep;
         }
       }
+      const uint32_t pick = (v_pair & 2) ? 0x07060302u : 0x05040100u;
+      const int shift = (v_pair & 1) * 8;
       u4v a, z;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -955,30 +947,31 @@ __global__ __launch_bounds__(WAVES * 64, (DP == 256 ? 1 : 2)) void prompt_kernel
         a[k] = as_bits(first);
         z[k] = as_bits(second);
       }
-      u4v* to_v = &lds_v[buf][(u * DB + w / 4) * 64 + h * 32 + (w & 3) * 8 + 2 * n2];
+      u4v* to_v = &lds_v[buf][(u * DB + v_dword / 4) * 64 + v_half * 32 + (v_dword & 3) * 8 + 2 * v_pair];
       to_v[0] = a;
       to_v[1] = z;
-    }
-    if (tid < TT) {
-      const bool ok = good(page_k) && t0 + tid < s.len;
-      const bool nan = ok && ((token_vs & 0x7c00u) == 0x7c00u || (token_vo & 0x7c00u) == 0x7c00u);
-      const unsigned long long valid = __ballot(ok), nans = __ballot(nan);
-      if (tid == 0) {
-        lds_valid[buf] = valid;
-        lds_nan[buf] = nans;
-      }
-      uint16_t* par = reinterpret_cast<uint16_t*>(&lds_kp[buf][tid / 4]) + (tid & 3);
-      par[0] = static_cast<uint16_t>(token_ks);
-      par[4] = static_cast<uint16_t>(token_ko);
-      if (FOLD) {
-        const bool keep = ok && !nan;
-        par = reinterpret_cast<uint16_t*>(&lds_vp[buf][tid / 4]) + (tid & 3);
-        par[0] = static_cast<uint16_t>(keep ? token_vs : 0);
-        par[4] = static_cast<uint16_t>(keep ? token_vo : 0);
+      if (has_token) {
+        const bool ok = good(page[i]) && tg + k_token < s.len;
+        const bool nan = ok && ((tok_v[i][0] & 0x7c00u) == 0x7c00u || (tok_v[i][1] & 0x7c00u) == 0x7c00u);
+        const uint64_t valid = __ballot(ok), nans = __ballot(nan);
+        if (in_group == 0) {
+          reinterpret_cast<uint16_t*>(&lds_valid[buf])[u] = static_cast<uint16_t>(valid);
+          reinterpret_cast<uint16_t*>(&lds_nan[buf])[u] = static_cast<uint16_t>(nans);
+        }
+        uint16_t* par = reinterpret_cast<uint16_t*>(&lds_kp[buf][t / 4]) + (t & 3);
+        par[0] = static_cast<uint16_t>(tok_k[i][0]);
+        par[4] = static_cast<uint16_t>(tok_k[i][1]);
+        if (FOLD) {
+          const bool keep = ok && !nan;
+          par = reinterpret_cast<uint16_t*>(&lds_vp[buf][t / 4]) + (t & 3);
+          par[0] = static_cast<uint16_t>(keep ? tok_v[i][0] : 0);
+          par[4] = static_cast<uint16_t>(keep ? tok_v[i][1] : 0);
+        }
       }
     }
   };
-  auto rescale = [&](float a) {
+  auto rescale = [&](float by) {  // after ref -= by
+    const float a = __builtin_amdgcn_exp2f(-by);
     l *= a;
     po *= a;
 #pragma unroll
@@ -991,22 +984,22 @@ __global__ __launch_bounds__(WAVES * 64, (DP == 256 ? 1 : 2)) void prompt_kernel
     stage(from, 0);
   }
   __syncthreads();
-  constexpr unsigned long long kAll = TT == 64 ? ~0ull : (1ull << (TT & 63)) - 1;
+  constexpr uint64_t kAll = TT == 64 ? ~0ull : (1ull << (TT & 63)) - 1;
   for (int t0 = from, buf = 0; t0 < to; t0 += TT, buf ^= 1) {
     const bool more = t0 + TT < to;
     if (more) fetch(t0 + TT);
-    if (!FOLD && lds_nan[buf] != 0) {  // values that are NaN reach the rows that see them through l, the products as zeros
+    const uint64_t valid = lds_valid[buf] & kAll, nans = lds_nan[buf] & kAll;
+    if (!FOLD && nans != 0) {  // values that are NaN reach the rows that see them through l, the products as zeros
       half8v* all = reinterpret_cast<half8v*>(lds_v[buf]);
-      for (int i = tid; i < U * DB * 64; i += THREADS) {
-        half8v a = all[i];
+      for (int k = tid; k < U * DB * 64; k += THREADS) {
+        half8v a = all[k];
 #pragma unroll
         for (int j = 0; j < 8; ++j) a[j] = a[j] == a[j] ? a[j] : static_cast<_Float16>(0);
-        all[i] = a;
+        all[k] = a;
       }
       __syncthreads();
     }
     if (t0 < w_to && t0 + TT > w_from) {
-      const unsigned long long valid = lds_valid[buf], nans = lds_nan[buf];
       const bool mask = valid != kAll || nans != 0 || t0 + TT > w_all_to || t0 < w_all_from;
 #pragma unroll
       for (int tb = 0; tb < TB; ++tb) {
@@ -1021,14 +1014,16 @@ __global__ __launch_bounds__(WAVES * 64, (DP == 256 ? 1 : 2)) void prompt_kernel
         for (int kk = 0; kk < KK; ++kk) sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[kk], q[kk], sc, 0, 0, 0);
 #pragma unroll
         for (int d = 0; d < DB; ++d) __builtin_memcpy(&vf[0][d], &lds_v[buf][(2 * tb * DB + d) * 64 + lane], 16);
+        u4v vp[FOLD ? 4 : 1];
         float p[16], top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const u4v par = lds_kp[buf][tb * 8 + 2 * i + hi];
+        for (int k = 0; k < 4; ++k) {
+          const u4v par = lds_kp[buf][tb * 8 + 2 * k + hi];
+          if constexpr (FOLD) vp[k] = lds_vp[buf][tb * 8 + 2 * k + hi];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float ks = (j & 1) ? high_half(par[j / 2]) : low_half(par[j / 2]), ko = (j & 1) ? high_half(par[2 + j / 2]) : low_half(par[2 + j / 2]);
-            p[4 * i + j] = fmaf(ks, sc[4 * i + j], ko * sumq);
+            p[4 * k + j] = fmaf(ks, sc[4 * k + j], fmaf(ko, sumq, 0.0f));
           }
         }
         if (mask) {
@@ -1045,15 +1040,13 @@ __global__ __launch_bounds__(WAVES * 64, (DP == 256 ? 1 : 2)) void prompt_kernel
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, p[r]);
         uint32_t most = 0;
-        u4v vp[4];
         if constexpr (FOLD) {
           typedef unsigned short us2 __attribute__((ext_vector_type(2)));
           us2 two = {0, 0};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            vp[i] = lds_vp[buf][tb * 8 + 2 * i + hi];
+          for (int k = 0; k < 4; ++k) {
             us2 x[2];
-            __builtin_memcpy(x, &vp[i], 8);
+            __builtin_memcpy(x, &vp[k], 8);
             two = __builtin_elementwise_max(two, __builtin_elementwise_max(x[0], x[1]));
           }
           most = two[0] > two[1] ? two[0] : two[1];
@@ -1065,14 +1058,14 @@ __global__ __launch_bounds__(WAVES * 64, (DP == 256 ? 1 : 2)) void prompt_kernel
               const float by = static_cast<float>(static_cast<int>((most >> 10) - (scale_bound >> 10)));
               scale_bound = most;
               ref -= by;
-              rescale(__builtin_amdgcn_exp2f(-by));
+              rescale(by);
             }
           }
           top = fmaxf(top, __shfl_xor(top, 32));
           if (top > m) {
             const float by = m == -INFINITY ? top * qs : (top - m) * qs;
             ref -= by;
-            rescale(m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(-by));
+            rescale(m == -INFINITY ? 0.0f : by);
             m = top;
             raise_at = top + 5.0f / qs;
           }
@@ -1085,7 +1078,8 @@ __global__ __launch_bounds__(WAVES * 64, (DP == 256 ? 1 : 2)) void prompt_kernel
           if constexpr (FOLD) {
             const uint32_t vs = vp[r / 4][r % 4 / 2], vo = vp[r / 4][2 + r % 4 / 2];
             po = fmaf(x, (r & 1) ? high_half(vo) : low_half(vo), po);
-            x *= (r & 1) ? high_half(vs) : low_half(vs);
+            x = fmaf(x, (r & 1) ? high_half(vs) : low_half(vs), 0.0f);
+            asm("" : "+v"(x));  // (merged with the conversion it would be an instruction that writes half a register, at twice the time)
           }
           pb[r / 8][r % 8] = static_cast<_Float16>(x);
         }
@@ -1104,7 +1098,7 @@ __global__ __launch_bounds__(WAVES * 64, (DP == 256 ? 1 : 2)) void prompt_kernel
 
   l += __shfl_xor(l, 32);
   if constexpr (FOLD) po += __shfl_xor(po, 32);
-  if (row >= rows) return;
+  if (!in) return;
   const int q_head = head * A.group + row % A.group;
   const int64_t q_row = s.first + row / A.group, at = q_row * A.o_st + q_head * A.o_sh;
   const bool empty = l == 0.0f;
@@ -1187,8 +1181,8 @@ void launch(const AttArgs& A, const Plan& plan, hipStream_t stream) {
     if constexpr (T == ITEXHIP_FLOAT) {
       rows_kernel<T, DP, NB><<<dim3((rows + 64 * NB - 1) / (64 * NB), A.kv_heads, A.num_seqs), dim3(256), 0, stream>>>(A);
     } else {
-      constexpr int WAVES = DP == 256 ? 4 : PWAVES;
-      prompt_kernel<T, DP, WAVES><<<dim3(A.kv_heads * ((rows + 32 * WAVES - 1) / (32 * WAVES)), 1, A.num_seqs), dim3(64 * WAVES), 0, stream>>>(A);
+      constexpr int tile = 32 * kWaves<DP>;
+      prompt_kernel<T, DP><<<dim3(A.kv_heads * ((rows + tile - 1) / tile), 1, A.num_seqs), dim3(2 * tile), 0, stream>>>(A);
     }
   }
 }
