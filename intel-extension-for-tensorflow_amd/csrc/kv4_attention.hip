@@ -803,8 +803,9 @@ __global__ __launch_bounds__(64 * kWaves<DP>, kWaves<DP> / 4) void prompt_kernel
   constexpr int WAVES = kWaves<DP>, TT = kTile<DP>, TB = TT / 32, KK = DP / 16, DB = DP / 32, U = TT / 16, THREADS = 64 * WAVES, DW = DP / 8;
   constexpr bool FOLD = T == ITEXHIP_HALF;  // scales of values go into the probabilities, as in Engine; else into the operands, a rounding to half
   typedef float f16v __attribute__((ext_vector_type(16)));
-  __shared__ u4v lds_k[2][TB * KK * 64], lds_v[2][U * DB * 64], lds_kp[2][TT / 4], lds_vp[2][TT / 4];
-  __shared__ uint64_t lds_valid[2], lds_nan[2];  // a bit a token
+  __shared__ u4v lds_k[2][TB * KK * 64], lds_v[2][U * DB * 64], lds_vp[2][TT / 4];
+  __shared__ f4 lds_kp[2][TT / 2];  // of two tokens: scale and offset - 72 scale, the excess of the codes taken back
+  __shared__ __align__(16) uint16_t lds_flags[2][2][4];  // a bit a token: [..][0] seen by some row, [..][1] its value is NaN
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, hi = lane >> 5;
   const int head = blockIdx.x % A.kv_heads, b = blockIdx.z;  // neighbouring workgroups, on different dies, take different heads
   const Seq s = sequence(A, b);
@@ -856,7 +857,6 @@ __global__ __launch_bounds__(64 * kWaves<DP>, kWaves<DP> / 4) void prompt_kernel
     sumq += __shfl_xor(sumq, 32);
   }
   float m = -INFINITY, raise_at = -INFINITY, l = 0.0f, po = 0.0f, ref = kProbExponent + (FOLD ? 15.0f : 0.0f);
-  const float corr = -72.0f * sumq;
   f16v o[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d)
@@ -868,33 +868,46 @@ __global__ __launch_bounds__(64 * kWaves<DP>, kWaves<DP> / 4) void prompt_kernel
   bits.pin();
   const Kv4Block block{A.page_size, DP};
   const uint8_t* head_base = A.cache + static_cast<int64_t>(head) * block.bytes();
-  const auto* table = (const __attribute__((address_space(4))) int32_t*)(A.table + b * A.table_stride);
+  const int32_t* table = A.table + b * A.table_stride;
   // Tasks of a group of 16 tokens: keys (token, pair of dwords), values (half, dword, pair of codes).  A wavefront has its tasks in one
   // group, or (DP = 256) in both one after the other.
-  constexpr int KG = 16 * DW / 2, VG = 2 * DW * 4, N = (U * VG + THREADS - 1) / THREADS;
-  static_assert(KG == VG && VG % 64 == 0 && (N == 1 || VG == THREADS), "the wavefronts of a group");
-  const bool stages = N > 1 || wave < U * VG / 64;
+  constexpr int KG = 16 * DW / 2, VG = 2 * DW * 4, STAGERS = U * VG / 64 < WAVES ? U * VG / 64 : WAVES, N = U * VG / (64 * STAGERS);
+  static_assert(KG == VG && VG % 64 == 0 && (64 * STAGERS) % VG == 0, "the wavefronts of a group");
+  const bool stages = wave < STAGERS;
   const int in_group = tid % VG;
-  auto group_of = [&](int i) { return N > 1 ? i : wave / (VG / 64); };
+  auto group_of = [&](int i) { return i * (64 * STAGERS / VG) + wave / (VG / 64); };
   const int k_token = in_group & 15, k_pair = in_group >> 4, v_pair = in_group & 3, v_dword = (in_group >> 2) % DW, v_half = (in_group >> 2) / DW;
   const uint32_t k_lane = k_token * (DP / 2) + 8 * k_pair, v_lane = block.value_codes(4 * v_half, v_dword), vp_lane = block.value_params(4 * v_half),
-                 par_lane = block.key_params(k_token);
-  const bool has_token = in_group < 16;
+                 par_lane = block.key_params(4 * (lane & 3)) + (lane & 4) * A.page_size;  // keys' of four tokens, values' of four tokens
   uint2 kraw[N];
   u4v vraw[N][2], vpar[N][2];
-  uint32_t tok_k[N][2], tok_v[N][2];
-  int page[N];
+  u4v par = {0, 0, 0, 0};
+  int page[N], par_page = -1, par_next = -1;  // parameters: a group for each of the first wavefronts, which the others wait for anyway
   auto good = [&](int p) { return p >= 0 && p < A.num_pages; };
-  int next[N];  // pages, read a tile ahead of the loads that need them
+  // Pages, read a tile ahead of the loads that need them; by vector loads, since the wait for a scalar one would be the wait for
+  // all of LDS too and come at once
+  int next[N];
   auto look_up = [&](int t0) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) next[i] = table[min(t0 + 16 * group_of(i), to - 1) >> A.page_shift];
+    for (int i = 0; i < N; ++i) {
+      int at = min(t0 + 16 * group_of(i), to - 1) >> A.page_shift;
+      asm("" : "+v"(at));
+      next[i] = table[at];
+    }
+    int at = min(t0 + 16 * (wave % U), to - 1) >> A.page_shift;
+    asm("" : "+v"(at));
+    par_next = table[at];
   };
   auto fetch = [&](int t0) {
-    if (!stages) return;
 #pragma unroll
-    for (int i = 0; i < N; ++i) page[i] = next[i];
+    for (int i = 0; i < N; ++i) page[i] = __builtin_amdgcn_readfirstlane(next[i]);
+    par_page = __builtin_amdgcn_readfirstlane(par_next);
     look_up(t0 + TT);
+    if (wave < U) {
+      const uint8_t* params = head_base + (good(par_page) ? par_page : 0) * A.page_bytes + ((t0 + 16 * wave) & (A.page_size - 1)) * 4;
+      if (lane < 8) par = *reinterpret_cast<const u4v*>(params + par_lane);
+    }
+    if (!stages) return;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int place = (t0 + 16 * group_of(i)) & (A.page_size - 1);
@@ -905,13 +918,6 @@ __global__ __launch_bounds__(64 * kWaves<DP>, kWaves<DP> / 4) void prompt_kernel
       for (int k = 0; k < 2; ++k) {
         vraw[i][k] = *reinterpret_cast<const u4v*>(codes + v_lane + k * (8 * DP / 2));
         if (!FOLD) vpar[i][k] = *reinterpret_cast<const u4v*>(params + vp_lane + k * 32);
-      }
-      if (has_token) {
-        const uint8_t *kp = params + par_lane, *vp = kp + A.page_size * 4;
-        tok_k[i][0] = *reinterpret_cast<const uint16_t*>(kp);
-        tok_k[i][1] = *reinterpret_cast<const uint16_t*>(kp + 8);
-        tok_v[i][0] = *reinterpret_cast<const uint16_t*>(vp);
-        tok_v[i][1] = *reinterpret_cast<const uint16_t*>(vp + 8);
       }
     }
   };
@@ -950,24 +956,49 @@ __global__ __launch_bounds__(64 * kWaves<DP>, kWaves<DP> / 4) void prompt_kernel
       u4v* to_v = &lds_v[buf][(u * DB + v_dword / 4) * 64 + v_half * 32 + (v_dword & 3) * 8 + 2 * v_pair];
       to_v[0] = a;
       to_v[1] = z;
-      if (has_token) {
-        const bool ok = good(page[i]) && tg + k_token < s.len;
-        const bool nan = ok && ((tok_v[i][0] & 0x7c00u) == 0x7c00u || (tok_v[i][1] & 0x7c00u) == 0x7c00u);
-        const uint64_t valid = __ballot(ok), nans = __ballot(nan);
-        if (in_group == 0) {
-          reinterpret_cast<uint16_t*>(&lds_valid[buf])[u] = static_cast<uint16_t>(valid);
-          reinterpret_cast<uint16_t*>(&lds_nan[buf])[u] = static_cast<uint16_t>(nans);
-        }
-        uint16_t* par = reinterpret_cast<uint16_t*>(&lds_kp[buf][t / 4]) + (t & 3);
-        par[0] = static_cast<uint16_t>(tok_k[i][0]);
-        par[4] = static_cast<uint16_t>(tok_k[i][1]);
-        if (FOLD) {
-          const bool keep = ok && !nan;
-          par = reinterpret_cast<uint16_t*>(&lds_vp[buf][t / 4]) + (t & 3);
-          par[0] = static_cast<uint16_t>(keep ? tok_v[i][0] : 0);
-          par[4] = static_cast<uint16_t>(keep ? tok_v[i][1] : 0);
+    }
+  };
+  auto stage_params = [&](int t0, int buf) {
+    if (wave >= U) return;
+    const int tg = t0 + 16 * wave;
+    auto odd = [](uint32_t x) { return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u; };
+    const bool nan = odd(par[0]) || odd(par[1]) || odd(par[2]) || odd(par[3]);
+    uint32_t valid = 0xffffu, nans = 0;
+    if (!good(par_page) || tg + 16 > s.len || __any(lane >= 4 && lane < 8 && nan)) {
+      const int n = good(par_page) ? min(max(s.len - tg, 0), 16) : 0;
+      valid = (1u << n) - 1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {  // token 4 (lane - 4) + j
+        const uint32_t vs = par[j / 2] >> (16 * (j & 1)), vo = par[2 + j / 2] >> (16 * (j & 1));
+        const bool is_nan = (vs & 0x7c00u) == 0x7c00u || (vo & 0x7c00u) == 0x7c00u;
+        const uint64_t lanes = __ballot(lane >= 4 && lane < 8 && is_nan) >> 4;
+        nans |= static_cast<uint32_t>((lanes & 1) | (lanes & 2) << 3 | (lanes & 4) << 6 | (lanes & 8) << 9) << j;
+      }
+      nans &= valid;
+      if (FOLD) {
+        const uint32_t keep = (valid & ~nans) >> (4 * (lane & 3));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (lane >= 4 && !(keep >> j & 1)) {
+            const uint32_t other = (j & 1) ? 0x0000ffffu : 0xffff0000u;
+            par[j / 2] &= other;
+            par[2 + j / 2] &= other;
+          }
         }
       }
+    }
+    if (lane == 0) {
+      lds_flags[buf][0][wave] = static_cast<uint16_t>(valid);
+      lds_flags[buf][1][wave] = static_cast<uint16_t>(nans);
+    }
+    if (lane < 4) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float ks0 = low_half(par[j]), ks1 = high_half(par[j]);
+        lds_kp[buf][2 * (4 * wave + lane) + j] = f4{ks0, fmaf(-72.0f, ks0, low_half(par[2 + j])), ks1, fmaf(-72.0f, ks1, high_half(par[2 + j]))};
+      }
+    } else if (lane < 8) {
+      lds_vp[buf][4 * wave + lane - 4] = par;
     }
   };
   auto rescale = [&](float by) {  // after ref -= by
@@ -981,14 +1012,16 @@ __global__ __launch_bounds__(64 * kWaves<DP>, kWaves<DP> / 4) void prompt_kernel
   if (from < to) {
     look_up(from);
     fetch(from);
+    stage_params(from, 0);
     stage(from, 0);
   }
   __syncthreads();
   constexpr uint64_t kAll = TT == 64 ? ~0ull : (1ull << (TT & 63)) - 1;
   for (int t0 = from, buf = 0; t0 < to; t0 += TT, buf ^= 1) {
     const bool more = t0 + TT < to;
+    const u4v flags = *reinterpret_cast<const u4v*>(lds_flags[buf]);
     if (more) fetch(t0 + TT);
-    const uint64_t valid = lds_valid[buf] & kAll, nans = lds_nan[buf] & kAll;
+    const uint64_t valid = (flags[0] | static_cast<uint64_t>(flags[1]) << 32) & kAll, nans = (flags[2] | static_cast<uint64_t>(flags[3]) << 32) & kAll;
     if (!FOLD && nans != 0) {  // values that are NaN reach the rows that see them through l, the products as zeros
       half8v* all = reinterpret_cast<half8v*>(lds_v[buf]);
       for (int k = tid; k < U * DB * 64; k += THREADS) {
@@ -1009,7 +1042,7 @@ __global__ __launch_bounds__(64 * kWaves<DP>, kWaves<DP> / 4) void prompt_kernel
         for (int kk = 0; kk < KK; ++kk) __builtin_memcpy(&kf[kk], &lds_k[buf][(tb * KK + kk) * 64 + lane], 16);
         f16v sc;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sc[r] = corr;
+        for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[kk], q[kk], sc, 0, 0, 0);
 #pragma unroll
@@ -1017,14 +1050,14 @@ __global__ __launch_bounds__(64 * kWaves<DP>, kWaves<DP> / 4) void prompt_kernel
         u4v vp[FOLD ? 4 : 1];
         float p[16], top = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const u4v par = lds_kp[buf][tb * 8 + 2 * k + hi];
-          if constexpr (FOLD) vp[k] = lds_vp[buf][tb * 8 + 2 * k + hi];
+        for (int k = 0; k < 8; ++k) {
+          const f4 par = lds_kp[buf][tb * 16 + 4 * (k / 2) + 2 * hi + k % 2];
+          p[2 * k] = fmaf(par[0], sc[2 * k], par[1] * sumq);
+          p[2 * k + 1] = fmaf(par[2], sc[2 * k + 1], par[3] * sumq);
+        }
+        if constexpr (FOLD) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float ks = (j & 1) ? high_half(par[j / 2]) : low_half(par[j / 2]), ko = (j & 1) ? high_half(par[2 + j / 2]) : low_half(par[2 + j / 2]);
-            p[4 * k + j] = fmaf(ks, sc[4 * k + j], fmaf(ko, sumq, 0.0f));
-          }
+          for (int k = 0; k < 4; ++k) vp[k] = lds_vp[buf][tb * 8 + 2 * k + hi];
         }
         if (mask) {
           const uint32_t here = static_cast<uint32_t>(valid >> (32 * tb)) >> (4 * hi), nan_here = static_cast<uint32_t>(nans >> (32 * tb)) >> (4 * hi);
@@ -1092,7 +1125,10 @@ __global__ __launch_bounds__(64 * kWaves<DP>, kWaves<DP> / 4) void prompt_kernel
         }
       }
     }
-    if (more) stage(t0 + TT, buf ^ 1);
+    if (more) {
+      stage_params(t0 + TT, buf ^ 1);
+      stage(t0 + TT, buf ^ 1);
+    }
     __syncthreads();
   }
 
