@@ -30,7 +30,7 @@ struct AttArgs {
   int64_t table_stride, total_q, page_bytes, num_pages;
   int64_t q_st, q_sh, o_st, o_sh;
   float scale;
-  int q_heads, kv_heads, group, num_seqs, max_q_len, causal, window, head_dim, page_size, page_shift, vec;
+  int q_heads, kv_heads, group, num_seqs, max_q_len, causal, window, head_dim, page_size, page_shift, vec, groups;
 };
 
 // One sequence's rows and tokens, whatever the arrays say
@@ -75,11 +75,7 @@ __device__ __forceinline__ float load_q(const void* q, int64_t i) {
   else return f16_bits_to_f32(static_cast<const uint16_t*>(q)[i]);
 }
 
-#ifndef OCC1
-#define OCC1 3
-#define OCC2 2
-#endif
-constexpr int occupancy_of(int nb, int dp) { return dp == 256 ? 1 : nb == 1 ? OCC1 : OCC2; }  // wavefronts a SIMD of a split kernel
+constexpr int occupancy_of(int nb, int dp) { return dp == 256 ? 1 : nb == 1 ? 3 : 2; }  // wavefronts a SIMD of a split kernel
 
 // A wavefront's 16 NB rows against 32 tokens at a time, everything in registers.
 //
@@ -246,7 +242,7 @@ struct Engine {
       } else {
 #pragma unroll
         for (int j = 0; j < NKK / 4; ++j) {
-          const u4v w = *reinterpret_cast<const u4v*>(kr + k_lane + 16 * j);
+          const u4v w = __builtin_nontemporal_load(reinterpret_cast<const u4v*>(kr + k_lane + 16 * j));
 #pragma unroll
           for (int n = 0; n < 4; ++n) kraw[i][4 * j + n] = w[n];
         }
@@ -260,7 +256,7 @@ struct Engine {
       int place;
       const uint8_t* base = tile(pages[i], t, i, &place);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) vraw[i][j] = *reinterpret_cast<const u4v*>(base + place * (DP / 2) + v_lane + 256 * j);
+      for (int j = 0; j < NV; ++j) vraw[i][j] = __builtin_nontemporal_load(reinterpret_cast<const u4v*>(base + place * (DP / 2) + v_lane + 256 * j));
       vp[i] = *reinterpret_cast<const u4v*>(base + place * 4 + vp_more + p_lane);
     }
   }
@@ -704,8 +700,9 @@ __global__ __launch_bounds__(256) void combine_kernel(const AttArgs A) {
   if (row >= s.n * A.group) return;
   const int item = head * tiles_of<NB>(A, s) + row / (16 * NB);
   const int64_t share = A.prefix[A.num_seqs], i0 = A.prefix[b] + item * s.steps;
-  const int64_t w0 = i0 / share, w1 = (i0 + s.steps - 1) / share;
-  if (w0 == w1) return;
+  if (share < 1 || i0 < 0) return;  // (another call is writing the workspace)
+  const int64_t w0 = i0 / share, w1 = min((i0 + s.steps - 1) / share, static_cast<int64_t>(A.groups) - 1);
+  if (w0 >= w1) return;
   const int count = static_cast<int>(w1 - w0 + 1);  // at most the workgroups of the split kernel, kMostGroups
   auto at = [&](int i) { return (2 * (w0 + i) + (i == 0 ? 1 : 0)) * 16 * NB + row % (16 * NB); };
   const int lane = tid % LANES, part = tid / LANES;
@@ -1286,6 +1283,7 @@ extern "C" int itexhip_kv4_attention(const itexhip_kv4_attention_params* p, cons
   A.head_dim = c->head_dim;
   A.page_size = c->page_size;
   A.page_shift = log2_of(c->page_size);
+  A.groups = static_cast<int>(plan.groups);
   A.vec = aligned(out, 4 * esize) && A.o_st % 4 == 0 && A.o_sh % 4 == 0;
   if (p->type == ITEXHIP_FLOAT) launch_dims<ITEXHIP_FLOAT>(A, plan, as_stream(stream));
   else if (p->type == ITEXHIP_BFLOAT16) launch_dims<ITEXHIP_BFLOAT16>(A, plan, as_stream(stream));
