@@ -15,7 +15,9 @@ typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 
 constexpr int kMostSplitRows = 64;     // rows of a sequence, times heads of a kv head, that split kernels take
 constexpr int kMostGroups = 1024;      // workgroups of a split kernel
-constexpr int kStep = 128;             // tokens a workgroup takes at a time, 32 a wavefront
+// Copies of the rows in a tile's 16 columns, see Engine; tokens that a workgroup of four wavefronts takes at a time
+constexpr int copies_of(bool f32, int64_t rows) { return f32 || rows > 8 ? 1 : rows > 4 ? 2 : 4; }
+constexpr int step_of(int copies) { return copies == 4 ? 256 : 128; }
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kProbExponent = 9.0f;  // probabilities are held as 2^9 p, up to 2^14 p above the maximum so far: half keeps 11 bits down to 2^-23
 
@@ -37,8 +39,9 @@ struct AttArgs {
 struct Seq {
   int64_t first;   // row of q
   int n, len, lo;  // new tokens, tokens, first token that any row sees (multiple of 32)
-  int64_t steps;   // of kStep tokens; at least one if there are rows
+  int64_t steps;   // of STEP tokens; at least one if there are rows
 };
+template <int STEP = 128>
 __device__ __forceinline__ Seq sequence(const AttArgs& A, int b) {
   Seq s;
   int64_t from = A.cu_q[b], to = A.cu_q[b + 1];
@@ -51,7 +54,7 @@ __device__ __forceinline__ Seq sequence(const AttArgs& A, int b) {
   s.len = static_cast<int>(len < 0 ? 0 : len > room ? room : len);
   int64_t lo = A.window > 0 ? static_cast<int64_t>(s.len) - s.n - A.window + 1 : 0;
   s.lo = static_cast<int>(lo < 0 ? 0 : lo) & ~31;
-  s.steps = s.n == 0 ? 0 : s.len > s.lo ? (s.len - s.lo + kStep - 1) / kStep : 1;
+  s.steps = s.n == 0 ? 0 : s.len > s.lo ? (s.len - s.lo + STEP - 1) / STEP : 1;
   return s;
 }
 
@@ -75,9 +78,13 @@ __device__ __forceinline__ float load_q(const void* q, int64_t i) {
   else return f16_bits_to_f32(static_cast<const uint16_t*>(q)[i]);
 }
 
-constexpr int occupancy_of(int nb, int dp) { return dp == 256 ? 1 : nb == 1 ? 3 : 2; }  // wavefronts a SIMD of a split kernel
+// Wavefronts a SIMD of a split kernel, and so its workgroups: registers for 2 (256) without spills, and longer shares than with 3, where
+// every other wait is for memory anyway; 3 where they fit and tokens are small or their products long.  Measured 2 : 3 in us, half or
+// bfloat16 heads of 128: one sequence of 131072 35 : 44, of 65536 (8 rows) 26 : 35, 64 of up to 8192 80 : 80; heads of 64: 32 sequences
+// of up to 4096 33.7 : 32.1, one of 32768 22.6 : 19.7; fp32, 32 sequences of up to 4096, 4 heads of 128 80 : 77.  4 spill (138 for 86).
+constexpr int occupancy_of(int nb, int dp, bool f32) { return dp == 256 ? 1 : nb == 1 && (dp == 64 || f32) ? 3 : 2; }
 
-// A wavefront's 16 NB rows against 32 tokens at a time, everything in registers.
+// A wavefront's 16 NB rows against 16 TILES tokens at a time, everything in registers.
 //
 // Scores are computed transposed, S^T = K Q^T: a lane then holds, for its query column c, the scores of tokens 4 g .. 4 g + 3
 // of each tile, which is the layout that the second product O^T = V^T P^T takes as its operand, so probabilities never
@@ -97,9 +104,17 @@ constexpr int occupancy_of(int nb, int dp) { return dp == 256 ? 1 : nb == 1 ? 3 
 //
 // Queries are multiplied by a power of two of their row so that half holds what bfloat16 does.  In fp32 the products are
 // fp32 MFMAs on fp32 operands.
-template <int T, int DP, int NB>
+//
+// Few rows (one token of a few heads) would leave most of the 16 columns empty and a softmax of nothing in most lanes.  They are
+// repeated COPIES times instead, and copy b of the columns (the lanes' `block`) has the softmax of tile b only: its lanes take their
+// scores from that tile's product, and put zeros into the other tiles' places of the second product.  Both products are what they were;
+// of the vector instructions those for scales, exponentials and sums are a COPIES-th a token.  The copies' maxima are
+// kept alike, their sums are added at the end.
+template <int T, int DP, int NB, int COPIES>
 struct Engine {
   static constexpr bool F32 = T == ITEXHIP_FLOAT;
+  static_assert(COPIES == 1 || (NB == 1 && !F32), "copies");
+  static constexpr int TILES = COPIES == 4 ? 4 : 2, TOKENS = 16 * TILES, OWN = COPIES == 1 ? TILES : 1, WIDTH = 16 / COPIES;  // OWN: tiles whose scores a lane has
   static constexpr int NKK = DP / 32, E = DP / 16, NV = DP <= 128 ? 1 : 2;
   static constexpr float kSlack = F32 ? 0.0f : 5.0f;  // log2 of how far a score may exceed the maximum that sums are relative to
   half8v q16[F32 ? 1 : NB][NKK];
@@ -111,10 +126,11 @@ struct Engine {
   f4 o[NB][E];
   int min_limit, max_start;  // over the wavefront's rows
   int seq_len;               // tokens of the sequence
-  int lane, c, g;
+  int lane, c, g, block;
   CodeBits bits;
-  uint32_t kraw[2][NKK];
-  u4v vraw[2][NV], kp[2], vp[2];
+  uint32_t kraw[TILES][NKK];
+  u4v vraw[TILES][NV], kp[OWN], vp[OWN];
+  const uint8_t* own_params;  // with copies: where kp came from
   const __attribute__((address_space(4))) int32_t* table;
   const uint8_t* head_base;
   int64_t page_bytes;
@@ -125,6 +141,7 @@ struct Engine {
     lane = threadIdx.x & 63;
     c = lane & 15;
     g = lane >> 4;
+    block = COPIES == 1 ? 0 : c / WIDTH;
     const int rows = s.n * A.group;
     const int before = s.len - s.n;  // position of the first row
     auto limit_of = [&](int row) { return A.causal ? max(before + row / A.group + 1, 0) : s.len; };
@@ -133,7 +150,7 @@ struct Engine {
     max_start = start_of(min(row0 + 16 * NB, rows) - 1);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const int row = row0 + nb * 16 + c;
+      const int row = row0 + nb * 16 + c % WIDTH;
       const bool in = row < rows;
       limit[nb] = in ? limit_of(row) : 0;
       start[nb] = in ? start_of(row) : 0;
@@ -213,10 +230,10 @@ struct Engine {
     p_lane = block.key_params(4 * g);
     vp_more = block.value_params(0) - block.key_params(0);
   }
-  // Pages of the tiles at t and t + 16 (beyond the last tile: that one's again, masked by its tokens)
-  __device__ __forceinline__ void fetch_pages(int t, int (&pages)[2]) const {
-    pages[0] = table[min(t, last_tile) >> shift];
-    pages[1] = table[min(t + 16, last_tile) >> shift];
+  // Pages of the tiles at t, t + 16, ... (beyond the last tile: that one's again, masked by its tokens)
+  __device__ __forceinline__ void fetch_pages(int t, int (&pages)[TILES]) const {
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) pages[i] = table[min(t + 16 * i, last_tile) >> shift];
   }
   // Where tile i of the step at t is; a page that is none: page 0 (masked)
   __device__ __forceinline__ const uint8_t* tile(int page, int t, int i, int* place) const {
@@ -225,13 +242,13 @@ struct Engine {
   }
   __device__ __forceinline__ bool valid(int page) const { return page >= 0 && page < num_pages; }
 
-  // What a lane (16 g + c) loads of a step's two tiles of 16 tokens:
+  // What a lane (16 g + c) loads of a step's tiles of 16 tokens:
   //   keys      token c of a tile, dwords g NKK .. g NKK + NKK - 1 of its row
   //   values    tokens 4 g .. 4 g + 3 of a tile, dword c (and c + 16; a half of dword c / 2 if a head has 8 of them)
-  //   params    of tokens 4 g .. 4 g + 3: four scales, four offsets
-  __device__ __forceinline__ void load_keys(const int (&pages)[2], int t) {
+  //   params    of tokens 4 g .. 4 g + 3 of the tiles that the lane has scores of: four scales, four offsets
+  __device__ __forceinline__ void load_keys(const int (&pages)[TILES], int t) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < TILES; ++i) {
       int place;
       const uint8_t* base = tile(pages[i], t, i, &place);
       const uint8_t* kr = base + place * (DP / 2);
@@ -247,18 +264,24 @@ struct Engine {
           for (int n = 0; n < 4; ++n) kraw[i][4 * j + n] = w[n];
         }
       }
-      kp[i] = *reinterpret_cast<const u4v*>(base + place * 4 + p_lane);
+      if constexpr (COPIES == 1) kp[i] = *reinterpret_cast<const u4v*>(base + place * 4 + p_lane);
+      else own_params = i == 0 || block == i ? base + place * 4 : own_params;
+    }
+    if constexpr (COPIES > 1) {
+      own_params += p_lane;
+      kp[0] = *reinterpret_cast<const u4v*>(own_params);
     }
   }
-  __device__ __forceinline__ void load_values(const int (&pages)[2], int t) {
+  __device__ __forceinline__ void load_values(const int (&pages)[TILES], int t) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < TILES; ++i) {
       int place;
       const uint8_t* base = tile(pages[i], t, i, &place);
 #pragma unroll
       for (int j = 0; j < NV; ++j) vraw[i][j] = __builtin_nontemporal_load(reinterpret_cast<const u4v*>(base + place * (DP / 2) + v_lane + 256 * j));
-      vp[i] = *reinterpret_cast<const u4v*>(base + place * 4 + vp_more + p_lane);
+      if constexpr (COPIES == 1) vp[i] = *reinterpret_cast<const u4v*>(base + place * 4 + vp_more + p_lane);
     }
+    if constexpr (COPIES > 1) vp[0] = *reinterpret_cast<const u4v*>(own_params + vp_more);
   }
 
   __device__ __forceinline__ half8v key_operand(uint32_t w) const {
@@ -276,10 +299,10 @@ struct Engine {
   }
 
   // The sums are held relative to a maximum of the scores and a power of two over the values' scales: either has grown
-  __device__ __forceinline__ void raise(const float (&p)[NB][8], uint32_t most) {
+  __device__ __forceinline__ void raise(const float (&p)[NB][4 * OWN], uint32_t most) {
     if constexpr (!F32) {
-      most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 16)));
-      most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 32)));
+#pragma unroll
+      for (int d = WIDTH; d < 64; d *= 2) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), d)));
       most = (most > 0x7bffu ? 0x7bffu : most) | 0x3ffu;  // NaN comes through the products
       if (most > scale_bound) {
         const float by = static_cast<float>(static_cast<int>((most >> 10) - (scale_bound >> 10)));
@@ -295,9 +318,9 @@ struct Engine {
     for (int nb = 0; nb < NB; ++nb) {
       float top = p[nb][0];
 #pragma unroll
-      for (int j = 1; j < 8; ++j) top = fmaxf(top, p[nb][j]);
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
+      for (int j = 1; j < 4 * OWN; ++j) top = fmaxf(top, p[nb][j]);
+#pragma unroll
+      for (int d = WIDTH; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
       const float was = m[nb];
       if (top > was) {
         m[nb] = top;
@@ -310,14 +333,14 @@ struct Engine {
   }
 
   // One step: `pages` are its own, `next` (at `tn`) those of the step to load behind it
-  __device__ __forceinline__ void step(bool mask, const int (&pages)[2], int t0, const int (&next)[2], int tn) {
-    bool ok[2] = {true, true};
-    uint32_t nan = 0;  // bit 4 i + j: the value of token 4 g + j of tile i is NaN and only some rows may see it
-    float p[NB][8];
+  __device__ __forceinline__ void step(bool mask, const int (&pages)[TILES], int t0, const int (&next)[TILES], int tn) {
+    auto tile_of = [&](int i) { return COPIES == 1 ? i : block; };  // of the lane's i-th four scores
+    float p[NB][4 * OWN];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
+      f4 own;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < TILES; ++i) {
         f4 s = corr[nb];
 #pragma unroll
         for (int kk = 0; kk < NKK; ++kk) {
@@ -329,11 +352,20 @@ struct Engine {
               s = __builtin_amdgcn_mfma_f32_16x16x4f32(static_cast<float>((kraw[i][kk] >> (4 * n)) & 15u), q32[nb][kk][n], s, 0, 0, 0);
           }
         }
+        if (COPIES == 1 || i == 0) {
+          own = s;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) own[j] = block == i ? s[j] : own[j];
+        }
+        if (COPIES > 1 && i + 1 < TILES) continue;
+        constexpr int last = OWN - 1;
+        const int k = COPIES == 1 ? i : last;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t sc = kp[i][j / 2], of = kp[i][2 + j / 2];
+          const uint32_t sc = kp[k][j / 2], of = kp[k][2 + j / 2];
           const float ks = (j & 1) ? high_half(sc) : low_half(sc), ko = (j & 1) ? high_half(of) : low_half(of);
-          p[nb][4 * i + j] = fmaf(ks, s[j], ko * sumq[nb]);
+          p[nb][4 * k + j] = fmaf(ks, own[j], fmaf(ko, sumq[nb], 0.0f));
         }
       }
     }
@@ -341,16 +373,21 @@ struct Engine {
     load_keys(next, tn);
     __builtin_amdgcn_sched_barrier(0);
     if (mask) {
-      ok[0] = valid(pages[0]);
-      ok[1] = valid(pages[1]);
+      uint32_t nan = 0;  // bit 4 i + j: the value of token 4 g + j of the lane's tile i is NaN and only some rows may see it
+      bool ok[OWN];
+#pragma unroll
+      for (int i = 0; i < TILES; ++i) {
+        if (COPIES == 1) ok[COPIES == 1 ? i : 0] = valid(pages[i]);
+        else ok[0] = i == 0 || block == i ? valid(pages[i]) : ok[0];
+      }
       // tokens beyond the last one hold whatever memory held: their values must not reach a product, not even times zero
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < OWN; ++i) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t keep = (j & 1) ? 0x0000ffffu : 0xffff0000u;
           const uint32_t sc = (vp[i][j / 2] >> (16 * (j & 1))) & 0x7fffu, of = (vp[i][2 + j / 2] >> (16 * (j & 1))) & 0x7fffu;
-          const bool beyond = t0 + 16 * i + 4 * g + j >= seq_len || !ok[i];
+          const bool beyond = t0 + 16 * tile_of(i) + 4 * g + j >= seq_len || !ok[i];
           if (beyond || sc >= 0x7c00u || of >= 0x7c00u) {
             if (!beyond) nan |= 1u << (4 * i + j);
             vp[i][j / 2] &= keep;
@@ -361,8 +398,8 @@ struct Engine {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int t = t0 + 16 * (k / 4) + 4 * g + k % 4;
+        for (int k = 0; k < 4 * OWN; ++k) {
+          const int t = t0 + 16 * tile_of(k / 4) + 4 * g + k % 4;
           const bool seen = ok[k / 4] && t < limit[nb] && t >= start[nb];
           p[nb][k] = seen ? p[nb][k] : -INFINITY;
           if (seen && (nan >> k & 1)) l[nb] = NAN;
@@ -373,48 +410,72 @@ struct Engine {
     bool over = false;
     if constexpr (!F32) {
       typedef unsigned short us2 __attribute__((ext_vector_type(2)));
-      auto v = [](uint32_t x) { us2 r; __builtin_memcpy(&r, &x, 4); return r; };
-      const us2 two = __builtin_elementwise_max(__builtin_elementwise_max(v(vp[0][0]), v(vp[0][1])), __builtin_elementwise_max(v(vp[1][0]), v(vp[1][1])));
+      us2 two = {0, 0};
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) {
+        us2 x[2];
+        __builtin_memcpy(x, &vp[i], 8);
+        two = __builtin_elementwise_max(two, __builtin_elementwise_max(x[0], x[1]));
+      }
       most = two[0] > two[1] ? two[0] : two[1];
       over = most > scale_bound;
     }
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const float top = fmaxf(fmaxf(fmaxf(p[nb][0], p[nb][1]), fmaxf(p[nb][2], p[nb][3])), fmaxf(fmaxf(p[nb][4], p[nb][5]), fmaxf(p[nb][6], p[nb][7])));
+      float top = p[nb][0];
+#pragma unroll
+      for (int j = 1; j < 4 * OWN; ++j) top = fmaxf(top, p[nb][j]);
       over = over || top > raise_at[nb];
     }
     if (__any(over)) raise(p, most);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < 4 * OWN; ++j) {
         p[nb][j] = __builtin_amdgcn_exp2f(fmaf(p[nb][j], qs[nb], ref[nb]));
         l[nb] += p[nb][j];
       }
     }
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (!F32) {
-      half8v pb[NB];
+      half8v pb[NB][TILES / 2];  // of tiles 2 u and 2 u + 1
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
+        uint32_t two[2 * OWN];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t sc = vp[j / 4][j % 4 / 2], of = vp[j / 4][2 + j % 4 / 2];
-          po[nb] = fmaf(p[nb][j], (j & 1) ? high_half(of) : low_half(of), po[nb]);
-          float x = fmaf(p[nb][j], (j & 1) ? high_half(sc) : low_half(sc), 0.0f);
-          asm("" : "+v"(x));  // (merged with the conversion it would be an instruction that writes half a register, at twice the time)
-          pb[nb][j] = static_cast<_Float16>(x);
+        for (int j = 0; j < 4 * OWN; j += 2) {
+          half2v h;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t sc = vp[j / 4][j % 4 / 2], of = vp[j / 4][2 + j % 4 / 2];
+            po[nb] = fmaf(p[nb][j + k], k ? high_half(of) : low_half(of), po[nb]);
+            float x = fmaf(p[nb][j + k], k ? high_half(sc) : low_half(sc), 0.0f);
+            asm("" : "+v"(x));  // (merged with the conversion it would be an instruction that writes half a register, at twice the time)
+            h[k] = static_cast<_Float16>(x);
+          }
+          two[j / 2] = as_bits(h);
+        }
+#pragma unroll
+        for (int u = 0; u < TILES / 2; ++u) {
+          u4v a;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if constexpr (COPIES == 1) a[k] = two[k];
+            else a[k] = block == 2 * u + k / 2 ? two[k & 1] : 0;
+          }
+          __builtin_memcpy(&pb[nb][u], &a, 16);
         }
       }
       // a lane's eight tokens of one dimension, two a register: first the halves of two tokens' dwords that hold its code
 #pragma unroll
-      for (int part = 0; part < E / 4; ++part) {  // four dimensions each: a half of a dword
+      for (int at = 0; at < TILES / 2 * (E / 4); ++at) {
+        const int u = at / (E / 4), part = at % (E / 4);  // two tiles, four dimensions: a half of a dword
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const u4v& d = vraw[i][part / 2 % NV];
+            const u4v& d = vraw[2 * u + i][part / 2 % NV];
             if constexpr (DP == 64) w[2 * i + j] = __builtin_amdgcn_perm(d[2 * j + 1], d[2 * j], (c & 1) ? 0x07060302u : 0x05040100u);
             else w[2 * i + j] = __builtin_amdgcn_perm(d[2 * j + 1], d[2 * j], (part & 1) ? 0x07060302u : 0x05040100u);
           }
@@ -433,7 +494,7 @@ struct Engine {
           __builtin_memcpy(&v, &a, 16);
           const int e = part * 4 + n;
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) o[nb][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pb[nb], o[nb][e], 0, 0, 0);
+          for (int nb = 0; nb < NB; ++nb) o[nb][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pb[nb][u], o[nb][e], 0, 0, 0);
         }
       }
     } else {
@@ -460,22 +521,28 @@ struct Engine {
     __builtin_amdgcn_sched_barrier(0);
   }
 
-  // Tokens from, from + stride, ..., 32 each, up to `to`
+  // Tokens from, from + stride, ..., TOKENS each, up to `to`
   __device__ __forceinline__ void run(const AttArgs& A, const int32_t* pages, int kv_head, int from, int to, int stride, int len) {
     if (from >= to) return;
     seq_len = len;
     bits.pin();
     open(A, pages, kv_head, to);
-    int now[2], next[2], later[2];
+    int now[TILES], next[TILES], later[TILES];
     fetch_pages(from, now);
     fetch_pages(from + stride, next);
     load_keys(now, from);
     load_values(now, from);
     for (int t = from; t < to; t += stride) {
       fetch_pages(t + 2 * stride, later);
-      step(!(valid(now[0]) && valid(now[1]) && t + 32 <= min_limit && t >= max_start), now, t, next, t + stride);
-      now[0] = next[0]; now[1] = next[1];
-      next[0] = later[0]; next[1] = later[1];
+      bool all = t + TOKENS <= min_limit && t >= max_start;
+#pragma unroll
+      for (int i = 0; i < TILES; ++i) all = all && valid(now[i]);
+      step(!all, now, t, next, t + stride);
+#pragma unroll
+      for (int i = 0; i < TILES; ++i) {
+        now[i] = next[i];
+        next[i] = later[i];
+      }
     }
   }
 
@@ -484,17 +551,28 @@ struct Engine {
     return DP == 64 ? 4 * (4 * g + r) + e : 8 * (4 * g + r) + (e & 7) + 128 * (e >> 3);
   }
 
-  // The parts of a column's sums that its four lanes hold apart
+  // The parts of a row's sums that the four lanes of a column, and the copies, hold apart
+  template <int BY>  // what the lane BY further on has, among 16
+  static __device__ __forceinline__ float turned(float x) { return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x120 + BY, 0xf, 0xf, true)); }
   __device__ __forceinline__ void close() {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      l[nb] += __shfl_xor(l[nb], 16);
-      l[nb] += __shfl_xor(l[nb], 32);
-      if constexpr (!F32) {
-        po[nb] += __shfl_xor(po[nb], 16);
-        po[nb] += __shfl_xor(po[nb], 32);
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[nb][e] += po[nb];
+      for (int d = WIDTH; d < 64; d *= 2) l[nb] += __shfl_xor(l[nb], d);
+      if constexpr (!F32) {
+#pragma unroll
+        for (int d = WIDTH; d < 64; d *= 2) po[nb] += __shfl_xor(po[nb], d);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          if constexpr (COPIES > 1) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              o[nb][e][r] += turned<8>(o[nb][e][r]);
+              if constexpr (COPIES == 4) o[nb][e][r] += turned<4>(o[nb][e][r]);
+            }
+          }
+          o[nb][e] += po[nb];
+        }
       }
     }
   }
@@ -542,8 +620,9 @@ struct Engine {
 // the two at its ends leave their sums in the workspace for combine_kernel.
 template <int NB>
 __device__ __forceinline__ int tiles_of(const AttArgs& A, const Seq& s) { return (s.n * A.group + 16 * NB - 1) / (16 * NB); }
-template <int T, int DP, int NB>
-__global__ __launch_bounds__(256, occupancy_of(NB, DP)) void split_kernel(const AttArgs A) {
+template <int T, int DP, int NB, int COPIES>
+__global__ __launch_bounds__(256, occupancy_of(NB, DP, T == ITEXHIP_FLOAT)) void split_kernel(const AttArgs A) {
+  constexpr int STEP = step_of(COPIES);
   __shared__ int64_t scan[5];
   __shared__ int64_t found[2];
   __shared__ float lds_ml[4][2][16 * NB];
@@ -555,7 +634,7 @@ __global__ __launch_bounds__(256, occupancy_of(NB, DP)) void split_kernel(const 
     const int b = base + tid;
     int64_t x = 0;
     if (b < A.num_seqs) {
-      const Seq s = sequence(A, b);
+      const Seq s = sequence<STEP>(A, b);
       x = s.steps * A.kv_heads * tiles_of<NB>(A, s);
     }
 #pragma unroll
@@ -584,7 +663,7 @@ __global__ __launch_bounds__(256, occupancy_of(NB, DP)) void split_kernel(const 
     const int b = base + tid;
     __syncthreads();
     if (b < A.num_seqs) {
-      const Seq s = sequence(A, b);
+      const Seq s = sequence<STEP>(A, b);
       const int64_t mine = s.steps * A.kv_heads * tiles_of<NB>(A, s), from = before + inclusive - mine;
       if (begin >= from && begin < from + mine) {
         found[0] = b;
@@ -601,7 +680,7 @@ __global__ __launch_bounds__(256, occupancy_of(NB, DP)) void split_kernel(const 
   int64_t from = found[1];
 
   for (int64_t at = begin; at < end;) {
-    const Seq s = sequence(A, b);
+    const Seq s = sequence<STEP>(A, b);
     if (s.steps == 0) {
       ++b;
       continue;
@@ -611,10 +690,10 @@ __global__ __launch_bounds__(256, occupancy_of(NB, DP)) void split_kernel(const 
     const int64_t s0 = rel - item * s.steps, left = s.steps - s0, n = left < end - at ? left : end - at;
     const bool whole = n == s.steps;
 
-    Engine<T, DP, NB> eng;
+    Engine<T, DP, NB, COPIES> eng;
     eng.init(A, s, head, row0);
-    const int first = s.lo + static_cast<int>(s0) * kStep, last = first + static_cast<int>(n) * kStep;
-    eng.run(A, A.table + b * A.table_stride, head, first + 32 * wave, last < s.len ? last : s.len, kStep, s.len);
+    const int first = s.lo + static_cast<int>(s0) * STEP, last = first + static_cast<int>(n) * STEP;
+    eng.run(A, A.table + b * A.table_stride, head, first + STEP / 4 * wave, last < s.len ? last : s.len, STEP, s.len);
     eng.close();
 
     // the four wavefronts' sums into those of the first
@@ -690,13 +769,14 @@ __global__ __launch_bounds__(256, occupancy_of(NB, DP)) void split_kernel(const 
 }
 
 // One row of a (sequence, kv head) that several workgroups shared: their sums, in the order of the tokens
-template <int T, int DP, int NB>
+template <int T, int DP, int NB, int COPIES>
 __global__ __launch_bounds__(256) void combine_kernel(const AttArgs A) {
+  constexpr int STEP = step_of(COPIES);
   constexpr int LANES = DP / 4, PARTS = 256 / LANES, CHUNK = kMostGroups;
   __shared__ float lds_o[PARTS][DP];
   __shared__ float lds_l[4], lds_top[4], weight[CHUNK];
   const int b = blockIdx.z, head = blockIdx.y, row = blockIdx.x, tid = threadIdx.x;
-  const Seq s = sequence(A, b);
+  const Seq s = sequence<STEP>(A, b);
   if (row >= s.n * A.group) return;
   const int item = head * tiles_of<NB>(A, s) + row / (16 * NB);
   const int64_t share = A.prefix[A.num_seqs], i0 = A.prefix[b] + item * s.steps;
@@ -764,7 +844,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const AttArgs A) {
   const Seq s = sequence(A, b);
   const int rows = s.n * A.group, row0 = (static_cast<int>(blockIdx.x) * 4 + wave) * 16 * NB;
   if (row0 >= rows) return;
-  Engine<T, DP, NB> eng;
+  Engine<T, DP, NB, 1> eng;
   eng.init(A, s, head, row0);
   const int first = row0 / A.group, last = (row0 + 16 * NB < rows ? row0 + 16 * NB - 1 : rows - 1) / A.group;
   int to = s.len, from = s.lo;
@@ -1159,6 +1239,7 @@ __global__ __launch_bounds__(64 * kWaves<DP>, kWaves<DP> / 4) void prompt_kernel
 // ---------------------------------------------------------------------------------------------------------------------
 struct Plan {
   int blocks;      // NB
+  int copies;
   bool split;
   int64_t groups;  // workgroups of the split kernel
   size_t prefix, ml, o, bytes;
@@ -1169,10 +1250,12 @@ Plan plan_of(const itexhip_kv4_attention_params* p, const itexhip_kv4_cache* c) 
   const int dp = kv4_padded(c->head_dim);
   const int64_t rows = static_cast<int64_t>(p->max_q_len) * (p->q_heads / c->kv_heads);
   plan.blocks = rows <= 16 || dp == 256 ? 1 : 2;
+  plan.copies = copies_of(p->type == ITEXHIP_FLOAT, rows);
   plan.split = rows <= kMostSplitRows;
   if (plan.split) {
-    const int64_t bound = static_cast<int64_t>(p->num_seqs) * c->kv_heads * ((p->table_stride * c->page_size + kStep - 1) / kStep) * ((rows + 16 * plan.blocks - 1) / (16 * plan.blocks));
-    const int64_t full = 256 * occupancy_of(plan.blocks, dp);
+    const int step = step_of(plan.copies);
+    const int64_t bound = static_cast<int64_t>(p->num_seqs) * c->kv_heads * ((p->table_stride * c->page_size + step - 1) / step) * ((rows + 16 * plan.blocks - 1) / (16 * plan.blocks));
+    const int64_t full = 256 * occupancy_of(plan.blocks, dp, p->type == ITEXHIP_FLOAT);
     plan.groups = bound < 1 ? 1 : bound < full ? bound : full;
     plan.prefix = (static_cast<size_t>(p->num_seqs) + 1) * 8 + 15 & ~size_t{15};
     plan.ml = static_cast<size_t>(plan.groups) * 2 * 16 * plan.blocks * 2 * 4;
@@ -1208,8 +1291,17 @@ template <int T, int DP, int NB>
 void launch(const AttArgs& A, const Plan& plan, hipStream_t stream) {
   const int rows = A.max_q_len * A.group;
   if (plan.split) {
-    split_kernel<T, DP, NB><<<dim3(static_cast<unsigned>(plan.groups)), dim3(256), 0, stream>>>(A);
-    if (plan.groups > 1) combine_kernel<T, DP, NB><<<dim3(rows, A.kv_heads, A.num_seqs), dim3(256), 0, stream>>>(A);
+    auto both = [&](auto copies) {
+      split_kernel<T, DP, NB, copies.value><<<dim3(static_cast<unsigned>(plan.groups)), dim3(256), 0, stream>>>(A);
+      if (plan.groups > 1) combine_kernel<T, DP, NB, copies.value><<<dim3(rows, A.kv_heads, A.num_seqs), dim3(256), 0, stream>>>(A);
+    };
+    if constexpr (T != ITEXHIP_FLOAT && NB == 1) {
+      if (plan.copies == 4) both(std::integral_constant<int, 4>{});
+      else if (plan.copies == 2) both(std::integral_constant<int, 2>{});
+      else both(std::integral_constant<int, 1>{});
+    } else {
+      both(std::integral_constant<int, 1>{});
+    }
   } else {
     if constexpr (T == ITEXHIP_FLOAT) {
       rows_kernel<T, DP, NB><<<dim3((rows + 64 * NB - 1) / (64 * NB), A.kv_heads, A.num_seqs), dim3(256), 0, stream>>>(A);
