@@ -561,7 +561,7 @@ typedef struct {
 int64_t itexhip_kv4_page_bytes(const itexhip_kv4_cache* c); /* 0: not a valid geometry */
 
 /* Norm, rotation and quantization of new keys, quantization of new values, into the cache, with the queries' norm and
- * rotation in the same launch (q may be NULL, then q_out is not written).  slots[t] (device) = page * page_size + place in
+ * rotation in the same call (q may be NULL, then q_out is not written; otherwise q_out is q or overlaps none of the inputs).  slots[t] (device) = page * page_size + place in
  * the page; a slot below 0 or beyond the cache writes nothing (padded rows).  A slot occurs once in a call: which of two
  * rows' codes, scales and offsets a slot given twice holds is not defined. */
 int itexhip_kv4_append(const itexhip_heads_params* p, const itexhip_kv4_cache* c, int64_t tokens, const void* q, const void* k,
@@ -569,7 +569,7 @@ int itexhip_kv4_append(const itexhip_heads_params* p, const itexhip_kv4_cache* c
                        const double* freqs, const int64_t* slots, void* q_out, void* cache, void* stream);
 
 /* The values that slots hold, [tokens, kv_heads, head_dim] of `type`; zeros for a slot outside the cache.  Either output may
- * be NULL. */
+ * be NULL; outputs are 16-byte aligned. */
 int itexhip_kv4_gather(const itexhip_kv4_cache* c, int type, int64_t tokens, const void* cache, const int64_t* slots, void* k_out,
                        void* v_out, void* stream);
 
@@ -579,7 +579,7 @@ int itexhip_kv4_gather(const itexhip_kv4_cache* c, int type, int64_t tokens, con
  * if window > 0.  q_heads is a multiple of kv_heads; consecutive query heads share a kv head.
  *   out = softmax(scale q k) v, rounded once; lse (NULL: not wanted; [total_q, q_heads] floats) the log of the sum of exponents
  * A row that sees nothing is 0 with lse -inf.  Rows outside every sequence are left as they are.  Keys and values a row does
- * not see do not reach it, whatever they hold.  A page outside the cache counts as tokens that no row sees; kv_len beyond the
+ * not see do not reach it, whatever they hold; a value that is NaN and seen makes the whole row of out and its lse NaN.  A page outside the cache counts as tokens that no row sees; kv_len beyond the
  * table is cut to it, a sequence's rows beyond max_q_len or total_q are not computed.
  * workspace: itexhip_kv4_attention_workspace bytes of device memory (16-byte aligned), contents irrelevant; calls that may
  * overlap in time need one each.  Results do not depend on timing: equal calls give equal bits. */
@@ -587,12 +587,12 @@ typedef struct {
   int type;             /* FLOAT | BFLOAT16 | HALF of q and out */
   int q_heads;
   int num_seqs;         /* 0 .. 65535 */
-  int max_q_len;        /* most rows of a sequence: decides, with the heads, which kernel runs */
+  int max_q_len;        /* most rows of a sequence: decides, with the heads, which kernel runs; times q_heads below 2^30 */
   int64_t total_q;      /* rows of q and out, below 2^31 */
-  float scale;          /* > 0 */
+  float scale;          /* finite and > 0 */
   int causal;
   int window;           /* 0: none */
-  int64_t table_stride; /* entries of block_table between sequences: the most pages of one */
+  int64_t table_stride; /* entries of block_table between sequences: the most pages of one; at most 2^30 tokens */
   int64_t q_strides[2], out_strides[2];
 } itexhip_kv4_attention_params;
 int64_t itexhip_kv4_attention_workspace(const itexhip_kv4_attention_params* p, const itexhip_kv4_cache* c); /* 0: not valid */

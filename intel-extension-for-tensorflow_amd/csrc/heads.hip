@@ -31,12 +31,14 @@ __device__ __forceinline__ float load1(const void* base, int64_t i) {
   else return f16_bits_to_f32(static_cast<const uint16_t*>(base)[i]);
 }
 template <int T>
-__device__ __forceinline__ void store4(void* base, int64_t i, const float (&x)[4]) {
+__device__ __forceinline__ void store8(void* base, int64_t i, const float (&x)[8]) {
   if constexpr (T == ITEXHIP_FLOAT) {
-    *reinterpret_cast<f4*>(static_cast<float*>(base) + i) = f4{x[0], x[1], x[2], x[3]};
+    f4* to = reinterpret_cast<f4*>(static_cast<float*>(base) + i);
+    to[0] = f4{x[0], x[1], x[2], x[3]};
+    to[1] = f4{x[4], x[5], x[6], x[7]};
   } else {
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + i) =
-        uint2{f32x2_to_bits16<T>(x[0], x[1]), f32x2_to_bits16<T>(x[2], x[3])};
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + i) =
+        uint4{f32x2_to_bits16<T>(x[0], x[1]), f32x2_to_bits16<T>(x[2], x[3]), f32x2_to_bits16<T>(x[4], x[5]), f32x2_to_bits16<T>(x[6], x[7])};
   }
 }
 
@@ -172,19 +174,21 @@ __device__ __forceinline__ void quantize_head(Runs<double, NPL>& v, bool mine, u
 // is worked on, and a token's cosines and sines are computed once for its passes in a share.
 //
 // Queries are normed and rotated in fp32.  Keys go through 64 bits all the way to their codes: a key computed by another call (a
-// shared prefix, a resumed sequence) has the same codes then, whichever way the arithmetic is ordered, and with eight kv heads to a
-// token it is a tenth of the vector instructions' time that the memory takes.
-#ifndef SPLIT_FROM
-#define SPLIT_FROM 512
-#endif
-#ifndef HA8
-#define HA8 2
-#define HA4 3
-#define HN8 4
-#endif
-template <int NPL, bool APPEND> constexpr int kHeadsOccupancy = APPEND ? (NPL == 8 ? HA8 : HA4) : NPL == 8 ? HN8 : 6;
+// shared prefix, a resumed sequence) has the same codes then, whichever way the arithmetic is ordered.
+//
+// Norm and rotation of 8192 tokens (32 heads and 8 of 128, bfloat16, 168 MB read and written) take 43 us, 3.9 TB/s, where a copy
+// has 5.1.  Appending them takes 32 us for the queries (4.2 TB/s) and 35 for keys and values, 34 MB and 9 MB of cache:
+// there the 64-bit instructions are what is waited for, with two wavefronts a SIMD to hide their latency (one token: 4 to 5 us, launch
+// and one chain of loads).
+//
+// Wavefronts a SIMD: what registers allow without spills.  Measured, 8192 tokens, in us: appending bfloat16 2 : 3 76 : 105, fp32
+// 3 : 4 119 : 111; norm and rotation bfloat16 3 : 4 : 6 43 : 43 : 77, fp32 3 : 4 : 6 : 8 73 : 71 : 76 : 110.
+constexpr int occupancy_of(int npl, bool vec, bool append) { return !append ? 4 : npl == 8 ? 2 : vec ? 4 : 3; }
+// Passes a wavefront from which an append's queries go through a launch of their own, which has more wavefronts and no 64-bit
+// registers: one launch : two, bfloat16 at 6 passes 24 : 26 us, 12 40 : 38, 18 67 : 59, 24 86 : 76; fp32 at 12 60 : 63, 24 113 : 111
+constexpr int kOwnLaunch = 16;
 template <int T, int NPL, int LPH, bool VEC, bool APPEND>
-__global__ __launch_bounds__(256, (kHeadsOccupancy<NPL, APPEND>)) void heads_kernel(const HeadsArgs A) {
+__global__ __launch_bounds__(256, occupancy_of(NPL, VEC, APPEND)) void heads_kernel(const HeadsArgs A) {
   constexpr bool DWORDS = VEC && NPL == 8;  // a run is a dword of codes
   constexpr int WORDS = VEC ? NPL * (T == ITEXHIP_FLOAT ? 4 : 2) / 4 : NPL;
   using Angle = std::conditional_t<APPEND, double, float>;
@@ -409,19 +413,17 @@ __global__ __launch_bounds__(256, (kHeadsOccupancy<NPL, APPEND>)) void heads_ker
   }
 }
 
-// Rows of the cache as values: one lane takes eight dimensions of a token's key and value
+// Rows of the cache as values: one lane takes eight dimensions of a token's key and value.  A launch has fewer than 2^32 of these
+// units, from `first` on, so a unit's place comes from divisions in 32 bits.
 template <int T>
-__global__ __launch_bounds__(256) void gather_kernel(const uint8_t* __restrict__ cache, const int64_t* __restrict__ slots, int64_t units,
-                                                     int kv_heads, int head_dim, int dp, int page_size, int page_shift, int64_t num_slots,
+__global__ __launch_bounds__(256) void gather_kernel(const uint8_t* __restrict__ cache, const int64_t* __restrict__ slots, int64_t first, uint32_t units,
+                                                     uint32_t kv_heads, int head_dim, int dp, int page_size, int page_shift, int64_t num_slots,
                                                      int64_t page_bytes, void* __restrict__ k_out, void* __restrict__ v_out) {
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const uint32_t unit = blockIdx.x * 256u + threadIdx.x;
   if (unit >= units) return;
-  const int chunks = head_dim / 8;
-  const int64_t row = unit / chunks;
-  const int dword = static_cast<int>(unit - row * chunks);
-  const int64_t token = row / kv_heads;
-  const int head = static_cast<int>(row - token * kv_heads);
-  const int64_t slot = slots[token];
+  const uint32_t chunks = static_cast<uint32_t>(head_dim) / 8, row = unit / chunks, token = row / kv_heads;
+  const int dword = static_cast<int>(unit - row * chunks), head = static_cast<int>(row - token * kv_heads);
+  const int64_t slot = slots[first + token], at = (first * kv_heads + row) * head_dim + 8 * dword;
   const bool in = slot >= 0 && slot < num_slots;
   const Kv4Block block{page_size, dp};
   const uint8_t* from = cache + (in ? (slot >> page_shift) * page_bytes : 0) + static_cast<int64_t>(head) * block.bytes();
@@ -430,14 +432,13 @@ __global__ __launch_bounds__(256) void gather_kernel(const uint8_t* __restrict__
     const uint32_t w = in ? *reinterpret_cast<const uint32_t*>(from + codes) : 0;
     const float scale = in ? f16_bits_to_f32(*reinterpret_cast<const uint16_t*>(from + params)) : 0.0f;
     const float offset = in ? f16_bits_to_f32(*reinterpret_cast<const uint16_t*>(from + params + 8)) : 0.0f;
-    float x[4], y[4];
+    float x[8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       x[j] = fmaf(scale, static_cast<float>(static_cast<int>((w >> (4 * j)) & 15u) - 8), offset);
-      y[j] = fmaf(scale, static_cast<float>(static_cast<int>((w >> (16 + 4 * j)) & 15u) - 8), offset);
+      x[4 + j] = fmaf(scale, static_cast<float>(static_cast<int>((w >> (16 + 4 * j)) & 15u) - 8), offset);
     }
-    store4<T>(out, row * head_dim + 8 * dword, x);
-    store4<T>(out, row * head_dim + 8 * dword + 4, y);
+    store8<T>(out, at, x);
   };
   if (k_out != nullptr) one(block.key_codes(place) + 4 * dword, block.key_params(place), k_out);
   if (v_out != nullptr) one(block.value_codes(place, dword), block.value_params(place), v_out);
@@ -465,7 +466,7 @@ int check_heads(const char* who, const itexhip_heads_params* p, int64_t tokens) 
 template <int T, int NPL, int LPH, bool VEC, bool APPEND>
 void launch(HeadsArgs& A, hipStream_t stream) {
   // as many wavefronts as the device holds at once, or one a pass
-  const int64_t all = A.tokens * A.passes, held = 1024 * kHeadsOccupancy<NPL, APPEND>;
+  const int64_t all = A.tokens * A.passes, held = 1024 * occupancy_of(NPL, VEC, APPEND);
   A.share = (all + held - 1) / held;
   const int64_t waves = (all + A.share - 1) / A.share;
   heads_kernel<T, NPL, LPH, VEC, APPEND><<<dim3(static_cast<unsigned>((waves + 3) / 4)), dim3(256), 0, stream>>>(A);
@@ -503,6 +504,14 @@ int run(HeadsArgs& A, hipStream_t stream, const char* who) {
   A.passes_v = APPEND ? A.passes_k : 0;
   A.passes = A.passes_k + A.passes_v + (A.q != nullptr ? (p.q_heads + group - 1) / group : 0);
   if (A.passes == 0 || A.tokens == 0) return ITEXHIP_OK;
+  if constexpr (APPEND) {
+    if (A.q != nullptr && A.tokens * A.passes >= kOwnLaunch * 1024ll * occupancy_of(npl, vec, true)) {
+      HeadsArgs Q = A;
+      Q.k = Q.v = nullptr;
+      if (const int st = run<false>(Q, stream, who)) return st;
+      A.passes = A.passes_k + A.passes_v;
+    }
+  }
   if (p.type == ITEXHIP_FLOAT) launch_runs<ITEXHIP_FLOAT, APPEND>(A, npl, lph, vec, stream);
   else if (p.type == ITEXHIP_BFLOAT16) launch_runs<ITEXHIP_BFLOAT16, APPEND>(A, npl, lph, vec, stream);
   else launch_runs<ITEXHIP_HALF, APPEND>(A, npl, lph, vec, stream);
@@ -603,12 +612,6 @@ extern "C" int itexhip_kv4_append(const itexhip_heads_params* p, const itexhip_k
   A.p = *p;
   A.q = q; A.k = k; A.v = v; A.q_weight = q_weight; A.k_weight = k_weight; A.positions = positions; A.freqs = freqs; A.slots = slots;
   A.q_out = q_out; A.cache = static_cast<uint8_t*>(cache); A.tokens = tokens;
-  if (q != nullptr && tokens >= SPLIT_FROM) {
-    HeadsArgs Q = A;
-    Q.k = Q.v = nullptr;
-    if (const int st = run<false>(Q, as_stream(stream), who)) return st;
-    A.q = nullptr;
-  }
   A.page_size = c->page_size;
   A.page_shift = log2_of(c->page_size);
   A.num_slots = c->num_pages * c->page_size;
@@ -630,13 +633,15 @@ extern "C" int itexhip_kv4_gather(const itexhip_kv4_cache* c, int type, int64_t 
   ITEXHIP_REQUIRE(cache != nullptr && slots != nullptr, "%s: null cache or slots", who);
   ITEXHIP_REQUIRE(aligned(cache, 16) && aligned(slots, 8) && aligned(k_out, 16) && aligned(v_out, 16),
                   "%s: cache and outputs are 16-byte aligned, slots to their elements", who);
-  const int64_t units = tokens * c->kv_heads * (c->head_dim / 8);
-  ITEXHIP_REQUIRE(units < (1ll << 31) * 128, "%s: too many values for one call", who);
+  const int64_t per_token = static_cast<int64_t>(c->kv_heads) * (c->head_dim / 8);
   const int dp = kv4_padded(c->head_dim);
-  const dim3 grid(static_cast<unsigned>((units + 255) / 256)), block(256);
   auto go = [&](auto kernel) {
-    kernel<<<grid, block, 0, as_stream(stream)>>>(static_cast<const uint8_t*>(cache), slots, units, c->kv_heads, c->head_dim, dp, c->page_size,
-                                                  log2_of(c->page_size), c->num_pages * c->page_size, itexhip_kv4_page_bytes(c), k_out, v_out);
+    in_pieces(0, tokens, [&](int64_t begin, int64_t end) {
+      const uint32_t units = static_cast<uint32_t>((end - begin) * per_token);
+      kernel<<<dim3((units + 255) / 256), dim3(256), 0, as_stream(stream)>>>(
+          static_cast<const uint8_t*>(cache), slots, begin, units, static_cast<uint32_t>(c->kv_heads), c->head_dim, dp, c->page_size,
+          log2_of(c->page_size), c->num_pages * c->page_size, itexhip_kv4_page_bytes(c), k_out, v_out);
+    }, kElementsPerLaunch / per_token);
   };
   if (type == ITEXHIP_FLOAT) go(gather_kernel<ITEXHIP_FLOAT>);
   else if (type == ITEXHIP_BFLOAT16) go(gather_kernel<ITEXHIP_BFLOAT16>);

@@ -220,23 +220,24 @@ def test_append_beyond_32_bits(hip, dev):
     assert torch.equal(ko.cpu(), want) and torch.equal(vo.cpu(), want)
 
 
-def test_many_tokens_are_cut_as_few_are(hip, dev):
-    """More passes than wavefronts: shares that begin and end inside a token, queries in a launch of their own; the same bits as token by token."""
-    tokens, hq, hk, d = 1500, 20, 4, 64
+@pytest.mark.parametrize("tokens", [1500, 9001])
+def test_many_tokens_are_cut_as_few_are(hip, dev, tokens):
+    """More passes than wavefronts: shares that begin and end inside a token, queries in a launch of their own; the same bits as by few tokens a call."""
+    hq, hk, d, pages = 20, 4, 64, tokens // 16 + 8
     x = rows(tokens, hq + 2 * hk, d, torch.bfloat16, 9).to(dev)
     freqs = torch.tensor(hip.rope_frequencies(d, 10000.0)[0], dtype=torch.float64, device=dev)
     pos = torch.arange(tokens, dtype=torch.int32, device=dev) * 3
     w = torch.rand(d, device=dev) + 0.5
     st = (x.stride(0), d)
     p = hip.heads_params(hip.BFLOAT16, d, hq, hk, rotary_dim=d, eps=1e-5, q_strides=st, k_strides=st, v_strides=st)
-    geometry = hip.kv4_cache(d, hk, 16, 100)
-    one, many = (torch.zeros(100, hip.kv4_page_bytes(geometry), dtype=torch.uint8, device=dev) for _ in range(2))
+    geometry = hip.kv4_cache(d, hk, 16, pages)
+    one, many = (torch.zeros(pages, hip.kv4_page_bytes(geometry), dtype=torch.uint8, device=dev) for _ in range(2))
     q1, q2 = torch.empty(tokens, hq, d, dtype=torch.bfloat16, device=dev), torch.empty(tokens, hq, d, dtype=torch.bfloat16, device=dev)
     slots = torch.arange(tokens, device=dev) + 50
     hip.kv4_append(p, geometry, tokens, x[:, :hq], x[:, hq:hq + hk], x[:, hq + hk:], w, w, pos, freqs, slots, q1, many)
     for i in range(0, tokens, 100):
         y = x[i:i + 100]
-        hip.kv4_append(p, geometry, 100, y[:, :hq], y[:, hq:hq + hk], y[:, hq + hk:], w, w, pos[i:], freqs, slots[i:], q2[i:], one)
+        hip.kv4_append(p, geometry, len(y), y[:, :hq], y[:, hq:hq + hk], y[:, hq + hk:], w, w, pos[i:], freqs, slots[i:], q2[i:], one)
     torch.cuda.synchronize()
     assert torch.equal(one, many)
     assert torch.equal(q1, q2)
@@ -244,9 +245,28 @@ def test_many_tokens_are_cut_as_few_are(hip, dev):
     q3 = torch.empty_like(q1)
     hip.qk_norm_rope(p, tokens, x[:, :hq], x[:, hq:], w, w, pos, freqs, q3, k1)
     for i in range(0, tokens, 100):
-        hip.qk_norm_rope(p, 100, x[i:i + 100, :hq], x[i:i + 100, hq:], w, w, pos[i:], freqs, q2[i:], k2[i:])
+        hip.qk_norm_rope(p, min(100, tokens - i), x[i:i + 100, :hq], x[i:i + 100, hq:], w, w, pos[i:], freqs, q2[i:], k2[i:])
     torch.cuda.synchronize()
     assert torch.equal(q3, q2) and torch.equal(k1, k2)
+
+
+def test_gather_of_more_values_than_a_launch_has(hip, dev):
+    """2^31 dwords of codes and some more: the launches' first and last rows, and those where one ends, are what calls of their own read."""
+    hk, d = 65535, 8
+    geometry = hip.kv4_cache(d, hk, 16, 1)
+    tokens = (1 << 31) // hk + 3
+    if torch.cuda.mem_get_info()[0] < tokens * hk * d * 2 + (4 << 30):
+        pytest.skip("memory for the rows")
+    g = torch.Generator(device=dev).manual_seed(1)
+    cache = torch.randint(0, 60, (hip.kv4_page_bytes(geometry),), dtype=torch.uint8, device=dev, generator=g)
+    slots = torch.arange(tokens, device=dev) * 5 % 16
+    out = torch.full((tokens, hk, d), 7, dtype=torch.half, device=dev)
+    hip.kv4_gather(geometry, hip.HALF, tokens, cache, slots, out, None)
+    once = torch.empty(16, hk, d, dtype=torch.half, device=dev)
+    hip.kv4_gather(geometry, hip.HALF, 16, cache, torch.arange(16, device=dev), once, None)
+    torch.cuda.synchronize()
+    for i in (0, 1, tokens // 2, tokens - 6, tokens - 5, tokens - 4, tokens - 3, tokens - 2, tokens - 1):
+        assert torch.equal(out[i], once[i * 5 % 16]), i
 
 
 def test_replayed_graph_reads_positions_and_slots_anew(hip, dev):
