@@ -131,23 +131,22 @@ __device__ __forceinline__ void rotate(Runs<Real, NPL>& v, bool across, int rota
   }
 }
 
-// Parameters and codes of a head whose dimensions are spread over LPH lanes (`mine`: this lane has some).
-template <int LPH, int NPL>
-__device__ __forceinline__ void quantize_head(Runs<double, NPL>& v, bool mine, uint32_t* scale_bits, uint32_t* offset_bits, uint32_t (&code)[2][NPL]) {
+// Parameters and codes of a head whose dimensions are spread over LPH lanes (`mine`: this lane has some).  Real: double for keys; values
+// are float until the quotient.
+template <int LPH, int NPL, class Real>
+__device__ __forceinline__ void quantize_head(Runs<Real, NPL>& v, bool mine, uint32_t* scale_bits, uint32_t* offset_bits, uint32_t (&code)[2][NPL]) {
   bool nan = false;
-  double hi = -65504.0, lo = 65504.0;
+  Real most = Real(-65504), least = Real(65504);
 #pragma unroll
   for (int j = 0; j < 2 * NPL; ++j) {
-    double& x = v.x[j / NPL][j % NPL];
+    Real& x = v.x[j / NPL][j % NPL];
     nan = nan || x != x;
-    x = fmin(fmax(x, -65504.0), 65504.0);
-    if (mine) {
-      hi = fmax(hi, x);
-      lo = fmin(lo, x);
-    }
+    x = fmin(fmax(x, Real(-65504)), Real(65504));
+    most = fmax(most, x);
+    least = fmin(least, x);
   }
-  hi = over_head<LPH>(hi, [](double a, double b) { return fmax(a, b); });
-  lo = over_head<LPH>(lo, [](double a, double b) { return fmin(a, b); });
+  const double hi = over_head<LPH>(mine ? most : Real(-65504), [](Real a, Real b) { return fmax(a, b); });
+  const double lo = over_head<LPH>(mine ? least : Real(65504), [](Real a, Real b) { return fmin(a, b); });
   const int lane = __lane_id();
   nan = ((__ballot(nan && mine) >> (lane & ~(LPH - 1))) & ((1ull << LPH) - 1)) != 0;
   const uint32_t sb = half_of((hi - lo) / 15.0);
@@ -155,13 +154,15 @@ __device__ __forceinline__ void quantize_head(Runs<double, NPL>& v, bool mine, u
   const uint32_t ob = half_of(fma(8.0, scale, lo));
   const double offset = f16_bits_to_f32(ob), inv = scale == 0.0 || nan ? 0.0 : 1.0 / scale;
   // A quotient that is a half exactly has to come out as one: the product with the reciprocal is off by 2^-52 of it, and adding
-  // and subtracting 3 2^11 rounds it to a multiple of 2^-40.
+  // and subtracting 3 2^11 rounds it to a multiple of 2^-40.  Then 3 2^51 + 8 brings 8 and the nearest integer, ties to even, into
+  // the low word (quotients are below 2^30: an offset is off by at most 16, a scale at least 2^-24).
 #pragma unroll
   for (int j = 0; j < 2 * NPL; ++j) {
-    double t = (v.x[j / NPL][j % NPL] - offset) * inv;
-    t = (t + 6144.0) - 6144.0;
-    const int r = static_cast<int>(rint(t));
-    code[j / NPL][j % NPL] = static_cast<uint32_t>((r < -8 ? -8 : r > 7 ? 7 : r) + 8);
+    double t = (static_cast<double>(v.x[j / NPL][j % NPL]) - offset) * inv;
+    t = ((t + 6144.0) - 6144.0) + 6755399441055752.0;
+    uint32_t word[2];
+    __builtin_memcpy(word, &t, 8);
+    code[j / NPL][j % NPL] = static_cast<uint32_t>(min(max(static_cast<int>(word[0]), 0), 15));
   }
   *scale_bits = nan ? 0x7e00u : sb;
   *offset_bits = nan ? 0x7e00u : ob;
@@ -177,9 +178,9 @@ __device__ __forceinline__ void quantize_head(Runs<double, NPL>& v, bool mine, u
 // shared prefix, a resumed sequence) has the same codes then, whichever way the arithmetic is ordered.
 //
 // Norm and rotation of 8192 tokens (32 heads and 8 of 128, bfloat16, 168 MB read and written) take 43 us, 3.9 TB/s, where a copy
-// has 5.1.  Appending them takes 32 us for the queries (4.2 TB/s) and 35 for keys and values, 34 MB and 9 MB of cache:
-// there the 64-bit instructions are what is waited for, with two wavefronts a SIMD to hide their latency (one token: 4 to 5 us, launch
-// and one chain of loads).
+// has 5.1.  Appending them takes 31 us for the queries (4.3 TB/s) and 34 for keys and values, 34 MB and 9 MB of cache: there a
+// SIMD's two wavefronts issue some 700 instructions for 16 dimensions a lane, a quarter of them in 64 bits, and that is what is
+// waited for.  One token takes 4 to 5 us: a launch and one chain of loads.
 //
 // Wavefronts a SIMD: what registers allow without spills.  Measured, 8192 tokens, in us: appending bfloat16 2 : 3 76 : 105, fp32
 // 3 : 4 119 : 111; norm and rotation bfloat16 3 : 4 : 6 43 : 43 : 77, fp32 3 : 4 : 6 : 8 73 : 71 : 76 : 110.
@@ -294,6 +295,9 @@ __global__ __launch_bounds__(256, occupancy_of(NPL, VEC, APPEND)) void heads_ker
   int64_t token = begin / A.passes;
   int pass = static_cast<int>(begin - token * A.passes);
   Pass now = pass_of(token, pass, raw);
+  double freq[2];
+#pragma unroll
+  for (int n = 0; n < 2; ++n) freq[n] = lane + 64 * n < half_rot ? A.freqs[lane + 64 * n] : 0.0;
   float weight[2][NPL];
   int64_t turned = -1;  // the token that lds_turns is for
   int weights_of = -1;
@@ -316,8 +320,11 @@ __global__ __launch_bounds__(256, occupancy_of(NPL, VEC, APPEND)) void heads_ker
       turned = now.token;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
-      for (int pair = lane; pair < half_rot; pair += 64) {
-        const double t = static_cast<double>(now.position) * A.freqs[pair];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int pair = lane + 64 * n;
+        if (pair >= half_rot) break;
+        const double t = static_cast<double>(now.position) * freq[n];
         double c, s;
         turn(t - rint(t), A.p.attention_factor, &c, &s);
         lds_turns[wave][pair][0] = static_cast<Angle>(c);
@@ -339,17 +346,21 @@ __global__ __launch_bounds__(256, occupancy_of(NPL, VEC, APPEND)) void heads_ker
       const int64_t st = now.role == kQueries ? A.p.q_out_strides[0] : A.p.k_out_strides[0], sh = now.role == kQueries ? A.p.q_out_strides[1] : A.p.k_out_strides[1];
       if (now.there) store(now.role == kQueries ? A.q_out : A.k_out, now.token * st + now.head * sh, v);
     } else if constexpr (APPEND) {
-      Runs<double, NPL> v;
-      widen(raw, v);
+      uint32_t code[2][NPL], scale_bits, offset_bits;
       if (now.role == kKeys) {
+        Runs<double, NPL> v;
+        widen(raw, v);
         if (w != nullptr) norm<LPH>(A, v, weight);
         rotate<VEC, NPL, double>(v, !VEC || split, rotated, turn_of);
+        quantize_head<LPH, NPL>(v, mine, &scale_bits, &offset_bits, code);
+      } else {
+        Runs<float, NPL> v;
+        widen(raw, v);
+        quantize_head<LPH, NPL>(v, mine, &scale_bits, &offset_bits, code);
       }
       const bool placed = now.slot >= 0 && now.slot < A.num_slots;
       const int64_t slot = placed ? now.slot : 0, page_at = (slot >> A.page_shift) * A.page_bytes;
       now.there = now.there && placed;
-      uint32_t code[2][NPL], scale_bits, offset_bits;
-      quantize_head<LPH, NPL>(v, mine, &scale_bits, &offset_bits, code);
       const Kv4Block block{A.page_size, A.dp};
       uint8_t* to = A.cache + page_at + static_cast<int64_t>(now.head) * block.bytes();
       const int place = static_cast<int>(slot & (A.page_size - 1));
