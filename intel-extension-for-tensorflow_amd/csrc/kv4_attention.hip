@@ -13,7 +13,7 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 
-constexpr int kMostSplitRows = 64;     // rows of a sequence, times heads of a kv head, that split kernels take
+constexpr int kMostSplitRows = 64;     // rows of a sequence, times heads of a kv head, that split kernels always take
 constexpr int kMostGroups = 1024;      // workgroups of a split kernel
 // Copies of the rows in a tile's 16 columns, see Engine; tokens that a workgroup of four wavefronts takes at a time
 constexpr int copies_of(bool f32, int64_t rows) { return f32 || rows > 8 ? 1 : rows > 4 ? 2 : 4; }
@@ -109,7 +109,9 @@ constexpr int occupancy_of(int nb, int dp, bool f32) { return dp == 256 ? 1 : nb
 // repeated COPIES times instead, and copy b of the columns (the lanes' `block`) has the softmax of tile b only: its lanes take their
 // scores from that tile's product, and put zeros into the other tiles' places of the second product.  Both products are what they were;
 // of the vector instructions those for scales, exponentials and sums are a COPIES-th a token.  The copies' maxima are
-// kept alike, their sums are added at the end.
+// kept alike, their sums are added at the end.  (64 sequences of up to 8192 tokens, 4 rows: 87 us without copies, 80 with four.)
+//
+// Codes are read once by one workgroup: nontemporal loads leave the caches to the rest (80 us for 91).
 template <int T, int DP, int NB, int COPIES>
 struct Engine {
   static constexpr bool F32 = T == ITEXHIP_FLOAT;
@@ -618,6 +620,12 @@ struct Engine {
 // row, [sequence][kv head][tile][step], are cut into equal shares, one a workgroup, whatever the lengths are and without the host
 // knowing them.  A share may end one (sequence, head), hold several whole ones and begin another: whole ones are written out,
 // the two at its ends leave their sums in the workspace for combine_kernel.
+//
+// What bounds it: 64 sequences of up to 8192 tokens (8 kv heads of 128, 378 MB) take 80 us with combine_kernel, 4.7 TB/s, where a copy
+// has 5.1 and a launch that only reads 6.9: vector instructions are issued for 59 % of the time (and-or, shift and subtraction of
+// the codes: 144 for 64 tokens of a wavefront's 400), matrix instructions for 15 %.  Loads two steps ahead instead of one: 85 us.  One
+// sequence of 131072 tokens (143 MB) takes 35 us.  One of 2000 takes 14, a chain of latencies: 10 us for lengths, pages, the
+// first codes and the sums of four wavefronts, 4 for the second launch.
 template <int NB>
 __device__ __forceinline__ int tiles_of(const AttArgs& A, const Seq& s) { return (s.n * A.group + 16 * NB - 1) / (16 * NB); }
 template <int T, int DP, int NB, int COPIES>
@@ -768,7 +776,9 @@ __global__ __launch_bounds__(256, occupancy_of(NB, DP, T == ITEXHIP_FLOAT)) void
   }
 }
 
-// One row of a (sequence, kv head) that several workgroups shared: their sums, in the order of the tokens
+// One row of a (sequence, kv head) that several workgroups shared: their sums, in the order of the tokens, so that equal calls give equal
+// bits.  All partial maxima and sums are read at once by as many threads, then the outputs by groups of DP / 4 (one thread going
+// through them: 54 us for a sequence of 131072 tokens where this took 39); 4 to 6 us, most of it the launch.
 template <int T, int DP, int NB, int COPIES>
 __global__ __launch_bounds__(256) void combine_kernel(const AttArgs A) {
   constexpr int STEP = step_of(COPIES);
@@ -837,7 +847,9 @@ __global__ __launch_bounds__(256) void combine_kernel(const AttArgs A) {
   for (int j = 0; j < 4; ++j) store_output<T>(A.out, to + j, o[j] * inv);
 }
 
-// Sequences of more rows: a wavefront takes 16 NB rows through all the tokens that they see
+// Sequences of more rows in fp32: a wavefront takes 16 NB rows through all the tokens that they see, codes straight from the caches to its
+// registers.  fp32 MFMAs (a 16th of half's rate) and a conversion for every code they take bound it: 2048 tokens, 32 heads
+// over 8 of 128, 690 us, 50 TFLOP/s.
 template <int T, int DP, int NB>
 __global__ __launch_bounds__(256) void rows_kernel(const AttArgs A) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), b = blockIdx.z, head = blockIdx.y;
@@ -871,6 +883,12 @@ __global__ __launch_bounds__(256) void rows_kernel(const AttArgs A) {
 //
 // LDS holds a fragment as 64 lanes of 16 bytes.  Keys: [32 tokens][16 dimensions], lane 32 h + token: dimensions 8 h .. 8 h + 7 in the
 // order of key_operand.  Values: [16 tokens][32 dimensions], lane 32 h + dimension: tokens 4 h .. 4 h + 3 and 8 + 4 h .. + 3.
+//
+// What bounds it: 8192 tokens, 32 heads over 8 kv heads of 128, bfloat16, take 720 us, 760 TFLOP/s of the two products.  The matrix cores
+// are busy for a third of that, vector instructions are issued for half of it (a scale, an exponential, a sum and a conversion for
+// each score), and a wavefront does one after the other: two on a SIMD overlap them in part.  Measured and slower: four wavefronts of
+// 32 rows (995), 64 rows a wavefront (1100), three wavefronts a SIMD (spills, 1280), the products pinned between the vector
+// instructions (737), staging by half the wavefronts (730), raised wave priorities (757).
 //
 // A wavefront stages tokens of one group of 16 at a time, which lie in one page: page and addresses are scalar.
 template <int DP> constexpr int kTile = DP == 256 ? 32 : 64;
@@ -1245,13 +1263,33 @@ struct Plan {
   size_t prefix, ml, o, bytes;
 };
 
+// Of more than kMostSplitRows rows, whether the tokens are divided (split_kernel) or the rows alone (prompt_kernel, rows_kernel).  Those
+// give a workgroup one tile of rows and all the tokens, and leave CUs idle where there are few tiles: as long as each has a CU of its own, the
+// time is that of one, 20 us and so much a token of the longest sequence.  split_kernel's is 25 us and so much a row and token, and
+// what combine_kernel takes for a row.  In us, 8 kv heads of 128 and 4 query heads each but where noted, rows alone : tokens
+// divided, a chunk of
+//   half, bfloat16  16 x 17 rows of 4096 tokens 142 : 60, 64 of 16384 599 : 56, 512 of 16384 632 : 269, 4 x 128 of 4096 177 : 101,
+//                   300 of 300 34 : 45, 1000 of 1000 62 : 99; heads of 256: 128 of 16384 1179 : 191
+//   fp32            128 of 4096 675 : 113, 4 x 128 of 4096 675 : 304, 512 of 4096 676 : 366; 12 heads of 64: 2048 of 2048 197 : 189
+// The longest sequence is the table's width (the host knows no lengths) or what a window leaves of it.
+bool tokens_are_divided(const itexhip_kv4_attention_params* p, const itexhip_kv4_cache* c, int64_t rows, int dp) {
+  const bool f32 = p->type == ITEXHIP_FLOAT;
+  const int64_t tile = f32 ? (dp == 256 ? 64 : 128) : dp == 256 ? 128 : 256, all = static_cast<int64_t>(p->num_seqs) * c->kv_heads;
+  if ((rows + tile - 1) / tile * all > 256) return false;
+  double tokens = static_cast<double>(p->table_stride) * c->page_size;
+  if (p->window > 0) tokens = fmin(tokens, static_cast<double>(p->window) + p->max_q_len);
+  const double by_rows = 20.0 + tokens * (f32 ? 0.165 : dp == 256 ? 0.072 : 0.0366);
+  const double divided = 25.0 + static_cast<double>(rows * all) * (tokens * (f32 ? 5.6e-6 : 1.1e-6) + 1.0 / 600.0);
+  return divided < by_rows;
+}
+
 Plan plan_of(const itexhip_kv4_attention_params* p, const itexhip_kv4_cache* c) {
   Plan plan = {};
   const int dp = kv4_padded(c->head_dim);
   const int64_t rows = static_cast<int64_t>(p->max_q_len) * (p->q_heads / c->kv_heads);
   plan.blocks = rows <= 16 || dp == 256 ? 1 : 2;
   plan.copies = copies_of(p->type == ITEXHIP_FLOAT, rows);
-  plan.split = rows <= kMostSplitRows;
+  plan.split = rows <= kMostSplitRows || tokens_are_divided(p, c, rows, dp);
   if (plan.split) {
     const int step = step_of(plan.copies);
     const int64_t bound = static_cast<int64_t>(p->num_seqs) * c->kv_heads * ((p->table_stride * c->page_size + step - 1) / step) * ((rows + 16 * plan.blocks - 1) / (16 * plan.blocks));

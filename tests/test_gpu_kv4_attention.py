@@ -74,6 +74,12 @@ def attend(hip, dev, name, batch, causal=True, window=0, rows_behind=3, scale=No
     return out[:rows].cpu(), lse[:rows].cpu(), q
 
 
+@pytest.fixture(params=[None, 100000], ids=["", "rows_alone"])
+def max_q(request):
+    """Of 100000 rows a sequence there are tiles for all CUs: the kernels that divide rows alone run, whatever the sequences then have."""
+    return request.param
+
+
 def check(out, lse, q, batch, causal=True, window=0, scale=None):
     d = batch.d
     scale = d ** -0.5 if scale is None else scale
@@ -122,10 +128,10 @@ RAGGED = [(3, 40), (1, 1), (5, 5), (0, 33), (2, 129), (7, 200), (4, 17), (1, 64)
 @pytest.mark.parametrize("name", list(TYPES))
 @pytest.mark.parametrize("heads,group,d,page,window", [(2, 4, 128, 16, 0), (1, 8, 64, 32, 0), (2, 1, 80, 16, 20), (1, 9, 256, 64, 0), (1, 3, 128, 16, 7), (1, 5, 64, 16, 0)])
 @pytest.mark.parametrize("causal", [True, False])
-def test_several_tokens(hip, dev, name, heads, group, d, page, window, causal):
+def test_several_tokens(hip, dev, max_q, name, heads, group, d, page, window, causal):
     """1 to 63 rows a sequence and kv head: the split kernels in one tile and several."""
     batch = Batch(RAGGED, heads, group, d, page, 3)
-    check(*attend(hip, dev, name, batch, causal=causal, window=window), batch, causal=causal, window=window)
+    check(*attend(hip, dev, name, batch, max_q=max_q, causal=causal, window=window), batch, causal=causal, window=window)
 
 
 PROMPTS = [(70, 70), (1, 90), (33, 150), (0, 10), (129, 129), (64, 64), (40, 41)]
@@ -134,25 +140,33 @@ PROMPTS = [(70, 70), (1, 90), (33, 150), (0, 10), (129, 129), (64, 64), (40, 41)
 @pytest.mark.parametrize("name", list(TYPES))
 @pytest.mark.parametrize("heads,group,d,page,window,causal", [(2, 2, 128, 16, 0, True), (1, 4, 64, 32, 0, True), (1, 1, 80, 16, 0, True), (1, 3, 256, 64, 0, True), (1, 2, 128, 16, 30, True),
                                                               (1, 2, 64, 64, 0, False), (1, 2, 200, 16, 50, True), (2, 1, 128, 128, 65, False), (1, 5, 8, 16, 0, True)])
-def test_prompts(hip, dev, name, heads, group, d, page, window, causal):
+def test_prompts(hip, dev, max_q, name, heads, group, d, page, window, causal):
     batch = Batch(PROMPTS, heads, group, d, page, 4)
-    check(*attend(hip, dev, name, batch, causal=causal, window=window), batch, causal=causal, window=window)
+    check(*attend(hip, dev, name, batch, max_q=max_q, causal=causal, window=window), batch, causal=causal, window=window)
+
+
+@pytest.mark.parametrize("name", list(TYPES))
+@pytest.mark.parametrize("heads,group,d,page,window,causal", [(2, 4, 128, 16, 0, True), (1, 2, 64, 64, 0, False), (1, 4, 256, 32, 0, True), (2, 3, 80, 16, 300, True)])
+def test_chunks_behind_long_contexts(hip, dev, max_q, name, heads, group, d, page, window, causal):
+    """Hundreds of rows of few sequences: the tokens are divided among workgroups."""
+    batch = Batch([(100, 2000), (150, 700), (0, 5), (3, 1500)], heads, group, d, page, 15)
+    check(*attend(hip, dev, name, batch, max_q=max_q, causal=causal, window=window), batch, causal=causal, window=window)
 
 
 @pytest.mark.parametrize("name", list(TYPES))
 @pytest.mark.parametrize("q_rows", [1, 9, 80])
-def test_rows_that_see_nothing(hip, dev, name, q_rows):
+def test_rows_that_see_nothing(hip, dev, max_q, name, q_rows):
     """More new tokens than tokens, sequences without any, none of them: 0 and lse -inf."""
     batch = Batch([(q_rows, 0), (q_rows, q_rows // 2), (1, 0), (q_rows, q_rows + 3), (0, 0)], 2, 2, 64, 16, 5)
-    check(*attend(hip, dev, name, batch), batch)
-    check(*attend(hip, dev, name, batch, causal=False), batch, causal=False)
+    check(*attend(hip, dev, name, batch, max_q=max_q), batch)
+    check(*attend(hip, dev, name, batch, max_q=max_q, causal=False), batch, causal=False)
     batch = Batch([(q_rows, 0)], 1, 1, 128, 16, 5)
-    check(*attend(hip, dev, name, batch), batch)
+    check(*attend(hip, dev, name, batch, max_q=max_q), batch)
 
 
 @pytest.mark.parametrize("name", list(TYPES))
 @pytest.mark.parametrize("lens", [[(1, 100), (1, 60)], [(4, 100), (2, 60)], [(80, 100), (1, 60)]])
-def test_nan_reaches_only_the_rows_that_see_it(hip, dev, name, lens):
+def test_nan_reaches_only_the_rows_that_see_it(hip, dev, max_q, name, lens):
     for which in (0, 1):
         batch = Batch(lens, 2, 2, 64, 16, 6)
         first, second = batch.table[0], batch.table[1]
@@ -160,7 +174,7 @@ def test_nan_reaches_only_the_rows_that_see_it(hip, dev, name, lens):
         batch.cache.scale[which, slot, 1] = batch.cache.offset[which, slot, 1] = math.nan
         early = second[3 // 16] * 16 + 3
         batch.cache.scale[which, early, 0] = batch.cache.offset[which, early, 0] = math.nan
-        out, lse, q = attend(hip, dev, name, batch)
+        out, lse, q = attend(hip, dev, name, batch, max_q=max_q)
         n = lens[0][0]
         assert bool(torch.isnan(out[:n, 2:]).any()) and not bool(torch.isnan(out[:n, :2]).any())
         want, want_lse, _ = ref.attention(q, batch.cache, batch.table, batch.cu, [100, 60], 64 ** -0.5)
@@ -177,12 +191,12 @@ def test_nan_reaches_only_the_rows_that_see_it(hip, dev, name, lens):
 
 @pytest.mark.parametrize("name", list(TYPES))
 @pytest.mark.parametrize("lens", [[(1, 200)], [(6, 200)], [(90, 200)]])
-def test_pages_outside_the_cache_are_not_seen(hip, dev, name, lens):
+def test_pages_outside_the_cache_are_not_seen(hip, dev, max_q, name, lens):
     batch = Batch(lens, 1, 2, 128, 32, 7)
     batch.table[0][1] = -1
     batch.table[0][3] = batch.cache.pages
     batch.table[0][4] = 2 ** 31 - 1
-    check(*attend(hip, dev, name, batch), batch)
+    check(*attend(hip, dev, name, batch, max_q=max_q), batch)
 
 
 @pytest.mark.parametrize("name", list(TYPES))
@@ -231,7 +245,7 @@ def test_long_contexts_shared_by_many_workgroups(hip, dev, name, heads, group, d
 
 
 @pytest.mark.parametrize("name", ["bfloat16", "half", "float"])
-def test_rising_scores_and_scales(hip, dev, name):
+def test_rising_scores_and_scales(hip, dev, max_q, name):
     """Maxima that grow step by step, values whose scales grow over 2^20, rows of very different size: the sums are rescaled."""
     batch = Batch([(1, 400), (3, 400), (100, 400)], 1, 2, 64, 16, 11)
     for b in range(3):
@@ -241,11 +255,11 @@ def test_rising_scores_and_scales(hip, dev, name):
             batch.cache.scale[1, slot] = torch.tensor(2.0 ** (-18 + t // 20)).double()
             batch.cache.offset[1, slot] = torch.tensor(2.0 ** (-16 + t // 20)).double()
     batch.q *= torch.logspace(-3, 1, batch.cu[-1])[:, None, None]
-    check(*attend(hip, dev, name, batch), batch)
+    check(*attend(hip, dev, name, batch, max_q=max_q), batch)
 
 
 @pytest.mark.parametrize("name", ["bfloat16", "half"])
-def test_queries_beyond_halves(hip, dev, name):
+def test_queries_beyond_halves(hip, dev, max_q, name):
     """bfloat16 queries far outside half's range, zero queries, tiny softmax scales."""
     batch = Batch([(1, 50), (2, 50), (70, 90)], 1, 2, 64, 16, 12)
     big = 1e30 if name == "bfloat16" else 6e4
@@ -254,7 +268,7 @@ def test_queries_beyond_halves(hip, dev, name):
     batch.q[5] *= 1e-30 if name == "bfloat16" else 1e-6
     q = batch.q.to(TYPES[name])
     for scale in (1.0 / big, 1e-38, 0.125 if name == "half" else 1e-30):
-        out, lse, _ = attend(hip, dev, name, batch, scale=scale, q=q)
+        out, lse, _ = attend(hip, dev, name, batch, max_q=max_q, scale=scale, q=q)
         want, want_lse, mass = ref.attention(q, batch.cache, batch.table, batch.cu, [n for _, n in batch.lens], scale)
         assert bool(torch.isfinite(out).all())
         if scale != 0.125:
