@@ -931,7 +931,11 @@ __global__ __launch_bounds__(64 * kWaves<DP>, kWaves<DP> / 4) void prompt_kernel
     for (int kk = 0; kk < KK; ++kk) {
       const int d0 = kk * 16 + hi * 8;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[kk][j] = in && d0 < A.head_dim ? load_q<T>(A.q, at + d0 + j) : 0.0f;
+      for (int j = 0; j < 8; ++j) x[kk][j] = 0.0f;
+      if (in && d0 < A.head_dim) {  // (a branch around all eight: they become one load)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[kk][j] = load_q<T>(A.q, at + d0 + j);
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[kk][j]));
     }
