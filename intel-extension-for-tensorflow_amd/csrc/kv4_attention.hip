@@ -624,7 +624,7 @@ struct Engine {
 // What bounds it: 64 sequences of up to 8192 tokens (8 kv heads of 128, 378 MB) take 80 us with combine_kernel, 4.7 TB/s, where a copy
 // has 5.1 and a launch that only reads 6.9: vector instructions are issued for 59 % of the time (and-or, shift and subtraction of
 // the codes: 144 for 64 tokens of a wavefront's 400), matrix instructions for 15 %.  Loads two steps ahead instead of one: 85 us.  One
-// sequence of 131072 tokens (143 MB) takes 35 us.  One of 2000 takes 14, a chain of latencies: 10 us for lengths, pages, the
+// sequence of 131072 tokens (143 MB) takes 34 us.  One of 2000 takes 13, a chain of latencies: 9 us for lengths, pages, the
 // first codes and the sums of four wavefronts, 4 for the second launch.
 template <int NB>
 __device__ __forceinline__ int tiles_of(const AttArgs& A, const Seq& s) { return (s.n * A.group + 16 * NB - 1) / (16 * NB); }
@@ -657,35 +657,47 @@ __global__ __launch_bounds__(256, occupancy_of(NB, DP, T == ITEXHIP_FLOAT)) void
     for (int w = 0; w < wave; ++w) x += scan[w];
     inclusive = x;
   };
-  int64_t total = 0, inclusive, all;
-  for (int base = 0; base < A.num_seqs; base += 256) {
-    prefix_of(base, inclusive, all);
-    total += all;
-  }
-  const int64_t share = (total + gridDim.x - 1) / gridDim.x;
-  const int64_t begin = share * blockIdx.x, end = begin + share < total ? begin + share : total;
-  if (tid == 0) found[0] = -1;
-  int64_t before = 0;
-  for (int base = 0; base < A.num_seqs; base += 256) {
-    if (base > 0 || A.num_seqs > 256) prefix_of(base, inclusive, all);
-    const int b = base + tid;
-    __syncthreads();
-    if (b < A.num_seqs) {
-      const Seq s = sequence<STEP>(A, b);
-      const int64_t mine = s.steps * A.kv_heads * tiles_of<NB>(A, s), from = before + inclusive - mine;
-      if (begin >= from && begin < from + mine) {
-        found[0] = b;
-        found[1] = from;
-      }
-      if (blockIdx.x == 0) A.prefix[b] = from;
+  int b = 0;
+  int64_t total = 0, from = 0, share, begin, end;
+  auto cut = [&] {
+    share = (total + gridDim.x - 1) / gridDim.x;
+    begin = share * blockIdx.x;
+    end = begin + share < total ? begin + share : total;
+  };
+  if (A.num_seqs == 1) {  // nothing to look for
+    const Seq s = sequence<STEP>(A, 0);
+    total = s.steps * A.kv_heads * tiles_of<NB>(A, s);
+    cut();
+    if (blockIdx.x == 0 && tid == 0) A.prefix[0] = 0;
+  } else {
+    int64_t inclusive, all, before = 0;
+    for (int base = 0; base < A.num_seqs; base += 256) {
+      prefix_of(base, inclusive, all);
+      total += all;
     }
-    before += all;
+    cut();
+    if (tid == 0) found[0] = -1;
+    for (int base = 0; base < A.num_seqs; base += 256) {
+      if (A.num_seqs > 256) prefix_of(base, inclusive, all);
+      const int at = base + tid;
+      __syncthreads();
+      if (at < A.num_seqs) {
+        const Seq s = sequence<STEP>(A, at);
+        const int64_t mine = s.steps * A.kv_heads * tiles_of<NB>(A, s), first = before + inclusive - mine;
+        if (begin >= first && begin < first + mine) {
+          found[0] = at;
+          found[1] = first;
+        }
+        if (blockIdx.x == 0) A.prefix[at] = first;
+      }
+      before += all;
+    }
+    __syncthreads();
+    b = static_cast<int>(found[0]);
+    from = found[1];
   }
   if (blockIdx.x == 0 && tid == 0) A.prefix[A.num_seqs] = share;
-  __syncthreads();
   if (begin >= end) return;
-  int b = static_cast<int>(found[0]);
-  int64_t from = found[1];
 
   for (int64_t at = begin; at < end;) {
     const Seq s = sequence<STEP>(A, b);
@@ -884,11 +896,12 @@ __global__ __launch_bounds__(256) void rows_kernel(const AttArgs A) {
 // LDS holds a fragment as 64 lanes of 16 bytes.  Keys: [32 tokens][16 dimensions], lane 32 h + token: dimensions 8 h .. 8 h + 7 in the
 // order of key_operand.  Values: [16 tokens][32 dimensions], lane 32 h + dimension: tokens 4 h .. 4 h + 3 and 8 + 4 h .. + 3.
 //
-// What bounds it: 8192 tokens, 32 heads over 8 kv heads of 128, bfloat16, take 720 us, 760 TFLOP/s of the two products.  The matrix cores
+// What bounds it: 8192 tokens, 32 heads over 8 kv heads of 128, bfloat16, take 675 to 700 us, 790 to 815 TFLOP/s of the two products.  The matrix cores
 // are busy for a third of that, vector instructions are issued for half of it (a scale, an exponential, a sum and a conversion for
 // each score), and a wavefront does one after the other: two on a SIMD overlap them in part.  Measured and slower: four wavefronts of
 // 32 rows (995), 64 rows a wavefront (1100), three wavefronts a SIMD (spills, 1280), the products pinned between the vector
-// instructions (737), staging by half the wavefronts (730), raised wave priorities (757).
+// instructions (737), staging by half the wavefronts (730), raised wave priorities (757), each beside 720 to 740 of its day; queries by single
+// elements cost every call 11 us.
 //
 // A wavefront stages tokens of one group of 16 at a time, which lie in one page: page and addresses are scalar.
 template <int DP> constexpr int kTile = DP == 256 ? 32 : 64;
@@ -1269,12 +1282,13 @@ struct Plan {
 
 // Of more than kMostSplitRows rows, whether the tokens are divided (split_kernel) or the rows alone (prompt_kernel, rows_kernel).  Those
 // give a workgroup one tile of rows and all the tokens, and leave CUs idle where there are few tiles: as long as each has a CU of its own, the
-// time is that of one, 20 us and so much a token of the longest sequence.  split_kernel's is 25 us and so much a row and token, and
+// time is that of one, 9 us and so much a token of the longest sequence.  split_kernel's is 25 us and so much a row and token, and
 // what combine_kernel takes for a row.  In us, 8 kv heads of 128 and 4 query heads each but where noted, rows alone : tokens
 // divided, a chunk of
-//   half, bfloat16  16 x 17 rows of 4096 tokens 142 : 60, 64 of 16384 599 : 56, 512 of 16384 632 : 269, 4 x 128 of 4096 177 : 101,
-//                   300 of 300 34 : 45, 1000 of 1000 62 : 99; heads of 256: 128 of 16384 1179 : 191
-//   fp32            128 of 4096 675 : 113, 4 x 128 of 4096 675 : 304, 512 of 4096 676 : 366; 12 heads of 64: 2048 of 2048 197 : 189
+//   half, bfloat16  16 x 17 rows of 4096 tokens 137 : 60, 64 of 16384 590 : 54, 512 of 16384 622 : 264, 4 x 128 of 4096 166 : 101, 100 of 2000
+//                   87 : 33, 2 x 200 of 1000 52 : 62, 300 of 300 23 : 45, 1000 of 1000 51 : 100, 1000 of 4096 173 : 216; heads of 256:
+//                   128 of 16384 1152 : 185; 12 heads of 64: 4 x 128 of 1024 37 : 30, 512 of 512 25 : 29
+//   fp32            128 of 4096 672 : 112, 4 x 128 of 4096 678 : 302, 512 of 4096 677 : 362; 12 heads of 64: 512 of 512 55 : 34, 2048 of 2048 194 : 188
 // The longest sequence is the table's width (the host knows no lengths) or what a window leaves of it.
 bool tokens_are_divided(const itexhip_kv4_attention_params* p, const itexhip_kv4_cache* c, int64_t rows, int dp) {
   const bool f32 = p->type == ITEXHIP_FLOAT;
@@ -1282,7 +1296,7 @@ bool tokens_are_divided(const itexhip_kv4_attention_params* p, const itexhip_kv4
   if ((rows + tile - 1) / tile * all > 256) return false;
   double tokens = static_cast<double>(p->table_stride) * c->page_size;
   if (p->window > 0) tokens = fmin(tokens, static_cast<double>(p->window) + p->max_q_len);
-  const double by_rows = 20.0 + tokens * (f32 ? 0.165 : dp == 256 ? 0.072 : 0.0366);
+  const double by_rows = 9.0 + tokens * (f32 ? 0.165 : dp == 256 ? 0.072 : 0.0366);
   const double divided = 25.0 + static_cast<double>(rows * all) * (tokens * (f32 ? 5.6e-6 : 1.1e-6) + 1.0 / 600.0);
   return divided < by_rows;
 }
