@@ -178,12 +178,12 @@ __device__ __forceinline__ void quantize_head(Runs<Real, NPL>& v, bool mine, uin
 // shared prefix, a resumed sequence) has the same codes then, whichever way the arithmetic is ordered.
 //
 // Norm and rotation of 8192 tokens (32 heads and 8 of 128, bfloat16, 168 MB read and written) take 43 us, 3.9 TB/s, where a copy
-// has 5.1.  Appending them takes 31 us for the queries (4.3 TB/s) and 34 for keys and values, 34 MB and 9 MB of cache: there a
-// SIMD's two wavefronts issue some 700 instructions for 16 dimensions a lane, a quarter of them in 64 bits, and that is what is
-// waited for.  One token takes 4 to 5 us: a launch and one chain of loads.
+// has 5.1.  Appending them takes 31 us for the queries (4.3 TB/s) and 32 for keys and values, 34 MB and 9 MB of cache: there a
+// SIMD's two wavefronts issue 500 vector instructions for a pass of 16 dimensions a lane, a good part of them in 64 bits, which is half
+// of the time, and wait for the other half.  One token takes 4 to 5 us: a launch and one chain of loads.
 //
-// Wavefronts a SIMD: what registers allow without spills.  Measured, 8192 tokens, in us: appending bfloat16 2 : 3 76 : 105, fp32
-// 3 : 4 119 : 111; norm and rotation bfloat16 3 : 4 : 6 43 : 43 : 77, fp32 3 : 4 : 6 : 8 73 : 71 : 76 : 110.
+// Wavefronts a SIMD: what registers allow without spills, or as nearly.  Measured, 8192 tokens, in us: appending bfloat16 2 : 3 72.6 : 72.2
+// (and more for few tokens), fp32 3 : 4 119 : 111; norm and rotation bfloat16 3 : 4 : 6 43 : 43 : 77, fp32 3 : 4 : 6 : 8 73 : 71 : 76 : 110.
 constexpr int occupancy_of(int npl, bool vec, bool append) { return !append ? 4 : npl == 8 ? 2 : vec ? 4 : 3; }
 // Passes a wavefront from which an append's queries go through a launch of their own, which has more wavefronts and no 64-bit
 // registers: one launch : two, bfloat16 at 6 passes 24 : 26 us, 12 40 : 38, 18 67 : 59, 24 86 : 76; fp32 at 12 60 : 63, 24 113 : 111
@@ -285,9 +285,12 @@ __global__ __launch_bounds__(256, occupancy_of(NPL, VEC, APPEND)) void heads_ker
     const int64_t sh = q.role == kQueries ? A.p.q_strides[1] : q.role == kKeys ? A.p.k_strides[1] : A.p.v_strides[1];
     q.head = (pass - first) * (64 / LPH) + group;
     q.there = q.head < heads;  // lanes beyond the last head run along on its values and store nothing
-    q.position = half_rot > 0 ? A.positions[token] : 0;
+    // by vector loads: the next wait for LDS would be a wait for a scalar one too, a pass before it is wanted
+    int at = static_cast<int>(token);
+    asm("" : "+v"(at));
+    q.position = half_rot > 0 ? A.positions[at] : 0;
     q.slot = 0;
-    if constexpr (APPEND) q.slot = A.slots[token];
+    if constexpr (APPEND) q.slot = A.slots[at];
     load(q.role == kQueries ? A.q : q.role == kKeys ? A.k : A.v, token * st + (q.there ? q.head : heads - 1) * sh, to);
     return q;
   };
@@ -358,8 +361,10 @@ __global__ __launch_bounds__(256, occupancy_of(NPL, VEC, APPEND)) void heads_ker
         widen(raw, v);
         quantize_head<LPH, NPL>(v, mine, &scale_bits, &offset_bits, code);
       }
-      const bool placed = now.slot >= 0 && now.slot < A.num_slots;
-      const int64_t slot = placed ? now.slot : 0, page_at = (slot >> A.page_shift) * A.page_bytes;
+      const int64_t its = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(now.slot >> 32))) << 32 |
+                          static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(now.slot)));
+      const bool placed = its >= 0 && its < A.num_slots;
+      const int64_t slot = placed ? its : 0, page_at = (slot >> A.page_shift) * A.page_bytes;
       now.there = now.there && placed;
       const Kv4Block block{A.page_size, A.dp};
       uint8_t* to = A.cache + page_at + static_cast<int64_t>(now.head) * block.bytes();
