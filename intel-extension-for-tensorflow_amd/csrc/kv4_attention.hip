@@ -1277,7 +1277,7 @@ struct Plan {
   int copies;
   bool split;
   int64_t groups;  // workgroups of the split kernel
-  size_t prefix, ml, o, bytes;
+  size_t prefix, ml, o;
 };
 
 // Of more than kMostSplitRows rows, whether the tokens are divided (split_kernel) or the rows alone (prompt_kernel, rows_kernel).  Those
@@ -1301,6 +1301,15 @@ bool tokens_are_divided(const itexhip_kv4_attention_params* p, const itexhip_kv4
   return divided < by_rows;
 }
 
+// Workgroups of a split kernel of `blocks` tiles of 16 rows: what the device holds, or one a step
+int64_t groups_of(const itexhip_kv4_attention_params* p, const itexhip_kv4_cache* c, int step, int blocks, int64_t rows) {
+  const int64_t full = 256 * occupancy_of(blocks, kv4_padded(c->head_dim), p->type == ITEXHIP_FLOAT);
+  const int64_t steps = static_cast<int64_t>(p->num_seqs) * c->kv_heads * ((p->table_stride * c->page_size + step - 1) / step);
+  const int64_t bound = (steps < full ? steps : full) * ((rows + 16 * blocks - 1) / (16 * blocks));
+  return bound < 1 ? 1 : bound < full ? bound : full;
+}
+size_t prefix_bytes(int num_seqs) { return (static_cast<size_t>(num_seqs) + 1) * 8 + 15 & ~size_t{15}; }
+
 Plan plan_of(const itexhip_kv4_attention_params* p, const itexhip_kv4_cache* c) {
   Plan plan = {};
   const int dp = kv4_padded(c->head_dim);
@@ -1309,16 +1318,22 @@ Plan plan_of(const itexhip_kv4_attention_params* p, const itexhip_kv4_cache* c) 
   plan.copies = copies_of(p->type == ITEXHIP_FLOAT, rows);
   plan.split = rows <= kMostSplitRows || tokens_are_divided(p, c, rows, dp);
   if (plan.split) {
-    const int step = step_of(plan.copies);
-    const int64_t bound = static_cast<int64_t>(p->num_seqs) * c->kv_heads * ((p->table_stride * c->page_size + step - 1) / step) * ((rows + 16 * plan.blocks - 1) / (16 * plan.blocks));
-    const int64_t full = 256 * occupancy_of(plan.blocks, dp, p->type == ITEXHIP_FLOAT);
-    plan.groups = bound < 1 ? 1 : bound < full ? bound : full;
-    plan.prefix = (static_cast<size_t>(p->num_seqs) + 1) * 8 + 15 & ~size_t{15};
+    plan.groups = groups_of(p, c, step_of(plan.copies), plan.blocks, rows);
+    plan.prefix = prefix_bytes(p->num_seqs);
     plan.ml = static_cast<size_t>(plan.groups) * 2 * 16 * plan.blocks * 2 * 4;
     plan.o = static_cast<size_t>(plan.groups) * 2 * 16 * plan.blocks * dp * 4;
   }
-  plan.bytes = plan.prefix + plan.ml + plan.o + 16;
   return plan;
+}
+
+// What the plan of this call and of every call of fewer sequences, rows or pages needs: which kernel takes a call goes by its own sizes, and
+// a program keeps one workspace for calls of many.
+size_t workspace_bytes(const itexhip_kv4_attention_params* p, const itexhip_kv4_cache* c) {
+  const int dp = kv4_padded(c->head_dim);
+  const int64_t rows = static_cast<int64_t>(p->max_q_len) * (p->q_heads / c->kv_heads), lone = dp == 256 ? rows : rows < 16 ? rows : 16;
+  const size_t part = 2 * 16 * static_cast<size_t>(dp + 2) * 4;
+  const size_t one = groups_of(p, c, 128, 1, lone) * part, two = rows > lone ? groups_of(p, c, 128, 2, rows) * 2 * part : 0;
+  return prefix_bytes(p->num_seqs) + (one > two ? one : two) + 16;
 }
 
 int check(const char* who, const itexhip_kv4_attention_params* p, const itexhip_kv4_cache* c) {
@@ -1387,7 +1402,7 @@ using namespace itexhip;
 
 extern "C" int64_t itexhip_kv4_attention_workspace(const itexhip_kv4_attention_params* p, const itexhip_kv4_cache* c) {
   if (check("itexhip_kv4_attention_workspace", p, c) != ITEXHIP_OK) return 0;
-  return static_cast<int64_t>(plan_of(p, c).bytes);
+  return static_cast<int64_t>(workspace_bytes(p, c));
 }
 
 extern "C" int itexhip_kv4_attention(const itexhip_kv4_attention_params* p, const itexhip_kv4_cache* c, const void* q, const void* cache,

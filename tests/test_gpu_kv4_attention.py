@@ -416,3 +416,30 @@ def test_another_device(hip):
     with torch.cuda.device(other):
         batch = Batch([(1, 20)], 1, 2, d, 16, 17)
         check(*attend(hip, other, "half", batch), batch)
+
+
+def placed(batch, b, t):
+    """The slot of a sequence's token."""
+    return batch.table[b][t // batch.cache.p] * batch.cache.p + t % batch.cache.p
+
+
+@pytest.mark.parametrize("name", list(TYPES))
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_workspace_serves_smaller_calls(hip, dev, name, d):
+    """A workspace of the largest call and what lies behind it, with calls of fewer rows, sequences and pages: prompts, chunks, single tokens."""
+    most = hip.kv4_attention_params(type_of(hip, name), 4, d, 3, 300, 1000, d ** -0.5, 60)
+    for lens in ([(1, 900), (1, 30), (1, 950)], [(4, 700), (9, 30)], [(30, 900)], [(300, 300), (2, 40)], [(70, 900)]):
+        batch = Batch(lens, 2, 2, d, 16, 23)
+        table = batch.table_tensor().to(dev)
+        geometry = hip.kv4_cache(d, 2, 16, batch.cache.pages)
+        size = hip.kv4_attention_workspace(most, geometry)
+        held = torch.full((size + 4096,), 0xa5, dtype=torch.uint8, device=dev)
+        out, lse, q = attend(hip, dev, name, batch)
+        p = hip.kv4_attention_params(type_of(hip, name), 4, d, len(lens), max(m for m, _ in lens), batch.cu[-1], d ** -0.5, table.shape[1])
+        assert hip.kv4_attention_workspace(p, geometry) <= size
+        again, lse2 = torch.empty_like(out, device=dev), torch.empty_like(lse, device=dev)
+        hip.kv4_attention(p, geometry, q.to(dev), batch.cache.pack().to(dev), table, torch.tensor(batch.cu, dtype=torch.int32, device=dev),
+                          torch.tensor([n for _, n in lens], dtype=torch.int32, device=dev), held, again, lse2)
+        torch.cuda.synchronize()
+        assert torch.equal(again.cpu(), out) and torch.equal(lse2.cpu(), lse)
+        assert bool((held[size:] == 0xa5).all())

@@ -232,3 +232,21 @@ def test_reference_quantizer_by_hand():
     assert scale.tolist() == [[1.0], [0.0]] and offset.tolist() == [[8.0], [2.0]]
     assert code.tolist() == [[0, 15, 8, 3], [8, 8, 8, 8]]      # (7.5 - 8) / 1 = -0.5 goes to even, 0
     assert ref.values(code, scale, offset).tolist() == [[0.0, 15.0, 8.0, 3.0], [2.0, 2.0, 2.0, 2.0]]
+
+
+@pytest.mark.parametrize("type", ["FLOAT", "BFLOAT16", "HALF"])
+@pytest.mark.parametrize("d,heads,group", [(64, 1, 2), (128, 8, 4), (128, 1, 1), (256, 2, 8), (80, 4, 16)])
+def test_a_workspace_serves_smaller_calls(hip, type, d, heads, group):
+    """Which kernel takes a call depends on its sizes: a prompt's may need less than a token's."""
+    c = hip.kv4_cache(d, heads, 16, 1000)
+    size = lambda seqs, rows, pages, **kw: hip.kv4_attention_workspace(
+        hip.kv4_attention_params(getattr(hip, type), heads * group, d, seqs, rows, seqs * max(rows, 1), 0.125, pages, **kw), c)
+    seqs, rows, pages = (1, 2, 64), (0, 1, 3, 5, 9, 17, 65, 90, 300, 8192, 100000), (0, 1, 19, 300, 8192)
+    sizes = {(b, m, n): size(b, m, n) for b in seqs for m in rows for n in pages}
+    for b, m, n in sizes:
+        assert sizes[b, m, n] == size(b, m, n, window=100) == size(b, m, n, causal=False)
+        for b2 in seqs:
+            for m2 in rows:
+                for n2 in pages:
+                    if b2 <= b and m2 <= m and n2 <= n:
+                        assert sizes[b2, m2, n2] <= sizes[b, m, n]
