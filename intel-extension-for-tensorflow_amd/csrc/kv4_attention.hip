@@ -1350,7 +1350,7 @@ int check(const char* who, const itexhip_kv4_attention_params* p, const itexhip_
   ITEXHIP_REQUIRE(p->total_q >= 0 && p->total_q < (1ll << 31), "%s: total_q is 0 to 2^31 - 1", who);
   ITEXHIP_REQUIRE(p->scale > 0.0f && isfinite(p->scale), "%s: scale is finite and positive", who);
   ITEXHIP_REQUIRE(p->window >= 0, "%s: window is not negative", who);
-  ITEXHIP_REQUIRE(p->table_stride >= 0 && p->table_stride * c->page_size <= (1ll << 30), "%s: table_stride times page_size is 0 to 2^30", who);
+  ITEXHIP_REQUIRE(p->table_stride >= 0 && p->table_stride <= (1ll << 30) / c->page_size, "%s: table_stride times page_size is 0 to 2^30", who);
   const int64_t* all[2] = {p->q_strides, p->out_strides};
   for (const int64_t* s : all)
     for (int i = 0; i < 2; ++i)

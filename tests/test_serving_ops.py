@@ -250,3 +250,19 @@ def test_a_workspace_serves_smaller_calls(hip, type, d, heads, group):
                 for n2 in pages:
                     if b2 <= b and m2 <= m and n2 <= n:
                         assert sizes[b2, m2, n2] <= sizes[b, m, n]
+
+
+@pytest.mark.parametrize("page,stride", [(256, (1 << 56) + 1), (256, 1 << 62), (256, (1 << 22) + 1), (16, 1 << 60), (16, (1 << 63) - 1), (16, (1 << 26) + 1), (128, (1 << 57) + 8)])
+def test_tables_beyond_the_bound_whatever_their_product_wraps_to(hip, page, stride):
+    c = hip.kv4_cache(64, 2, page, 4)
+    p = hip.kv4_attention_params(hip.BFLOAT16, 8, 64, 2, 1, 2, 0.125, stride)
+    with pytest.raises(hip.ItexHipError, match="table_stride"):
+        hip.kv4_attention_workspace(p, c)
+    with pytest.raises(hip.ItexHipError, match="table_stride"):
+        hip.kv4_attention(p, c, 64, 64, 64, 64, 64, 64, 64)
+
+
+@pytest.mark.parametrize("page", [16, 256])
+def test_the_widest_table_is_taken(hip, page):
+    p = hip.kv4_attention_params(hip.BFLOAT16, 8, 64, 2, 1, 2, 0.125, (1 << 30) // page)
+    assert hip.kv4_attention_workspace(p, hip.kv4_cache(64, 2, page, 4)) > 0
