@@ -913,7 +913,10 @@ __global__ __launch_bounds__(64 * kWaves<DP>, kWaves<DP> / 4) void prompt_kernel
   typedef float f16v __attribute__((ext_vector_type(16)));
   __shared__ u4v lds_k[2][TB * KK * 64], lds_v[2][U * DB * 64], lds_vp[2][TT / 4];
   __shared__ f4 lds_kp[2][TT / 2];  // of two tokens: scale and offset - 72 scale, the excess of the codes taken back
-  __shared__ __align__(16) uint16_t lds_flags[2][2][4];  // a bit a token: [..][0] seen by some row, [..][1] its value is NaN
+  // A bit a token: [..][0] seen by some row, [..][1] its value is not finite; without FOLD [..][1] is all of 16 tokens if some value of
+  // theirs may be none as a half, and lds_nans says which are not finite
+  __shared__ __align__(16) uint16_t lds_flags[2][2][4];
+  __shared__ __align__(8) uint16_t lds_nans[2][4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, hi = lane >> 5;
   const int head = blockIdx.x % A.kv_heads, b = blockIdx.z;  // neighbouring workgroups, on different dies, take different heads
   const Seq s = sequence(A, b);
@@ -1074,9 +1077,12 @@ __global__ __launch_bounds__(64 * kWaves<DP>, kWaves<DP> / 4) void prompt_kernel
     if (wave >= U) return;
     const int tg = t0 + 16 * wave;
     auto odd = [](uint32_t x) { return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u; };
-    const bool nan = odd(par[0]) || odd(par[1]) || odd(par[2]) || odd(par[3]);
+    // without FOLD: a value is at most 8 |scale| + |offset|; what append saturated comes to up to 65536, which a half does not hold
+    auto most = [&](int j) { return as_bits(__builtin_elementwise_fma(as_half2(par[j] & 0x7fff7fffu), half2v{8, 8}, as_half2(par[2 + j] & 0x7fff7fffu))); };
+    const bool far = FOLD ? odd(par[0]) || odd(par[1]) || odd(par[2]) || odd(par[3]) : odd(most(0)) || odd(most(1));
+    const bool any_far = !FOLD && __any(lane >= 4 && lane < 8 && far);
     uint32_t valid = 0xffffu, nans = 0;
-    if (!good(par_page) || tg + 16 > s.len || __any(lane >= 4 && lane < 8 && nan)) {
+    if (!good(par_page) || tg + 16 > s.len || (FOLD ? __any(lane >= 4 && lane < 8 && far) : any_far)) {
       const int n = good(par_page) ? min(max(s.len - tg, 0), 16) : 0;
       valid = (1u << n) - 1;
 #pragma unroll
@@ -1101,7 +1107,8 @@ __global__ __launch_bounds__(64 * kWaves<DP>, kWaves<DP> / 4) void prompt_kernel
     }
     if (lane == 0) {
       lds_flags[buf][0][wave] = static_cast<uint16_t>(valid);
-      lds_flags[buf][1][wave] = static_cast<uint16_t>(nans);
+      lds_flags[buf][1][wave] = static_cast<uint16_t>(FOLD ? nans : any_far ? 0xffffu : 0u);
+      if (!FOLD) lds_nans[buf][wave] = static_cast<uint16_t>(nans);
     }
     if (lane < 4) {
 #pragma unroll
@@ -1133,16 +1140,24 @@ __global__ __launch_bounds__(64 * kWaves<DP>, kWaves<DP> / 4) void prompt_kernel
     const bool more = t0 + TT < to;
     const u4v flags = *reinterpret_cast<const u4v*>(lds_flags[buf]);
     if (more) fetch(t0 + TT);
-    const uint64_t valid = (flags[0] | static_cast<uint64_t>(flags[1]) << 32) & kAll, nans = (flags[2] | static_cast<uint64_t>(flags[3]) << 32) & kAll;
-    if (!FOLD && nans != 0) {  // values that are NaN reach the rows that see them through l, the products as zeros
-      half8v* all = reinterpret_cast<half8v*>(lds_v[buf]);
-      for (int k = tid; k < U * DB * 64; k += THREADS) {
-        half8v a = all[k];
+    const uint64_t valid = (flags[0] | static_cast<uint64_t>(flags[1]) << 32) & kAll;
+    uint64_t nans = (flags[2] | static_cast<uint64_t>(flags[3]) << 32) & kAll;
+    if constexpr (!FOLD) {
+      // values that are not finite reach the rows that see them through l, the products as finite ones; values beyond a half are its
+      // largest, 65504 for at most 65536: 2^-11 of it
+      if (nans != 0) {
+        const uint2 bits_of = *reinterpret_cast<const uint2*>(lds_nans[buf]);
+        nans = (bits_of.x | static_cast<uint64_t>(bits_of.y) << 32) & kAll;
+        half8v* all = reinterpret_cast<half8v*>(lds_v[buf]);
+        constexpr _Float16 top = static_cast<_Float16>(65504.0f);
+        for (int k = tid; k < U * DB * 64; k += THREADS) {
+          half8v a = all[k];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) a[j] = a[j] == a[j] ? a[j] : static_cast<_Float16>(0);
-        all[k] = a;
+          for (int j = 0; j < 8; ++j) a[j] = a[j] != a[j] ? static_cast<_Float16>(0) : a[j] > top ? top : a[j] < -top ? -top : a[j];
+          all[k] = a;
+        }
+        __syncthreads();
       }
-      __syncthreads();
     }
     if (t0 < w_to && t0 + TT > w_from) {
       const bool mask = valid != kAll || nans != 0 || t0 + TT > w_all_to || t0 < w_all_from;

@@ -443,3 +443,25 @@ def test_a_workspace_serves_smaller_calls(hip, dev, name, d):
         torch.cuda.synchronize()
         assert torch.equal(again.cpu(), out) and torch.equal(lse2.cpu(), lse)
         assert bool((held[size:] == 0xa5).all())
+
+
+
+@pytest.mark.parametrize("name", list(TYPES))
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("lens", [[(1, 200), (1, 60)], [(6, 200), (3, 60)], [(90, 200), (70, 90)]])
+def test_saturated_values(hip, dev, max_q, name, lens, d):
+    """Rows of values with an element of 65504 or more: the codes of the largest stand for up to 65536, beyond what a half holds."""
+    batch = Batch(lens, 2, 2, d, 16, 18)
+    rows = torch.full((3, d), 0.5, dtype=torch.float64)
+    rows[0, 3], rows[1, 5], rows[2, 1], rows[2, 2] = 65504.0, math.inf, math.inf, -math.inf
+    rows[:, 7] = 0.0
+    code, scale, offset = ref.quantize(rows)
+    assert float(ref.values(code, scale, offset).max()) == 65536.0 and float(ref.values(code, scale, offset)[0].max()) == 65520.0
+    for b, (m, n) in enumerate(lens):
+        for head in range(2):
+            for i, t in enumerate((n - 2 if head else 9, 20 + head, n - m // 2 - 1)):    # some rows see them, all do, some of a tile do not
+                slot = placed(batch, b, t)
+                batch.cache.code[1, slot, head], batch.cache.scale[1, slot, head], batch.cache.offset[1, slot, head] = code[i], scale[i, 0], offset[i, 0]
+    out, lse, q = attend(hip, dev, name, batch, max_q=max_q)
+    assert bool(torch.isfinite(out).all()) and bool(torch.isfinite(lse).all())
+    check(out, lse, q, batch)
