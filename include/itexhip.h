@@ -579,7 +579,8 @@ int itexhip_kv4_gather(const itexhip_kv4_cache* c, int type, int64_t tokens, con
  * if window > 0.  q_heads is a multiple of kv_heads; consecutive query heads share a kv head.
  *   out = softmax(scale q k) v, rounded once; lse (NULL: not wanted; [total_q, q_heads] floats) the log of the sum of exponents
  * A row that sees nothing is 0 with lse -inf.  Rows outside every sequence are left as they are.  Keys and values a row does
- * not see do not reach it, whatever they hold; a value that is NaN and seen makes the whole row of out and its lse NaN.
+ * not see do not reach it, whatever they hold; a value that is seen and whose scale or offset is not finite makes the whole row of out
+ * and its lse NaN.
  * Prompts in bfloat16 hold values as halves: one beyond +-65504 (codes of saturated elements stand for up to 65536) counts
  * as that.  A page outside the cache counts as tokens that no row sees; kv_len beyond the table is cut to it, a sequence's
  * rows beyond max_q_len or total_q are not computed.

@@ -576,6 +576,7 @@ struct Engine {
           o[nb][e] += po[nb];
         }
       }
+      l[nb] = fmaf(0.0f, o[nb][0][0], l[nb]);  // a value that is not finite and that all rows of a step saw is in all dimensions' sums so far
     }
   }
   // What the sums are relative to, in units of log2

@@ -445,7 +445,6 @@ def test_a_workspace_serves_smaller_calls(hip, dev, name, d):
         assert bool((held[size:] == 0xa5).all())
 
 
-
 @pytest.mark.parametrize("name", list(TYPES))
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("lens", [[(1, 200), (1, 60)], [(6, 200), (3, 60)], [(90, 200), (70, 90)]])
@@ -465,3 +464,28 @@ def test_saturated_values(hip, dev, max_q, name, lens, d):
     out, lse, q = attend(hip, dev, name, batch, max_q=max_q)
     assert bool(torch.isfinite(out).all()) and bool(torch.isfinite(lse).all())
     check(out, lse, q, batch)
+
+
+@pytest.mark.parametrize("name", list(TYPES))
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("lens,d", [([(1, 100), (1, 300)], 64), ([(4, 100), (2, 300)], 128), ([(80, 100), (40, 300)], 128), ([(4, 100), (40, 200)], 256), ([(1, 100), (30, 60)], 256)])
+def test_values_that_are_not_finite(hip, dev, max_q, name, bad, lens, d):
+    """A scale or an offset of a value that is NaN or infinite: rows that see it are NaN in out and lse, whether or not other rows of a step see it too,
+    and the others are what they are without it."""
+    for which in ("both", "scale", "offset"):
+        for b, t in ((0, 98), (0, 3), (1, 3)):                         # seen by the first sequence's last rows; by all rows of one
+            batch = Batch(lens, 2, 2, d, 16, 19)
+            plain = Batch(lens, 2, 2, d, 16, 19)
+            slot = placed(batch, b, t)
+            if which != "offset":
+                batch.cache.scale[1, slot, 1] = bad
+            if which != "scale":
+                batch.cache.offset[1, slot, 1] = bad
+            out, lse, q = attend(hip, dev, name, batch, max_q=max_q)
+            rows, hit = torch.arange(batch.cu[-1]), torch.zeros(batch.cu[-1], 4, dtype=torch.bool)
+            m, n = lens[b]
+            hit[:, 2:] = ((rows >= batch.cu[b]) & (rows < batch.cu[b + 1]) & (n - m + rows - batch.cu[b] >= t))[:, None]
+            assert torch.equal(torch.isnan(lse), hit) and torch.equal(torch.isnan(out), hit[..., None].expand_as(out))
+            want, want_lse, mass = ref.attention(q, plain.cache, plain.table, plain.cu, [n for _, n in lens], d ** -0.5)
+            out, lse = torch.where(hit[..., None], want.to(out.dtype), out), torch.where(hit, want_lse.float(), lse)
+            check(out, lse, q, plain)
