@@ -583,7 +583,7 @@ int itexhip_kv4_gather(const itexhip_kv4_cache* c, int type, int64_t tokens, con
  * and its lse NaN.
  * Prompts in bfloat16 hold values as halves: one beyond +-65504 (codes of saturated elements stand for up to 65536) counts
  * as that.  A page outside the cache counts as tokens that no row sees; kv_len beyond the table is cut to it, a sequence's
- * rows beyond max_q_len or total_q are not computed.
+ * rows beyond max_q_len or total_q are not computed (the others sit where they would without that).
  * workspace: itexhip_kv4_attention_workspace bytes of device memory (16-byte aligned), contents irrelevant; it serves every
  * call of the same type, cache and q_heads whose num_seqs, max_q_len and table_stride are no larger; calls that may overlap
  * in time need one each.  Results do not depend on timing: equal calls give equal bits. */

@@ -38,21 +38,23 @@ struct AttArgs {
 // One sequence's rows and tokens, whatever the arrays say
 struct Seq {
   int64_t first;   // row of q
-  int n, len, lo;  // new tokens, tokens, first token that any row sees (multiple of 32)
+  int n, len, lo;  // rows to compute, tokens, first token that any row sees (multiple of 32)
+  int before;      // position of the first row, by all rows that the sequence has; not below -2^30, where no row sees a token either
   int64_t steps;   // of STEP tokens; at least one if there are rows
 };
 template <int STEP = 128>
 __device__ __forceinline__ Seq sequence(const AttArgs& A, int b) {
   Seq s;
-  int64_t from = A.cu_q[b], to = A.cu_q[b + 1];
+  int64_t from = A.cu_q[b], end = A.cu_q[b + 1];
   from = from < 0 ? 0 : from > A.total_q ? A.total_q : from;
-  to = to < from ? from : to > A.total_q ? A.total_q : to;
+  const int64_t all = end < from ? 0 : end - from, n = all < A.total_q - from ? all : A.total_q - from;
   s.first = from;
-  s.n = static_cast<int>(to - from < A.max_q_len ? to - from : A.max_q_len);
+  s.n = static_cast<int>(n < A.max_q_len ? n : A.max_q_len);
   const int64_t room = A.table_stride << A.page_shift;
   int64_t len = A.kv_len[b];
   s.len = static_cast<int>(len < 0 ? 0 : len > room ? room : len);
-  int64_t lo = A.window > 0 ? static_cast<int64_t>(s.len) - s.n - A.window + 1 : 0;
+  s.before = static_cast<int>(s.len - all < -(1ll << 30) ? -(1ll << 30) : s.len - all);
+  int64_t lo = A.window > 0 ? static_cast<int64_t>(s.before) - A.window + 1 : 0;
   s.lo = static_cast<int>(lo < 0 ? 0 : lo) & ~31;
   s.steps = s.n == 0 ? 0 : s.len > s.lo ? (s.len - s.lo + STEP - 1) / STEP : 1;
   return s;
@@ -145,9 +147,8 @@ struct Engine {
     g = lane >> 4;
     block = COPIES == 1 ? 0 : c / WIDTH;
     const int rows = s.n * A.group;
-    const int before = s.len - s.n;  // position of the first row
-    auto limit_of = [&](int row) { return A.causal ? max(before + row / A.group + 1, 0) : s.len; };
-    auto start_of = [&](int row) { return A.window > 0 ? max(before + row / A.group - A.window + 1, 0) : 0; };
+    auto limit_of = [&](int row) { return A.causal ? max(s.before + row / A.group + 1, 0) : s.len; };
+    auto start_of = [&](int row) { return A.window > 0 ? max(s.before + row / A.group - A.window + 1, 0) : 0; };
     min_limit = limit_of(row0);
     max_start = start_of(min(row0 + 16 * NB, rows) - 1);
 #pragma unroll
@@ -874,11 +875,11 @@ __global__ __launch_bounds__(256) void rows_kernel(const AttArgs A) {
   const int first = row0 / A.group, last = (row0 + 16 * NB < rows ? row0 + 16 * NB - 1 : rows - 1) / A.group;
   int to = s.len, from = s.lo;
   if (A.causal) {
-    to = s.len - s.n + last + 1;
+    to = s.before + last + 1;
     to = to < 0 ? 0 : to;
   }
   if (A.window > 0) {
-    from = s.len - s.n + first - A.window + 1;
+    from = s.before + first - A.window + 1;
     from = (from < 0 ? 0 : from) & ~31;
   }
   eng.run(A, A.table + b * A.table_stride, head, from, to, 32, s.len);
@@ -926,9 +927,8 @@ __global__ __launch_bounds__(64 * kWaves<DP>, kWaves<DP> / 4) void prompt_kernel
   const int at_tile = tiles - 1 - static_cast<int>(blockIdx.x / A.kv_heads);  // the longest first
   if (at_tile < 0) return;
   const int row0 = at_tile * tile_rows + 32 * wave, row = row0 + c;
-  const int before = s.len - s.n;  // position of the first row
-  auto limit_of = [&](int r) { return A.causal ? max(before + r / A.group + 1, 0) : s.len; };
-  auto start_of = [&](int r) { return A.window > 0 ? max(before + r / A.group - A.window + 1, 0) : 0; };
+  auto limit_of = [&](int r) { return A.causal ? max(s.before + r / A.group + 1, 0) : s.len; };
+  auto start_of = [&](int r) { return A.window > 0 ? max(s.before + r / A.group - A.window + 1, 0) : 0; };
   // of the workgroup and the wavefront
   const int first_row = at_tile * tile_rows, last_row = min(first_row + tile_rows, rows) - 1;
   const int from = start_of(first_row) & ~(TT - 1), to = min(limit_of(last_row), s.len);

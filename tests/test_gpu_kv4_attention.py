@@ -489,3 +489,33 @@ def test_values_that_are_not_finite(hip, dev, max_q, name, bad, lens, d):
             want, want_lse, mass = ref.attention(q, plain.cache, plain.table, plain.cu, [n for _, n in lens], d ** -0.5)
             out, lse = torch.where(hit[..., None], want.to(out.dtype), out), torch.where(hit, want_lse.float(), lse)
             check(out, lse, q, plain)
+
+
+@pytest.mark.parametrize("name", list(TYPES))
+@pytest.mark.parametrize("heads,group,d,window,causal", [(2, 2, 64, 0, True), (1, 4, 128, 0, True), (1, 3, 256, 0, True), (2, 2, 64, 20, True), (1, 3, 128, 9, False)])
+@pytest.mark.parametrize("lens,most", [([(8, 100), (1, 60), (5, 5)], 4), ([(120, 170), (3, 60), (70, 70), (80, 50)], 66), ([(8, 100), (3, 2), (6, 90)], 1)])
+def test_rows_that_are_not_computed_keep_the_others_positions(hip, dev, name, lens, most, heads, group, d, window, causal):
+    """Sequences with more rows than max_q_len, and one with rows beyond total_q: row i of n sits at kv_len - n + i all the same."""
+    batch = Batch(lens, heads, group, d, 16, 20)
+    dtype, hq = TYPES[name], heads * group
+    for total in (batch.cu[-1], batch.cu[-1] - 2):
+        q = batch.q.to(dtype)
+        table = batch.table_tensor().to(dev)
+        geometry = hip.kv4_cache(d, heads, 16, batch.cache.pages)
+        for bound in (most, 100000):
+            p = hip.kv4_attention_params(type_of(hip, name), hq, d, len(lens), bound, total, d ** -0.5, table.shape[1], causal=causal, window=window)
+            ws = torch.empty(hip.kv4_attention_workspace(p, geometry), dtype=torch.uint8, device=dev)
+            out, lse = torch.full((batch.cu[-1], hq, d), 3.0, dtype=dtype, device=dev), torch.full((batch.cu[-1], hq), 3.0, device=dev)
+            hip.kv4_attention(p, geometry, q.to(dev), batch.cache.pack().to(dev), table, torch.tensor(batch.cu, dtype=torch.int32, device=dev),
+                              torch.tensor([n for _, n in lens], dtype=torch.int32, device=dev), ws, out, lse)
+            torch.cuda.synchronize()
+            out, lse = out.cpu(), lse.cpu()
+            rows = torch.arange(batch.cu[-1])
+            done = rows < total
+            for b, (m, _) in enumerate(lens):
+                done &= ~((rows >= batch.cu[b] + bound) & (rows < batch.cu[b + 1]))
+            assert int(done.sum()) < len(rows) or bound == 100000
+            assert bool((out[~done] == 3.0).all()) and bool((lse[~done] == 3.0).all())
+            want, want_lse, _ = ref.attention(q, batch.cache, batch.table, batch.cu, [n for _, n in lens], d ** -0.5, causal, window)
+            out[~done], lse[~done] = want[~done].to(dtype), want_lse[~done].float()
+            check(out, lse, q, batch, causal=causal, window=window)
