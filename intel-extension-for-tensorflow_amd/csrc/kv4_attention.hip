@@ -1458,7 +1458,7 @@ extern "C" int itexhip_kv4_attention(const itexhip_kv4_attention_params* p, cons
   A.num_seqs = p->num_seqs;
   A.max_q_len = p->max_q_len;
   A.causal = p->causal != 0;
-  A.window = p->window;
+  A.window = p->window < 1 << 30 ? p->window : 1 << 30;  // no sequence is longer; positions from -2^30 on less this stay in 32 bits
   A.head_dim = c->head_dim;
   A.page_size = c->page_size;
   A.page_shift = log2_of(c->page_size);

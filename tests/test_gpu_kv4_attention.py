@@ -519,3 +519,13 @@ def test_rows_that_are_not_computed_keep_the_others_positions(hip, dev, name, le
             want, want_lse, _ = ref.attention(q, batch.cache, batch.table, batch.cu, [n for _, n in lens], d ** -0.5, causal, window)
             out[~done], lse[~done] = want[~done].to(dtype), want_lse[~done].float()
             check(out, lse, q, batch, causal=causal, window=window)
+
+
+@pytest.mark.parametrize("name", list(TYPES))
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 30])
+@pytest.mark.parametrize("q_rows", [5, 9, 80])
+def test_windows_beyond_every_length(hip, dev, max_q, name, q_rows, window):
+    """Among sequences of more new tokens than tokens, whose first rows sit before position 0."""
+    batch = Batch([(q_rows, q_rows // 2), (1, 40), (q_rows, q_rows + 3), (q_rows, 1), (0, 0)], 2, 2, 64, 16, 21)
+    for causal in (True, False):
+        check(*attend(hip, dev, name, batch, max_q=max_q, causal=causal, window=window), batch, causal=causal, window=window)
