@@ -21,6 +21,23 @@ constexpr int step_of(int copies) { return copies == 4 ? 256 : 128; }
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kProbExponent = 9.0f;  // probabilities are held as 2^9 p, up to 2^14 p above the maximum so far: half keeps 11 bits down to 2^-23
 
+// Probabilities times scales as halves: 2^(score log2(e) + ref) scale.  ref goes by the largest score and a power of two over the scales
+// (scale_bound, an exponent more than was seen), so that they are below 2^10, and 5 bits are left for scores to rise in
+// without a look at them (kMostExponent).  The largest score and the largest scale may be different tokens', though, and a large
+// scale without probability would take the others' bits: ref falls no further than to where the largest product of a token's own
+// probability and scale is 2^4, of which 2^-29 is lost then.  Where that holds ref above what scale_bound asks for,
+// scale_bound becomes the present tile's, and scores above raise_at come to be looked at again.
+constexpr float kMostExponent = 15.0f, kOwnExponent = 4.0f;
+// log2 of a half: a straight line between powers of two, at most 0.09 below it; above it for subnormals, by 9 at most (2^-5 in place of 2^4)
+__device__ __forceinline__ float log2_of_half(uint32_t bits) { return fmaf(static_cast<float>(bits & 0x7fffu), 1.0f / 1024.0f, -15.0f); }
+__device__ __forceinline__ float log2_over(uint32_t bound) { return static_cast<float>(static_cast<int>(bound >> 10) - 14); }
+__device__ __forceinline__ uint32_t bound_of(uint32_t bound, uint32_t most) { return most > bound ? min(most + 0x400u, 0x7bffu) : bound; }
+// ref for a tile whose largest score asks for `bound` (with the bound of the scales), its largest product for `own`
+__device__ __forceinline__ float lower(float ref, bool first, float bound, float own) {
+  const float to = fmaxf(kProbExponent + 1.0f - bound, kOwnExponent - own);
+  return first ? to : fminf(ref, to);
+}
+
 struct AttArgs {
   const void* q;
   const uint8_t* cache;
@@ -101,8 +118,7 @@ constexpr int occupancy_of(int nb, int dp, bool f32) { return dp == 256 ? 1 : nb
 // rounded to half, and offset times probability is summed apart in fp32: codes and products of 11 bits are exact, the one
 // rounding is that of the probability.
 //
-// Probabilities times scales have to fit a half: they are held relative to a power of two that bounds the scales seen so far,
-// which grows like the maximum of the scores does; both are in `ref`, p = 2^(score log2(e) + ref).
+// Probabilities times scales have to fit a half: see above for `ref`, p = 2^(score log2(e) + ref).
 //
 // Queries are multiplied by a power of two of their row so that half holds what bfloat16 does.  In fp32 the products are
 // fp32 MFMAs on fp32 operands.
@@ -120,12 +136,11 @@ struct Engine {
   static_assert(COPIES == 1 || (NB == 1 && !F32), "copies");
   static constexpr int TILES = COPIES == 4 ? 4 : 2, TOKENS = 16 * TILES, OWN = COPIES == 1 ? TILES : 1, WIDTH = 16 / COPIES;  // OWN: tiles whose scores a lane has
   static constexpr int NKK = DP / 32, E = DP / 16, NV = DP <= 128 ? 1 : 2;
-  static constexpr float kSlack = F32 ? 0.0f : 5.0f;  // log2 of how far a score may exceed the maximum that sums are relative to
   half8v q16[F32 ? 1 : NB][NKK];
   float q32[F32 ? NB : 1][NKK][8];
   f4 corr[NB];  // what a product starts from: minus the excess of the codes
   float sumq[NB], qs[NB], m[NB], raise_at[NB], ref[NB], l[NB], po[NB];
-  uint32_t scale_bound;  // half bits that no value's scale so far exceeds: an exponent with all ones below
+  uint32_t scale_bound;  // half bits that no value's scale exceeds without a look: an exponent with all ones below
   int limit[NB], start[NB];  // the tokens that column c of block nb sees: start <= t < limit
   f4 o[NB][E];
   int min_limit, max_start;  // over the wavefront's rows
@@ -301,37 +316,56 @@ struct Engine {
     for (int e = 0; e < E; ++e) o[nb][e] *= a;
   }
 
-  // The sums are held relative to a maximum of the scores and a power of two over the values' scales: either has grown
+  // The sums are held relative to 2^-ref, which falls with the maximum of the scores and with the scales: either has grown
   __device__ __forceinline__ void raise(const float (&p)[NB][4 * OWN], uint32_t most) {
-    if constexpr (!F32) {
+    auto over_lanes = [](float x) {
+#pragma unroll
+      for (int d = WIDTH; d < 64; d *= 2) x = fmaxf(x, __shfl_xor(x, d));
+      return x;
+    };
+    if constexpr (F32) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        float top = p[nb][0];
+#pragma unroll
+        for (int j = 1; j < 4 * OWN; ++j) top = fmaxf(top, p[nb][j]);
+        top = over_lanes(top);
+        const float was = m[nb];
+        if (top > was) {
+          m[nb] = raise_at[nb] = top;
+          const float by = was == -INFINITY ? top * qs[nb] : (top - was) * qs[nb];
+          ref[nb] -= by;
+          rescale(nb, was == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(-by));
+        }
+      }
+    } else {
 #pragma unroll
       for (int d = WIDTH; d < 64; d *= 2) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), d)));
       most = (most > 0x7bffu ? 0x7bffu : most) | 0x3ffu;  // NaN comes through the products
-      if (most > scale_bound) {
-        const float by = static_cast<float>(static_cast<int>((most >> 10) - (scale_bound >> 10)));
-        scale_bound = most;
+      scale_bound = bound_of(scale_bound, most);
+      bool held = false;
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          ref[nb] -= by;
-          rescale(nb, __builtin_amdgcn_exp2f(-by));
+      for (int nb = 0; nb < NB; ++nb) {
+        float top = p[nb][0], own = -INFINITY;
+#pragma unroll
+        for (int j = 1; j < 4 * OWN; ++j) top = fmaxf(top, p[nb][j]);
+        top = over_lanes(top);
+#pragma unroll
+        for (int j = 0; j < 4 * OWN; ++j) own = fmaxf(own, fmaf(p[nb][j], qs[nb], log2_of_half(vp[j / 4][j % 4 / 2] >> (16 * (j & 1)))));
+        own = over_lanes(own);
+        if (top > -INFINITY) {
+          const float bound = fmaf(top, qs[nb], log2_over(scale_bound)), to = lower(ref[nb], m[nb] == -INFINITY, bound, own);
+          if (to != ref[nb]) {
+            rescale(nb, m[nb] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(to - ref[nb]));
+            ref[nb] = to;
+          }
+          m[nb] = fmaxf(m[nb], top);
+          held = held || to + bound > kMostExponent;
         }
       }
-    }
+      if (__any(held)) scale_bound = most;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      float top = p[nb][0];
-#pragma unroll
-      for (int j = 1; j < 4 * OWN; ++j) top = fmaxf(top, p[nb][j]);
-#pragma unroll
-      for (int d = WIDTH; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-      const float was = m[nb];
-      if (top > was) {
-        m[nb] = top;
-        const float by = was == -INFINITY ? top * qs[nb] : (top - was) * qs[nb];
-        ref[nb] -= by;
-        rescale(nb, was == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(-by));
-        raise_at[nb] = top + kSlack / qs[nb];
-      }
+      for (int nb = 0; nb < NB; ++nb) raise_at[nb] = m[nb] == -INFINITY ? -INFINITY : (kMostExponent - log2_over(scale_bound) - ref[nb]) * __builtin_amdgcn_rcpf(qs[nb]);
     }
   }
 
@@ -1213,17 +1247,40 @@ __global__ __launch_bounds__(64 * kWaves<DP>, kWaves<DP> / 4) void prompt_kernel
           most = two[0] > two[1] ? two[0] : two[1];
         }
         if (__any(top > raise_at || (FOLD && most > scale_bound))) {
-          if constexpr (FOLD) {
-            most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 32))) | 0x3ffu;
-            if (most > scale_bound) {
-              const float by = static_cast<float>(static_cast<int>((most >> 10) - (scale_bound >> 10)));
-              scale_bound = most;
-              ref -= by;
-              rescale(by);
-            }
-          }
           top = fmaxf(top, __shfl_xor(top, 32));
-          if (top > m) {
+          if constexpr (FOLD) {
+            most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 32)));
+            most = (most > 0x7bffu ? 0x7bffu : most) | 0x3ffu;
+            scale_bound = bound_of(scale_bound, most);
+            uint32_t least = 0xffffu;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              uint32_t x = vp[k / 2][k % 2];
+              asm volatile("" : "+v"(x));  // (not ahead of the branch, where the results would take registers that spill)
+              least = min(least, min(x & 0xffffu, x >> 16));
+            }
+            float own = INFINITY;  // where no scale is far below the bound, that holds for the products too
+            if (__any(log2_over(scale_bound) - log2_of_half(least) > kProbExponent + 1.0f - kOwnExponent)) {
+              own = -INFINITY;
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                uint32_t x = vp[r / 4][r % 4 / 2];
+                asm volatile("" : "+v"(x));
+                own = fmaxf(own, fmaf(p[r], qs, log2_of_half(x >> (16 * (r & 1)))));
+              }
+              own = fmaxf(own, __shfl_xor(own, 32));
+            }
+            bool held = false;
+            if (top > -INFINITY) {
+              const float bound = fmaf(top, qs, log2_over(scale_bound)), to = lower(ref, m == -INFINITY, bound, own);
+              if (to != ref) rescale(m == -INFINITY ? 0.0f : ref - to);
+              ref = to;
+              m = fmaxf(m, top);
+              held = to + bound > kMostExponent;
+            }
+            if (__any(held)) scale_bound = most;
+            raise_at = m == -INFINITY ? -INFINITY : (kMostExponent - log2_over(scale_bound) - ref) * __builtin_amdgcn_rcpf(qs);
+          } else if (top > m) {
             const float by = m == -INFINITY ? top * qs : (top - m) * qs;
             ref -= by;
             rescale(m == -INFINITY ? 0.0f : by);

@@ -529,3 +529,46 @@ def test_windows_beyond_every_length(hip, dev, max_q, name, q_rows, window):
     batch = Batch([(q_rows, q_rows // 2), (1, 40), (q_rows, q_rows + 3), (q_rows, 1), (0, 0)], 2, 2, 64, 16, 21)
     for causal in (True, False):
         check(*attend(hip, dev, name, batch, max_q=max_q, causal=causal, window=window), batch, causal=causal, window=window)
+
+
+@pytest.mark.parametrize("name", list(TYPES))
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("order", ["large first", "large at first", "falling", "large unseen", "large among small", "larger scores of smaller scales", "any"])
+def test_falling_scales(hip, dev, max_q, name, d, order):
+    """Values whose scales differ by up to 2^30, the large ones without probability in the end: what is left keeps its bits.  Keys' offsets times a sum of
+    queries of about 10 / scale order the scores; two tokens have nearly all of the probability, so that no average hides what they lost."""
+    lens = [(1, 900), (3, 900), (100, 900)]
+    batch = Batch(lens, 1, 2, d, 16, 22, q_scale=0.05)
+    batch.q += 10.0 / math.sqrt(d)
+    batch.cache.scale[0] = torch.tensor(0.02).half().double()
+    g = torch.Generator().manual_seed(24)
+    for b, (_, n) in enumerate(lens):
+        for t in range(n):
+            slot = placed(batch, b, t)
+            large = {"large first": t == 5, "large at first": t < 20, "large unseen": t == n - 1, "large among small": t % 8 == 3}.get(order, False)
+            scale, low = (4096.0, -4.0) if large else (2.0 ** -18, 0.0)
+            if order == "falling":
+                scale, low = 2.0 ** max(12 - t // 16, -18), 4.0 * (min(t, 600) / 600 - 1)
+            if order == "larger scores of smaller scales":
+                scale, low = 2.0 ** ((t * 7) % 24 - 18), -0.1 * ((t * 7) % 24)
+            if order == "any":
+                scale, low = 2.0 ** float(torch.rand(1, generator=g) * 30 - 18), -4.0 * float(torch.rand(1, generator=g))
+            if t in (690, 700):                                      # all rows see them
+                scale, low = 2.0 ** -18, 1.93 if t == 690 else 2.0
+            batch.cache.scale[1, slot], batch.cache.offset[0, slot], batch.cache.offset[1, slot] = 1.37 * scale, low, 0.0
+    batch.cache.offset, batch.cache.scale = batch.cache.offset.half().double(), batch.cache.scale.half().double()
+    out, lse, q = attend(hip, dev, name, batch, max_q=max_q)
+    want, want_lse, mass = ref.attention(q, batch.cache, batch.table, batch.cu, [n for _, n in lens], d ** -0.5)
+    qf, eps, tiny = q.double(), torch.finfo(out.dtype).eps, torch.finfo(out.dtype).tiny
+    lead = qf.abs().sum(-1) * 15 + qf.cumsum(-1).abs().amax(-1) * 2 * (72 if name != "float" else 8)
+    e = d ** -0.5 * (0.02 * d * U * lead + 4 * U * (0.02 * 9 + 4) * qf.abs().sum(-1) + d * 2.0 ** -25 * qf.abs().amax(-1) * 0.02 * 8)
+    assert float(((lse.double() - want_lse).abs() - e - 8 * U * want_lse.abs() - 40 * U).max()) <= 0
+    rounding = 2.0 ** -10 if name != "float" else 0.0
+    tol = eps / 2 * want.abs() * (1 + 2.0 ** -8) + tiny * eps + ((2 * e + 40 * U + rounding) * mass)[..., None]
+    if name == "bfloat16" and max_q:
+        # prompts take a probability to a half apart from its value's scale, as 2^9 of the largest so far or more: below 2^-14 it is off by up to 2^-25, that is
+        # 2^-34 of the largest, which is at most 1 of the sum: 2^-34 of each value's magnitude
+        total = torch.stack([8.0 * batch.cache.scale[1, [placed(batch, b, t) for t in range(n)], 0].sum() for b, (_, n) in enumerate(lens)])
+        tol += 2.0 ** -34 * total.repeat_interleave(torch.tensor([m for m, _ in lens]))[:, None, None]
+    off = (out.double() - want).abs() - tol
+    assert float(off.max()) <= 0, (float(off.max()), float(((out.double() - want).abs() / mass[..., None]).max()))
