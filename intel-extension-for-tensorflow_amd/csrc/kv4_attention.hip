@@ -62,17 +62,14 @@ struct Seq {
 template <int STEP = 128>
 __device__ __forceinline__ Seq sequence(const AttArgs& A, int b) {
   Seq s;
-  int64_t from = A.cu_q[b], end = A.cu_q[b + 1];
-  from = from < 0 ? 0 : from > A.total_q ? A.total_q : from;
-  const int64_t all = end < from ? 0 : end - from, n = all < A.total_q - from ? all : A.total_q - from;
+  const int total = static_cast<int>(A.total_q), end = A.cu_q[b + 1], from = min(max(A.cu_q[b], 0), total);
+  const int all = end < from ? 0 : end - from;
   s.first = from;
-  s.n = static_cast<int>(n < A.max_q_len ? n : A.max_q_len);
-  const int64_t room = A.table_stride << A.page_shift;
-  int64_t len = A.kv_len[b];
-  s.len = static_cast<int>(len < 0 ? 0 : len > room ? room : len);
-  s.before = static_cast<int>(s.len - all < -(1ll << 30) ? -(1ll << 30) : s.len - all);
-  int64_t lo = A.window > 0 ? static_cast<int64_t>(s.before) - A.window + 1 : 0;
-  s.lo = static_cast<int>(lo < 0 ? 0 : lo) & ~31;
+  s.n = min(min(all, total - from), A.max_q_len);
+  const int room = static_cast<int>(A.table_stride << A.page_shift);  // at most 2^30
+  s.len = min(max(A.kv_len[b], 0), room);
+  s.before = max(s.len - all, -(1 << 30));
+  s.lo = A.window > 0 ? max(s.before - A.window + 1, 0) & ~31 : 0;
   s.steps = s.n == 0 ? 0 : s.len > s.lo ? (s.len - s.lo + STEP - 1) / STEP : 1;
   return s;
 }
