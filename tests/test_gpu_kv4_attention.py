@@ -572,3 +572,15 @@ def test_falling_scales(hip, dev, max_q, name, d, order):
         tol += 2.0 ** -34 * total.repeat_interleave(torch.tensor([m for m, _ in lens]))[:, None, None]
     off = (out.double() - want).abs() - tol
     assert float(off.max()) <= 0, (float(off.max()), float(((out.double() - want).abs() / mass[..., None]).max()))
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("lens", [[(1, 300)], [(5, 300), (2, 90)], [(90, 300)]])
+def test_zeros_add_nothing_in_float(hip, dev, max_q, lens, d):
+    """Keys that are zero (codes of 8, no offset) beside large queries: every product is zero exactly, the sums are counts of tokens."""
+    batch = Batch(lens, 2, 2, d, 16, 25, q_scale=100.0)
+    batch.cache.code[0], batch.cache.scale[0], batch.cache.offset[0] = 8, 4.0, 0.0
+    out, lse, q = attend(hip, dev, "float", batch, max_q=max_q)
+    want, want_lse, mass = ref.attention(q, batch.cache, batch.table, batch.cu, [n for _, n in lens], d ** -0.5)
+    assert float(((lse.double() - want_lse).abs() - 8 * U * want_lse.abs() - 40 * U).max()) <= 0
+    assert float(((out.double() - want).abs() - 2.0 ** -24 * want.abs() - 40 * U * mass[..., None]).max()) <= 0
