@@ -548,7 +548,8 @@ int itexhip_qk_norm_rope(const itexhip_heads_params* p, int64_t tokens, const vo
  * (or value) of one head is held as scale * (code - 8) + offset: codes of 0 .. 15, scale and offset in half precision,
  *   scale = half((max - min) / 15), offset = half(min + 8 scale), code = 8 + clamp(rne((x - offset) / scale), -8, 7)
  * of the dimensions after norm and rotation, clamped to +-65504, evaluated in 64 bits (codes do not depend on the
- * call that made them); scale 0: all codes are 8; a NaN among the dimensions: scale and offset are NaN, all codes 8.
+ * call that made them; half(x) goes by way of a float); scale 0: all codes are 8; a NaN among the dimensions: scale and
+ * offset are NaN, all codes 8.
  * A page holds, for each kv head, [page_size][DP / 2] bytes of key codes (lower dimension in the low bits), [page_size / 4]
  * [DP / 8][4 tokens][4] bytes of value codes, [page_size / 4][4 scales, 4 offsets] of the keys and the same of the values;
  * DP is head_dim rounded up to 64, 128 or 256.  (Four tokens' value codes of eight dimensions are one 16-byte load.) */
@@ -561,9 +562,9 @@ typedef struct {
 int64_t itexhip_kv4_page_bytes(const itexhip_kv4_cache* c); /* 0: not a valid geometry */
 
 /* Norm, rotation and quantization of new keys, quantization of new values, into the cache, with the queries' norm and
- * rotation in the same call (q may be NULL, then q_out is not written; otherwise q_out is q or overlaps none of the inputs).  slots[t] (device) = page * page_size + place in
- * the page; a slot below 0 or beyond the cache writes nothing (padded rows).  A slot occurs once in a call: which of two
- * rows' codes, scales and offsets a slot given twice holds is not defined. */
+ * rotation in the same call (q may be NULL, then q_out is not written; otherwise q_out is q or overlaps none of the inputs).
+ * slots[t] (device) = page * page_size + place in the page; a slot below 0 or beyond the cache writes nothing (padded rows).
+ * A slot occurs once in a call: which of two rows' codes, scales and offsets a slot given twice holds is not defined. */
 int itexhip_kv4_append(const itexhip_heads_params* p, const itexhip_kv4_cache* c, int64_t tokens, const void* q, const void* k,
                        const void* v, const float* q_weight, const float* k_weight, const int32_t* positions,
                        const double* freqs, const int64_t* slots, void* q_out, void* cache, void* stream);
@@ -577,13 +578,17 @@ int itexhip_kv4_gather(const itexhip_kv4_cache* c, int type, int64_t tokens, con
  * cu_q[b + 1] - 1 of q and out, and kv_len[b] tokens in the pages block_table[b * table_stride + token / page_size]; row i of
  * n sits at position kv_len - n + i and sees the tokens up to there (all of them if not causal), of these the last `window`
  * if window > 0.  q_heads is a multiple of kv_heads; consecutive query heads share a kv head.
- *   out = softmax(scale q k) v, rounded once; lse (NULL: not wanted; [total_q, q_heads] floats) the log of the sum of exponents
+ *   out = softmax(scale q k) v; lse (NULL: not wanted; [total_q, q_heads] floats) the log of the sum of exponents
+ * All sums are fp32 and out is rounded to its type at the end.  FLOAT holds nothing in fewer bits.  BFLOAT16 and HALF have
+ * operands of half precision: codes exactly; a row's queries, times a power of two, off by at most 2^-25 of the row's
+ * largest (exactly but for elements below 2^-14 of it); a probability times its value's scale to 11 bits, or to 2^-29 of the row's
+ * largest such product if that is more (up to 2^-20 where scales are subnormal); in BFLOAT16 prompts instead a probability to 11
+ * bits or 2^-34 of the row's largest, and a value (scale (code - 8) + offset) to 11 bits, one beyond +-65504 (codes of saturated
+ * elements stand for up to 65536) as that.
  * A row that sees nothing is 0 with lse -inf.  Rows outside every sequence are left as they are.  Keys and values a row does
- * not see do not reach it, whatever they hold; a value that is seen and whose scale or offset is not finite makes the whole row of out
- * and its lse NaN.
- * Prompts in bfloat16 hold values as halves: one beyond +-65504 (codes of saturated elements stand for up to 65536) counts
- * as that.  A page outside the cache counts as tokens that no row sees; kv_len beyond the table is cut to it, a sequence's
- * rows beyond max_q_len or total_q are not computed (the others sit where they would without that).
+ * not see do not reach it, whatever they hold; a value that is seen and whose scale or offset is not finite makes the whole
+ * row of out and its lse NaN.  A page outside the cache counts as tokens that no row sees; kv_len beyond the table is cut to
+ * it, a sequence's rows beyond max_q_len or total_q are not computed (the others sit where they would without that).
  * workspace: itexhip_kv4_attention_workspace bytes of device memory (16-byte aligned), contents irrelevant; it serves every
  * call of the same type, cache and q_heads whose num_seqs, max_q_len and table_stride are no larger; calls that may overlap
  * in time need one each.  Results do not depend on timing: equal calls give equal bits. */

@@ -94,8 +94,10 @@ __device__ __forceinline__ float load_q(const void* q, int64_t i) {
   else return f16_bits_to_f32(static_cast<const uint16_t*>(q)[i]);
 }
 
-// Wavefronts a SIMD of a split kernel, and so its workgroups: registers for 2 (256) without spills, and longer shares than with 3, where
-// every other wait is for memory anyway; 3 where they fit and tokens are small or their products long.  Measured 2 : 3 in us, half or
+// Wavefronts a SIMD of a split kernel, and so its workgroups: registers for 2 (256; two tiles of rows of 128 dimensions spill 2 of theirs in
+// 16-bit types and 28 in fp32, other kernels none), and longer shares than with 3, where every other wait is for memory
+// anyway; 3 where they fit (fp32 of 128: but for 2) and tokens are small or their products long.  44 to 157 scalar
+// registers are held in lanes of vector registers.  Measured 2 : 3 in us, half or
 // bfloat16 heads of 128: one sequence of 131072 35 : 44, of 65536 (8 rows) 26 : 35, 64 of up to 8192 80 : 80; heads of 64: 32 sequences
 // of up to 4096 33.7 : 32.1, one of 32768 22.6 : 19.7; fp32, 32 sequences of up to 4096, 4 heads of 128 80 : 77.  4 spill (138 for 86).
 constexpr int occupancy_of(int nb, int dp, bool f32) { return dp == 256 ? 1 : nb == 1 && (dp == 64 || f32) ? 3 : 2; }
@@ -654,10 +656,10 @@ struct Engine {
 // knowing them.  A share may end one (sequence, head), hold several whole ones and begin another: whole ones are written out,
 // the two at its ends leave their sums in the workspace for combine_kernel.
 //
-// What bounds it: 64 sequences of up to 8192 tokens (8 kv heads of 128, 378 MB) take 80 us with combine_kernel, 4.7 TB/s, where a copy
-// has 5.1 and a launch that only reads 6.9: vector instructions are issued for 59 % of the time (and-or, shift and subtraction of
+// What bounds it: 64 sequences of up to 8192 tokens (8 kv heads of 128, 378 MB) take 79 us with combine_kernel, 4.8 TB/s, where a copy
+// has 5.1 and a launch that only reads 6.9: vector instructions are issued for 60 % of the time (and-or, shift and subtraction of
 // the codes: 144 for 64 tokens of a wavefront's 400), matrix instructions for 15 %.  Loads two steps ahead instead of one: 85 us.  One
-// sequence of 131072 tokens (143 MB) takes 34 us.  One of 2000 takes 13, a chain of latencies: 9 us for lengths, pages, the
+// sequence of 131072 tokens (143 MB) takes 33 us.  One of 2000 takes 13, a chain of latencies: 9 us for lengths, pages, the
 // first codes and the sums of four wavefronts, 4 for the second launch.
 template <int NB>
 __device__ __forceinline__ int tiles_of(const AttArgs& A, const Seq& s) { return (s.n * A.group + 16 * NB - 1) / (16 * NB); }
@@ -894,7 +896,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const AttArgs A) {
 
 // Sequences of more rows in fp32: a wavefront takes 16 NB rows through all the tokens that they see, codes straight from the caches to its
 // registers.  fp32 MFMAs (a 16th of half's rate) and a conversion for every code they take bound it: 2048 tokens, 32 heads
-// over 8 of 128, 690 us, 50 TFLOP/s.
+// over 8 of 128, 698 us, 49 TFLOP/s.
 template <int T, int DP, int NB>
 __global__ __launch_bounds__(256) void rows_kernel(const AttArgs A) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), b = blockIdx.z, head = blockIdx.y;
@@ -929,7 +931,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const AttArgs A) {
 // LDS holds a fragment as 64 lanes of 16 bytes.  Keys: [32 tokens][16 dimensions], lane 32 h + token: dimensions 8 h .. 8 h + 7 in the
 // order of key_operand.  Values: [16 tokens][32 dimensions], lane 32 h + dimension: tokens 4 h .. 4 h + 3 and 8 + 4 h .. + 3.
 //
-// What bounds it: 8192 tokens, 32 heads over 8 kv heads of 128, bfloat16, take 675 to 700 us, 790 to 815 TFLOP/s of the two products.  The matrix cores
+// What bounds it: 8192 tokens, 32 heads over 8 kv heads of 128, bfloat16, take 665 to 700 us, 785 to 830 TFLOP/s of the two products.  The matrix cores
 // are busy for a third of that, vector instructions are issued for half of it (a scale, an exponential, a sum and a conversion for
 // each score), and a wavefront does one after the other: two on a SIMD overlap them in part.  Measured and slower: four wavefronts of
 // 32 rows (995), 64 rows a wavefront (1100), three wavefronts a SIMD (spills, 1280), the products pinned between the vector
@@ -1353,13 +1355,13 @@ struct Plan {
 // Of more than kMostSplitRows rows, whether the tokens are divided (split_kernel) or the rows alone (prompt_kernel, rows_kernel).  Those
 // give a workgroup one tile of rows and all the tokens, and leave CUs idle where there are few tiles: as long as each has a CU of its own, the
 // time is that of one, 9 us and so much a token of the longest sequence.  split_kernel's is 25 us and so much a row and token, and
-// what combine_kernel takes for a row.  In us, 8 kv heads of 128 and 4 query heads each but where noted, rows alone : tokens
-// divided, a chunk of
-//   half, bfloat16  16 x 17 rows of 4096 tokens 137 : 60, 64 of 16384 590 : 54, 512 of 16384 622 : 264, 4 x 128 of 4096 166 : 101, 100 of 2000
-//                   87 : 33, 2 x 200 of 1000 52 : 62, 300 of 300 23 : 45, 1000 of 1000 51 : 100, 1000 of 4096 173 : 216; heads of 256:
-//                   128 of 16384 1152 : 185; 12 heads of 64: 4 x 128 of 1024 37 : 30, 512 of 512 25 : 29
-//   fp32            128 of 4096 672 : 112, 4 x 128 of 4096 678 : 302, 512 of 4096 677 : 362; 12 heads of 64: 512 of 512 55 : 34, 2048 of 2048 194 : 188
-// The longest sequence is the table's width (the host knows no lengths) or what a window leaves of it.
+// what combine_kernel takes for a row.  In us, 8 kv heads of 128 and 4 query heads each but where noted (the constants are these sizes'; others
+// go by the formula), rows alone : tokens divided, sequences x rows of tokens
+//   bfloat16  16 x 17 of 4096 137 : 90, 64 of 16384 595 : 57, 512 of 16384 599 : 288, 4 x 128 of 4096 158 : 95, 100 of 2000 83 : 32, 2 x 200 of
+//             1000 49 : 64, 300 of 300 22 : 46, 1000 of 1000 47 : 95, 1000 of 4096 161 : 203; heads of 256: 128 of 16384 1218 : 204;
+//             12 heads of 64: 4 x 128 of 1024 37 : 36, 512 of 512 25 : 28
+//   fp32      128 of 4096 676 : 110, 4 x 128 of 4096 676 : 353, 512 of 4096 674 : 355; 12 heads of 64: 512 of 512 54 : 34, 2048 of 2048 193 : 194
+// The longest sequence is taken to be as long as the table is wide (the host knows no lengths) or what a window leaves of it.
 bool tokens_are_divided(const itexhip_kv4_attention_params* p, const itexhip_kv4_cache* c, int64_t rows, int dp) {
   const bool f32 = p->type == ITEXHIP_FLOAT;
   const int64_t tile = f32 ? (dp == 256 ? 64 : 128) : dp == 256 ? 128 : 256, all = static_cast<int64_t>(p->num_seqs) * c->kv_heads;
