@@ -180,13 +180,14 @@ __device__ __forceinline__ void quantize_head(Runs<Real, NPL>& v, bool mine, uin
 // Norm and rotation of 8192 tokens (32 heads and 8 of 128, bfloat16, 168 MB read and written) take 43 us, 3.9 TB/s, where a copy
 // has 5.1.  Appending them takes 31 us for the queries (4.3 TB/s) and 32 for keys and values, 34 MB and 9 MB of cache: there a
 // SIMD's two wavefronts issue 500 vector instructions for a pass of 16 dimensions a lane, a good part of them in 64 bits, which is half
-// of the time, and wait for the other half.  One token takes 4 to 5 us: a launch and one chain of loads.
+// of the time, and wait for the other half.  12 heads and 1 of 80 keep a third of the lanes at work: norm and rotation of 8192 tokens 20 us,
+// 1.7 TB/s, appending 38.  One token takes 4 to 5 us: a launch and one chain of loads.
 //
-// Wavefronts a SIMD: what registers allow without spills, or as nearly.  Measured, 8192 tokens, in us: appending bfloat16 2 : 3 72.6 : 72.2
+// Wavefronts a SIMD: what registers allow without spills, or as nearly.  Measured, 8192 tokens, in us: appending and reading back bfloat16 2 : 3 72.6 : 72.2
 // (and more for few tokens), fp32 3 : 4 119 : 111; norm and rotation bfloat16 3 : 4 : 6 43 : 43 : 77, fp32 3 : 4 : 6 : 8 73 : 71 : 76 : 110.
 constexpr int occupancy_of(int npl, bool vec, bool append) { return !append ? 4 : npl == 8 ? 2 : vec ? 4 : 3; }
 // Passes a wavefront from which an append's queries go through a launch of their own, which has more wavefronts and no 64-bit
-// registers: one launch : two, bfloat16 at 6 passes 24 : 26 us, 12 40 : 38, 18 67 : 59, 24 86 : 76; fp32 at 12 60 : 63, 24 113 : 111
+// registers: one launch : two, with the read-back, bfloat16 at 6 passes 24 : 26 us, 12 40 : 38, 18 67 : 59, 24 86 : 76; fp32 at 12 60 : 63, 24 113 : 111
 constexpr int kOwnLaunch = 16;
 template <int T, int NPL, int LPH, bool VEC, bool APPEND>
 __global__ __launch_bounds__(256, occupancy_of(NPL, VEC, APPEND)) void heads_kernel(const HeadsArgs A) {
