@@ -585,6 +585,7 @@ int itexhip_kv4_gather(const itexhip_kv4_cache* c, int type, int64_t tokens, con
  * largest such product if that is more (up to 2^-20 where scales are subnormal); in BFLOAT16 prompts instead a probability to 11
  * bits or 2^-34 of the row's largest, and a value (scale (code - 8) + offset) to 11 bits, one beyond +-65504 (codes of saturated
  * elements stand for up to 65536) as that.
+ * out and lse overlap none of the inputs.
  * A row that sees nothing is 0 with lse -inf.  Rows outside every sequence are left as they are.  Keys and values a row does
  * not see do not reach it, whatever they hold; a value that is seen and whose scale or offset is not finite makes the whole
  * row of out and its lse NaN.  A page outside the cache counts as tokens that no row sees; kv_len beyond the table is cut to
