@@ -610,6 +610,105 @@ int itexhip_kv4_attention(const itexhip_kv4_attention_params* p, const itexhip_k
                           const int32_t* block_table, const int32_t* cu_q, const int32_t* kv_len, void* workspace, void* out,
                           float* lse, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Linears whose weights a token chooses: routing to experts, the experts' quantized products, low-rank adapters beside a shared
+ * projection.  The reference has no such ops; they complete a served decoder whose MLP is a mixture of experts over the
+ * quantized MatMuls above, or whose linears are shared by requests with adapters of their own.
+ *
+ * The rule of the operators above holds: what a router chose, orders, ranks and scales are device arrays that a captured graph reads
+ * anew at every replay; nothing is read back to the host, no call allocates.  Outputs overlap no input unless stated otherwise.
+ * A workspace is device memory, 16-byte aligned, whose contents do not matter; it serves every call of the same sizes and of
+ * fewer tokens, and calls that may overlap in time need one each.  Equal calls give equal bits.
+ * ---------------------------------------------------------------------------------------- */
+
+/* The experts of each token and their weights, from a router's logits [tokens, experts] (rows logits_stride elements apart):
+ *   score   softmax of the token's logits, or sigmoid of each
+ *   rank    score + bias (NULL: none), which balances the experts' load and is no part of the weights
+ *   groups  if there are several, the experts are that many equal runs; a group's value is the sum of its group_best best ranks and
+ *           only the experts of the top_groups groups of the largest value are left
+ *   experts_out[t, 0 .. top_k - 1]  the experts of the largest ranks, largest first, of equal ones the lowest index first
+ *   weights_out[t, j]  score, divided by the sum of the chosen scores if renormalise (a sum of 0 gives weights of 0), times scale
+ * Scores and ranks are held in 64 bits, weights are rounded to fp32 once.  A rank or a group's value that is not a number counts as -infinity; weights
+ * follow the formula (a logit of +infinity or NaN makes a softmax token's weights NaN; one of -infinity has the score 0; a
+ * token of nothing but -infinity has scores of 0). */
+enum { ITEXHIP_ROUTE_SOFTMAX = 0, ITEXHIP_ROUTE_SIGMOID = 1 };
+typedef struct {
+  int type;        /* FLOAT | BFLOAT16 | HALF of the logits */
+  int experts;     /* 1 .. 1024 */
+  int top_k;       /* 1 .. 32, no more than the experts of top_groups groups */
+  int score;       /* ITEXHIP_ROUTE_* */
+  int groups;      /* 1 .. 64, divides experts */
+  int top_groups;  /* 1 .. groups */
+  int group_best;  /* 1, or 2 where a group has two experts */
+  int renormalise;
+  float scale;     /* finite */
+  int64_t logits_stride;
+} itexhip_route_params;
+int itexhip_route(const itexhip_route_params* p, int64_t tokens, const void* logits, const float* bias, int32_t* experts_out,
+                  float* weights_out, void* stream);
+
+/* The order of n rows by group: rows_out is a permutation of 0 .. n - 1 that lists the rows of group 0 first, then those of group 1 ...,
+ * within a group in their own order, and at the end, in their own order, those whose group_of is not in 0 .. groups - 1;
+ * group g has the places offsets_out[g] .. offsets_out[g + 1] - 1.  1 <= groups <= 1024, n < 2^30. */
+int64_t itexhip_group_rows_workspace(int64_t n, int groups); /* 0: not valid */
+int itexhip_group_rows(int64_t n, int groups, const int32_t* group_of, int32_t* offsets_out, int32_t* rows_out, void* workspace,
+                       void* stream);
+
+/* The experts' products on int8 weights.  A slot is a token's choice, token * top_k + j; `offsets` and `rows` are the order of the
+ * slots by expert (itexhip_group_rows of the chosen experts; ids outside 0 .. experts - 1 belong to another device and are
+ * left out).  A row of activations becomes int8 codes by its own largest absolute value:
+ *   s = max(fp32(absmax / 127), 2^-100), code = rne(x / s)  (the quotient itself, not a rounded one); a row that holds an infinity
+ *   or NaN has s = NaN.
+ * up:   h[place, n] = act(v0[n]) * v1[n] if gated, else act(v0[n]);  v = fp32(sum of codes) * (s * scales[e, which, n]) with the codes of the
+ *       token of slot rows[place] and e's weights, the products summed exactly; h has top_k * tokens rows of `inner`, in the
+ *       order's places, and those behind offsets[experts] are left as they are.
+ * down: out[t, n] = addend[t, n] + sum over j of weights[t, j] * v[n] of slot t * top_k + j, from the row of h in that slot's place; in fp32, j upwards,
+ *       rounded to the type once; choices whose experts[t, j] is not in 0 .. experts - 1 are no part of it.  addend may be NULL
+ *       (zero) or `out` itself.
+ * packed: [experts][2 if gated, else 1][itexhip_qgemm_packed_bytes(K, N)] of itexhip_qgemm_prepack_b (16-byte aligned), gate first; K = hidden
+ * and N = inner for up, the other way round for down.  scales: [experts][2 or 1][N], the weight that a code of 1 stands for.
+ * activation: ITEXHIP_ACT_NONE, RELU, GELU_APPROX, GELU_EXACT or SWISH (for up). */
+typedef struct {
+  int type;           /* FLOAT | BFLOAT16 | HALF of x, h, addend and out */
+  int experts;        /* 1 .. 1024 */
+  int top_k;          /* 1 .. 32 */
+  int activation;
+  int gated;
+  int64_t tokens;     /* tokens * top_k below 2^30 */
+  int64_t hidden, inner;                       /* 1 .. 65536 */
+  int64_t x_stride, addend_stride, out_stride; /* elements between tokens, at least hidden */
+} itexhip_experts_params;
+int64_t itexhip_experts_workspace(const itexhip_experts_params* p); /* of either call; 0: not valid */
+int itexhip_experts_up(const itexhip_experts_params* p, const void* x, const int32_t* offsets, const int32_t* rows,
+                       const int8_t* packed, const float* scales, void* h, void* workspace, void* stream);
+int itexhip_experts_down(const itexhip_experts_params* p, const void* h, const int32_t* experts, const int32_t* offsets,
+                         const int32_t* rows, const int8_t* packed, const float* scales, const float* weights,
+                         const void* addend, void* out, void* workspace, void* stream);
+
+/* Low-rank adapters of many requests beside a shared projection:
+ *   out[t] = base[t] + scales[g] * (x[t] A_g^T) B_g^T   for the tokens of group g in the order (offsets, rows), out[t] = base[t] for the others
+ * a: [adapters][n_slices * rank][in], b: [adapters][out][rank], scales: [adapters] floats.  Columns slice_end[i - 1] .. slice_end[i] - 1 of
+ * the output use the rows i * rank .. of A (queries, keys and values of one projection); slice_end[n_slices - 1] = out.
+ * ranks (NULL: all have `rank`): [adapters], the rows of each slice of A and the columns of B that an adapter has, the rest is
+ * neither read nor counted; cut to 0 .. rank.  x A^T is held in fp32; BFLOAT16 and HALF multiply it as the sum of two
+ * numbers of the type (16 bits of it, 22 of the row's largest), FLOAT as it is; sums are fp32, out is rounded once.  A token whose x A^T holds an
+ * infinity or NaN has no finite results in that slice.  `base` may be `out` (tokens without an adapter are not touched then). */
+enum { ITEXHIP_ADAPTER_MAX_SLICES = 4 };
+typedef struct {
+  int type;           /* FLOAT | BFLOAT16 | HALF of x, a, b, base and out */
+  int adapters;       /* 1 .. 1024 */
+  int rank;           /* a multiple of 8, 8 .. 256 */
+  int n_slices;       /* 1 .. 4 */
+  int64_t tokens;     /* below 2^30 */
+  int64_t in;         /* 1 .. 2^20 */
+  int64_t slice_end[ITEXHIP_ADAPTER_MAX_SLICES]; /* ascending, the last one at most 2^20 */
+  int64_t x_stride, base_stride, out_stride;     /* elements between tokens */
+} itexhip_adapters_params;
+int64_t itexhip_adapters_workspace(const itexhip_adapters_params* p); /* 0: not valid */
+int itexhip_adapters(const itexhip_adapters_params* p, const void* x, const int32_t* offsets, const int32_t* rows, const void* a,
+                     const void* b, const int32_t* ranks, const float* scales, const void* base, void* out, void* workspace,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -28,10 +28,11 @@ namespace {
   X(minmax_i32_per_channel) X(minmax_f32) X(qgemm) X(qgemm_tile) X(qgemv) X(qgemm_sum) X(qmatmul) X(qmatmul_per_row)  \
   X(qmatmul_device_range) X(qmatmul_unpacked) X(quantize_dynamic) X(quantize_dynamic_static) X(quantize_dynamic_rows) \
   X(qbatch_matmul) X(pad_nhwc8) X(qconv2d) X(qconv2d_sum) X(qdepthwise_conv2d)                                        \
-  X(qk_norm_rope) X(kv4_append) X(kv4_gather) X(kv4_attention)
+  X(qk_norm_rope) X(kv4_append) X(kv4_gather) X(kv4_attention)                                                        \
+  X(route) X(group_rows) X(experts_up) X(experts_down) X(adapters)
 
-// MatmulParams, Epilogue, BmmParams, ConvGeometry, HeadsParams, Kv4Cache, Kv4AttentionParams
-constexpr int kStructs = 7;
+// MatmulParams, Epilogue, BmmParams, ConvGeometry, HeadsParams, Kv4Cache, Kv4AttentionParams, RouteParams, ExpertsParams, AdaptersParams
+constexpr int kStructs = 10;
 
 // All zero until init
 struct State {
@@ -62,6 +63,9 @@ template <class T> constexpr int struct_index() {
   if (std::is_same_v<T, itexhip_heads_params>) return 4;
   if (std::is_same_v<T, itexhip_kv4_cache>) return 5;
   if (std::is_same_v<T, itexhip_kv4_attention_params>) return 6;
+  if (std::is_same_v<T, itexhip_route_params>) return 7;
+  if (std::is_same_v<T, itexhip_experts_params>) return 8;
+  if (std::is_same_v<T, itexhip_adapters_params>) return 9;
   return -1;
 }
 
@@ -201,7 +205,8 @@ PyObject* f_transpose(PyObject* self, PyObject* const* args, Py_ssize_t n) {
 PyObject* init(PyObject* self, PyObject* args) {
   State& st = *state_of(self);
   PyObject *addresses, *check, *s[kStructs];
-  if (!PyArg_ParseTuple(args, "OO(OOOOOOO)", &addresses, &check, &s[0], &s[1], &s[2], &s[3], &s[4], &s[5], &s[6])) return nullptr;
+  if (!PyArg_ParseTuple(args, "OO(OOOOOOOOOO)", &addresses, &check, &s[0], &s[1], &s[2], &s[3], &s[4], &s[5], &s[6], &s[7],
+                        &s[8], &s[9])) return nullptr;
   for (PyObject* t : s)
     if (!PyType_Check(t)) { PyErr_SetString(PyExc_TypeError, "structures are types"); return nullptr; }
   bool ok = true;

@@ -1,0 +1,89 @@
+// What the kernels share whose rows are grouped by the weights they chose: loads of the three types, and the tiles of rows of a
+// grouped order.
+#ifndef ITEXHIP_CHOSEN_HPP_
+#define ITEXHIP_CHOSEN_HPP_
+
+#include "common.hpp"
+
+namespace itexhip {
+
+constexpr int kMaxGroups = 1024;
+constexpr int64_t kMaxRows = 1 << 30;
+
+inline bool is_chosen_type(int t) { return t == ITEXHIP_FLOAT || is_float16_type(t); }
+inline int64_t element_size(int t) { return t == ITEXHIP_FLOAT ? 4 : 2; }
+
+template <int T>
+__device__ __forceinline__ float load_value(const void* base, int64_t i) {
+  if constexpr (T == ITEXHIP_FLOAT) return static_cast<const float*>(base)[i];
+  else if constexpr (T == ITEXHIP_BFLOAT16) return bf16_bits_to_f32(static_cast<const uint16_t*>(base)[i]);
+  else return f16_bits_to_f32(static_cast<const uint16_t*>(base)[i]);
+}
+
+// Eight elements from the i-th on; the address of the first is a multiple of 16 bytes
+template <int T>
+__device__ __forceinline__ void load8(const void* base, int64_t i, float (&x)[8]) {
+  if constexpr (T == ITEXHIP_FLOAT) {
+    const f4* from = reinterpret_cast<const f4*>(static_cast<const float*>(base) + i);
+    const f4 a = from[0], b = from[1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { x[j] = a[j]; x[4 + j] = b[j]; }
+  } else {
+    const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + i);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t h = (w[j / 2] >> (16 * (j % 2))) & 0xffffu;
+      x[j] = T == ITEXHIP_BFLOAT16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
+    }
+  }
+}
+
+// Launches of up to 2^23 workgroups, since a grid has fewer than 2^32 threads: f(first, count) for each
+template <class F>
+inline void launch_blocks(int64_t blocks, F&& f) {
+  in_pieces(0, blocks, [&](int64_t begin, int64_t end) { f(begin, static_cast<unsigned>(end - begin)); }, 1LL << 23);
+}
+
+// Tiles of up to `per_tile` places of the order, group by group; with REST the rows of no group are a group of their own behind the
+// others.  How many there are is known on the device only: a launch has room for tiles_bound of them, and those beyond the
+// last find group = -1.
+inline int64_t tiles_bound(int64_t n, int groups, int per_tile, bool rest) {
+  const int64_t parts = groups + (rest ? 1 : 0);
+  const int64_t open = n < parts ? n : parts;  // groups that can have a tile that is not full
+  return open + (n - open) / per_tile;
+}
+struct RowTile {
+  int group;       // groups: the rows of no group
+  int begin, rows; // places
+  int first;       // of the group's places
+};
+// By all lanes of a wavefront, the same for all.  Offsets are cut to 0 .. n, so that whatever they hold, places are.
+template <bool REST>
+__device__ __forceinline__ RowTile find_tile(const int32_t* __restrict__ offsets, int groups, int n, int per_tile, int index) {
+  const int lane = static_cast<int>(__lane_id());
+  const int parts = groups + (REST ? 1 : 0), each = (parts + 63) / 64;
+  const int begin = lane * each, end = min(begin + each, parts);
+  auto at = [&](int g) { return g > groups ? n : min(max(offsets[g], 0), n); };
+  auto tiles_of = [&](int g) { return (max(at(g + 1) - at(g), 0) + per_tile - 1) / per_tile; };
+  int mine = 0;
+  for (int g = begin; g < end; ++g) mine += tiles_of(g);
+  int sum = mine;  // of the lanes up to this one
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int below = __shfl_up(sum, d);
+    if (lane >= d) sum += below;
+  }
+  const unsigned long long past = __ballot(sum > index);
+  if (past == 0) return RowTile{-1, 0, 0, 0};
+  const int owner = __builtin_ctzll(past);
+  int rank = index - (__builtin_amdgcn_readlane(sum, owner) - __builtin_amdgcn_readlane(mine, owner));
+  for (int g = owner * each;; ++g) {
+    const int first = at(g), rows = max(at(g + 1) - first, 0), tiles = (rows + per_tile - 1) / per_tile;
+    if (rank < tiles) return RowTile{g, first + rank * per_tile, min(per_tile, rows - rank * per_tile), first};
+    rank -= tiles;
+  }
+}
+
+}  // namespace itexhip
+#endif  // ITEXHIP_CHOSEN_HPP_

@@ -1,0 +1,353 @@
+// A router's choice of experts, and the order of rows by what they chose.
+#include <math.h>
+
+#include "chosen.hpp"
+
+namespace itexhip {
+namespace {
+
+// ------------------------------------------------------------------------------------------------
+// Router.  LPT lanes hold a token's ranks in 64 bits, PER consecutive experts each, so that LPT = 16 lets a wavefront choose for
+// four tokens at once.  What is chosen or left out becomes NaN, which neither a maximum nor an equality sees: top_k rounds of
+// one maximum over the lanes and the lowest expert that equals it.
+// ------------------------------------------------------------------------------------------------
+struct RouteArgs {
+  itexhip_route_params p;
+  const void* logits;
+  const float* bias;
+  int32_t* experts;
+  float* weights;
+  int64_t tokens, first;  // first: workgroup of the launch
+};
+
+template <int LPT, class V, class F>
+__device__ __forceinline__ V over_lanes(V x, F&& f) {
+#pragma unroll
+  for (int d = 1; d < LPT; d *= 2) x = f(x, __shfl_xor(x, d));
+  return x;
+}
+
+__device__ __forceinline__ double sigmoid(double x) { return 1.0 / (1.0 + exp(-x)); }
+
+template <int T, int LPT, int PER>
+__global__ __launch_bounds__(256) void route_kernel(const RouteArgs A) {
+  constexpr int TOKENS = 256 / LPT;  // of a workgroup
+  extern __shared__ __align__(16) uint8_t lds[];
+  const int local = threadIdx.x / LPT, sub = threadIdx.x & (LPT - 1);
+  const int64_t token = (A.first + blockIdx.x) * TOKENS + local;
+  const bool live = token < A.tokens;
+  const int E = A.p.experts, k = A.p.top_k;
+  const bool softmax = A.p.score == ITEXHIP_ROUTE_SOFTMAX;
+  const int64_t row = (live ? token : A.tokens - 1) * A.p.logits_stride;
+  const double inf = __builtin_inf(), nan = __builtin_nan("");
+  auto max_of = [](double a, double b) { return fmax(a, b); };
+  auto sum_of = [](double a, double b) { return a + b; };
+
+  double rank[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = sub * PER + i;
+    rank[i] = e < E ? static_cast<double>(load_value<T>(A.logits, row + e)) : nan;
+  }
+  double top = 0.0, total = 1.0;
+  if (softmax) {
+    top = -inf;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) top = fmax(top, rank[i]);
+    top = over_lanes<LPT>(top, max_of);
+    if (top == -inf) top = 0.0;  // nothing but -infinity: scores of 0
+    total = 0.0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const double z = exp(rank[i] - top);
+      if (sub * PER + i < E) total += z;
+      rank[i] = z;
+    }
+    total = over_lanes<LPT>(total, sum_of);
+    const double inv = total == 0.0 ? 1.0 : total;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) rank[i] = rank[i] / inv;
+    total = inv;
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) rank[i] = sigmoid(rank[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = sub * PER + i;
+    if (A.bias != nullptr && e < E) rank[i] += static_cast<double>(A.bias[e]);
+    rank[i] = e >= E ? nan : rank[i] != rank[i] ? -inf : rank[i];
+  }
+
+  if (A.p.groups > 1) {
+    const int G = A.p.groups, size = E / G;
+    double* const ranks = reinterpret_cast<double*>(lds) + static_cast<size_t>(local) * (LPT * PER + 64);
+    double* const values = ranks + LPT * PER;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) ranks[sub * PER + i] = rank[i];
+    __syncthreads();
+    for (int g = sub; g < G; g += LPT) {
+      double best = -inf, second = -inf;
+      for (int i = 0; i < size; ++i) {
+        const double r = ranks[g * size + i];
+        second = fmax(second, fmin(best, r));
+        best = fmax(best, r);
+      }
+      const double value = A.p.group_best == 2 ? best + second : best;
+      values[g] = value != value ? -inf : value;
+    }
+    __syncthreads();
+    unsigned long long open = 0;  // groups that are left, the same in all of a token's lanes
+    for (int g = sub; g < G; g += LPT) {
+      int ahead = 0;
+      for (int o = 0; o < G; ++o) ahead += values[o] > values[g] || (values[o] == values[g] && o < g);
+      if (ahead < A.p.top_groups) open |= 1ull << g;
+    }
+    open = over_lanes<LPT>(open, [](unsigned long long a, unsigned long long b) { return a | b; });
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int g = min(sub * PER + i, E - 1) / size;
+      if (!((open >> g) & 1)) rank[i] = nan;
+    }
+  }
+
+  // the j-th choice and its score stay with lane j % LPT, which has up to two (32 / LPT) of them
+  constexpr int KEEP = 32 / LPT > 0 ? (32 + LPT - 1) / LPT : 1;
+  int chosen[KEEP];
+#pragma unroll
+  for (int n = 0; n < KEEP; ++n) chosen[n] = 0;
+  for (int j = 0; j < k; ++j) {
+    double best = rank[0];
+#pragma unroll
+    for (int i = 1; i < PER; ++i) best = fmax(best, rank[i]);
+    best = over_lanes<LPT>(best, max_of);
+    int id = 1 << 30;
+#pragma unroll
+    for (int i = PER - 1; i >= 0; --i)
+      if (rank[i] == best) id = sub * PER + i;
+    id = over_lanes<LPT>(id, [](int a, int b) { return min(a, b); });
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (sub * PER + i == id) rank[i] = nan;
+#pragma unroll
+    for (int n = 0; n < KEEP; ++n)
+      if (n * LPT + sub == j) chosen[n] = min(id, E - 1);
+  }
+  double score[KEEP], sum = 0.0;
+#pragma unroll
+  for (int n = 0; n < KEEP; ++n) {
+    const double x = load_value<T>(A.logits, row + chosen[n]);
+    score[n] = softmax ? exp(x - top) / total : sigmoid(x);
+    if (n * LPT + sub < k) sum += score[n];
+  }
+  sum = A.p.renormalise ? over_lanes<LPT>(sum, sum_of) : 1.0;
+#pragma unroll
+  for (int n = 0; n < KEEP; ++n) {
+    const int j = n * LPT + sub;
+    if (!live || j >= k) continue;
+    A.experts[token * k + j] = chosen[n];
+    A.weights[token * k + j] = static_cast<float>((sum == 0.0 ? 0.0 : score[n] / sum) * static_cast<double>(A.p.scale));
+  }
+}
+
+template <int T, int LPT, int PER>
+void launch_route(RouteArgs A, hipStream_t st) {
+  constexpr int TOKENS = 256 / LPT;
+  const size_t lds = A.p.groups > 1 ? TOKENS * (LPT * PER + 64) * sizeof(double) : 0;
+  launch_blocks((A.tokens + TOKENS - 1) / TOKENS, [&](int64_t first, unsigned count) {
+    A.first = first;
+    route_kernel<T, LPT, PER><<<count, 256, lds, st>>>(A);
+  });
+}
+template <int T>
+void launch_route(const RouteArgs& A, hipStream_t st) {
+  if (A.p.experts <= 64) launch_route<T, 16, 4>(A, st);
+  else if (A.p.experts <= 256) launch_route<T, 16, 16>(A, st);
+  else launch_route<T, 64, 16>(A, st);
+}
+
+// ------------------------------------------------------------------------------------------------
+// Order of rows by group: a counting sort.  The rows are cut into runs, one a workgroup, whose wavefronts take consecutive shares.
+// A first launch counts each run's groups; in the second a wavefront knows where its rows of a group begin: behind all smaller
+// groups, the group's rows of earlier runs and those of the run's earlier wavefronts.  Rows of one group within 64 keep their
+// order by their number among the lanes.  One workgroup does both where there are few rows.
+// ------------------------------------------------------------------------------------------------
+constexpr int kOrderWaves = 4;
+constexpr int kRunRows = 1024, kMostRuns = 256;
+int runs_of(int64_t n) {
+  const int64_t runs = (n + kRunRows - 1) / kRunRows;
+  return static_cast<int>(runs < kMostRuns ? runs : kMostRuns);
+}
+
+__device__ __forceinline__ int key_of(const int32_t* group_of, int i, int groups) {
+  const int g = group_of[i];
+  return g < 0 || g >= groups ? groups : g;
+}
+
+// counts of each wavefront's share [begin, end) of the rows into LDS
+__device__ __forceinline__ void count_share(const int32_t* group_of, int begin, int end, int groups, int* bins) {
+  const int lane = threadIdx.x & 63;
+  for (int g = lane; g <= groups; g += 64) bins[g] = 0;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  for (int i = begin + lane; i < end; i += 64) atomicAdd(&bins[key_of(group_of, i, groups)], 1);
+}
+
+__global__ __launch_bounds__(64 * kOrderWaves) void count_rows_kernel(const int32_t* __restrict__ group_of, int n, int groups, int per_run,
+                                                                      int32_t* __restrict__ counts) {
+  extern __shared__ int bins[];
+  const int wave = threadIdx.x >> 6, stride = groups + 1, share = (per_run + kOrderWaves - 1) / kOrderWaves;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * per_run;
+  const int last = static_cast<int>(min(first + per_run, static_cast<int64_t>(n)));
+  const int begin = static_cast<int>(min(first + static_cast<int64_t>(wave) * share, static_cast<int64_t>(last)));
+  count_share(group_of, begin, min(begin + share, last), groups, bins + wave * stride);
+  __syncthreads();
+  for (int g = threadIdx.x; g <= groups; g += 64 * kOrderWaves) {
+    int sum = 0;
+    for (int w = 0; w < kOrderWaves; ++w) sum += bins[w * stride + g];
+    counts[static_cast<int64_t>(blockIdx.x) * stride + g] = sum;
+  }
+}
+
+// counts: of the runs, or null where there is but one
+__global__ __launch_bounds__(64 * kOrderWaves) void order_rows_kernel(const int32_t* __restrict__ group_of, int n, int groups, int per_run,
+                                                                      const int32_t* __restrict__ counts, int32_t* __restrict__ offsets,
+                                                                      int32_t* __restrict__ rows) {
+  extern __shared__ int bins[];  // of the wavefronts, then the total of each group
+  __shared__ int wave_sum[kOrderWaves];
+  constexpr int THREADS = 64 * kOrderWaves;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, stride = groups + 1, share = (per_run + kOrderWaves - 1) / kOrderWaves;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * per_run;
+  const int last = static_cast<int>(min(first + per_run, static_cast<int64_t>(n)));
+  const int begin = static_cast<int>(min(first + static_cast<int64_t>(wave) * share, static_cast<int64_t>(last))), end = min(begin + share, last);
+  int* const total = bins + kOrderWaves * stride;
+  count_share(group_of, begin, end, groups, bins + wave * stride);
+  __syncthreads();
+  // each thread a run of groups: totals, where the groups begin, and from there where each wavefront's rows do
+  const int each = (stride + THREADS - 1) / THREADS;
+  const int g0 = min(static_cast<int>(threadIdx.x) * each, stride), g1 = min(g0 + each, stride);
+  for (int g = threadIdx.x; g < stride; g += THREADS) {
+    int all = 0, before = 0;
+    if (counts != nullptr) {
+      for (int r = 0; r < static_cast<int>(gridDim.x); ++r) {
+        const int c = counts[static_cast<int64_t>(r) * stride + g];
+        all += c;
+        before += r < static_cast<int>(blockIdx.x) ? c : 0;
+      }
+    } else {
+      for (int w = 0; w < kOrderWaves; ++w) all += bins[w * stride + g];
+    }
+    total[g] = all;
+    int at = before;
+    for (int w = 0; w < kOrderWaves; ++w) {
+      const int c = bins[w * stride + g];
+      bins[w * stride + g] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+  int mine = 0;
+  for (int g = g0; g < g1; ++g) mine += total[g];
+  int sum = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int below = __shfl_up(sum, d);
+    if (lane >= d) sum += below;
+  }
+  if (lane == 63) wave_sum[wave] = sum;
+  __syncthreads();
+  int start = sum - mine;
+  for (int w = 0; w < wave; ++w) start += wave_sum[w];
+  for (int g = g0; g < g1; ++g) {
+    if (blockIdx.x == 0) offsets[g] = start;  // offsets[groups]: where the rows of no group begin
+    for (int w = 0; w < kOrderWaves; ++w) bins[w * stride + g] += start;
+    start += total[g];
+  }
+  __syncthreads();
+  int* const next = bins + wave * stride;
+  int bits = 1;
+  while ((1 << bits) <= groups) ++bits;
+  for (int i0 = begin; i0 < end; i0 += 64) {
+    const int i = i0 + lane;
+    const bool there = i < end;
+    const int key = there ? key_of(group_of, i, groups) : 0;
+    unsigned long long same = __ballot(there);  // lanes with this lane's group
+    for (int b = 0; b < bits; ++b) {
+      const bool set = (key >> b) & 1;
+      const unsigned long long with = __ballot(set);
+      same &= set ? with : ~with;
+    }
+    const int ahead = __popcll(same & ((1ull << lane) - 1));
+    const int at = there ? next[key] + ahead : 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (there) {
+      rows[at] = i;
+      if (ahead == 0) next[key] = at + __popcll(same);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+int check_groups(int64_t n, int groups) {
+  ITEXHIP_REQUIRE(groups >= 1 && groups <= kMaxGroups, "itexhip_group_rows: 1 .. 1024 groups, got %d", groups);
+  ITEXHIP_REQUIRE(n >= 0 && n < kMaxRows, "itexhip_group_rows: rows are 0 .. 2^30 - 1");
+  return ITEXHIP_OK;
+}
+
+}  // namespace
+}  // namespace itexhip
+
+using namespace itexhip;
+
+extern "C" int itexhip_route(const itexhip_route_params* p, int64_t tokens, const void* logits, const float* bias, int32_t* experts_out,
+                             float* weights_out, void* stream) {
+  ITEXHIP_REQUIRE(p != nullptr, "itexhip_route: null parameters");
+  ITEXHIP_REQUIRE(is_chosen_type(p->type), "itexhip_route: the type is float, bfloat16 or half");
+  ITEXHIP_REQUIRE(p->experts >= 1 && p->experts <= kMaxGroups, "itexhip_route: 1 .. 1024 experts, got %d", p->experts);
+  ITEXHIP_REQUIRE(p->score == ITEXHIP_ROUTE_SOFTMAX || p->score == ITEXHIP_ROUTE_SIGMOID, "itexhip_route: score is softmax or sigmoid");
+  ITEXHIP_REQUIRE(p->groups >= 1 && p->groups <= 64 && p->experts % p->groups == 0, "itexhip_route: 1 .. 64 groups of equally many experts");
+  ITEXHIP_REQUIRE(p->top_groups >= 1 && p->top_groups <= p->groups, "itexhip_route: top_groups is 1 .. groups");
+  const int size = p->experts / p->groups;
+  ITEXHIP_REQUIRE(p->group_best == 1 || (p->group_best == 2 && size >= 2), "itexhip_route: group_best is 1, or 2 where groups have two experts");
+  ITEXHIP_REQUIRE(p->top_k >= 1 && p->top_k <= 32 && p->top_k <= size * p->top_groups,
+                  "itexhip_route: top_k is 1 .. 32 and no more than the experts of top_groups groups");
+  ITEXHIP_REQUIRE(isfinite(p->scale), "itexhip_route: scale is finite");
+  ITEXHIP_REQUIRE(tokens >= 0 && tokens < kMaxRows, "itexhip_route: tokens are 0 .. 2^30 - 1");
+  ITEXHIP_REQUIRE(p->logits_stride >= 0 && p->logits_stride < (1LL << 31), "itexhip_route: bad logits_stride");
+  if (tokens == 0) return ITEXHIP_OK;
+  ITEXHIP_REQUIRE(logits && experts_out && weights_out, "itexhip_route: null buffer");
+  ITEXHIP_REQUIRE(aligned(logits, element_size(p->type)) && aligned(bias, 4) && aligned(experts_out, 4) && aligned(weights_out, 4),
+                  "itexhip_route: buffers are aligned to their elements");
+  const RouteArgs A{*p, logits, bias, experts_out, weights_out, tokens, 0};
+  hipStream_t st = as_stream(stream);
+  if (p->type == ITEXHIP_FLOAT) launch_route<ITEXHIP_FLOAT>(A, st);
+  else if (p->type == ITEXHIP_BFLOAT16) launch_route<ITEXHIP_BFLOAT16>(A, st);
+  else launch_route<ITEXHIP_HALF>(A, st);
+  ITEXHIP_CHECK_LAUNCH("itexhip_route");
+  return ITEXHIP_OK;
+}
+
+extern "C" int64_t itexhip_group_rows_workspace(int64_t n, int groups) {
+  if (check_groups(n, groups) != ITEXHIP_OK) return 0;
+  return (static_cast<int64_t>(runs_of(n)) * (groups + 1) * 4 + 16 + 15) / 16 * 16;
+}
+
+extern "C" int itexhip_group_rows(int64_t n, int groups, const int32_t* group_of, int32_t* offsets_out, int32_t* rows_out, void* workspace,
+                                  void* stream) {
+  if (const int e = check_groups(n, groups)) return e;
+  ITEXHIP_REQUIRE(offsets_out && (n == 0 || (group_of && rows_out && workspace)), "itexhip_group_rows: null buffer");
+  ITEXHIP_REQUIRE(aligned(group_of, 4) && aligned(offsets_out, 4) && aligned(rows_out, 4) && aligned(workspace, 16),
+                  "itexhip_group_rows: buffers are aligned to their elements, the workspace to 16 bytes");
+  hipStream_t st = as_stream(stream);
+  const int runs = n == 0 ? 1 : runs_of(n), per_run = n == 0 ? 1 : static_cast<int>((n + runs - 1) / runs);
+  const size_t bins = static_cast<size_t>(groups + 1) * 4;
+  int32_t* const counts = runs > 1 ? static_cast<int32_t*>(workspace) : nullptr;
+  if (runs > 1)
+    count_rows_kernel<<<runs, 64 * kOrderWaves, bins * kOrderWaves, st>>>(group_of, static_cast<int>(n), groups, per_run, counts);
+  order_rows_kernel<<<runs, 64 * kOrderWaves, bins * (kOrderWaves + 1), st>>>(group_of, static_cast<int>(n), groups, per_run, counts, offsets_out,
+                                                                               rows_out);
+  ITEXHIP_CHECK_LAUNCH("itexhip_group_rows");
+  return ITEXHIP_OK;
+}

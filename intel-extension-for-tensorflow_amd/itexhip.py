@@ -21,6 +21,7 @@ ACT_NONE, ACT_RELU, ACT_RELU6, ACT_LEAKYRELU, ACT_GELU_APPROX, ACT_GELU_EXACT = 
 ACT_ELU, ACT_SIGMOID, ACT_TANH, ACT_SWISH, ACT_MISH = 6, 7, 8, 9, 10
 ELT_RELU, ELT_CLIP, ELT_LINEAR, ELT_GELU_TANH, ELT_GELU_ERF, ELT_SUM = 1, 2, 3, 4, 5, 6
 ELT_ELU, ELT_LOGISTIC, ELT_TANH, ELT_SWISH, ELT_MISH = 7, 8, 9, 10, 11
+ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
 ROPE_NONE, ROPE_LINEAR, ROPE_NTK, ROPE_LLAMA3, ROPE_YARN = 0, 1, 2, 3, 4
 
 EXPORTS = [
@@ -39,6 +40,8 @@ EXPORTS = [
     "itexhip_qconv2d_implicit_ok", "itexhip_qconv2d", "itexhip_qgemm_sum", "itexhip_qconv2d_sum", "itexhip_qdepthwise_conv2d",
     "itexhip_rope_frequencies", "itexhip_qk_norm_rope", "itexhip_kv4_page_bytes", "itexhip_kv4_append", "itexhip_kv4_gather",
     "itexhip_kv4_attention_workspace", "itexhip_kv4_attention",
+    "itexhip_route", "itexhip_group_rows_workspace", "itexhip_group_rows", "itexhip_experts_workspace", "itexhip_experts_up",
+    "itexhip_experts_down", "itexhip_adapters_workspace", "itexhip_adapters",
 ]
 
 
@@ -662,5 +665,90 @@ def kv4_attention(p, c, q, cache, block_table, cu_q, kv_len, workspace, out, lse
                                          _addr(workspace), _addr(out), _addr(lse), _addr(stream)))
 
 
+# ---- linears whose weights a token chooses -----------------------------------------------------------
+class RouteParams(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("type", "experts", "top_k", "score", "groups", "top_groups", "group_best", "renormalise")] + \
+               [("scale", C.c_float), ("logits_stride", C.c_int64)]
+
+
+class ExpertsParams(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("type", "experts", "top_k", "activation", "gated")] + \
+               [(n, C.c_int64) for n in ("tokens", "hidden", "inner", "x_stride", "addend_stride", "out_stride")]
+
+
+class AdaptersParams(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("type", "adapters", "rank", "n_slices")] + [("tokens", C.c_int64), ("in_", C.c_int64), ("slice_end", C.c_int64 * 4)] + \
+               [(n, C.c_int64) for n in ("x_stride", "base_stride", "out_stride")]
+
+
+_CHOSEN = {name: _bind("itexhip_" + name, signature) for name, signature in (
+    ("route", "plppppp"), ("group_rows", "lippppp"), ("experts_up", "ppppppppp"), ("experts_down", "pppppppppppp"), ("adapters", "pppppppppppp"))}
+for _name in ("group_rows_workspace", "experts_workspace", "adapters_workspace"):
+    getattr(_lib, "itexhip_" + _name).restype = C.c_int64
+
+
+def route_params(type, experts, top_k, score=ROUTE_SOFTMAX, groups=1, top_groups=1, group_best=1, renormalise=False, scale=1.0, logits_stride=None):
+    return RouteParams(type, int(experts), int(top_k), int(score), int(groups), int(top_groups), int(group_best), int(bool(renormalise)), scale,
+                       int(experts if logits_stride is None else logits_stride))
+
+
+def route(p, tokens, logits, bias, experts_out, weights_out, stream=0):
+    if not _call.route(p, tokens, logits, bias, experts_out, weights_out, stream):
+        _check(_CHOSEN["route"](C.byref(p), int(tokens), _addr(logits), _addr(bias), _addr(experts_out), _addr(weights_out), _addr(stream)))
+
+
+def group_rows_workspace(n, groups):
+    """Bytes of device memory that group_rows needs besides its arguments."""
+    return _size(_lib.itexhip_group_rows_workspace(_i64(n), C.c_int(int(groups))))
+
+
+def group_rows(n, groups, group_of, offsets_out, rows_out, workspace, stream=0):
+    if not _call.group_rows(n, groups, group_of, offsets_out, rows_out, workspace, stream):
+        _check(_CHOSEN["group_rows"](int(n), int(groups), _addr(group_of), _addr(offsets_out), _addr(rows_out), _addr(workspace), _addr(stream)))
+
+
+def experts_params(type, experts, top_k, tokens, hidden, inner, activation=ACT_SWISH, gated=True, x_stride=None, addend_stride=None, out_stride=None):
+    """Strides (between tokens) in elements, hidden where not given."""
+    x, a, o = (int(hidden if s is None else s) for s in (x_stride, addend_stride, out_stride))
+    return ExpertsParams(type, int(experts), int(top_k), int(activation), int(bool(gated)), int(tokens), int(hidden), int(inner), x, a, o)
+
+
+def experts_workspace(p):
+    """Bytes of device memory that experts_up and experts_down need besides their arguments."""
+    return _size(_lib.itexhip_experts_workspace(C.byref(p)))
+
+
+def experts_up(p, x, offsets, rows, packed, scales, h, workspace, stream=0):
+    if not _call.experts_up(p, x, offsets, rows, packed, scales, h, workspace, stream):
+        _check(_CHOSEN["experts_up"](C.byref(p), _addr(x), _addr(offsets), _addr(rows), _addr(packed), _addr(scales), _addr(h), _addr(workspace),
+                                     _addr(stream)))
+
+
+def experts_down(p, h, experts, offsets, rows, packed, scales, weights, addend, out, workspace, stream=0):
+    if not _call.experts_down(p, h, experts, offsets, rows, packed, scales, weights, addend, out, workspace, stream):
+        _check(_CHOSEN["experts_down"](C.byref(p), _addr(h), _addr(experts), _addr(offsets), _addr(rows), _addr(packed), _addr(scales), _addr(weights),
+                                       _addr(addend), _addr(out), _addr(workspace), _addr(stream)))
+
+
+def adapters_params(type, adapters, rank, tokens, in_dim, slice_ends, x_stride=None, base_stride=None, out_stride=None):
+    """slice_ends: the column behind each slice, the last one the width of the output; strides (between tokens) in elements, dense where not given."""
+    ends = [int(n) for n in slice_ends]
+    x = int(in_dim if x_stride is None else x_stride)
+    base, out = (int(ends[-1] if s is None else s) for s in (base_stride, out_stride))
+    return AdaptersParams(type, int(adapters), int(rank), len(ends), int(tokens), int(in_dim), (C.c_int64 * 4)(*ends[:4]), x, base, out)
+
+
+def adapters_workspace(p):
+    """Bytes of device memory that adapters needs besides its arguments."""
+    return _size(_lib.itexhip_adapters_workspace(C.byref(p)))
+
+
+def adapters(p, x, offsets, rows, a, b, ranks, scales, base, out, workspace, stream=0):
+    if not _call.adapters(p, x, offsets, rows, a, b, ranks, scales, base, out, workspace, stream):
+        _check(_CHOSEN["adapters"](C.byref(p), _addr(x), _addr(offsets), _addr(rows), _addr(a), _addr(b), _addr(ranks), _addr(scales), _addr(base),
+                                   _addr(out), _addr(workspace), _addr(stream)))
+
+
 _call.init(lambda name: C.cast(getattr(_lib, name), C.c_void_p).value, _check,
-           (MatmulParams, Epilogue, BmmParams, ConvGeometry, HeadsParams, Kv4Cache, Kv4AttentionParams))
+           (MatmulParams, Epilogue, BmmParams, ConvGeometry, HeadsParams, Kv4Cache, Kv4AttentionParams, RouteParams,
+            ExpertsParams, AdaptersParams))
