@@ -56,11 +56,17 @@ inline int64_t tiles_bound(int64_t n, int groups, int per_tile, bool rest) {
 struct RowTile {
   int group;       // groups: the rows of no group
   int begin, rows; // places
-  int first;       // of the group's places
 };
-// By all lanes of a wavefront, the same for all.  Offsets are cut to 0 .. n, so that whatever they hold, places are.
+// The group of the index-th of its tiles' `units` (as many of each tile), by all lanes of a wavefront and the same for all.
+// Offsets are cut to 0 .. n, so that whatever they hold, places are.
+struct GroupUnit {
+  int group;          // -1: there are no more than `total` units
+  int begin, rows;    // the group's places
+  int tiles;          // of the group
+  int64_t index, total;
+};
 template <bool REST>
-__device__ __forceinline__ RowTile find_tile(const int32_t* __restrict__ offsets, int groups, int n, int per_tile, int index) {
+__device__ __forceinline__ GroupUnit find_unit(const int32_t* __restrict__ offsets, int groups, int n, int per_tile, int64_t units, int64_t index) {
   const int lane = static_cast<int>(__lane_id());
   const int parts = groups + (REST ? 1 : 0), each = (parts + 63) / 64;
   const int begin = lane * each, end = min(begin + each, parts);
@@ -74,15 +80,22 @@ __device__ __forceinline__ RowTile find_tile(const int32_t* __restrict__ offsets
     const int below = __shfl_up(sum, d);
     if (lane >= d) sum += below;
   }
-  const unsigned long long past = __ballot(sum > index);
-  if (past == 0) return RowTile{-1, 0, 0, 0};
+  const int64_t total = __builtin_amdgcn_readlane(sum, 63) * units;
+  const unsigned long long past = __ballot(sum * units > index);
+  if (past == 0) return GroupUnit{-1, 0, 0, 0, 0, total};
   const int owner = __builtin_ctzll(past);
-  int rank = index - (__builtin_amdgcn_readlane(sum, owner) - __builtin_amdgcn_readlane(mine, owner));
+  int64_t rank = index - (__builtin_amdgcn_readlane(sum, owner) - __builtin_amdgcn_readlane(mine, owner)) * units;
   for (int g = owner * each;; ++g) {
     const int first = at(g), rows = max(at(g + 1) - first, 0), tiles = (rows + per_tile - 1) / per_tile;
-    if (rank < tiles) return RowTile{g, first + rank * per_tile, min(per_tile, rows - rank * per_tile), first};
-    rank -= tiles;
+    if (rank < tiles * units) return GroupUnit{g, first, rows, tiles, rank, total};
+    rank -= tiles * units;
   }
+}
+template <bool REST>
+__device__ __forceinline__ RowTile find_tile(const int32_t* __restrict__ offsets, int groups, int n, int per_tile, int index) {
+  const GroupUnit u = find_unit<REST>(offsets, groups, n, per_tile, 1, index);
+  const int before = static_cast<int>(u.index) * per_tile;
+  return RowTile{u.group, u.begin + before, min(per_tile, u.rows - before)};
 }
 
 }  // namespace itexhip

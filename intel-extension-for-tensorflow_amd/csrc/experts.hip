@@ -190,6 +190,215 @@ __global__ __launch_bounds__(256) void experts_stream_kernel(const ProductArgs A
   });
 }
 
+// ------------------------------------------------------------------------------------------------
+// Many rows an expert: tiles of BM places of one expert and BN channels (gated: BN / 2 of the gate and the same BN / 2 of the up weight, so
+// that a wavefront ends with both sums of a value), K in steps of 64.  Four wavefronts of (BM / 2) x (BN / 2) accumulators in
+// MFMA tiles of 32 x 32.  Both operands reach LDS by direct loads, three steps ahead in a ring of four; a step's fragments are read
+// during the step before it, one load or read behind each MFMA, so that one wavefront a SIMD keeps the matrix core fed.
+// Activation rows lie in LDS 16 to a KiB, a row's four 16-byte pieces in the lanes of a quad, turned by (row / 4) so that the 16 lanes
+// served at a time read 16 different bank groups; weights are packed in fragment order and copied as they are.
+//
+// Tiles are numbered expert by expert, within an expert in groups of up to 8 tiles of rows, there column by column, and each XCD has
+// a contiguous run of the numbers: its 32 workgroups share a few columns of weights and up to 8 tiles of rows in their L2.
+// ------------------------------------------------------------------------------------------------
+constexpr int kTileGroup = 8;  // tiles of rows that share a column
+
+template <int OUT, bool GATED, int BM, int BN>
+__global__ __launch_bounds__(256) void experts_tile_kernel(const ProductArgs A) {
+  constexpr bool UP = OUT != 0;
+  constexpr int EACH = GATED ? 2 : 1, NSTAGE = 4, AHEAD = 3;
+  constexpr int TM = BM / 64, TN = BN / 64;                       // MFMA tiles of a wavefront
+  constexpr int A_LOADS = BM / 16, B_LOADS = BN / 16;             // of 1 KiB a step
+  constexpr int A_PER_WAVE = A_LOADS / 4, B_PER_WAVE = B_LOADS / 4, NLD = A_PER_WAVE + B_PER_WAVE;
+  constexpr int STAGE = (A_LOADS + B_LOADS) * kChunkBytes, B_REGION = A_LOADS * kChunkBytes;
+  constexpr int NSLICE = 2 * TN, FA = 2 * TM;
+  constexpr int OUT_TN = TN / EACH, WIDTH = BN / EACH;            // MFMA tiles of results; channels of a tile
+  static_assert(A_LOADS % 4 == 0 && B_LOADS % 4 == 0 && TN % EACH == 0 && NSLICE % 4 == 0, "loads and tiles divide among wavefronts");
+  extern __shared__ __align__(16) uint8_t lds[];
+  const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)lds));
+  float* const panel = reinterpret_cast<float*>(lds + NSTAGE * STAGE);  // scales of the tile's BN channels, wavefront by wavefront
+
+  const int columns = (A.N + WIDTH - 1) / WIDTH;
+  const int64_t id = A.first + blockIdx.x, local = id >> 3;
+  // the run of this XCD: total / 8 of the numbers, whose count only the offsets tell
+  GroupUnit u = find_unit<false>(A.offsets, A.experts, A.slots, BM, columns, 0);
+  const int64_t run = (u.total + 7) >> 3, number = (id & 7) * run + local;
+  if (local >= run || number >= u.total) return;
+  u = find_unit<false>(A.offsets, A.experts, A.slots, BM, columns, number);
+  const int group = static_cast<int>(u.index / (kTileGroup * columns));
+  const int in_group = static_cast<int>(u.index - static_cast<int64_t>(group) * (kTileGroup * columns));
+  const int group_rows = min(kTileGroup, u.tiles - group * kTileGroup);
+  const int tile_n = in_group / group_rows, tile_m = group * kTileGroup + in_group - tile_n * group_rows;
+  const int begin = u.begin + tile_m * BM, rows = min(BM, u.rows - tile_m * BM), n_base = tile_n * WIDTH;
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wm = wave & 1, wn = wave >> 1, lrow = lane & 31, lgrp = lane >> 5;
+
+  // channels of column tile c of the block: which weight, first channel
+  auto which_of = [](int c) { return GATED ? c % TN / OUT_TN : 0; };
+  auto channel_of = [&](int c) { return n_base + (GATED ? c / TN * OUT_TN + c % OUT_TN : c) * 32; };
+  const int8_t* const weights = A.packed + static_cast<int64_t>(u.group) * EACH * A.panel;
+  if (threadIdx.x < BN) {
+    const int c = threadIdx.x >> 5, n = min(channel_of(c) + static_cast<int>(threadIdx.x & 31), A.N - 1);
+    panel[threadIdx.x] = A.scales[(static_cast<int64_t>(u.group) * EACH + which_of(c)) * A.N + n];
+  }
+
+  const int q_row = lane >> 2, q_piece = (lane & 3) ^ ((q_row >> 2) & 3);
+  const int8_t* src_a[A_PER_WAVE];
+  const int8_t* src_b[B_PER_WAVE];
+  static_for<A_PER_WAVE>([&](auto c) {
+    const int place = begin + min((wave * A_PER_WAVE + static_cast<int>(c)) * 16 + q_row, rows - 1);
+    const int row = UP ? slot_of(A, place) / A.top_k : place;
+    src_a[c] = A.codes + static_cast<int64_t>(row) * A.pitch + q_piece * 16;
+  });
+  static_for<B_PER_WAVE>([&](auto c) {
+    const int ld = wave * B_PER_WAVE + static_cast<int>(c), strip = min(channel_of(ld >> 1) >> 5, A.strips - 1);
+    src_b[c] = weights + which_of(ld >> 1) * A.panel + (static_cast<int64_t>(strip) * A.chunks + (ld & 1)) * kChunkBytes;
+  });
+  const uint32_t lane16 = lane * 16;
+  auto issue = [&](auto c, int kt, int stage) {
+    constexpr int ci = decltype(c)::value;
+    const uint32_t to = lds_base + stage * STAGE;
+    if constexpr (ci < A_PER_WAVE)
+      lds_dma16(src_a[ci] + kt * 64, to + (wave * A_PER_WAVE + ci) * kChunkBytes);
+    else
+      lds_dma16(src_b[ci - A_PER_WAVE] + static_cast<int64_t>(kt) * (2 * kChunkBytes), lane16, to + B_REGION + (wave * B_PER_WAVE + ci - A_PER_WAVE) * kChunkBytes);
+  };
+  const int fq = lrow & 15, fh = lrow >> 4;
+  const uint32_t frag_a[2] = {static_cast<uint32_t>(fh * kChunkBytes + ((4 * fq + ((0 + lgrp) ^ ((fq >> 2) & 3))) << 4)),
+                              static_cast<uint32_t>(fh * kChunkBytes + ((4 * fq + ((2 + lgrp) ^ ((fq >> 2) & 3))) << 4))};
+  auto read_a = [&](int stage, int kc, int i) {
+    return *reinterpret_cast<const v4i*>(lds + stage * STAGE + (wm * TM + i) * (2 * kChunkBytes) + frag_a[kc]);
+  };
+  auto read_b = [&](int stage, int kc, int j) {
+    return *reinterpret_cast<const v4i*>(lds + stage * STAGE + B_REGION + ((wn * TN + j) * 2 + kc) * kChunkBytes + lane * 16);
+  };
+
+  const int KT = A.chunks / 2;
+  static_for<AHEAD>([&](auto k) {
+    static_for<NLD>([&](auto c) { issue(c, min(decltype(k)::value, KT - 1), decltype(k)::value); });
+  });
+  v16i acc[TN * TM];
+  static_for<TN * TM>([&](auto t) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[t][r] = 0;
+  });
+  wait_vmcnt<(AHEAD - 2) * NLD>();
+  __syncthreads();
+
+  v4i fa0[FA], fa1[FA], fb[4];
+  static_for<FA>([&](auto x) { fa0[x] = read_a(0, decltype(x)::value / TM, decltype(x)::value % TM); });
+  static_for<2>([&](auto d) { fb[d] = read_b(0, decltype(d)::value / TN, decltype(d)::value % TN); });
+  // No branches: behind the last step the loads fetch that step again, into stages that nobody reads
+  auto step = [&](int kt, const v4i (&now)[FA], v4i (&next)[FA]) {
+    const int st_now = kt & (NSTAGE - 1), st_next = (kt + 1) & (NSTAGE - 1), st_fill = (kt + AHEAD) & (NSTAGE - 1);
+    const int kt_load = min(kt + AHEAD, KT - 1);
+    static_for<NSLICE>([&](auto sl) {
+      constexpr int s = decltype(sl)::value, kc = s / TN, j = s % TN;
+      static_for<TM>([&](auto i) {
+        constexpr int ii = decltype(i)::value, t = j * TM + ii;
+        acc[t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[s % 4], now[kc * TM + ii], acc[t], 0, 0, 0);
+        if constexpr (ii == 0) {
+          constexpr int sn = s + 2;  // weight fragments are read two slices ahead
+          if constexpr (sn < NSLICE) fb[sn % 4] = read_b(st_now, sn / TN, sn % TN);
+          else fb[sn % 4] = read_b(st_next, (sn - NSLICE) / TN, (sn - NSLICE) % TN);
+        }
+        if constexpr (ii == TM - 1) {
+          static_for<NLD>([&](auto c) {
+            if constexpr (decltype(c)::value * NSLICE / NLD == s) issue(c, kt_load, st_fill);
+          });
+        }
+        if constexpr (s < NSLICE / 2) {  // activation fragments of the next step during the first half
+          constexpr int Q = NSLICE / 2 * TM, q = s * TM + ii, shift = Q >= 2 * FA ? 1 : 0;
+          static_for<FA>([&](auto x) {
+            if constexpr (decltype(x)::value * Q / FA + shift == q) next[decltype(x)::value] = read_a(st_next, decltype(x)::value / TM, decltype(x)::value % TM);
+          });
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    });
+    wait_vmcnt<(AHEAD - 2) * NLD>();
+    __syncthreads();
+  };
+  int kt = 0;
+  if (KT & 1) {
+    step(0, fa0, fa1);
+    static_for<FA>([&](auto x) { fa0[x] = fa1[x]; });
+    kt = 1;
+  }
+  for (; kt < KT; kt += 2) {
+    step(kt, fa0, fa1);
+    step(kt + 1, fa1, fa0);
+  }
+  wait_vmcnt<0>();  // no load may still be writing LDS
+  __syncthreads();
+
+  // ---- results.  A lane has groups of 4 channels of one row; they go through a private piece of LDS (32 rows of 64 channels and a
+  // pad) to rows of contiguous bytes.
+  constexpr int ESZ = UP ? (OUT == ITEXHIP_FLOAT ? 4 : 2) : 4;
+  constexpr int PAIR = OUT_TN >= 2 ? 2 : 1, ROWB = PAIR * 32 * ESZ, PITCH = ROWB + 16;
+  uint8_t* const buffer = lds + wave * (32 * PITCH);
+  static_assert(4 * 32 * PITCH <= NSTAGE * STAGE, "the buffers fit the ring");
+  constexpr int LPR = ROWB / 16, RPP = 64 / LPR;   // lanes a row, rows a store
+  const bool whole_rows = ((static_cast<uint32_t>(A.N) * ESZ | static_cast<uint32_t>(reinterpret_cast<uintptr_t>(A.out))) & 15) == 0;
+  const float* const scale0 = panel + wn * TN * 32 + lgrp * 4;
+  static_for<TM>([&](auto tile) {
+    constexpr int i = decltype(tile)::value;
+    const int m0 = wm * (BM / 2) + i * 32;
+    if (m0 >= rows) return;  // the same for the whole wavefront
+    const int place = begin + min(m0 + lrow, rows - 1);
+    const float s = A.row_scales[UP ? slot_of(A, place) / A.top_k : place];
+    static_for<OUT_TN / PAIR>([&](auto pair) {
+      static_for<PAIR>([&](auto half) {
+        constexpr int j = decltype(pair)::value * PAIR + decltype(half)::value;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f4 of0 = *reinterpret_cast<const f4*>(scale0 + j * 32 + g * 8);
+          float y[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) y[r] = static_cast<float>(acc[j * TM + i][g * 4 + r]) * (s * of0[r]);
+          if constexpr (UP) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[r] = activate(A.activation, y[r]);
+          }
+          if constexpr (GATED) {
+            const f4 of1 = *reinterpret_cast<const f4*>(scale0 + (OUT_TN + j) * 32 + g * 8);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[r] = y[r] * (static_cast<float>(acc[(OUT_TN + j) * TM + i][g * 4 + r]) * (s * of1[r]));
+          }
+          uint8_t* const to = buffer + lrow * PITCH + (decltype(half)::value * 32 + g * 8 + lgrp * 4) * ESZ;
+          if constexpr (ESZ == 4) *reinterpret_cast<f4*>(to) = f4{y[0], y[1], y[2], y[3]};
+          else *reinterpret_cast<uint2*>(to) = uint2{f32x2_to_bits16<UP ? OUT : ITEXHIP_HALF>(y[0], y[1]), f32x2_to_bits16<UP ? OUT : ITEXHIP_HALF>(y[2], y[3])};
+        }
+      });
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      const int n0 = n_base + (wn * OUT_TN + decltype(pair)::value * PAIR) * 32;
+#pragma unroll
+      for (int p = 0; p < 32 / RPP; ++p) {
+        const int r = p * RPP + lane / LPR, n = n0 + lane % LPR * (16 / ESZ);
+        const v4i v = *reinterpret_cast<const v4i*>(buffer + r * PITCH + lane % LPR * 16);
+        if (m0 + r >= rows || n >= A.N) continue;
+        const int at = begin + m0 + r;
+        const int64_t row = UP ? at : slot_of(A, at);
+        uint8_t* const to = static_cast<uint8_t*>(A.out) + (row * A.N + n) * ESZ;
+        if (whole_rows) {
+          *reinterpret_cast<v4i*>(to) = v;
+        } else {
+#pragma unroll
+          for (int w = 0; w < 16 / ESZ; ++w) {
+            if (n + w >= A.N) continue;
+            if constexpr (ESZ == 4) *reinterpret_cast<int*>(to + w * 4) = v[w];
+            else *reinterpret_cast<uint16_t*>(to + w * 2) = static_cast<uint16_t>(static_cast<uint32_t>(v[w / 2]) >> (16 * (w % 2)));
+          }
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    });
+  });
+}
+
 // out[t] = addend[t] + sum of the weighted results of the token's choices, in their order
 template <int T, bool VEC>
 __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ experts, const float* __restrict__ weights,
@@ -276,10 +485,30 @@ void launch_stream(ProductArgs A, hipStream_t st) {
     experts_stream_kernel<OUT, GATED, RT><<<count, 256, 0, st>>>(A);
   });
 }
+template <int OUT, bool GATED, int BM, int BN>
+int launch_tiles(ProductArgs A, hipStream_t st) {
+  constexpr int WIDTH = GATED ? BN / 2 : BN, LDS = 4 * (BM + BN) * 64 + BN * 4;
+  static unsigned long long configured;
+  const auto kernel = experts_tile_kernel<OUT, GATED, BM, BN>;
+  if (!device_bit(&configured, false)) {
+    const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    if (err != hipSuccess) return hip_fail(err, "hipFuncSetAttribute(experts_tile_kernel)");
+    device_bit(&configured, true);
+  }
+  const int64_t tiles = tiles_bound(A.slots, A.experts, BM, false) * ((A.N + WIDTH - 1) / WIDTH);
+  launch_blocks((tiles + 7) / 8 * 8, [&](int64_t first, unsigned count) {
+    A.first = first;
+    kernel<<<count, 256, LDS, st>>>(A);
+  });
+  return ITEXHIP_OK;
+}
 template <int OUT, bool GATED>
-void launch_products(const ProductArgs& A, hipStream_t st) {
-  if (A.slots > 64 * A.experts) launch_stream<OUT, GATED, 4>(A, st);
-  else launch_stream<OUT, GATED, 1>(A, st);
+int launch_products(const ProductArgs& A, hipStream_t st) {
+  const int64_t each = A.slots / A.experts;
+  if (each > 128) return launch_tiles<OUT, GATED, 256, 256>(A, st);
+  if (each > 64) return launch_tiles<OUT, GATED, 128, 256>(A, st);
+  launch_stream<OUT, GATED, 1>(A, st);
+  return ITEXHIP_OK;
 }
 
 ProductArgs product_args(const itexhip_experts_params& p, bool up, const Layout& l, void* workspace, const int32_t* offsets, const int32_t* rows,
@@ -306,27 +535,27 @@ ProductArgs product_args(const itexhip_experts_params& p, bool up, const Layout&
 }
 
 template <int T>
-void run_up(const itexhip_experts_params& p, const void* x, const int32_t* offsets, const int32_t* rows, const int8_t* packed, const float* scales,
+int run_up(const itexhip_experts_params& p, const void* x, const int32_t* offsets, const int32_t* rows, const int8_t* packed, const float* scales,
             void* h, void* workspace, hipStream_t st) {
   const Layout l = layout_of(p, true);
   const ProductArgs A = product_args(p, true, l, workspace, offsets, rows, packed, scales, h);
   launch_quantize<T>(x, p.x_stride, p.tokens, p.hidden, const_cast<int8_t*>(A.codes), const_cast<float*>(A.row_scales), st);
-  if (p.gated) launch_products<T, true>(A, st);
-  else launch_products<T, false>(A, st);
+  return p.gated ? launch_products<T, true>(A, st) : launch_products<T, false>(A, st);
 }
 
 template <int T>
-void run_down(const itexhip_experts_params& p, const void* h, const int32_t* experts, const int32_t* offsets, const int32_t* rows, const int8_t* packed,
+int run_down(const itexhip_experts_params& p, const void* h, const int32_t* experts, const int32_t* offsets, const int32_t* rows, const int8_t* packed,
               const float* scales, const float* weights, const void* addend, void* out, void* workspace, hipStream_t st) {
   const Layout l = layout_of(p, false);
   float* const results = reinterpret_cast<float*>(static_cast<char*>(workspace) + l.results);
   const ProductArgs A = product_args(p, false, l, workspace, offsets, rows, packed, scales, results);
   launch_quantize<T>(h, p.inner, A.slots, p.inner, const_cast<int8_t*>(A.codes), const_cast<float*>(A.row_scales), st);
-  launch_products<0, false>(A, st);
+  if (const int e = launch_products<0, false>(A, st)) return e;
   const auto combine = p.hidden % 4 == 0 ? combine_kernel<T, true> : combine_kernel<T, false>;
   launch_blocks(p.tokens, [&](int64_t first, unsigned count) {
     combine<<<count, 256, 0, st>>>(results, experts, weights, addend, p.addend_stride, out, p.out_stride, p.experts, p.top_k, A.N, first);
   });
+  return ITEXHIP_OK;
 }
 
 }  // namespace
@@ -349,9 +578,10 @@ extern "C" int itexhip_experts_up(const itexhip_experts_params* p, const void* x
                   "itexhip_experts_up: buffers are aligned to their elements");
   ITEXHIP_REQUIRE(aligned(packed, 16) && aligned(workspace, 16), "itexhip_experts_up: packed weights and workspace are aligned to 16 bytes");
   hipStream_t st = as_stream(stream);
-  if (p->type == ITEXHIP_FLOAT) run_up<ITEXHIP_FLOAT>(*p, x, offsets, rows, packed, scales, h, workspace, st);
-  else if (p->type == ITEXHIP_BFLOAT16) run_up<ITEXHIP_BFLOAT16>(*p, x, offsets, rows, packed, scales, h, workspace, st);
-  else run_up<ITEXHIP_HALF>(*p, x, offsets, rows, packed, scales, h, workspace, st);
+  const int status = p->type == ITEXHIP_FLOAT      ? run_up<ITEXHIP_FLOAT>(*p, x, offsets, rows, packed, scales, h, workspace, st)
+                     : p->type == ITEXHIP_BFLOAT16 ? run_up<ITEXHIP_BFLOAT16>(*p, x, offsets, rows, packed, scales, h, workspace, st)
+                                                   : run_up<ITEXHIP_HALF>(*p, x, offsets, rows, packed, scales, h, workspace, st);
+  if (status != ITEXHIP_OK) return status;
   ITEXHIP_CHECK_LAUNCH("itexhip_experts_up");
   return ITEXHIP_OK;
 }
@@ -368,9 +598,10 @@ extern "C" int itexhip_experts_down(const itexhip_experts_params* p, const void*
                   "itexhip_experts_down: buffers are aligned to their elements");
   ITEXHIP_REQUIRE(aligned(packed, 16) && aligned(workspace, 16), "itexhip_experts_down: packed weights and workspace are aligned to 16 bytes");
   hipStream_t st = as_stream(stream);
-  if (p->type == ITEXHIP_FLOAT) run_down<ITEXHIP_FLOAT>(*p, h, experts, offsets, rows, packed, scales, weights, addend, out, workspace, st);
-  else if (p->type == ITEXHIP_BFLOAT16) run_down<ITEXHIP_BFLOAT16>(*p, h, experts, offsets, rows, packed, scales, weights, addend, out, workspace, st);
-  else run_down<ITEXHIP_HALF>(*p, h, experts, offsets, rows, packed, scales, weights, addend, out, workspace, st);
+  const int status = p->type == ITEXHIP_FLOAT      ? run_down<ITEXHIP_FLOAT>(*p, h, experts, offsets, rows, packed, scales, weights, addend, out, workspace, st)
+                     : p->type == ITEXHIP_BFLOAT16 ? run_down<ITEXHIP_BFLOAT16>(*p, h, experts, offsets, rows, packed, scales, weights, addend, out, workspace, st)
+                                                   : run_down<ITEXHIP_HALF>(*p, h, experts, offsets, rows, packed, scales, weights, addend, out, workspace, st);
+  if (status != ITEXHIP_OK) return status;
   ITEXHIP_CHECK_LAUNCH("itexhip_experts_down");
   return ITEXHIP_OK;
 }
