@@ -57,43 +57,61 @@ struct RowTile {
   int group;       // groups: the rows of no group
   int begin, rows; // places
 };
-// The group of the index-th of its tiles' `units` (as many of each tile), by all lanes of a wavefront and the same for all.
-// Offsets are cut to 0 .. n, so that whatever they hold, places are.
+// The groups' tiles, counted by all lanes of a wavefront; a lane has `each` neighbouring groups.  Offsets are cut to 0 .. n, so that
+// whatever they hold, places are.
 struct GroupUnit {
-  int group;          // -1: there are no more than `total` units
+  int group;          // -1: there are not that many units
   int begin, rows;    // the group's places
   int tiles;          // of the group
-  int64_t index, total;
+  int64_t index;      // within the group
 };
 template <bool REST>
-__device__ __forceinline__ GroupUnit find_unit(const int32_t* __restrict__ offsets, int groups, int n, int per_tile, int64_t units, int64_t index) {
-  const int lane = static_cast<int>(__lane_id());
-  const int parts = groups + (REST ? 1 : 0), each = (parts + 63) / 64;
-  const int begin = lane * each, end = min(begin + each, parts);
-  auto at = [&](int g) { return g > groups ? n : min(max(offsets[g], 0), n); };
-  auto tiles_of = [&](int g) { return (max(at(g + 1) - at(g), 0) + per_tile - 1) / per_tile; };
-  int mine = 0;
-  for (int g = begin; g < end; ++g) mine += tiles_of(g);
-  int sum = mine;  // of the lanes up to this one
+struct TileCount {
+  const int32_t* offsets;
+  int groups, n, per_tile, each;
+  int begin, rows;    // of the lane's first group
+  int mine, sum;      // tiles of the lane's groups; and with those of the lanes below
+  __device__ __forceinline__ int at(int g) const { return g > groups ? n : min(max(offsets[g], 0), n); }
+  __device__ __forceinline__ TileCount(const int32_t* offsets, int groups, int n, int per_tile)
+      : offsets(offsets), groups(groups), n(n), per_tile(per_tile) {
+    const int lane = static_cast<int>(__lane_id()), parts = groups + (REST ? 1 : 0);
+    each = (parts + 63) / 64;
+    const int g0 = min(lane * each, parts), g1 = min(g0 + each, parts);
+    begin = rows = mine = 0;
+    if (g0 < g1) {
+      begin = at(g0);
+      rows = max(at(g0 + 1) - begin, 0);
+      mine = (rows + per_tile - 1) / per_tile;
+      for (int g = g0 + 1; g < g1; ++g) mine += (max(at(g + 1) - at(g), 0) + per_tile - 1) / per_tile;
+    }
+    sum = mine;
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int below = __shfl_up(sum, d);
-    if (lane >= d) sum += below;
+    for (int d = 1; d < 64; d *= 2) {
+      const int below = __shfl_up(sum, d);
+      if (lane >= d) sum += below;
+    }
   }
-  const int64_t total = __builtin_amdgcn_readlane(sum, 63) * units;
-  const unsigned long long past = __ballot(sum * units > index);
-  if (past == 0) return GroupUnit{-1, 0, 0, 0, 0, total};
-  const int owner = __builtin_ctzll(past);
-  int64_t rank = index - (__builtin_amdgcn_readlane(sum, owner) - __builtin_amdgcn_readlane(mine, owner)) * units;
-  for (int g = owner * each;; ++g) {
-    const int first = at(g), rows = max(at(g + 1) - first, 0), tiles = (rows + per_tile - 1) / per_tile;
-    if (rank < tiles * units) return GroupUnit{g, first, rows, tiles, rank, total};
-    rank -= tiles * units;
+  __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(sum, 63); }
+  // Whose the index-th unit is where every tile has `units` of them; the same for all lanes
+  __device__ __forceinline__ GroupUnit find(int64_t units, int64_t index) const {
+    const unsigned long long past = __ballot(sum * units > index);
+    if (past == 0) return GroupUnit{-1, 0, 0, 0, 0};
+    const int owner = __builtin_ctzll(past);
+    int64_t rank = index - (__builtin_amdgcn_readlane(sum, owner) - __builtin_amdgcn_readlane(mine, owner)) * units;
+    int first = __builtin_amdgcn_readlane(begin, owner), count = __builtin_amdgcn_readlane(rows, owner);
+    for (int g = owner * each;;) {
+      const int tiles = (count + per_tile - 1) / per_tile;
+      if (rank < tiles * units) return GroupUnit{g, first, count, tiles, rank};
+      rank -= tiles * units;
+      ++g;
+      first = __builtin_amdgcn_readfirstlane(at(g));
+      count = __builtin_amdgcn_readfirstlane(max(at(g + 1) - first, 0));
+    }
   }
-}
+};
 template <bool REST>
 __device__ __forceinline__ RowTile find_tile(const int32_t* __restrict__ offsets, int groups, int n, int per_tile, int index) {
-  const GroupUnit u = find_unit<REST>(offsets, groups, n, per_tile, 1, index);
+  const GroupUnit u = TileCount<REST>(offsets, groups, n, per_tile).find(1, index);
   const int before = static_cast<int>(u.index) * per_tile;
   return RowTile{u.group, u.begin + before, min(per_tile, u.rows - before)};
 }

@@ -27,7 +27,8 @@ __device__ __forceinline__ float scale_of(uint32_t absmax_bits) {
   return fmaxf(__uint_as_float(absmax_bits) / 127.0f, kLeastScale);
 }
 
-template <int T, bool VEC>
+// HELD: runs of 8 elements that a thread keeps between the two passes (0: it reads them again)
+template <int T, bool VEC, int HELD>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const void* __restrict__ x, int64_t stride, int K, int pitch, int8_t* __restrict__ codes,
                                                             float* __restrict__ scales, int64_t first) {
   __shared__ uint32_t most[4];
@@ -41,11 +42,22 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const void* __restri
     }
   };
   uint32_t top = 0;
-  for (int k = threadIdx.x * 8; k < K; k += 2048) {
-    float v[8];
-    load(k, v);
+  auto largest = [&](const float (&v)[8]) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+  };
+  float held[HELD > 0 ? HELD : 1][8];
+  if constexpr (HELD > 0) {
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) load(h * 2048 + threadIdx.x * 8, held[h]);
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) largest(held[h]);
+  } else {
+    for (int k = threadIdx.x * 8; k < K; k += 2048) {
+      float v[8];
+      load(k, v);
+      largest(v);
+    }
   }
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d)));
@@ -55,13 +67,22 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const void* __restri
   const float s = scale_of(top), inv = 1.0f / s;
   const bool finite = s == s;
   if (threadIdx.x == 0) scales[row] = s;
-  for (int k = threadIdx.x * 8; k < pitch; k += 2048) {
-    float v[8];
-    load(k, v);
+  auto store = [&](int k, const float (&v)[8]) {
     int c[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) c[j] = finite ? code_of(v[j], s, inv) : 0;
     *reinterpret_cast<uint2*>(codes + row * pitch + k) = uint2{pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7])};
+  };
+  if constexpr (HELD > 0) {
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+      if (h * 2048 + static_cast<int>(threadIdx.x) * 8 < pitch) store(h * 2048 + threadIdx.x * 8, held[h]);
+  } else {
+    for (int k = threadIdx.x * 8; k < pitch; k += 2048) {
+      float v[8];
+      load(k, v);
+      store(k, v);
+    }
   }
 }
 
@@ -193,17 +214,48 @@ __global__ __launch_bounds__(256) void experts_stream_kernel(const ProductArgs A
 // ------------------------------------------------------------------------------------------------
 // Many rows an expert: tiles of BM places of one expert and BN channels (gated: BN / 2 of the gate and the same BN / 2 of the up weight, so
 // that a wavefront ends with both sums of a value), K in steps of 64.  Four wavefronts of (BM / 2) x (BN / 2) accumulators in
-// MFMA tiles of 32 x 32.  Both operands reach LDS by direct loads, three steps ahead in a ring of four; a step's fragments are read
+// MFMA tiles of 32 x 32, the tiles of rows in turns.  Both operands reach LDS by direct loads, three steps ahead in a ring of four; a step's fragments are read
 // during the step before it, one load or read behind each MFMA, so that one wavefront a SIMD keeps the matrix core fed.
 // Activation rows lie in LDS 16 to a KiB, a row's four 16-byte pieces in the lanes of a quad, turned by (row / 4) so that the 16 lanes
 // served at a time read 16 different bank groups; weights are packed in fragment order and copied as they are.
 //
 // Tiles are numbered expert by expert, within an expert in groups of up to 8 tiles of rows, there column by column, and each XCD has
-// a contiguous run of the numbers: its 32 workgroups share a few columns of weights and up to 8 tiles of rows in their L2.
+// a contiguous run of the numbers: its 32 workgroups share a few columns of weights and up to 8 tiles of rows in their L2.  A workgroup
+// stays for all its tiles: the last steps of one fetch the first ones of the next, which then travel while results are written.
 // ------------------------------------------------------------------------------------------------
 constexpr int kTileGroup = 8;  // tiles of rows that share a column
+constexpr int kTileSteps = 4;  // K steps that a tile has to have
+// MFMA tiles of results that go through a wavefront's piece of LDS at a time: 128 bytes of a row
+constexpr int tile_pair(int element, int out_tn) { return element == 2 && out_tn >= 2 ? 2 : 1; }
+constexpr int tile_lds(int element, int out_tn, int bm, int bn) {
+  return 4 * (bm + bn) * 64 + 3 * bn * 4 + 4 * 32 * (tile_pair(element, out_tn) * 32 * element + 16);
+}
 
-template <int OUT, bool GATED, int BM, int BN>
+// The activation of 16 values, chosen once for them
+__device__ __forceinline__ void activate16(int activation, float (&y)[16]) {
+#define ITEXHIP_EACH(ACT) _Pragma("unroll") for (int r = 0; r < 16; ++r) y[r] = activate(ACT, y[r])
+  if (activation == ITEXHIP_ACT_SWISH) ITEXHIP_EACH(ITEXHIP_ACT_SWISH);
+  else if (activation == ITEXHIP_ACT_RELU) ITEXHIP_EACH(ITEXHIP_ACT_RELU);
+  else if (activation == ITEXHIP_ACT_GELU_APPROX) ITEXHIP_EACH(ITEXHIP_ACT_GELU_APPROX);
+  else if (activation == ITEXHIP_ACT_GELU_EXACT) ITEXHIP_EACH(ITEXHIP_ACT_GELU_EXACT);
+#undef ITEXHIP_EACH
+}
+
+// A pointer that all lanes have, in scalar registers
+__device__ __forceinline__ const int8_t* uniform(const int8_t* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int>(v)), hi = __builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32));
+  return reinterpret_cast<const int8_t*>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// lds_dma16 to OFFSET behind lds_addr, the sum formed in m0
+template <int OFFSET>
+__device__ __forceinline__ void lds_dma16_at(const void* base, uint32_t lane_offset, uint32_t lds_addr) {
+  asm volatile("s_add_u32 m0, %2, %3\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(lane_offset), "s"(base), "s"(lds_addr), "i"(OFFSET) : "memory", "m0", "scc");
+}
+
+// SWISH: the activation, known when compiled; with the others beside it this one's code would be fetched around them
+template <int OUT, bool GATED, bool SWISH, int BM, int BN>
 __global__ __launch_bounds__(256) void experts_tile_kernel(const ProductArgs A) {
   constexpr bool UP = OUT != 0;
   constexpr int EACH = GATED ? 2 : 1, NSTAGE = 4, AHEAD = 3;
@@ -211,192 +263,248 @@ __global__ __launch_bounds__(256) void experts_tile_kernel(const ProductArgs A) 
   constexpr int A_LOADS = BM / 16, B_LOADS = BN / 16;             // of 1 KiB a step
   constexpr int A_PER_WAVE = A_LOADS / 4, B_PER_WAVE = B_LOADS / 4, NLD = A_PER_WAVE + B_PER_WAVE;
   constexpr int STAGE = (A_LOADS + B_LOADS) * kChunkBytes, B_REGION = A_LOADS * kChunkBytes;
-  constexpr int NSLICE = 2 * TN, FA = 2 * TM;
+  constexpr int NSLICE = 2 * TN;
   constexpr int OUT_TN = TN / EACH, WIDTH = BN / EACH;            // MFMA tiles of results; channels of a tile
   static_assert(A_LOADS % 4 == 0 && B_LOADS % 4 == 0 && TN % EACH == 0 && NSLICE % 4 == 0, "loads and tiles divide among wavefronts");
   extern __shared__ __align__(16) uint8_t lds[];
   const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)lds));
-  float* const panel = reinterpret_cast<float*>(lds + NSTAGE * STAGE);  // scales of the tile's BN channels, wavefront by wavefront
+  // behind the ring: scales of a tile's BN channels, wavefront by wavefront, for three tiles; the wavefronts' pieces for results
+  float* const panels = reinterpret_cast<float*>(lds + NSTAGE * STAGE);
+  uint8_t* const buffers = lds + NSTAGE * STAGE + 3 * BN * 4;
 
   const int columns = (A.N + WIDTH - 1) / WIDTH;
-  const int64_t id = A.first + blockIdx.x, local = id >> 3;
-  // the run of this XCD: total / 8 of the numbers, whose count only the offsets tell
-  GroupUnit u = find_unit<false>(A.offsets, A.experts, A.slots, BM, columns, 0);
-  const int64_t run = (u.total + 7) >> 3, number = (id & 7) * run + local;
-  if (local >= run || number >= u.total) return;
-  u = find_unit<false>(A.offsets, A.experts, A.slots, BM, columns, number);
-  const int group = static_cast<int>(u.index / (kTileGroup * columns));
-  const int in_group = static_cast<int>(u.index - static_cast<int64_t>(group) * (kTileGroup * columns));
-  const int group_rows = min(kTileGroup, u.tiles - group * kTileGroup);
-  const int tile_n = in_group / group_rows, tile_m = group * kTileGroup + in_group - tile_n * group_rows;
-  const int begin = u.begin + tile_m * BM, rows = min(BM, u.rows - tile_m * BM), n_base = tile_n * WIDTH;
+  const TileCount<false> count(A.offsets, A.experts, A.slots, BM);
+  // the run of this XCD: an eighth of the numbers, whose count only the offsets tell
+  const int64_t total = static_cast<int64_t>(count.total()) * columns, run = (total + 7) >> 3, run_begin = (blockIdx.x & 7) * run;
+  const int64_t stride = gridDim.x >> 3;
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = wave & 1, wn = wave >> 1, lrow = lane & 31, lgrp = lane >> 5;
-
-  // channels of column tile c of the block: which weight, first channel
-  auto which_of = [](int c) { return GATED ? c % TN / OUT_TN : 0; };
-  auto channel_of = [&](int c) { return n_base + (GATED ? c / TN * OUT_TN + c % OUT_TN : c) * 32; };
-  const int8_t* const weights = A.packed + static_cast<int64_t>(u.group) * EACH * A.panel;
-  if (threadIdx.x < BN) {
-    const int c = threadIdx.x >> 5, n = min(channel_of(c) + static_cast<int>(threadIdx.x & 31), A.N - 1);
-    panel[threadIdx.x] = A.scales[(static_cast<int64_t>(u.group) * EACH + which_of(c)) * A.N + n];
-  }
-
   const int q_row = lane >> 2, q_piece = (lane & 3) ^ ((q_row >> 2) & 3);
-  const int8_t* src_a[A_PER_WAVE];
-  const int8_t* src_b[B_PER_WAVE];
-  static_for<A_PER_WAVE>([&](auto c) {
-    const int place = begin + min((wave * A_PER_WAVE + static_cast<int>(c)) * 16 + q_row, rows - 1);
-    const int row = UP ? slot_of(A, place) / A.top_k : place;
-    src_a[c] = A.codes + static_cast<int64_t>(row) * A.pitch + q_piece * 16;
-  });
-  static_for<B_PER_WAVE>([&](auto c) {
-    const int ld = wave * B_PER_WAVE + static_cast<int>(c), strip = min(channel_of(ld >> 1) >> 5, A.strips - 1);
-    src_b[c] = weights + which_of(ld >> 1) * A.panel + (static_cast<int64_t>(strip) * A.chunks + (ld & 1)) * kChunkBytes;
-  });
+  // column tile c of the block: which weight, and its first channel from the tile's on
+  auto which_of = [](int c) { return GATED ? c % TN / OUT_TN : 0; };
+  auto channel_of = [](int c) { return (GATED ? c / TN * OUT_TN + c % OUT_TN : c) * 32; };
+
+  struct Work {
+    bool there;
+    int begin, rows, n_base;
+  };
+  // Where a tile's operands are loaded from: bases that are the same for the wavefront, and a lane's offsets from them
+  struct Source {
+    const int8_t* a;
+    uint32_t row[A_PER_WAVE];
+    const int8_t* b[B_PER_WAVE];
+  };
+  auto find = [&](int64_t local, Work& w, Source& src, float* panel) {
+    const int64_t number = run_begin + local;
+    w.there = local < run && number < total;
+    if (!w.there) return;
+    const GroupUnit u = count.find(columns, number);
+    const int group = __builtin_amdgcn_readfirstlane(static_cast<int>(u.index / (kTileGroup * columns)));
+    const int in_group = static_cast<int>(u.index - static_cast<int64_t>(group) * (kTileGroup * columns));
+    const int group_rows = min(kTileGroup, u.tiles - group * kTileGroup);
+    const int tile_n = __builtin_amdgcn_readfirstlane(in_group / group_rows), tile_m = group * kTileGroup + in_group - tile_n * group_rows;
+    w.begin = u.begin + tile_m * BM;
+    w.rows = min(BM, u.rows - tile_m * BM);
+    w.n_base = tile_n * WIDTH;
+    static_for<A_PER_WAVE>([&](auto c) {
+      const int in_tile = min((wave * A_PER_WAVE + static_cast<int>(c)) * 16 + q_row, w.rows - 1);
+      const uint32_t row = UP ? slot_of(A, w.begin + in_tile) / A.top_k : in_tile;
+      src.row[c] = row * static_cast<uint32_t>(A.pitch) + q_piece * 16;  // up: all codes are below 4 GiB, which the host checks
+    });
+    src.a = UP ? A.codes : A.codes + static_cast<int64_t>(w.begin) * A.pitch;
+    const int8_t* const weights = A.packed + static_cast<int64_t>(u.group) * EACH * A.panel;
+    static_for<B_PER_WAVE>([&](auto c) {
+      const int ld = wave * B_PER_WAVE + static_cast<int>(c), strip = min((w.n_base + channel_of(ld >> 1)) >> 5, A.strips - 1);
+      src.b[c] = weights + which_of(ld >> 1) * A.panel + (static_cast<int64_t>(strip) * A.chunks + (ld & 1)) * kChunkBytes;
+    });
+    if (threadIdx.x < BN) {
+      const int c = threadIdx.x >> 5, n = min(w.n_base + channel_of(c) + static_cast<int>(threadIdx.x & 31), A.N - 1);
+      panel[threadIdx.x] = A.scales[(static_cast<int64_t>(u.group) * EACH + which_of(c)) * A.N + n];
+    }
+  };
   const uint32_t lane16 = lane * 16;
-  auto issue = [&](auto c, int kt, int stage) {
+  auto issue = [&](auto c, const Source& src, uint32_t step_b, int stage) {
     constexpr int ci = decltype(c)::value;
-    const uint32_t to = lds_base + stage * STAGE;
-    if constexpr (ci < A_PER_WAVE)
-      lds_dma16(src_a[ci] + kt * 64, to + (wave * A_PER_WAVE + ci) * kChunkBytes);
-    else
-      lds_dma16(src_b[ci - A_PER_WAVE] + static_cast<int64_t>(kt) * (2 * kChunkBytes), lane16, to + B_REGION + (wave * B_PER_WAVE + ci - A_PER_WAVE) * kChunkBytes);
+    const uint32_t to = lds_base + stage * STAGE + wave * (ci < A_PER_WAVE ? A_PER_WAVE : B_PER_WAVE) * kChunkBytes;
+    if constexpr (ci < A_PER_WAVE) lds_dma16_at<ci * kChunkBytes>(src.a, src.row[ci], to);
+    else lds_dma16_at<B_REGION + (ci - A_PER_WAVE) * kChunkBytes>(src.b[ci - A_PER_WAVE], step_b, to);
   };
   const int fq = lrow & 15, fh = lrow >> 4;
   const uint32_t frag_a[2] = {static_cast<uint32_t>(fh * kChunkBytes + ((4 * fq + ((0 + lgrp) ^ ((fq >> 2) & 3))) << 4)),
                               static_cast<uint32_t>(fh * kChunkBytes + ((4 * fq + ((2 + lgrp) ^ ((fq >> 2) & 3))) << 4))};
   auto read_a = [&](int stage, int kc, int i) {
-    return *reinterpret_cast<const v4i*>(lds + stage * STAGE + (wm * TM + i) * (2 * kChunkBytes) + frag_a[kc]);
+    return *reinterpret_cast<const v4i*>(lds + stage * STAGE + (2 * i + wm) * (2 * kChunkBytes) + frag_a[kc]);
   };
   auto read_b = [&](int stage, int kc, int j) {
     return *reinterpret_cast<const v4i*>(lds + stage * STAGE + B_REGION + ((wn * TN + j) * 2 + kc) * kChunkBytes + lane * 16);
   };
 
-  const int KT = A.chunks / 2;
+  const int KT = A.chunks / 2;  // at least AHEAD: the last steps of a tile fetch the first ones of the next
+  int64_t local = blockIdx.x >> 3;
+  Work now, next;
+  Source src, next_src;   // src: of the step that is loaded next; its second offset:
+  uint32_t step_b = lane16;
+  find(local, now, src, panels);
+  if (!now.there) return;
+  auto make_uniform = [](Source& s) {
+    s.a = uniform(s.a);
+    static_for<B_PER_WAVE>([&](auto c) { s.b[c] = uniform(s.b[c]); });
+  };
+  make_uniform(src);
   static_for<AHEAD>([&](auto k) {
-    static_for<NLD>([&](auto c) { issue(c, min(decltype(k)::value, KT - 1), decltype(k)::value); });
-  });
-  v16i acc[TN * TM];
-  static_for<TN * TM>([&](auto t) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[t][r] = 0;
+    static_for<NLD>([&](auto c) { issue(c, src, step_b, decltype(k)::value); });
+    src.a += 64;
+    step_b += 2 * kChunkBytes;
   });
   wait_vmcnt<(AHEAD - 2) * NLD>();
   __syncthreads();
 
-  v4i fa0[FA], fa1[FA], fb[4];
-  static_for<FA>([&](auto x) { fa0[x] = read_a(0, decltype(x)::value / TM, decltype(x)::value % TM); });
-  static_for<2>([&](auto d) { fb[d] = read_b(0, decltype(d)::value / TN, decltype(d)::value % TN); });
-  // No branches: behind the last step the loads fetch that step again, into stages that nobody reads
-  auto step = [&](int kt, const v4i (&now)[FA], v4i (&next)[FA]) {
-    const int st_now = kt & (NSTAGE - 1), st_next = (kt + 1) & (NSTAGE - 1), st_fill = (kt + AHEAD) & (NSTAGE - 1);
-    const int kt_load = min(kt + AHEAD, KT - 1);
-    static_for<NSLICE>([&](auto sl) {
-      constexpr int s = decltype(sl)::value, kc = s / TN, j = s % TN;
-      static_for<TM>([&](auto i) {
-        constexpr int ii = decltype(i)::value, t = j * TM + ii;
-        acc[t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[s % 4], now[kc * TM + ii], acc[t], 0, 0, 0);
-        if constexpr (ii == 0) {
-          constexpr int sn = s + 2;  // weight fragments are read two slices ahead
-          if constexpr (sn < NSLICE) fb[sn % 4] = read_b(st_now, sn / TN, sn % TN);
-          else fb[sn % 4] = read_b(st_next, (sn - NSLICE) / TN, (sn - NSLICE) % TN);
-        }
-        if constexpr (ii == TM - 1) {
-          static_for<NLD>([&](auto c) {
-            if constexpr (decltype(c)::value * NSLICE / NLD == s) issue(c, kt_load, st_fill);
-          });
-        }
-        if constexpr (s < NSLICE / 2) {  // activation fragments of the next step during the first half
-          constexpr int Q = NSLICE / 2 * TM, q = s * TM + ii, shift = Q >= 2 * FA ? 1 : 0;
-          static_for<FA>([&](auto x) {
-            if constexpr (decltype(x)::value * Q / FA + shift == q) next[decltype(x)::value] = read_a(st_next, decltype(x)::value / TM, decltype(x)::value % TM);
-          });
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      });
+  int ring = 0;  // stage of the tile's first step
+  for (int slot = 0;; slot = slot == 2 ? 0 : slot + 1) {
+    // (a third panel: a wavefront may be here while another one still is at the results of the tile before)
+    find(local += stride, next, next_src, panels + (slot == 2 ? 0 : slot + 1) * BN);
+    const bool more = __builtin_amdgcn_readfirstlane(next.there);  // what is fetched behind the last tile is not used
+    v16i acc[TN * TM];
+    static_for<TN * TM>([&](auto t) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[t][r] = 0;
     });
-    wait_vmcnt<(AHEAD - 2) * NLD>();
-    __syncthreads();
-  };
-  int kt = 0;
-  if (KT & 1) {
-    step(0, fa0, fa1);
-    static_for<FA>([&](auto x) { fa0[x] = fa1[x]; });
-    kt = 1;
-  }
-  for (; kt < KT; kt += 2) {
-    step(kt, fa0, fa1);
-    step(kt + 1, fa1, fa0);
-  }
-  wait_vmcnt<0>();  // no load may still be writing LDS
-  __syncthreads();
-
-  // ---- results.  A lane has groups of 4 channels of one row; they go through a private piece of LDS (32 rows of 64 channels and a
-  // pad) to rows of contiguous bytes.
-  constexpr int ESZ = UP ? (OUT == ITEXHIP_FLOAT ? 4 : 2) : 4;
-  constexpr int PAIR = OUT_TN >= 2 ? 2 : 1, ROWB = PAIR * 32 * ESZ, PITCH = ROWB + 16;
-  uint8_t* const buffer = lds + wave * (32 * PITCH);
-  static_assert(4 * 32 * PITCH <= NSTAGE * STAGE, "the buffers fit the ring");
-  constexpr int LPR = ROWB / 16, RPP = 64 / LPR;   // lanes a row, rows a store
-  const bool whole_rows = ((static_cast<uint32_t>(A.N) * ESZ | static_cast<uint32_t>(reinterpret_cast<uintptr_t>(A.out))) & 15) == 0;
-  const float* const scale0 = panel + wn * TN * 32 + lgrp * 4;
-  static_for<TM>([&](auto tile) {
-    constexpr int i = decltype(tile)::value;
-    const int m0 = wm * (BM / 2) + i * 32;
-    if (m0 >= rows) return;  // the same for the whole wavefront
-    const int place = begin + min(m0 + lrow, rows - 1);
-    const float s = A.row_scales[UP ? slot_of(A, place) / A.top_k : place];
-    static_for<OUT_TN / PAIR>([&](auto pair) {
-      static_for<PAIR>([&](auto half) {
-        constexpr int j = decltype(pair)::value * PAIR + decltype(half)::value;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const f4 of0 = *reinterpret_cast<const f4*>(scale0 + j * 32 + g * 8);
-          float y[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) y[r] = static_cast<float>(acc[j * TM + i][g * 4 + r]) * (s * of0[r]);
-          if constexpr (UP) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) y[r] = activate(A.activation, y[r]);
-          }
-          if constexpr (GATED) {
-            const f4 of1 = *reinterpret_cast<const f4*>(scale0 + (OUT_TN + j) * 32 + g * 8);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) y[r] = y[r] * (static_cast<float>(acc[(OUT_TN + j) * TM + i][g * 4 + r]) * (s * of1[r]));
-          }
-          uint8_t* const to = buffer + lrow * PITCH + (decltype(half)::value * 32 + g * 8 + lgrp * 4) * ESZ;
-          if constexpr (ESZ == 4) *reinterpret_cast<f4*>(to) = f4{y[0], y[1], y[2], y[3]};
-          else *reinterpret_cast<uint2*>(to) = uint2{f32x2_to_bits16<UP ? OUT : ITEXHIP_HALF>(y[0], y[1]), f32x2_to_bits16<UP ? OUT : ITEXHIP_HALF>(y[2], y[3])};
+    // The steps of a tile whose wavefronts use TU of their TM tiles of rows: the last tile of an expert costs by 64 rows
+    auto multiply = [&](auto used) {
+      constexpr int TU = decltype(used)::value, FA = 2 * TU;
+      v4i fa0[FA], fa1[FA], fb[4];
+      static_for<FA>([&](auto x) { fa0[x] = read_a(ring, decltype(x)::value / TU, decltype(x)::value % TU); });
+      static_for<2>([&](auto d) { fb[d] = read_b(ring, decltype(d)::value / TN, decltype(d)::value % TN); });
+      auto step = [&](int kt, const v4i (&at)[FA], v4i (&then)[FA]) {
+        const int st_now = (ring + kt) & (NSTAGE - 1), st_next = (ring + kt + 1) & (NSTAGE - 1), st_fill = (ring + kt + AHEAD) & (NSTAGE - 1);
+        if (kt + AHEAD == KT) {
+          if (more) src = next_src;
+          else src.a -= static_cast<int64_t>(KT) * 64;
+          make_uniform(src);
+          step_b = lane16;
         }
-      });
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      const int n0 = n_base + (wn * OUT_TN + decltype(pair)::value * PAIR) * 32;
-#pragma unroll
-      for (int p = 0; p < 32 / RPP; ++p) {
-        const int r = p * RPP + lane / LPR, n = n0 + lane % LPR * (16 / ESZ);
-        const v4i v = *reinterpret_cast<const v4i*>(buffer + r * PITCH + lane % LPR * 16);
-        if (m0 + r >= rows || n >= A.N) continue;
-        const int at = begin + m0 + r;
-        const int64_t row = UP ? at : slot_of(A, at);
-        uint8_t* const to = static_cast<uint8_t*>(A.out) + (row * A.N + n) * ESZ;
-        if (whole_rows) {
-          *reinterpret_cast<v4i*>(to) = v;
-        } else {
-#pragma unroll
-          for (int w = 0; w < 16 / ESZ; ++w) {
-            if (n + w >= A.N) continue;
-            if constexpr (ESZ == 4) *reinterpret_cast<int*>(to + w * 4) = v[w];
-            else *reinterpret_cast<uint16_t*>(to + w * 2) = static_cast<uint16_t>(static_cast<uint32_t>(v[w / 2]) >> (16 * (w % 2)));
-          }
-        }
+        static_for<NSLICE>([&](auto sl) {
+          constexpr int s = decltype(sl)::value, kc = s / TN, j = s % TN;
+          static_for<TU>([&](auto i) {
+            constexpr int ii = decltype(i)::value, t = j * TM + ii;
+            acc[t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[s % 4], at[kc * TU + ii], acc[t], 0, 0, 0);
+            if constexpr (ii == 0) {
+              constexpr int sn = s + 2;  // weight fragments are read two slices ahead
+              if constexpr (sn < NSLICE) fb[sn % 4] = read_b(st_now, sn / TN, sn % TN);
+              else fb[sn % 4] = read_b(st_next, (sn - NSLICE) / TN, (sn - NSLICE) % TN);
+            }
+            if constexpr (ii == TU - 1) {
+              static_for<NLD>([&](auto c) {
+                if constexpr (decltype(c)::value * NSLICE / NLD == s) issue(c, src, step_b, st_fill);
+              });
+            }
+            if constexpr (s < NSLICE / 2) {  // activation fragments of the next step during the first half
+              constexpr int Q = NSLICE / 2 * TU, q = s * TU + ii, shift = Q >= 2 * FA ? 1 : 0;
+              static_for<FA>([&](auto x) {
+                if constexpr (decltype(x)::value * Q / FA + shift == q) then[decltype(x)::value] = read_a(st_next, decltype(x)::value / TU, decltype(x)::value % TU);
+              });
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          });
+        });
+        src.a += 64;
+        step_b += 2 * kChunkBytes;
+        wait_vmcnt<(AHEAD - 2) * NLD>();
+        __syncthreads();
+      };
+      int kt = 0;
+      if (KT & 1) {
+        step(0, fa0, fa1);
+        static_for<FA>([&](auto x) { fa0[x] = fa1[x]; });
+        kt = 1;
       }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
+      for (; kt < KT; kt += 2) {
+        step(kt, fa0, fa1);
+        step(kt + 1, fa1, fa0);
+      }
+    };
+    const int used = __builtin_amdgcn_readfirstlane((now.rows + 63) / 64);
+    static_for<TM>([&](auto less) {
+      if (used == static_cast<int>(less) + 1) multiply(std::integral_constant<int, decltype(less)::value + 1>{});
     });
-  });
+    ring = (ring + KT) & (NSTAGE - 1);
+
+    // ---- results.  A lane has groups of 4 channels of one row; they go through a private piece of LDS (32 rows of a few channels and
+    // a pad) to rows of contiguous bytes.
+    // (lane numbers that the compiler does not know: what follows from them is not kept in registers, of which there are none, throughout the steps)
+    int el = lane;
+    asm volatile("" : "+v"(el));
+    const int erow = el & 31, egrp = el >> 5;
+    constexpr int ESZ = UP ? (OUT == ITEXHIP_FLOAT ? 4 : 2) : 4;
+    constexpr int PAIR = tile_pair(ESZ, OUT_TN), ROWB = PAIR * 32 * ESZ, PITCH = ROWB + 16;
+    uint8_t* const buffer = buffers + wave * (32 * PITCH);
+    constexpr int LPR = ROWB / 16, RPP = 64 / LPR;   // lanes a row, rows a store
+    const bool whole_rows = ((static_cast<uint32_t>(A.N) * ESZ | static_cast<uint32_t>(reinterpret_cast<uintptr_t>(A.out))) & 15) == 0;
+    const float* const scale0 = panels + slot * BN + wn * TN * 32 + egrp * 4;
+    static_for<TM>([&](auto tile) {
+      constexpr int i = decltype(tile)::value;
+      const int m0 = (2 * i + wm) * 32;
+      if (m0 >= now.rows) return;  // the same for the whole wavefront
+      const int place = now.begin + min(m0 + erow, now.rows - 1);
+      const float s = A.row_scales[UP ? slot_of(A, place) / A.top_k : place];
+      static_for<OUT_TN / PAIR>([&](auto pair) {
+        static_for<PAIR>([&](auto half) {
+          constexpr int j = decltype(pair)::value * PAIR + decltype(half)::value;
+          float y[16];
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const f4 of = *reinterpret_cast<const f4*>(scale0 + j * 32 + g * 8);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[g * 4 + r] = static_cast<float>(acc[j * TM + i][g * 4 + r]) * (s * of[r]);
+          }
+          if constexpr (UP) activate16(SWISH ? ITEXHIP_ACT_SWISH : A.activation, y);
+          if constexpr (GATED) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const f4 of = *reinterpret_cast<const f4*>(scale0 + (OUT_TN + j) * 32 + g * 8);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) y[g * 4 + r] *= static_cast<float>(acc[(OUT_TN + j) * TM + i][g * 4 + r]) * (s * of[r]);
+            }
+          }
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            uint8_t* const to = buffer + erow * PITCH + (decltype(half)::value * 32 + g * 8 + egrp * 4) * ESZ;
+            const float* const v = y + g * 4;
+            if constexpr (ESZ == 4) *reinterpret_cast<f4*>(to) = f4{v[0], v[1], v[2], v[3]};
+            else *reinterpret_cast<uint2*>(to) = uint2{f32x2_to_bits16<UP ? OUT : ITEXHIP_HALF>(v[0], v[1]), f32x2_to_bits16<UP ? OUT : ITEXHIP_HALF>(v[2], v[3])};
+          }
+        });
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const int n0 = now.n_base + (wn * OUT_TN + decltype(pair)::value * PAIR) * 32;
+#pragma unroll
+        for (int p = 0; p < 32 / RPP; ++p) {
+          const int r = p * RPP + el / LPR, n = n0 + el % LPR * (16 / ESZ);
+          const v4i v = *reinterpret_cast<const v4i*>(buffer + r * PITCH + el % LPR * 16);
+          if (m0 + r >= now.rows || n >= A.N) continue;
+          const int at = now.begin + m0 + r;
+          const int64_t row = UP ? at : slot_of(A, at);
+          uint8_t* const to = static_cast<uint8_t*>(A.out) + (row * A.N + n) * ESZ;
+          if (whole_rows) {
+            *reinterpret_cast<v4i*>(to) = v;
+          } else {
+#pragma unroll
+            for (int w = 0; w < 16 / ESZ; ++w) {
+              if (n + w >= A.N) continue;
+              if constexpr (ESZ == 4) *reinterpret_cast<int*>(to + w * 4) = v[w];
+              else *reinterpret_cast<uint16_t*>(to + w * 2) = static_cast<uint16_t>(static_cast<uint32_t>(v[w / 2]) >> (16 * (w % 2)));
+            }
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      });
+    });
+    if (!more) break;
+    now = next;
+  }
+  wait_vmcnt<0>();  // no load may still be writing LDS when another workgroup has it
 }
 
 // out[t] = addend[t] + sum of the weighted results of the token's choices, in their order
@@ -472,7 +580,12 @@ Layout layout_of(const itexhip_experts_params& p, bool up) {
 template <int T>
 void launch_quantize(const void* x, int64_t stride, int64_t rows, int64_t K, int8_t* codes, float* scales, hipStream_t st) {
   const bool vec = aligned(x, 16) && (stride * element_size(T)) % 16 == 0;
-  const auto kernel = vec ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>;
+  const auto kernel = !vec           ? quantize_rows_kernel<T, false, 0>
+                      : K <= 1 * 2048 ? quantize_rows_kernel<T, true, 1>
+                      : K <= 2 * 2048 ? quantize_rows_kernel<T, true, 2>
+                      : K <= 4 * 2048 ? quantize_rows_kernel<T, true, 4>
+                      : K <= 7 * 2048 ? quantize_rows_kernel<T, true, 7>
+                                      : quantize_rows_kernel<T, true, 0>;
   launch_blocks(rows, [&](int64_t first, unsigned count) {
     kernel<<<count, 256, 0, st>>>(x, stride, static_cast<int>(K), static_cast<int>(pitch_of(K)), codes, scales, first);
   });
@@ -485,28 +598,32 @@ void launch_stream(ProductArgs A, hipStream_t st) {
     experts_stream_kernel<OUT, GATED, RT><<<count, 256, 0, st>>>(A);
   });
 }
-template <int OUT, bool GATED, int BM, int BN>
+constexpr int kWorkgroups = 256;  // one for each CU; they take the tiles in turns
+
+template <int OUT, bool GATED, bool SWISH, int BM, int BN>
 int launch_tiles(ProductArgs A, hipStream_t st) {
-  constexpr int WIDTH = GATED ? BN / 2 : BN, LDS = 4 * (BM + BN) * 64 + BN * 4;
+  constexpr int WIDTH = GATED ? BN / 2 : BN, LDS = tile_lds(OUT == ITEXHIP_BFLOAT16 || OUT == ITEXHIP_HALF ? 2 : 4, WIDTH / 64, BM, BN);
+  static_assert(LDS <= 160 * 1024, "LDS of a CU");
   static unsigned long long configured;
-  const auto kernel = experts_tile_kernel<OUT, GATED, BM, BN>;
+  const auto kernel = experts_tile_kernel<OUT, GATED, SWISH, BM, BN>;
   if (!device_bit(&configured, false)) {
     const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
     if (err != hipSuccess) return hip_fail(err, "hipFuncSetAttribute(experts_tile_kernel)");
     device_bit(&configured, true);
   }
   const int64_t tiles = tiles_bound(A.slots, A.experts, BM, false) * ((A.N + WIDTH - 1) / WIDTH);
-  launch_blocks((tiles + 7) / 8 * 8, [&](int64_t first, unsigned count) {
-    A.first = first;
-    kernel<<<count, 256, LDS, st>>>(A);
-  });
+  const int64_t grid = tiles < kWorkgroups ? (tiles + 7) / 8 * 8 : kWorkgroups;
+  kernel<<<static_cast<unsigned>(grid), 256, LDS, st>>>(A);
   return ITEXHIP_OK;
 }
 template <int OUT, bool GATED>
 int launch_products(const ProductArgs& A, hipStream_t st) {
   const int64_t each = A.slots / A.experts;
-  if (each > 128) return launch_tiles<OUT, GATED, 256, 256>(A, st);
-  if (each > 64) return launch_tiles<OUT, GATED, 128, 256>(A, st);
+  const bool near = OUT == 0 || A.slots / A.top_k * static_cast<int64_t>(A.pitch) < (1LL << 32);  // up: codes in reach of 32 bits
+  if (each > 64 && A.chunks >= 2 * kTileSteps && near) {
+    if (GATED && A.activation == ITEXHIP_ACT_SWISH) return launch_tiles<OUT, GATED, GATED, 256, 256>(A, st);
+    return launch_tiles<OUT, GATED, false, 256, 256>(A, st);
+  }
   launch_stream<OUT, GATED, 1>(A, st);
   return ITEXHIP_OK;
 }
