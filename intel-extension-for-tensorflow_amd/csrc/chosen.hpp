@@ -65,13 +65,17 @@ struct GroupUnit {
   int tiles;          // of the group
   int64_t index;      // within the group
 };
-template <bool REST>
+enum Tiles : int { kAllTiles, kFullTiles, kLastTiles };  // of a group; kLastTiles: those that are not full
+template <bool REST, int KIND = kAllTiles>
 struct TileCount {
   const int32_t* offsets;
   int groups, n, per_tile, each;
   int begin, rows;    // of the lane's first group
   int mine, sum;      // tiles of the lane's groups; and with those of the lanes below
   __device__ __forceinline__ int at(int g) const { return g > groups ? n : min(max(offsets[g], 0), n); }
+  __device__ __forceinline__ int tiles_of(int rows) const {
+    return KIND == kFullTiles ? rows / per_tile : KIND == kLastTiles ? rows % per_tile != 0 : (rows + per_tile - 1) / per_tile;
+  }
   __device__ __forceinline__ TileCount(const int32_t* offsets, int groups, int n, int per_tile)
       : offsets(offsets), groups(groups), n(n), per_tile(per_tile) {
     const int lane = static_cast<int>(__lane_id()), parts = groups + (REST ? 1 : 0);
@@ -81,8 +85,8 @@ struct TileCount {
     if (g0 < g1) {
       begin = at(g0);
       rows = max(at(g0 + 1) - begin, 0);
-      mine = (rows + per_tile - 1) / per_tile;
-      for (int g = g0 + 1; g < g1; ++g) mine += (max(at(g + 1) - at(g), 0) + per_tile - 1) / per_tile;
+      mine = tiles_of(rows);
+      for (int g = g0 + 1; g < g1; ++g) mine += tiles_of(max(at(g + 1) - at(g), 0));
     }
     sum = mine;
 #pragma unroll
@@ -100,7 +104,7 @@ struct TileCount {
     int64_t rank = index - (__builtin_amdgcn_readlane(sum, owner) - __builtin_amdgcn_readlane(mine, owner)) * units;
     int first = __builtin_amdgcn_readlane(begin, owner), count = __builtin_amdgcn_readlane(rows, owner);
     for (int g = owner * each;;) {
-      const int tiles = (count + per_tile - 1) / per_tile;
+      const int tiles = tiles_of(count);
       if (rank < tiles * units) return GroupUnit{g, first, count, tiles, rank};
       rank -= tiles * units;
       ++g;

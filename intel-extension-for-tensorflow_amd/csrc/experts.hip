@@ -220,7 +220,7 @@ __global__ __launch_bounds__(256) void experts_stream_kernel(const ProductArgs A
 // served at a time read 16 different bank groups; weights are packed in fragment order and copied as they are.
 //
 // Tiles are numbered expert by expert, within an expert in groups of up to 8 tiles of rows, there column by column, and each XCD has
-// a contiguous run of the numbers: its 32 workgroups share a few columns of weights and up to 8 tiles of rows in their L2.  A workgroup
+// a contiguous run of the experts' last tiles, which are not full, and then of the others: its 32 workgroups share a few columns of weights and up to 8 tiles of rows in their L2.  A workgroup
 // stays for all its tiles: the last steps of one fetch the first ones of the next, which then travel while results are written.
 // ------------------------------------------------------------------------------------------------
 constexpr int kTileGroup = 8;  // tiles of rows that share a column
@@ -228,7 +228,7 @@ constexpr int kTileSteps = 4;  // K steps that a tile has to have
 // MFMA tiles of results that go through a wavefront's piece of LDS at a time: 128 bytes of a row
 constexpr int tile_pair(int element, int out_tn) { return element == 2 && out_tn >= 2 ? 2 : 1; }
 constexpr int tile_lds(int element, int out_tn, int bm, int bn) {
-  return 4 * (bm + bn) * 64 + 3 * bn * 4 + 4 * 32 * (tile_pair(element, out_tn) * 32 * element + 16);
+  return 4 * (bm + bn) * 64 + 3 * (bn + 2 * bm) * 4 + 4 * 32 * (tile_pair(element, out_tn) * 32 * element + 16);
 }
 
 // The activation of 16 values, chosen once for them
@@ -268,15 +268,20 @@ __global__ __launch_bounds__(256) void experts_tile_kernel(const ProductArgs A) 
   static_assert(A_LOADS % 4 == 0 && B_LOADS % 4 == 0 && TN % EACH == 0 && NSLICE % 4 == 0, "loads and tiles divide among wavefronts");
   extern __shared__ __align__(16) uint8_t lds[];
   const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)lds));
-  // behind the ring: scales of a tile's BN channels, wavefront by wavefront, for three tiles; the wavefronts' pieces for results
+  // behind the ring, for three tiles: scales of its BN channels, wavefront by wavefront, scales of its rows and their slots; then the
+  // wavefronts' pieces for results
+  constexpr int PANEL = BN + 2 * BM;
   float* const panels = reinterpret_cast<float*>(lds + NSTAGE * STAGE);
-  uint8_t* const buffers = lds + NSTAGE * STAGE + 3 * BN * 4;
+  uint8_t* const buffers = lds + NSTAGE * STAGE + 3 * PANEL * 4;
 
   const int columns = (A.N + WIDTH - 1) / WIDTH;
-  const TileCount<false> count(A.offsets, A.experts, A.slots, BM);
-  // the run of this XCD: an eighth of the numbers, whose count only the offsets tell
-  const int64_t total = static_cast<int64_t>(count.total()) * columns, run = (total + 7) >> 3, run_begin = (blockIdx.x & 7) * run;
-  const int64_t stride = gridDim.x >> 3;
+  // this XCD's tiles: an eighth of the experts' last ones, which are not full, then an eighth of the others; only the offsets tell how many
+  const TileCount<false, kFullTiles> full(A.offsets, A.experts, A.slots, BM);
+  const TileCount<false, kLastTiles> last(A.offsets, A.experts, A.slots, BM);
+  const int xcd = blockIdx.x & 7;
+  const int64_t all_full = static_cast<int64_t>(full.total()) * columns, all_last = static_cast<int64_t>(last.total()) * columns;
+  const int64_t last_begin = all_last * xcd / 8, last_run = all_last * (xcd + 1) / 8 - last_begin;
+  const int64_t full_begin = all_full * xcd / 8, run = last_run + all_full * (xcd + 1) / 8 - full_begin;
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = wave & 1, wn = wave >> 1, lrow = lane & 31, lgrp = lane >> 5;
@@ -296,14 +301,21 @@ __global__ __launch_bounds__(256) void experts_tile_kernel(const ProductArgs A) 
     const int8_t* b[B_PER_WAVE];
   };
   auto find = [&](int64_t local, Work& w, Source& src, float* panel) {
-    const int64_t number = run_begin + local;
-    w.there = local < run && number < total;
+    w.there = local < run;
     if (!w.there) return;
-    const GroupUnit u = count.find(columns, number);
-    const int group = __builtin_amdgcn_readfirstlane(static_cast<int>(u.index / (kTileGroup * columns)));
-    const int in_group = static_cast<int>(u.index - static_cast<int64_t>(group) * (kTileGroup * columns));
-    const int group_rows = min(kTileGroup, u.tiles - group * kTileGroup);
-    const int tile_n = __builtin_amdgcn_readfirstlane(in_group / group_rows), tile_m = group * kTileGroup + in_group - tile_n * group_rows;
+    const bool whole = local >= last_run;
+    const GroupUnit u = whole ? full.find(columns, full_begin + local - last_run) : last.find(columns, last_begin + local);
+    int tile_m, tile_n;
+    if (whole) {
+      const int group = __builtin_amdgcn_readfirstlane(static_cast<int>(u.index / (kTileGroup * columns)));
+      const int in_group = static_cast<int>(u.index - static_cast<int64_t>(group) * (kTileGroup * columns));
+      const int group_rows = min(kTileGroup, u.tiles - group * kTileGroup);
+      tile_n = __builtin_amdgcn_readfirstlane(in_group / group_rows);
+      tile_m = group * kTileGroup + in_group - tile_n * group_rows;
+    } else {
+      tile_n = static_cast<int>(u.index);
+      tile_m = u.rows / BM;
+    }
     w.begin = u.begin + tile_m * BM;
     w.rows = min(BM, u.rows - tile_m * BM);
     w.n_base = tile_n * WIDTH;
@@ -318,7 +330,11 @@ __global__ __launch_bounds__(256) void experts_tile_kernel(const ProductArgs A) 
       const int ld = wave * B_PER_WAVE + static_cast<int>(c), strip = min((w.n_base + channel_of(ld >> 1)) >> 5, A.strips - 1);
       src.b[c] = weights + which_of(ld >> 1) * A.panel + (static_cast<int64_t>(strip) * A.chunks + (ld & 1)) * kChunkBytes;
     });
-    if (threadIdx.x < BN) {
+    static_assert(BM == 256 && BN == 256, "a thread for each row and channel");
+    {
+      const int place = w.begin + min(static_cast<int>(threadIdx.x), w.rows - 1), slot = slot_of(A, place);
+      panel[BN + threadIdx.x] = A.row_scales[UP ? slot / A.top_k : place];
+      reinterpret_cast<int*>(panel)[BN + BM + threadIdx.x] = slot;
       const int c = threadIdx.x >> 5, n = min(w.n_base + channel_of(c) + static_cast<int>(threadIdx.x & 31), A.N - 1);
       panel[threadIdx.x] = A.scales[(static_cast<int64_t>(u.group) * EACH + which_of(c)) * A.N + n];
     }
@@ -341,11 +357,10 @@ __global__ __launch_bounds__(256) void experts_tile_kernel(const ProductArgs A) 
   };
 
   const int KT = A.chunks / 2;  // at least AHEAD: the last steps of a tile fetch the first ones of the next
-  int64_t local = blockIdx.x >> 3;
   Work now, next;
   Source src, next_src;   // src: of the step that is loaded next; its second offset:
   uint32_t step_b = lane16;
-  find(local, now, src, panels);
+  find(blockIdx.x >> 3, now, src, panels);
   if (!now.there) return;
   auto make_uniform = [](Source& s) {
     s.a = uniform(s.a);
@@ -361,9 +376,11 @@ __global__ __launch_bounds__(256) void experts_tile_kernel(const ProductArgs A) 
   __syncthreads();
 
   int ring = 0;  // stage of the tile's first step
+  int number = blockIdx.x >> 3;
   for (int slot = 0;; slot = slot == 2 ? 0 : slot + 1) {
     // (a third panel: a wavefront may be here while another one still is at the results of the tile before)
-    find(local += stride, next, next_src, panels + (slot == 2 ? 0 : slot + 1) * BN);
+    number += static_cast<int>(gridDim.x >> 3);
+    find(number, next, next_src, panels + (slot == 2 ? 0 : slot + 1) * PANEL);
     const bool more = __builtin_amdgcn_readfirstlane(next.there);  // what is fetched behind the last tile is not used
     v16i acc[TN * TM];
     static_for<TN * TM>([&](auto t) {
@@ -441,13 +458,14 @@ __global__ __launch_bounds__(256) void experts_tile_kernel(const ProductArgs A) 
     uint8_t* const buffer = buffers + wave * (32 * PITCH);
     constexpr int LPR = ROWB / 16, RPP = 64 / LPR;   // lanes a row, rows a store
     const bool whole_rows = ((static_cast<uint32_t>(A.N) * ESZ | static_cast<uint32_t>(reinterpret_cast<uintptr_t>(A.out))) & 15) == 0;
-    const float* const scale0 = panels + slot * BN + wn * TN * 32 + egrp * 4;
+    const float* const scale0 = panels + slot * PANEL + wn * TN * 32 + egrp * 4;
+    const float* const row_scale = panels + slot * PANEL + BN;
+    const int* const slots = reinterpret_cast<const int*>(row_scale + BM);
     static_for<TM>([&](auto tile) {
       constexpr int i = decltype(tile)::value;
       const int m0 = (2 * i + wm) * 32;
       if (m0 >= now.rows) return;  // the same for the whole wavefront
-      const int place = now.begin + min(m0 + erow, now.rows - 1);
-      const float s = A.row_scales[UP ? slot_of(A, place) / A.top_k : place];
+      const float s = row_scale[m0 + erow];
       static_for<OUT_TN / PAIR>([&](auto pair) {
         static_for<PAIR>([&](auto half) {
           constexpr int j = decltype(pair)::value * PAIR + decltype(half)::value;
@@ -483,8 +501,7 @@ __global__ __launch_bounds__(256) void experts_tile_kernel(const ProductArgs A) 
           const int r = p * RPP + el / LPR, n = n0 + el % LPR * (16 / ESZ);
           const v4i v = *reinterpret_cast<const v4i*>(buffer + r * PITCH + el % LPR * 16);
           if (m0 + r >= now.rows || n >= A.N) continue;
-          const int at = now.begin + m0 + r;
-          const int64_t row = UP ? at : slot_of(A, at);
+          const int64_t row = UP ? now.begin + m0 + r : slots[m0 + r];
           uint8_t* const to = static_cast<uint8_t*>(A.out) + (row * A.N + n) * ESZ;
           if (whole_rows) {
             *reinterpret_cast<v4i*>(to) = v;
@@ -578,7 +595,7 @@ Layout layout_of(const itexhip_experts_params& p, bool up) {
 }
 
 template <int T>
-void launch_quantize(const void* x, int64_t stride, int64_t rows, int64_t K, int8_t* codes, float* scales, hipStream_t st) {
+void launch_quantize(const void* x, int64_t stride, int64_t rows, int64_t K, const ProductArgs& A, hipStream_t st) {
   const bool vec = aligned(x, 16) && (stride * element_size(T)) % 16 == 0;
   const auto kernel = !vec           ? quantize_rows_kernel<T, false, 0>
                       : K <= 1 * 2048 ? quantize_rows_kernel<T, true, 1>
@@ -587,7 +604,7 @@ void launch_quantize(const void* x, int64_t stride, int64_t rows, int64_t K, int
                       : K <= 7 * 2048 ? quantize_rows_kernel<T, true, 7>
                                       : quantize_rows_kernel<T, true, 0>;
   launch_blocks(rows, [&](int64_t first, unsigned count) {
-    kernel<<<count, 256, 0, st>>>(x, stride, static_cast<int>(K), static_cast<int>(pitch_of(K)), codes, scales, first);
+    kernel<<<count, 256, 0, st>>>(x, stride, static_cast<int>(K), A.pitch, const_cast<int8_t*>(A.codes), const_cast<float*>(A.row_scales), first);
   });
 }
 
@@ -656,7 +673,7 @@ int run_up(const itexhip_experts_params& p, const void* x, const int32_t* offset
             void* h, void* workspace, hipStream_t st) {
   const Layout l = layout_of(p, true);
   const ProductArgs A = product_args(p, true, l, workspace, offsets, rows, packed, scales, h);
-  launch_quantize<T>(x, p.x_stride, p.tokens, p.hidden, const_cast<int8_t*>(A.codes), const_cast<float*>(A.row_scales), st);
+  launch_quantize<T>(x, p.x_stride, p.tokens, p.hidden, A, st);
   return p.gated ? launch_products<T, true>(A, st) : launch_products<T, false>(A, st);
 }
 
@@ -666,7 +683,7 @@ int run_down(const itexhip_experts_params& p, const void* h, const int32_t* expe
   const Layout l = layout_of(p, false);
   float* const results = reinterpret_cast<float*>(static_cast<char*>(workspace) + l.results);
   const ProductArgs A = product_args(p, false, l, workspace, offsets, rows, packed, scales, results);
-  launch_quantize<T>(h, p.inner, A.slots, p.inner, const_cast<int8_t*>(A.codes), const_cast<float*>(A.row_scales), st);
+  launch_quantize<T>(h, p.inner, A.slots, p.inner, A, st);
   if (const int e = launch_products<0, false>(A, st)) return e;
   const auto combine = p.hidden % 4 == 0 ? combine_kernel<T, true> : combine_kernel<T, false>;
   launch_blocks(p.tokens, [&](int64_t first, unsigned count) {
