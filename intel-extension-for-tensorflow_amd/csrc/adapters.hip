@@ -23,7 +23,8 @@ struct AdapterArgs {
   int tokens, deep, splits, per_split;  // deep = n_slices * rank; per_split: K steps of 32 of a share
   int in, columns;  // of x; of the output
   int64_t first;    // workgroup of the launch
-  int blocks[ITEXHIP_ADAPTER_MAX_SLICES];  // blocks of 64 columns up to the end of each slice
+  int vec;          // runs of columns of base and out are aligned
+  int blocks[ITEXHIP_ADAPTER_MAX_SLICES];  // a workgroup's columns: how many such blocks there are up to the end of each slice
 };
 
 __device__ __forceinline__ int token_of(const AdapterArgs& A, int place) { return min(max(A.rows[place], 0), A.tokens - 1); }
@@ -83,6 +84,47 @@ __device__ __forceinline__ operand_t<T> load_operand(const void* base, int64_t r
   return o;
 }
 
+// N neighbouring elements (an even number), aligned to 16 bytes, or to all of them if that is less
+template <int T, int N>
+constexpr int run_alignment() { return N * (T == ITEXHIP_FLOAT ? 4 : 2) < 16 ? N * (T == ITEXHIP_FLOAT ? 4 : 2) : 16; }
+template <int T, int N>
+struct Run {
+  static constexpr int WORDS = N * (T == ITEXHIP_FLOAT ? 4 : 2) / 4;
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void load(const void* base, int64_t i) {
+    __builtin_memcpy(w, __builtin_assume_aligned(static_cast<const char*>(base) + i * (T == ITEXHIP_FLOAT ? 4 : 2), run_alignment<T, N>()), 4 * WORDS);
+  }
+  __device__ __forceinline__ void store(void* base, int64_t i) const {
+    __builtin_memcpy(__builtin_assume_aligned(static_cast<char*>(base) + i * (T == ITEXHIP_FLOAT ? 4 : 2), run_alignment<T, N>()), w, 4 * WORDS);
+  }
+  __device__ __forceinline__ float at(int j) const {
+    if constexpr (T == ITEXHIP_FLOAT) return __uint_as_float(w[j]);
+    const uint32_t h = (w[j / 2] >> (16 * (j % 2))) & 0xffffu;
+    return T == ITEXHIP_BFLOAT16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
+  }
+  __device__ __forceinline__ void set(int j, float x, float y) {  // elements j and j + 1, j even
+    if constexpr (T == ITEXHIP_FLOAT) {
+      w[j] = __float_as_uint(x);
+      w[j + 1] = __float_as_uint(y);
+    } else {
+      w[j / 2] = f32x2_to_bits16<T>(x, y);
+    }
+  }
+  // one by one, of a row that ends `count` elements on
+  __device__ __forceinline__ void load_some(const void* base, int64_t i, int count) {
+#pragma unroll
+    for (int j = 0; j < N; j += 2) set(j, j < count ? load_value<T>(base, i + j) : 0.0f, j + 1 < count ? load_value<T>(base, i + j + 1) : 0.0f);
+  }
+  __device__ __forceinline__ void store_some(void* base, int64_t i, int count) const {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j < count) {
+        if constexpr (T == ITEXHIP_FLOAT) static_cast<uint32_t*>(base)[i + j] = w[j];
+        else static_cast<uint16_t*>(base)[i + j] = static_cast<uint16_t>(w[j / 2] >> (16 * (j % 2)));
+      }
+  }
+};
+
 // the elements from the count-th on become zeros
 template <int T>
 __device__ __forceinline__ void cut(operand_t<T>& o, int count) {
@@ -98,35 +140,82 @@ __device__ __forceinline__ void cut(operand_t<T>& o, int count) {
   }
 }
 
-// x A^T.  A workgroup has 16 places of one adapter, 16 of its rows of A and a share of K, which its wavefronts divide.
-template <int T, bool VEC>
+// x A^T.  A workgroup has 16 RT places of one adapter, up to 16 CT of one slice's rows of A and a share of K.  Its wavefronts take the
+// share's steps of 32 in turns, so that together they read 256 consecutive bytes of a row, and add up in LDS.  Operands go straight from
+// memory to registers: x is read once, A stays in L2.
+template <int T, bool VEC, int RT, int CT>
 __global__ __launch_bounds__(256) void shrink_kernel(const AdapterArgs A) {
-  __shared__ __align__(16) float sums[4][16 * 16];
+  constexpr int PITCH = 16 * CT + 4;
+  __shared__ __align__(16) float sums[4][16 * RT * PITCH];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t id = A.first + blockIdx.x;
-  const int tile_of_a = static_cast<int>(id % ((A.deep + 15) / 16)), rest = static_cast<int>(id / ((A.deep + 15) / 16));
-  const int split = rest % A.splits;
-  const RowTile t = find_tile<false>(A.offsets, A.p.adapters, A.tokens, 16, rest / A.splits);
+  const int groups_of = (A.p.rank + 16 * CT - 1) / (16 * CT);
+  int64_t id = A.first + blockIdx.x;
+  const int split = static_cast<int>(id % A.splits);
+  id /= A.splits;
+  const int which = static_cast<int>(id % (groups_of * A.p.n_slices)), slice = which / groups_of, r0 = which % groups_of * 16 * CT;
+  const RowTile t = find_tile<false>(A.offsets, A.p.adapters, A.tokens, 16 * RT, static_cast<int>(id / (groups_of * A.p.n_slices)));
   if (t.group < 0) return;
-  const int r = tile_of_a * 16 + (lane & 15), rank = rank_of(A, t.group);
-  const bool there = r < A.deep && r % A.p.rank < rank;
-  const int64_t x_row = static_cast<int64_t>(token_of(A, t.begin + min(lane & 15, t.rows - 1))) * A.p.x_stride;
-  const int64_t a_row = (static_cast<int64_t>(t.group) * A.deep + min(r, A.deep - 1)) * A.in;
-  const int first = split * A.per_split, last = min(first + A.per_split, (A.in + 31) / 32);
-  v4f d = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int c = first + wave; c < last; c += 4) {
-    const int k = c * 32 + (lane >> 4) * 8;
-    const operand_t<T> a = load_operand<T, VEC>(A.a, a_row, k, there ? A.in : 0);
-    const operand_t<T> x = load_operand<T, VEC>(A.x, x_row, k, A.in);
-    d = product<T>(a, x, d);
+  const int rank = rank_of(A, t.group), k0 = (lane >> 4) * 8;
+  int64_t x_row[RT], a_row[CT];
+  int there[CT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) x_row[i] = static_cast<int64_t>(token_of(A, t.begin + min(i * 16 + (lane & 15), t.rows - 1))) * A.p.x_stride;
+#pragma unroll
+  for (int j = 0; j < CT; ++j) {
+    const int r = r0 + j * 16 + (lane & 15);
+    there[j] = r < rank ? A.in : 0;  // rows behind the rank are not read
+    a_row[j] = (static_cast<int64_t>(t.group) * A.deep + slice * A.p.rank + min(r, A.p.rank - 1)) * A.in;
   }
-  *reinterpret_cast<v4f*>(&sums[wave][(lane & 15) * 16 + (lane >> 4) * 4]) = d;
+  const int first = split * A.per_split, last = min(first + A.per_split, (A.in + 31) / 32);
+  v4f d[RT][CT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int j = 0; j < CT; ++j) d[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  auto load = [&](int c, operand_t<T> (&x)[RT], operand_t<T> (&a)[CT]) {
+    const int k = c * 32 + k0;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) x[i] = load_operand<T, VEC>(A.x, x_row[i], k, A.in);
+#pragma unroll
+    for (int j = 0; j < CT; ++j) a[j] = load_operand<T, VEC>(A.a, a_row[j], k, there[j]);
+  };
+  auto multiply = [&](const operand_t<T> (&x)[RT], const operand_t<T> (&a)[CT]) {
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int j = 0; j < CT; ++j) d[i][j] = product<T>(a[j], x[i], d[i][j]);
+  };
+  constexpr int AT_ONCE = 4;
+  int c = first + wave;
+  for (; c + 4 * (AT_ONCE - 1) < last; c += 4 * AT_ONCE) {
+    operand_t<T> x[AT_ONCE][RT], a[AT_ONCE][CT];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) load(c + 4 * u, x[u], a[u]);
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) multiply(x[u], a[u]);
+  }
+  for (; c < last; c += 4) {
+    operand_t<T> x[RT], a[CT];
+    load(c, x, a);
+    multiply(x, a);
+  }
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int j = 0; j < CT; ++j) *reinterpret_cast<v4f*>(&sums[wave][(i * 16 + (lane & 15)) * PITCH + j * 16 + (lane >> 4) * 4]) = d[i][j];
   __syncthreads();
-  const int place = threadIdx.x >> 4, column = tile_of_a * 16 + (threadIdx.x & 15);
-  if (place < t.rows && column < A.deep) {
-    float sum = sums[0][threadIdx.x];
-    for (int w = 1; w < 4; ++w) sum += sums[w][threadIdx.x];
-    A.middle[(static_cast<int64_t>(split) * A.tokens + t.begin + place) * A.deep + column] = sum;
+  constexpr int FOURS = 4 * CT;  // of a row
+  for (int n = threadIdx.x; n < 16 * RT * FOURS; n += 256) {
+    const int place = n / FOURS, r = n % FOURS * 4;
+    if (place >= t.rows || r0 + r >= A.p.rank) continue;  // (rank is a multiple of 8)
+    v4f sum = *reinterpret_cast<const v4f*>(&sums[0][place * PITCH + r]);
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      const v4f more = *reinterpret_cast<const v4f*>(&sums[w][place * PITCH + r]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] += more[i];
+    }
+    *reinterpret_cast<v4f*>(A.middle + (static_cast<int64_t>(split) * A.tokens + t.begin + place) * A.deep + slice * A.p.rank + r0 + r) = sum;
   }
 }
 
@@ -137,108 +226,143 @@ __device__ __forceinline__ void power_of(uint32_t bits, float* up, float* down) 
   *down = __uint_as_float(static_cast<uint32_t>(e - 8) << 23);
 }
 
-// out = base + scale (x A^T) B^T.  A wavefront has 16 places of one adapter and 64 columns of one slice: a product's row q = 4 g + i of
-// its j-th tile of B stands for column 16 g + 4 j + i, so that a lane ends with 16 neighbouring columns of a row.  The middle's values are the sum of two
-// numbers of the type; in half precision times a power of two that keeps a row's largest in range.
-template <int T>
+// out = base + scale (x A^T) B^T.  A wavefront has 16 NT columns of one slice, whose rows of B it keeps in registers (KS steps of 32 of the rank),
+// and goes through up to ROWS places of one adapter, 16 at a time.  A lane's column of the j-th tile is NT (lane % 16) + j of them, so that it ends
+// with NT neighbouring columns of four rows and 16 lanes with a run of 16 NT.  The workgroup adds up the shares of x A^T and holds them in LDS as operands: the
+// sum of two numbers of the type; in half precision times a power of two that keeps a row's largest in range.
+template <int T, int KS, int NT, int ROWS>
 __global__ __launch_bounds__(256) void expand_kernel(const AdapterArgs A) {
+  constexpr int SIZE = T == ITEXHIP_FLOAT ? 4 : 2, PARTS = T == ITEXHIP_FLOAT ? 1 : 2;
+  constexpr int PITCH = KS * 32 * SIZE + 16;
+  __shared__ __align__(16) uint8_t operands[2][PARTS][16 * PITCH];
+  __shared__ float downs[2][16];
+  __shared__ int tokens[ROWS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int all = A.blocks[A.p.n_slices - 1];
   const int64_t id = A.first + blockIdx.x;
-  const int fours = (A.blocks[A.p.n_slices - 1] + 3) / 4, index = static_cast<int>(id / fours);
-  const int block = static_cast<int>(id - static_cast<int64_t>(index) * fours) * 4 + wave;
-  if (block >= A.blocks[A.p.n_slices - 1]) return;
-  const RowTile t = find_tile<true>(A.offsets, A.p.adapters, A.tokens, 16, index);
+  const int index = static_cast<int>(id / all), block = static_cast<int>(id - static_cast<int64_t>(index) * all);
+  const RowTile t = find_tile<true>(A.offsets, A.p.adapters, A.tokens, ROWS, index);
   if (t.group < 0) return;
   const bool none = t.group == A.p.adapters;
   if (none && A.out == A.base) return;
   int slice = 0;
   while (block >= A.blocks[slice]) ++slice;
   const int slice_begin = slice == 0 ? 0 : static_cast<int>(A.p.slice_end[slice - 1]), slice_end = static_cast<int>(A.p.slice_end[slice]);
-  const int column0 = slice_begin + (block - (slice == 0 ? 0 : A.blocks[slice - 1])) * 64;
-  const int place = t.begin + min(lane & 15, t.rows - 1), group4 = lane >> 4;
-  v4f d[4];
+  const int column0 = slice_begin + ((block - (slice == 0 ? 0 : A.blocks[slice - 1])) * 4 + wave) * (16 * NT);
+  const int column = column0 + (lane & 15) * NT;  // the lane's first
+  const int rank = none ? 0 : rank_of(A, t.group);
+  const float scale = none ? 0.0f : A.scales[t.group];
+  const bool vec = A.vec && column + NT <= slice_end;
+
+  operand_t<T> b[KS][NT];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) d[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-  float scale = 0.0f, down = 1.0f;
-  if (!none) {
-    const int rank = rank_of(A, t.group);
-    scale = A.scales[t.group];
-    const int64_t at = static_cast<int64_t>(place) * A.deep + slice * A.p.rank, share = static_cast<int64_t>(A.tokens) * A.deep;
-    auto middle = [&](int r, float (&v)[8]) {
-      if (r < rank) {
-        load8<ITEXHIP_FLOAT>(A.middle, at + r, v);
-        for (int s = 1; s < A.splits; ++s) {
-          float w[8];
-          load8<ITEXHIP_FLOAT>(A.middle, at + s * share + r, w);
+  for (int s = 0; s < KS; ++s)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] += w[i];
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (r + i >= rank) v[i] = 0.0f;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-      }
-    };
-    float up = 1.0f;
-    if constexpr (T == ITEXHIP_HALF) {
-      uint32_t top = 0;
-      for (int r0 = 0; r0 < rank; r0 += 32) {
-        float v[8];
-        middle(r0 + group4 * 8, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-      }
-      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
-      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
-      power_of(top, &up, &down);
+    for (int j = 0; j < NT; ++j) {
+      const int r = s * 32 + (lane >> 4) * 8;
+      const int64_t row = (static_cast<int64_t>(none ? 0 : t.group) * A.columns + min(column + j, slice_end - 1)) * A.p.rank;
+      b[s][j] = load_operand<T, true>(A.b, row, r, (rank + 7) / 8 * 8);
+      if (rank % 8 != 0) cut<T>(b[s][j], rank - r);
     }
-    for (int r0 = 0; r0 < rank; r0 += 32) {
-      const int r = r0 + group4 * 8;
-      float v[8];
-      middle(r, v);
-      operand_t<T> hi, lo;
-      if constexpr (T == ITEXHIP_FLOAT) {
+
+  for (int n = threadIdx.x; n < ROWS; n += 256) tokens[n] = token_of(A, t.begin + min(n, t.rows - 1));
+  __syncthreads();
+  const int row = threadIdx.x >> 4, part = threadIdx.x & 15;  // 16 threads a row of operands
+  constexpr int EACH = KS * 2;  // r that a thread has, in pairs from 2 part on
+  struct Round {
+    float v[EACH];
+    Run<T, NT> base[4];  // of the lane's rows, 4 (lane / 16) .. + 3
+  };
+  auto load = [&](int n, Round& q) {
+    const float* from = A.middle + static_cast<int64_t>(t.begin + min(n * 16 + row, t.rows - 1)) * A.deep + slice * A.p.rank + part * 2;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) hi.v[i] = v[i];
-      } else {
-        uint32_t wh[4], wl[4];
+    for (int s = 0; s < KS; ++s) {
+      float2 sum = {0.0f, 0.0f};
+      if (s * 32 + part * 2 < rank) {
+        sum = *reinterpret_cast<const float2*>(from + s * 32);
+        for (int o = 1; o < A.splits; o += 5) {  // five at a time on their way
+          float2 more[5];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float a = v[2 * i] * up, b = v[2 * i + 1] * up;
-          wh[i] = f32x2_to_bits16<T>(a, b);
-          const float ha = T == ITEXHIP_BFLOAT16 ? bf16_bits_to_f32(wh[i] & 0xffffu) : f16_bits_to_f32(wh[i] & 0xffffu);
-          const float hb = T == ITEXHIP_BFLOAT16 ? bf16_bits_to_f32(wh[i] >> 16) : f16_bits_to_f32(wh[i] >> 16);
-          wl[i] = f32x2_to_bits16<T>(a - ha, b - hb);
+          for (int i = 0; i < 5; ++i) more[i] = *reinterpret_cast<const float2*>(from + s * 32 + static_cast<int64_t>(min(o + i, A.splits - 1)) * A.tokens * A.deep);
+#pragma unroll
+          for (int i = 0; i < 5; ++i) {
+            sum.x += o + i < A.splits ? more[i].x : 0.0f;
+            sum.y += o + i < A.splits ? more[i].y : 0.0f;
+          }
         }
-        __builtin_memcpy(&hi, wh, 16);
-        __builtin_memcpy(&lo, wl, 16);
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int q = lane & 15, column = column0 + (q >> 2) * 16 + j * 4 + (q & 3);
-        const int64_t b_row = (static_cast<int64_t>(t.group) * A.columns + min(column, slice_end - 1)) * A.p.rank;
-        operand_t<T> b = load_operand<T, true>(A.b, b_row, r, (rank + 7) / 8 * 8);
-        if (rank % 8 != 0) cut<T>(b, rank - r);
-        d[j] = product<T>(b, hi, d[j]);
-        if constexpr (T != ITEXHIP_FLOAT) d[j] = product<T>(b, lo, d[j]);
-      }
+      q.v[2 * s] = sum.x;
+      q.v[2 * s + 1] = s * 32 + part * 2 + 1 < rank ? sum.y : 0.0f;
     }
-  }
-  if ((lane & 15) >= t.rows) return;
-  const int64_t token = token_of(A, place);
-  const int first = column0 + group4 * 16;
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int column = first + j * 4 + i;
-      if (column >= slice_end) continue;
-      const float base = load_value<T>(A.base, token * A.p.base_stride + column);
-      if (none) store_output<T>(A.out, token * A.p.out_stride + column, base);
-      else store_output<T>(A.out, token * A.p.out_stride + column, base + scale * (d[j][i] * down));
+      const int m = n * 16 + (lane >> 4) * 4 + i;
+      if (m >= t.rows || column >= slice_end) continue;
+      const int64_t at = static_cast<int64_t>(tokens[m]) * A.p.base_stride + column;
+      if (vec) q.base[i].load(A.base, at);
+      else q.base[i].load_some(A.base, at, slice_end - column);
     }
+  };
+  const int rounds = (t.rows + 15) / 16;
+  Round now, next;
+  load(0, now);
+  for (int n = 0; n < rounds; ++n) {
+    const int parity = n & 1;
+    float up = 1.0f, down = 1.0f;
+    if constexpr (T == ITEXHIP_HALF) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) top = max(top, __float_as_uint(now.v[i]) & 0x7fffffffu);
+#pragma unroll
+      for (int d = 1; d < 16; d *= 2) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d)));
+      power_of(top, &up, &down);
+      if (part == 0) downs[parity][row] = down;
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      uint8_t* const to = operands[parity][0] + row * PITCH + (s * 32 + part * 2) * SIZE;
+      if constexpr (T == ITEXHIP_FLOAT) {
+        *reinterpret_cast<float2*>(to) = float2{now.v[2 * s], now.v[2 * s + 1]};
+      } else {
+        const float a = now.v[2 * s] * up, c = now.v[2 * s + 1] * up;
+        const uint32_t hi = f32x2_to_bits16<T>(a, c);
+        const float ha = T == ITEXHIP_BFLOAT16 ? bf16_bits_to_f32(hi & 0xffffu) : f16_bits_to_f32(hi & 0xffffu);
+        const float hc = T == ITEXHIP_BFLOAT16 ? bf16_bits_to_f32(hi >> 16) : f16_bits_to_f32(hi >> 16);
+        *reinterpret_cast<uint32_t*>(to) = hi;
+        *reinterpret_cast<uint32_t*>(operands[parity][PARTS - 1] + row * PITCH + (s * 32 + part * 2) * SIZE) = f32x2_to_bits16<T>(a - ha, c - hc);
+      }
+    }
+    __syncthreads();  // (one a round: the next one's operands go to the other half)
+    if (n + 1 < rounds) load(n + 1, next);
+    v4f d[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) d[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int h = 0; h < PARTS; ++h) {
+        operand_t<T> o;
+        __builtin_memcpy(&o, operands[parity][h] + (lane & 15) * PITCH + (s * 32 + (lane >> 4) * 8) * SIZE, sizeof(o));
+#pragma unroll
+        for (int j = 0; j < NT; ++j) d[j] = product<T>(o, b[s][j], d[j]);
+      }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int m = n * 16 + (lane >> 4) * 4 + i;
+      if (m >= t.rows || column >= slice_end) continue;
+      const float factor = T == ITEXHIP_HALF ? downs[parity][(lane >> 4) * 4 + i] : 1.0f;
+      Run<T, NT> y = now.base[i];
+      if (!none) {
+#pragma unroll
+        for (int j = 0; j < NT; j += 2)
+          y.set(j, now.base[i].at(j) + scale * (d[j][i] * factor), now.base[i].at(j + 1) + scale * (d[j + 1][i] * factor));
+      }
+      const int64_t at = static_cast<int64_t>(tokens[m]) * A.p.out_stride + column;
+      if (vec) y.store(A.out, at);
+      else y.store_some(A.out, at, slice_end - column);
+    }
+    now = next;
+  }
 }
 
 int check(const itexhip_adapters_params* p, const char* name) {
@@ -260,26 +384,73 @@ int check(const itexhip_adapters_params* p, const char* name) {
   return ITEXHIP_OK;
 }
 
-// Shares of K for one tile of rows: enough workgroups for the device where tokens are few
-int splits_of(int64_t in) {
-  const int64_t n = (in + 511) / 512;
+// Many places an adapter: tiles of 64 of them (16 where most would be empty), which read A a quarter as often
+bool long_tiles(int64_t tokens, int adapters) { return tokens > 32 * static_cast<int64_t>(adapters); }
+// Shares of K: enough workgroups for the device where tiles are few, of at least 256 k each
+constexpr int kEnoughTiles = 512;
+int splits_of(int64_t tokens, int adapters, int64_t parts, int64_t in) {
+  const int64_t tiles = tiles_bound(tokens, adapters, long_tiles(tokens, adapters) ? 64 : 16, false) * parts;
+  int64_t n = tiles == 0 ? 1 : (kEnoughTiles + tiles - 1) / tiles;
+  n = n < (in + 255) / 256 ? n : (in + 255) / 256;
   return static_cast<int>(n < kMaxSplits ? n : kMaxSplits);
+}
+// Rows of the middle that any call of up to this many tokens needs: a share's tiles hold at most 64 tokens each
+int64_t middle_rows(int64_t tokens) {
+  const int64_t most = kMaxSplits * tokens, few = 64 * 2 * kEnoughTiles;
+  return most < few ? most : few > tokens ? few : tokens;
+}
+
+template <int T, bool VEC, int RT, int CT>
+void launch_shrink(AdapterArgs A, hipStream_t st) {
+  const int64_t parts = static_cast<int64_t>((A.p.rank + 16 * CT - 1) / (16 * CT)) * A.p.n_slices;
+  const int steps = (A.in + 31) / 32;
+  A.per_split = (steps + A.splits - 1) / A.splits;
+  launch_blocks(tiles_bound(A.tokens, A.p.adapters, 16 * RT, false) * parts * A.splits, [&](int64_t first, unsigned count) {
+    A.first = first;
+    shrink_kernel<T, VEC, RT, CT><<<count, 256, 0, st>>>(A);
+  });
+}
+template <int T, bool VEC, int RT>
+void launch_shrink(const AdapterArgs& A, hipStream_t st) {
+  if (A.p.rank <= 16) launch_shrink<T, VEC, RT, 1>(A, st);
+  else if (A.p.rank <= 32) launch_shrink<T, VEC, RT, 2>(A, st);
+  else launch_shrink<T, VEC, RT, 4>(A, st);
+}
+int shrink_parts(int rank) { return rank <= 64 ? 1 : (rank + 63) / 64; }
+
+template <int T, int KS, int NT, int ROWS>
+void launch_expand(AdapterArgs A, hipStream_t st) {
+  int64_t begin = 0;
+  for (int i = 0, blocks = 0; i < A.p.n_slices; ++i) {
+    blocks += static_cast<int>((A.p.slice_end[i] - begin + 64 * NT - 1) / (64 * NT));
+    A.blocks[i] = blocks;
+    begin = A.p.slice_end[i];
+  }
+  launch_blocks(tiles_bound(A.tokens, A.p.adapters, ROWS, true) * A.blocks[A.p.n_slices - 1], [&](int64_t first, unsigned count) {
+    A.first = first;
+    expand_kernel<T, KS, NT, ROWS><<<count, 256, 0, st>>>(A);
+  });
+}
+template <int T, int ROWS>
+void launch_expand(const AdapterArgs& A, hipStream_t st) {
+  constexpr int NT = T == ITEXHIP_FLOAT ? 4 : 8;  // 16 bytes of a lane's row; fewer where more would not fit the registers
+  if (A.p.rank <= 32) launch_expand<T, 1, NT, ROWS>(A, st);
+  else if (A.p.rank <= 64) launch_expand<T, 2, NT, ROWS>(A, st);
+  else if (A.p.rank <= 128) launch_expand<T, 4, 4, ROWS>(A, st);
+  else launch_expand<T, 8, T == ITEXHIP_FLOAT ? 2 : 4, ROWS>(A, st);
 }
 
 template <int T>
 void run_adapters(AdapterArgs A, hipStream_t st) {
-  const bool vec = A.in % 8 == 0 && aligned(A.x, 16) && aligned(A.a, 16) && (A.p.x_stride * element_size(T)) % 16 == 0;
-  const int steps = (A.in + 31) / 32;
-  A.per_split = (steps + A.splits - 1) / A.splits;
-  const auto shrink = vec ? shrink_kernel<T, true> : shrink_kernel<T, false>;
-  launch_blocks(tiles_bound(A.tokens, A.p.adapters, 16, false) * A.splits * ((A.deep + 15) / 16), [&](int64_t first, unsigned count) {
-    A.first = first;
-    shrink<<<count, 256, 0, st>>>(A);
-  });
-  launch_blocks(tiles_bound(A.tokens, A.p.adapters, 16, true) * ((A.blocks[A.p.n_slices - 1] + 3) / 4), [&](int64_t first, unsigned count) {
-    A.first = first;
-    expand_kernel<T><<<count, 256, 0, st>>>(A);
-  });
+  const int64_t size = element_size(T);
+  const bool vec = A.in % 8 == 0 && aligned(A.x, 16) && aligned(A.a, 16) && (A.p.x_stride * size) % 16 == 0;
+  A.vec = aligned(A.base, 16) && aligned(A.out, 16) && (A.p.base_stride * size) % 16 == 0 && (A.p.out_stride * size) % 16 == 0;
+  for (int i = 0; i + 1 < A.p.n_slices; ++i) A.vec = A.vec && (A.p.slice_end[i] * size) % 16 == 0;
+  const bool wide = long_tiles(A.tokens, A.p.adapters);
+  if (vec) wide ? launch_shrink<T, true, 4>(A, st) : launch_shrink<T, true, 1>(A, st);
+  else wide ? launch_shrink<T, false, 4>(A, st) : launch_shrink<T, false, 1>(A, st);
+  if (wide) launch_expand<T, 128>(A, st);
+  else launch_expand<T, 16>(A, st);
 }
 
 }  // namespace
@@ -289,7 +460,7 @@ using namespace itexhip;
 
 extern "C" int64_t itexhip_adapters_workspace(const itexhip_adapters_params* p) {
   if (check(p, "itexhip_adapters_workspace") != ITEXHIP_OK) return 0;
-  return (static_cast<int64_t>(splits_of(p->in)) * p->tokens * p->n_slices * p->rank * 4 + 255) / 256 * 256 + 256;
+  return (middle_rows(p->tokens) * p->n_slices * p->rank * 4 + 255) / 256 * 256 + 256;
 }
 
 extern "C" int itexhip_adapters(const itexhip_adapters_params* p, const void* x, const int32_t* offsets, const int32_t* rows, const void* a, const void* b,
@@ -317,15 +488,9 @@ extern "C" int itexhip_adapters(const itexhip_adapters_params* p, const void* x,
   A.middle = static_cast<float*>(workspace);
   A.tokens = static_cast<int>(p->tokens);
   A.deep = p->n_slices * p->rank;
-  A.splits = splits_of(p->in);
+  A.splits = splits_of(p->tokens, p->adapters, static_cast<int64_t>(p->n_slices) * shrink_parts(p->rank), p->in);
   A.in = static_cast<int>(p->in);
   A.columns = static_cast<int>(p->slice_end[p->n_slices - 1]);
-  int64_t begin = 0;
-  for (int i = 0, blocks = 0; i < p->n_slices; ++i) {
-    blocks += static_cast<int>((p->slice_end[i] - begin + 63) / 64);
-    A.blocks[i] = blocks;
-    begin = p->slice_end[i];
-  }
   hipStream_t st = as_stream(stream);
   if (p->type == ITEXHIP_FLOAT) run_adapters<ITEXHIP_FLOAT>(A, st);
   else if (p->type == ITEXHIP_BFLOAT16) run_adapters<ITEXHIP_BFLOAT16>(A, st);
