@@ -11,7 +11,7 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
-constexpr int kMaxSplits = 16;
+constexpr int kMaxSplits = 6;
 
 struct AdapterArgs {
   itexhip_adapters_params p;
@@ -231,7 +231,7 @@ __device__ __forceinline__ void power_of(uint32_t bits, float* up, float* down) 
 // with NT neighbouring columns of four rows and 16 lanes with a run of 16 NT.  The workgroup adds up the shares of x A^T and holds them in LDS as operands: the
 // sum of two numbers of the type; in half precision times a power of two that keeps a row's largest in range.
 template <int T, int KS, int NT, int ROWS>
-__global__ __launch_bounds__(256) void expand_kernel(const AdapterArgs A) {
+__global__ __launch_bounds__(256, KS <= 2 ? 3 : 2) void expand_kernel(const AdapterArgs A) {
   constexpr int SIZE = T == ITEXHIP_FLOAT ? 4 : 2, PARTS = T == ITEXHIP_FLOAT ? 1 : 2;
   constexpr int PITCH = KS * 32 * SIZE + 16;
   __shared__ __align__(16) uint8_t operands[2][PARTS][16 * PITCH];
@@ -449,7 +449,7 @@ void run_adapters(AdapterArgs A, hipStream_t st) {
   const bool wide = long_tiles(A.tokens, A.p.adapters);
   if (vec) wide ? launch_shrink<T, true, 4>(A, st) : launch_shrink<T, true, 1>(A, st);
   else wide ? launch_shrink<T, false, 4>(A, st) : launch_shrink<T, false, 1>(A, st);
-  if (wide) launch_expand<T, 128>(A, st);
+  if (wide) launch_expand<T, 64>(A, st);
   else launch_expand<T, 16>(A, st);
 }
 
