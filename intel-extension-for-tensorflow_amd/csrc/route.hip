@@ -20,16 +20,73 @@ struct RouteArgs {
   int64_t tokens, first;  // first: workgroup of the launch
 };
 
+// Over a token's lanes.  Lanes 1, 2, 4 and 8 apart meet within the vector unit; of a mirrored row any lane of the other half will
+// do, since its half agrees by then.
+template <int CTRL, class V>
+__device__ __forceinline__ V from_lane(V x) {
+  static_assert(sizeof(V) == 4 || sizeof(V) == 8, "one or two registers");
+  int w[sizeof(V) / 4];
+  __builtin_memcpy(w, &x, sizeof(V));
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(V) / 4; ++i) w[i] = __builtin_amdgcn_update_dpp(w[i], w[i], CTRL, 0xf, 0xf, false);
+  __builtin_memcpy(&x, w, sizeof(V));
+  return x;
+}
 template <int LPT, class V, class F>
 __device__ __forceinline__ V over_lanes(V x, F&& f) {
-#pragma unroll
-  for (int d = 1; d < LPT; d *= 2) x = f(x, __shfl_xor(x, d));
+  static_assert(LPT == 16 || LPT == 64, "lanes a token");
+  x = f(x, from_lane<0xb1>(x));    // quad_perm 1 0 3 2
+  x = f(x, from_lane<0x4e>(x));    // quad_perm 2 3 0 1
+  x = f(x, from_lane<0x141>(x));   // row_half_mirror
+  x = f(x, from_lane<0x140>(x));   // row_mirror
+  if constexpr (LPT > 16) {
+    x = f(x, __shfl_xor(x, 16));
+    x = f(x, __shfl_xor(x, 32));
+  }
   return x;
 }
 
-__device__ __forceinline__ double sigmoid(double x) { return 1.0 / (1.0 + exp(-x)); }
+// e^x to about 2^-52: n ln 2 taken off with ln 2 in two parts, so that |r| <= ln 2 / 2, and the Taylor sum of e^r (the first term left
+// out is r^14 / 14! < 5e-18).  Below 2^-1074 it is 0, beyond 2^1024 infinite; NaN stays.
+__device__ __forceinline__ double exp64(double x) {
+  x = x < -800.0 ? -800.0 : x > 800.0 ? 800.0 : x;
+  const double n = rint(x * 1.4426950408889634);
+  double r = fma(n, -0x1.62e42fefa38p-1, x);
+  r = fma(n, -0x1.ef35793c7673p-45, r);
+  double p = fma(r, 1.0 / 6227020800.0, 1.0 / 479001600.0);
+  p = fma(r, p, 1.0 / 39916800.0);
+  p = fma(r, p, 1.0 / 3628800.0);
+  p = fma(r, p, 1.0 / 362880.0);
+  p = fma(r, p, 1.0 / 40320.0);
+  p = fma(r, p, 1.0 / 5040.0);
+  p = fma(r, p, 1.0 / 720.0);
+  p = fma(r, p, 1.0 / 120.0);
+  p = fma(r, p, 1.0 / 24.0);
+  p = fma(r, p, 1.0 / 6.0);
+  p = fma(r, p, 0.5);
+  p = fma(r, p, 1.0);
+  p = fma(r, p, 1.0);
+  return ldexp(p, static_cast<int>(n));
+}
+// 1 / (1 + e^-x): the reciprocal instruction's value and two steps of Newton's iteration (the sum is 1 at least; infinite from 2^1024 on)
+__device__ __forceinline__ double sigmoid(double x) {
+  const double d = 1.0 + exp64(-x);
+  double r = __builtin_amdgcn_rcp(d);
+  r = fma(fma(-d, r, 1.0), r, r);
+  r = fma(fma(-d, r, 1.0), r, r);
+  return d > 1e308 ? 0.0 : r;
+}
+// x is not a number any more: its upper word decides that
+__device__ __forceinline__ double spoiled_if(bool condition, double x) {
+  uint32_t w[2];
+  __builtin_memcpy(w, &x, 8);
+  w[1] = condition ? 0x7ff80000u : w[1];
+  __builtin_memcpy(&x, w, 8);
+  return x;
+}
 
-template <int T, int LPT, int PER>
+// VEC: a lane's logits are aligned to 16 bytes and there are as many as it can hold, or none
+template <int T, int LPT, int PER, bool VEC>
 __global__ __launch_bounds__(256) void route_kernel(const RouteArgs A) {
   constexpr int TOKENS = 256 / LPT;  // of a workgroup
   extern __shared__ __align__(16) uint8_t lds[];
@@ -44,10 +101,21 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs A) {
   auto sum_of = [](double a, double b) { return a + b; };
 
   double rank[PER];
+  if constexpr (VEC) {
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int e = sub * PER + i;
-    rank[i] = e < E ? static_cast<double>(load_value<T>(A.logits, row + e)) : nan;
+    for (int i = 0; i < PER; i += 8) {
+      float x[8];
+      load8<T>(A.logits, row + min(sub * PER, E - PER) + i, x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) rank[i + j] = sub * PER < E ? static_cast<double>(x[j]) : nan;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = sub * PER + i;
+      const double x = load_value<T>(A.logits, row + min(e, E - 1));
+      rank[i] = e < E ? x : nan;
+    }
   }
   double top = 0.0, total = 1.0;
   if (softmax) {
@@ -59,15 +127,15 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs A) {
     total = 0.0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const double z = exp(rank[i] - top);
+      const double z = exp64(rank[i] - top);
       if (sub * PER + i < E) total += z;
       rank[i] = z;
     }
     total = over_lanes<LPT>(total, sum_of);
-    const double inv = total == 0.0 ? 1.0 : total;
+    total = total == 0.0 ? 1.0 : total;
+    const double inv = 1.0 / total;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) rank[i] = rank[i] / inv;
-    total = inv;
+    for (int i = 0; i < PER; ++i) rank[i] = rank[i] * inv;
   } else {
 #pragma unroll
     for (int i = 0; i < PER; ++i) rank[i] = sigmoid(rank[i]);
@@ -83,18 +151,35 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs A) {
     const int G = A.p.groups, size = E / G;
     double* const ranks = reinterpret_cast<double*>(lds) + static_cast<size_t>(local) * (LPT * PER + 64);
     double* const values = ranks + LPT * PER;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) ranks[sub * PER + i] = rank[i];
-    __syncthreads();
-    for (int g = sub; g < G; g += LPT) {
-      double best = -inf, second = -inf;
-      for (int i = 0; i < size; ++i) {
-        const double r = ranks[g * size + i];
-        second = fmax(second, fmin(best, r));
-        best = fmax(best, r);
-      }
+    auto put = [&](int g, double best, double second) {
       const double value = A.p.group_best == 2 ? best + second : best;
       values[g] = value != value ? -inf : value;
+    };
+    auto take = [](double r, double& best, double& second) {
+      second = fmax(second, fmin(best, r));
+      best = fmax(best, r);
+    };
+    const int lanes = size / PER;  // of a group, where groups are whole lanes
+    const bool whole = size % PER == 0 && (lanes & (lanes - 1)) == 0;
+    if (whole) {
+      double best = -inf, second = -inf;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) take(rank[i], best, second);
+      for (int d = 1; d < lanes; d *= 2) {
+        const double b = __shfl_xor(best, d), s = __shfl_xor(second, d);
+        second = fmax(fmin(best, b), fmax(second, s));
+        best = fmax(best, b);
+      }
+      if (sub % lanes == 0 && sub * PER < E) put(sub / lanes, best, second);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) ranks[sub * PER + i] = rank[i];
+      __syncthreads();
+      for (int g = sub; g < G; g += LPT) {
+        double best = -inf, second = -inf;
+        for (int i = 0; i < size; ++i) take(ranks[g * size + i], best, second);
+        put(g, best, second);
+      }
     }
     __syncthreads();
     unsigned long long open = 0;  // groups that are left, the same in all of a token's lanes
@@ -104,10 +189,16 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs A) {
       if (ahead < A.p.top_groups) open |= 1ull << g;
     }
     open = over_lanes<LPT>(open, [](unsigned long long a, unsigned long long b) { return a | b; });
+    if (whole) {
+      const bool shut = !((open >> min(sub / lanes, G - 1)) & 1);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int g = min(sub * PER + i, E - 1) / size;
-      if (!((open >> g) & 1)) rank[i] = nan;
+      for (int i = 0; i < PER; ++i) rank[i] = spoiled_if(shut, rank[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int g = min(sub * PER + i, E - 1) / size;
+        rank[i] = spoiled_if(!((open >> g) & 1), rank[i]);
+      }
     }
   }
 
@@ -123,12 +214,12 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs A) {
     best = over_lanes<LPT>(best, max_of);
     int id = 1 << 30;
 #pragma unroll
-    for (int i = PER - 1; i >= 0; --i)
-      if (rank[i] == best) id = sub * PER + i;
+    for (int i = PER - 1; i >= 0; --i) id = rank[i] == best ? i : id;
+    id += id < PER ? sub * PER : 0;
     id = over_lanes<LPT>(id, [](int a, int b) { return min(a, b); });
+    const int mine = id - sub * PER;
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (sub * PER + i == id) rank[i] = nan;
+    for (int i = 0; i < PER; ++i) rank[i] = spoiled_if(i == mine, rank[i]);
 #pragma unroll
     for (int n = 0; n < KEEP; ++n)
       if (n * LPT + sub == j) chosen[n] = min(id, E - 1);
@@ -137,7 +228,7 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs A) {
 #pragma unroll
   for (int n = 0; n < KEEP; ++n) {
     const double x = load_value<T>(A.logits, row + chosen[n]);
-    score[n] = softmax ? exp(x - top) / total : sigmoid(x);
+    score[n] = softmax ? exp64(x - top) / total : sigmoid(x);
     if (n * LPT + sub < k) sum += score[n];
   }
   sum = A.p.renormalise ? over_lanes<LPT>(sum, sum_of) : 1.0;
@@ -153,10 +244,12 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs A) {
 template <int T, int LPT, int PER>
 void launch_route(RouteArgs A, hipStream_t st) {
   constexpr int TOKENS = 256 / LPT;
+  const bool vec = PER >= 8 && A.p.experts % PER == 0 && aligned(A.logits, 16) && (A.p.logits_stride * element_size(T)) % 16 == 0;
+  const auto kernel = vec ? route_kernel<T, LPT, PER, PER >= 8> : route_kernel<T, LPT, PER, false>;
   const size_t lds = A.p.groups > 1 ? TOKENS * (LPT * PER + 64) * sizeof(double) : 0;
   launch_blocks((A.tokens + TOKENS - 1) / TOKENS, [&](int64_t first, unsigned count) {
     A.first = first;
-    route_kernel<T, LPT, PER><<<count, 256, lds, st>>>(A);
+    kernel<<<count, 256, lds, st>>>(A);
   });
 }
 template <int T>
@@ -229,10 +322,17 @@ __global__ __launch_bounds__(64 * kOrderWaves) void order_rows_kernel(const int3
   for (int g = threadIdx.x; g < stride; g += THREADS) {
     int all = 0, before = 0;
     if (counts != nullptr) {
-      for (int r = 0; r < static_cast<int>(gridDim.x); ++r) {
-        const int c = counts[static_cast<int64_t>(r) * stride + g];
-        all += c;
-        before += r < static_cast<int>(blockIdx.x) ? c : 0;
+      constexpr int AT_ONCE = 16;
+      const int runs = gridDim.x, run = blockIdx.x;
+      for (int r = 0; r < runs; r += AT_ONCE) {
+        int c[AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) c[i] = counts[static_cast<int64_t>(min(r + i, runs - 1)) * stride + g];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+          all += r + i < runs ? c[i] : 0;
+          before += r + i < run ? c[i] : 0;
+        }
       }
     } else {
       for (int w = 0; w < kOrderWaves; ++w) all += bins[w * stride + g];
