@@ -96,8 +96,13 @@ struct ProductArgs {
   const float* scales;       // [experts][each][N]
   const int32_t *offsets, *rows;
   void* out;                 // up: h, [place][N];  down: fp32, [slot][N]
+  const void* x;             // the source itself, for kernels that make the codes
+  int64_t x_stride;
+  bool x_vec;                // its rows are aligned to 16 bytes
   int64_t panel;
   int experts, slots, top_k; // slots = tokens * top_k
+  int K;
+  int few;                   // rows of a tile whose workgroups make its codes, at most kFewRows
   int pitch, chunks, N;      // chunks of 32 k, an even number
   int strips;                // of 32 channels
   int64_t first;             // workgroup of the launch
@@ -117,25 +122,76 @@ __device__ __forceinline__ float activate(int activation, float x) {
 // Where a place's codes are, and (down) where its result goes.  What `rows` holds is cut to the slots there are.
 __device__ __forceinline__ int slot_of(const ProductArgs& A, int place) { return min(max(A.rows[place], 0), A.slots - 1); }
 
-// Few rows an expert: each wavefront streams a share of the K chunks of a strip of 32 channels past up to 32 RT rows, whose
-// codes come from the caches; the shares' sums meet in LDS.  OUT: type of h (up), or 0: fp32 by slot (down).
-template <int OUT, bool GATED, int RT>
-__global__ __launch_bounds__(256) void experts_stream_kernel(const ProductArgs A) {
-  constexpr int WAVES = 4, EACH = GATED ? 2 : 1, PITCH = 36;
-  constexpr bool UP = OUT != 0;
+// Codes and scales of a few rows in LDS, by all wavefronts of a workgroup: each has a share of one row.  `at` gives a row's first element.
+// All of them wait twice.
+constexpr int kFewRows = 16;
+template <int T, int WAVES, class F>
+__device__ __forceinline__ void quantize_few(const void* x, bool vec, int rows, int K, int pitch, int8_t* codes, float* scales, uint32_t (&most)[WAVES], F&& at) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int shares = max(1, WAVES / rows), share = wave / rows;
+  for (int r0 = 0; r0 < rows; r0 += WAVES) {  // (more rows than wavefronts: in turns)
+    const int row = r0 + (rows <= WAVES ? wave % rows : wave);
+    const bool there = row < rows && share < shares;
+    const int64_t base = at(min(row, rows - 1));
+    auto load = [&](int k, float (&v)[8]) {
+      if (vec && k + 8 <= K) {
+        load8<T>(x, base + k, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = k + j < K ? load_value<T>(x, base + k + j) : 0.0f;
+      }
+    };
+    uint32_t top = 0;
+    if (there) {
+      for (int k = (share * 64 + lane) * 8; k < K; k += shares * 512) {
+        float v[8];
+        load(k, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+      }
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d)));
+    if (lane == 0) most[wave] = top;
+    __syncthreads();
+    if (there) {
+      if (rows <= WAVES)
+        for (int o = 0; o < shares; ++o) top = max(top, most[row + o * rows]);
+      const float s = scale_of(top), inv = 1.0f / s;
+      if (share == 0 && lane == 0) scales[row] = s;
+      for (int k = (share * 64 + lane) * 8; k < pitch; k += shares * 512) {
+        float v[8];
+        load(k, v);
+        int c[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) c[j] = s == s ? code_of(v[j], s, inv) : 0;
+        *reinterpret_cast<uint2*>(codes + row * pitch + k) = uint2{pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7])};
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Weights that one workgroup reads once: past the caches' order of use
+__device__ __forceinline__ v4i load_once(const int8_t* p) { return __builtin_nontemporal_load(reinterpret_cast<const v4i*>(p)); }
+
+// Few rows an expert: each wavefront streams a share of the K chunks of a strip of 32 channels past up to 32 RT rows, the next chunks on
+// their way while the last ones are multiplied; the shares' sums meet in LDS.  The rows' codes come from the caches, or (SOURCE: the
+// type of x) the workgroup makes them itself, which saves a launch where rows are very few.
+// OUT: type of h (up), or 0: fp32 by slot (down).
+template <int OUT, bool GATED, int RT, int WAVES, int SOURCE>
+__global__ __launch_bounds__(64 * WAVES) void experts_stream_kernel(const ProductArgs A) {
+  constexpr int EACH = GATED ? 2 : 1, PITCH = 36;
+  constexpr bool UP = OUT != 0, FUSED = SOURCE != 0;
   __shared__ __align__(16) int sums[EACH][WAVES][32 * PITCH];
+  __shared__ float few_scales[kFewRows];
+  __shared__ uint32_t most[WAVES];
+  extern __shared__ __align__(16) int8_t few_codes[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t id = A.first + blockIdx.x;
   const int index = static_cast<int>(id / A.strips), strip = static_cast<int>(id - static_cast<int64_t>(index) * A.strips);
-  const RowTile t = find_tile<false>(A.offsets, A.experts, A.slots, 32 * RT, index);
+  const RowTile t = find_tile<false>(A.offsets, A.experts, A.slots, FUSED ? A.few : 32 * RT, index);
   if (t.group < 0) return;
-  const int8_t* source[RT];
-#pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    const int place = t.begin + min(i * 32 + (lane & 31), t.rows - 1);
-    const int row = UP ? slot_of(A, place) / A.top_k : place;
-    source[i] = A.codes + static_cast<int64_t>(row) * A.pitch + (lane >> 5) * 16;
-  }
   const int8_t* weights = A.packed + static_cast<int64_t>(t.group) * EACH * A.panel + static_cast<int64_t>(strip) * A.chunks * kChunkBytes + lane * 16;
   v16i acc[EACH][RT];
 #pragma unroll
@@ -144,31 +200,48 @@ __global__ __launch_bounds__(256) void experts_stream_kernel(const ProductArgs A
     for (int i = 0; i < RT; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[w][i][r] = 0;
-  auto load = [&](int c, v4i (&b)[EACH], v4i (&a)[RT]) {
-#pragma unroll
-    for (int w = 0; w < EACH; ++w) b[w] = *reinterpret_cast<const v4i*>(weights + w * A.panel + static_cast<int64_t>(c) * kChunkBytes);
-#pragma unroll
-    for (int i = 0; i < RT; ++i) a[i] = *reinterpret_cast<const v4i*>(source[i] + c * 32);
-  };
-  auto multiply = [&](const v4i (&b)[EACH], const v4i (&a)[RT]) {
-#pragma unroll
-    for (int w = 0; w < EACH; ++w)
-#pragma unroll
-      for (int i = 0; i < RT; ++i) acc[w][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(b[w], a[i], acc[w][i], 0, 0, 0);
-  };
   constexpr int AT_ONCE = 4;
-  int c = wave;
-  for (; c + (AT_ONCE - 1) * WAVES < A.chunks; c += AT_ONCE * WAVES) {
-    v4i b[AT_ONCE][EACH], a[AT_ONCE][RT];
+  struct Batch {
+    v4i b[AT_ONCE][EACH];
+  };
+  // chunks c, c + WAVES ...; behind the last one that chunk again, which is not multiplied
+  auto load = [&](int c, Batch& to) {
 #pragma unroll
-    for (int u = 0; u < AT_ONCE; ++u) load(c + u * WAVES, b[u], a[u]);
+    for (int u = 0; u < AT_ONCE; ++u)
 #pragma unroll
-    for (int u = 0; u < AT_ONCE; ++u) multiply(b[u], a[u]);
+      for (int w = 0; w < EACH; ++w) to.b[u][w] = load_once(weights + w * A.panel + static_cast<int64_t>(min(c + u * WAVES, A.chunks - 1)) * kChunkBytes);
+  };
+  Batch now, next;
+  load(wave, now);
+  const int8_t* source[RT];
+  if constexpr (FUSED) {
+    quantize_few<SOURCE, WAVES>(A.x, A.x_vec, t.rows, A.K, A.pitch, few_codes, few_scales, most,
+                                [&](int r) { return static_cast<int64_t>(slot_of(A, t.begin + r) / A.top_k) * A.x_stride; });
+    source[0] = few_codes + min(lane & 31, t.rows - 1) * A.pitch + (lane >> 5) * 16;
+  } else {
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const int place = t.begin + min(i * 32 + (lane & 31), t.rows - 1);
+      const int row = UP ? slot_of(A, place) / A.top_k : place;
+      source[i] = A.codes + static_cast<int64_t>(row) * A.pitch + (lane >> 5) * 16;
+    }
   }
-  for (; c < A.chunks; c += WAVES) {
-    v4i b[EACH], a[RT];
-    load(c, b, a);
-    multiply(b, a);
+  for (int c = wave; c < A.chunks; c += AT_ONCE * WAVES) {
+    v4i a[AT_ONCE][RT];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+      for (int i = 0; i < RT; ++i) a[u][i] = *reinterpret_cast<const v4i*>(source[i] + min(c + u * WAVES, A.chunks - 1) * 32);
+    if (c + AT_ONCE * WAVES < A.chunks) load(c + AT_ONCE * WAVES, next);
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      if (c + u * WAVES >= A.chunks) break;
+#pragma unroll
+      for (int w = 0; w < EACH; ++w)
+#pragma unroll
+        for (int i = 0; i < RT; ++i) acc[w][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(now.b[u][w], a[u][i], acc[w][i], 0, 0, 0);
+    }
+    now = next;
   }
   // row tile by row tile: the shares' sums, then four channels of a row a thread
   const int m = threadIdx.x >> 3, n0 = strip * 32 + (threadIdx.x & 7) * 4;
@@ -183,10 +256,10 @@ __global__ __launch_bounds__(256) void experts_stream_kernel(const ProductArgs A
         *reinterpret_cast<v4i*>(&sums[w][wave][(lane & 31) * PITCH + g * 8 + (lane >> 5) * 4]) =
             v4i{acc[w][i][4 * g], acc[w][i][4 * g + 1], acc[w][i][4 * g + 2], acc[w][i][4 * g + 3]};
     __syncthreads();
-    if (i * 32 + m >= t.rows) return;
+    if (m >= 32 || i * 32 + m >= t.rows) return;
     const int place = t.begin + i * 32 + m;
-    const int slot = slot_of(A, place), row = UP ? slot / A.top_k : place;
-    const float s = A.row_scales[row];
+    const int slot = slot_of(A, place);
+    const float s = FUSED ? few_scales[m % kFewRows] : A.row_scales[UP ? slot / A.top_k : place];
     float v[EACH][4];
 #pragma unroll
     for (int w = 0; w < EACH; ++w) {
@@ -209,6 +282,100 @@ __global__ __launch_bounds__(256) void experts_stream_kernel(const ProductArgs A
       }
     }
   });
+}
+
+// The way back of very few choices in one launch: a workgroup has a strip of 32 channels of every expert that is chosen.  Its
+// wavefronts divide the experts and, within one, the chunks of K; every place of the order is a row of every product, and where the sums meet each place
+// takes its own expert's.  Then the strip's part of each token is all there.
+struct FewArgs {
+  const int32_t* experts;
+  const float* weights;
+  const void* addend;
+  int64_t addend_stride, out_stride;
+  int tokens;
+};
+constexpr int kFewPlaces = 16, kFewWaves = 16;
+template <int T>
+__global__ __launch_bounds__(64 * kFewWaves) void experts_few_down_kernel(const ProductArgs A, const FewArgs F) {
+  constexpr int PITCH = 36;
+  __shared__ __align__(16) int sums[kFewWaves][kFewPlaces * PITCH];
+  __shared__ float results[kFewPlaces][32];
+  __shared__ float row_scales[kFewPlaces];
+  __shared__ uint32_t most[kFewWaves];
+  extern __shared__ __align__(16) int8_t few_codes[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), strip = blockIdx.x;
+  // the lane's place (all lanes hold them again from kFewPlaces on), its slot and expert, -1: none here
+  const int place = lane & (kFewPlaces - 1);
+  const int slot = slot_of(A, min(place, A.slots - 1));
+  int expert = F.experts[slot];
+  if (place >= A.slots || expert < 0 || expert >= A.experts) expert = -1;
+  // experts in the order of their first places
+  int order = -1, number = 0;
+  for (int p = 0; p < A.slots; ++p) {
+    const int e = __builtin_amdgcn_readlane(expert, p);
+    if (e < 0) continue;
+    const unsigned long long same = __ballot(expert == e) & ((1ull << kFewPlaces) - 1);
+    if (__builtin_ctzll(same) != p) continue;
+    if (expert == e) order = number;
+    ++number;
+  }
+  number = __builtin_amdgcn_readfirstlane(number);
+  if (number > 0) {  // (the same for all wavefronts: they all waited for the same values)
+    const int shares = kFewWaves / number, mine = wave % number, share = wave / number;
+    const unsigned long long of_mine = __ballot(order == mine && lane < kFewPlaces);
+    const int e = __builtin_amdgcn_readlane(expert, __builtin_ctzll(of_mine));
+    const int8_t* weights = A.packed + static_cast<int64_t>(e) * A.panel + static_cast<int64_t>(strip) * A.chunks * kChunkBytes + lane * 16;
+    constexpr int AT_ONCE = 8;
+    v4i now[AT_ONCE], next[AT_ONCE];
+    auto load = [&](int c, v4i (&to)[AT_ONCE]) {
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) to[u] = load_once(weights + static_cast<int64_t>(min(c + u * shares, A.chunks - 1)) * kChunkBytes);
+    };
+    if (share < shares) load(share, now);
+    quantize_few<T, kFewWaves>(A.x, A.x_vec, A.slots, A.K, A.pitch, few_codes, row_scales, most, [&](int r) { return r * A.x_stride; });
+    v16i acc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] = 0;
+    const int8_t* source = few_codes + min(lane & 31, A.slots - 1) * A.pitch + (lane >> 5) * 16;
+    if (share < shares) {
+      for (int c = share; c < A.chunks; c += AT_ONCE * shares) {
+        if (c + AT_ONCE * shares < A.chunks) load(c + AT_ONCE * shares, next);
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+          if (c + u * shares >= A.chunks) break;
+          acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(now[u], *reinterpret_cast<const v4i*>(source + (c + u * shares) * 32), acc, 0, 0, 0);
+        }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) now[u] = next[u];
+      }
+    }
+    if ((lane & 31) < kFewPlaces) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<v4i*>(&sums[wave][(lane & 31) * PITCH + g * 8 + (lane >> 5) * 4]) = v4i{acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
+    }
+    __syncthreads();
+    // a thread for each place and channel
+    const int p = threadIdx.x >> 5, n = threadIdx.x & 31;
+    if (p < kFewPlaces) {
+      const int to = __shfl(slot, p), which = __shfl(order, p), its = __shfl(expert, p);
+      if (p < A.slots && which >= 0) {
+        int sum = 0;
+        for (int o = 0; o < shares; ++o) sum += sums[which + o * number][p * PITCH + n];
+        results[to % kFewPlaces][n] = static_cast<float>(sum) * (row_scales[p] * A.scales[static_cast<int64_t>(its) * A.N + min(strip * 32 + n, A.N - 1)]);
+      }
+    }
+    __syncthreads();
+  }
+  const int token = threadIdx.x >> 5, n = strip * 32 + (threadIdx.x & 31);
+  if (token >= F.tokens || n >= A.N) return;
+  float sum = 0.0f;
+  for (int c = 0; c < A.top_k; ++c) {
+    const int its = F.experts[token * A.top_k + c];
+    if (its >= 0 && its < A.experts) sum = sum + F.weights[token * A.top_k + c] * results[token * A.top_k + c][threadIdx.x & 31];
+  }
+  if (F.addend != nullptr) sum = sum + load_value<T>(F.addend, token * F.addend_stride + n);
+  store_output<T>(A.out, token * F.out_stride + n, sum);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -594,6 +761,15 @@ Layout layout_of(const itexhip_experts_params& p, bool up) {
   return l;
 }
 
+// Codes that a workgroup keeps in LDS
+constexpr int kFewBytes = 48 * 1024;
+// up: a workgroup makes the codes of its tokens itself, up to 32 elements a thread; beyond, a launch that makes them once is shorter
+bool few_up(const ProductArgs& A) {
+  const int64_t tokens = A.slots / A.top_k;
+  return tokens <= kFewRows && tokens * A.pitch <= 8192;
+}
+bool few_down(const ProductArgs& A) { return A.slots <= kFewPlaces && static_cast<int64_t>(A.slots) * A.pitch <= kFewBytes; }
+
 template <int T>
 void launch_quantize(const void* x, int64_t stride, int64_t rows, int64_t K, const ProductArgs& A, hipStream_t st) {
   const bool vec = aligned(x, 16) && (stride * element_size(T)) % 16 == 0;
@@ -608,12 +784,23 @@ void launch_quantize(const void* x, int64_t stride, int64_t rows, int64_t K, con
   });
 }
 
-template <int OUT, bool GATED, int RT>
-void launch_stream(ProductArgs A, hipStream_t st) {
-  launch_blocks(tiles_bound(A.slots, A.experts, 32 * RT, false) * A.strips, [&](int64_t first, unsigned count) {
+template <int OUT, bool GATED, int RT, int WAVES, int SOURCE>
+int launch_stream(ProductArgs A, hipStream_t st) {
+  A.few = A.slots / A.top_k;  // (tokens: an expert has no more rows, unless a token names it twice, which is one more tile)
+  const int per_tile = SOURCE != 0 ? A.few : 32 * RT, lds = SOURCE != 0 ? A.few * A.pitch : 0;
+  constexpr int STATIC = (GATED ? 2 : 1) * WAVES * 32 * 36 * 4 + 1024;
+  static unsigned long long configured;
+  const auto kernel = experts_stream_kernel<OUT, GATED, RT, WAVES, SOURCE>;
+  if (STATIC + lds > 64 * 1024 && !device_bit(&configured, false)) {
+    const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kFewBytes);
+    if (err != hipSuccess) return hip_fail(err, "hipFuncSetAttribute(experts_stream_kernel)");
+    device_bit(&configured, true);
+  }
+  launch_blocks(tiles_bound(A.slots, A.experts, per_tile, false) * A.strips, [&](int64_t first, unsigned count) {
     A.first = first;
-    experts_stream_kernel<OUT, GATED, RT><<<count, 256, 0, st>>>(A);
+    kernel<<<count, 64 * WAVES, lds, st>>>(A);
   });
+  return ITEXHIP_OK;
 }
 constexpr int kWorkgroups = 256;  // one for each CU; they take the tiles in turns
 
@@ -641,8 +828,10 @@ int launch_products(const ProductArgs& A, hipStream_t st) {
     if (GATED && A.activation == ITEXHIP_ACT_SWISH) return launch_tiles<OUT, GATED, GATED, 256, 256>(A, st);
     return launch_tiles<OUT, GATED, false, 256, 256>(A, st);
   }
-  launch_stream<OUT, GATED, 1>(A, st);
-  return ITEXHIP_OK;
+  if (each > 16) return launch_stream<OUT, GATED, 2, 4, 0>(A, st);
+  // few strips: more wavefronts for each, so that the device has enough on their way
+  const int64_t strips = tiles_bound(A.slots, A.experts, 32, false) * A.strips;
+  return strips >= 1024 ? launch_stream<OUT, GATED, 1, 4, 0>(A, st) : launch_stream<OUT, GATED, 1, 8, 0>(A, st);
 }
 
 ProductArgs product_args(const itexhip_experts_params& p, bool up, const Layout& l, void* workspace, const int32_t* offsets, const int32_t* rows,
@@ -660,6 +849,7 @@ ProductArgs product_args(const itexhip_experts_params& p, bool up, const Layout&
   A.experts = p.experts;
   A.slots = static_cast<int>(p.tokens * p.top_k);
   A.top_k = p.top_k;
+  A.K = static_cast<int>(K);
   A.pitch = static_cast<int>(pitch_of(K));
   A.chunks = A.pitch / 32;
   A.N = static_cast<int>(N);
@@ -672,7 +862,15 @@ template <int T>
 int run_up(const itexhip_experts_params& p, const void* x, const int32_t* offsets, const int32_t* rows, const int8_t* packed, const float* scales,
             void* h, void* workspace, hipStream_t st) {
   const Layout l = layout_of(p, true);
-  const ProductArgs A = product_args(p, true, l, workspace, offsets, rows, packed, scales, h);
+  ProductArgs A = product_args(p, true, l, workspace, offsets, rows, packed, scales, h);
+  A.x = x;
+  A.x_stride = p.x_stride;
+  A.x_vec = aligned(x, 16) && (p.x_stride * element_size(T)) % 16 == 0;
+  if (few_up(A)) {
+    const int64_t strips = tiles_bound(A.slots, A.experts, 32, false) * A.strips;
+    if (p.gated) return strips >= 1024 ? launch_stream<T, true, 1, 4, T>(A, st) : launch_stream<T, true, 1, 8, T>(A, st);
+    return strips >= 1024 ? launch_stream<T, false, 1, 4, T>(A, st) : launch_stream<T, false, 1, 8, T>(A, st);
+  }
   launch_quantize<T>(x, p.x_stride, p.tokens, p.hidden, A, st);
   return p.gated ? launch_products<T, true>(A, st) : launch_products<T, false>(A, st);
 }
@@ -682,7 +880,23 @@ int run_down(const itexhip_experts_params& p, const void* h, const int32_t* expe
               const float* scales, const float* weights, const void* addend, void* out, void* workspace, hipStream_t st) {
   const Layout l = layout_of(p, false);
   float* const results = reinterpret_cast<float*>(static_cast<char*>(workspace) + l.results);
-  const ProductArgs A = product_args(p, false, l, workspace, offsets, rows, packed, scales, results);
+  ProductArgs A = product_args(p, false, l, workspace, offsets, rows, packed, scales, results);
+  A.x = h;
+  A.x_stride = p.inner;
+  A.x_vec = aligned(h, 16) && (p.inner * element_size(T)) % 16 == 0;
+  if (few_down(A)) {
+    static unsigned long long configured;
+    const auto kernel = experts_few_down_kernel<T>;
+    if (!device_bit(&configured, false)) {
+      const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kFewBytes);
+      if (err != hipSuccess) return hip_fail(err, "hipFuncSetAttribute(experts_few_down_kernel)");
+      device_bit(&configured, true);
+    }
+    A.out = out;
+    const FewArgs F{experts, weights, addend, p.addend_stride, p.out_stride, static_cast<int>(p.tokens)};
+    kernel<<<static_cast<unsigned>(A.strips), 64 * kFewWaves, static_cast<size_t>(A.slots) * A.pitch, st>>>(A, F);
+    return ITEXHIP_OK;
+  }
   launch_quantize<T>(h, p.inner, A.slots, p.inner, A, st);
   if (const int e = launch_products<0, false>(A, st)) return e;
   const auto combine = p.hidden % 4 == 0 ? combine_kernel<T, true> : combine_kernel<T, false>;
