@@ -175,11 +175,11 @@ __device__ __forceinline__ void quantize_few(const void* x, bool vec, int rows, 
 // Weights that one workgroup reads once: past the caches' order of use
 __device__ __forceinline__ v4i load_once(const int8_t* p) { return __builtin_nontemporal_load(reinterpret_cast<const v4i*>(p)); }
 
-// Few rows an expert: each wavefront streams a share of the K chunks of a strip of 32 channels past up to 32 RT rows, the next chunks on
+// Few rows an expert: each wavefront streams a share of the K chunks of a strip of 32 channels past up to 32 rows, the next chunks on
 // their way while the last ones are multiplied; the shares' sums meet in LDS.  The rows' codes come from the caches, or (SOURCE: the
 // type of x) the workgroup makes them itself, which saves a launch where rows are very few.
 // OUT: type of h (up), or 0: fp32 by slot (down).
-template <int OUT, bool GATED, int RT, int WAVES, int SOURCE>
+template <int OUT, bool GATED, int WAVES, int SOURCE>
 __global__ __launch_bounds__(64 * WAVES) void experts_stream_kernel(const ProductArgs A) {
   constexpr int EACH = GATED ? 2 : 1, PITCH = 36;
   constexpr bool UP = OUT != 0, FUSED = SOURCE != 0;
@@ -190,16 +190,14 @@ __global__ __launch_bounds__(64 * WAVES) void experts_stream_kernel(const Produc
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t id = A.first + blockIdx.x;
   const int index = static_cast<int>(id / A.strips), strip = static_cast<int>(id - static_cast<int64_t>(index) * A.strips);
-  const RowTile t = find_tile<false>(A.offsets, A.experts, A.slots, FUSED ? A.few : 32 * RT, index);
+  const RowTile t = find_tile<false>(A.offsets, A.experts, A.slots, FUSED ? A.few : 32, index);
   if (t.group < 0) return;
   const int8_t* weights = A.packed + static_cast<int64_t>(t.group) * EACH * A.panel + static_cast<int64_t>(strip) * A.chunks * kChunkBytes + lane * 16;
-  v16i acc[EACH][RT];
+  v16i acc[EACH];
 #pragma unroll
   for (int w = 0; w < EACH; ++w)
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[w][i][r] = 0;
+    for (int r = 0; r < 16; ++r) acc[w][r] = 0;
   constexpr int AT_ONCE = 4;
   struct Batch {
     v4i b[AT_ONCE][EACH];
@@ -213,75 +211,63 @@ __global__ __launch_bounds__(64 * WAVES) void experts_stream_kernel(const Produc
   };
   Batch now, next;
   load(wave, now);
-  const int8_t* source[RT];
+  const int8_t* source;
   if constexpr (FUSED) {
     quantize_few<SOURCE, WAVES>(A.x, A.x_vec, t.rows, A.K, A.pitch, few_codes, few_scales, most,
                                 [&](int r) { return static_cast<int64_t>(slot_of(A, t.begin + r) / A.top_k) * A.x_stride; });
-    source[0] = few_codes + min(lane & 31, t.rows - 1) * A.pitch + (lane >> 5) * 16;
+    source = few_codes + min(lane & 31, t.rows - 1) * A.pitch + (lane >> 5) * 16;
   } else {
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      const int place = t.begin + min(i * 32 + (lane & 31), t.rows - 1);
-      const int row = UP ? slot_of(A, place) / A.top_k : place;
-      source[i] = A.codes + static_cast<int64_t>(row) * A.pitch + (lane >> 5) * 16;
-    }
+    const int place = t.begin + min(lane & 31, t.rows - 1);
+    const int row = UP ? slot_of(A, place) / A.top_k : place;
+    source = A.codes + static_cast<int64_t>(row) * A.pitch + (lane >> 5) * 16;
   }
   for (int c = wave; c < A.chunks; c += AT_ONCE * WAVES) {
-    v4i a[AT_ONCE][RT];
+    v4i a[AT_ONCE];
 #pragma unroll
-    for (int u = 0; u < AT_ONCE; ++u)
-#pragma unroll
-      for (int i = 0; i < RT; ++i) a[u][i] = *reinterpret_cast<const v4i*>(source[i] + min(c + u * WAVES, A.chunks - 1) * 32);
+    for (int u = 0; u < AT_ONCE; ++u) a[u] = *reinterpret_cast<const v4i*>(source + min(c + u * WAVES, A.chunks - 1) * 32);
     if (c + AT_ONCE * WAVES < A.chunks) load(c + AT_ONCE * WAVES, next);
 #pragma unroll
     for (int u = 0; u < AT_ONCE; ++u) {
       if (c + u * WAVES >= A.chunks) break;
 #pragma unroll
-      for (int w = 0; w < EACH; ++w)
-#pragma unroll
-        for (int i = 0; i < RT; ++i) acc[w][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(now.b[u][w], a[u][i], acc[w][i], 0, 0, 0);
+      for (int w = 0; w < EACH; ++w) acc[w] = __builtin_amdgcn_mfma_i32_32x32x32_i8(now.b[u][w], a[u], acc[w], 0, 0, 0);
     }
     now = next;
   }
-  // row tile by row tile: the shares' sums, then four channels of a row a thread
+  // the shares' sums, then four channels of a row a thread
   const int m = threadIdx.x >> 3, n0 = strip * 32 + (threadIdx.x & 7) * 4;
-  static_for<RT>([&](auto tile) {
-    constexpr int i = decltype(tile)::value;
-    if (i * 32 >= t.rows) return;  // the same for all
-    if (i > 0) __syncthreads();
 #pragma unroll
-    for (int w = 0; w < EACH; ++w)
+  for (int w = 0; w < EACH; ++w)
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<v4i*>(&sums[w][wave][(lane & 31) * PITCH + g * 8 + (lane >> 5) * 4]) =
-            v4i{acc[w][i][4 * g], acc[w][i][4 * g + 1], acc[w][i][4 * g + 2], acc[w][i][4 * g + 3]};
-    __syncthreads();
-    if (m >= 32 || i * 32 + m >= t.rows) return;
-    const int place = t.begin + i * 32 + m;
-    const int slot = slot_of(A, place);
-    const float s = FUSED ? few_scales[m % kFewRows] : A.row_scales[UP ? slot / A.top_k : place];
-    float v[EACH][4];
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<v4i*>(&sums[w][wave][(lane & 31) * PITCH + g * 8 + (lane >> 5) * 4]) =
+          v4i{acc[w][4 * g], acc[w][4 * g + 1], acc[w][4 * g + 2], acc[w][4 * g + 3]};
+  __syncthreads();
+  if (m >= t.rows) return;
+  const int place = t.begin + m;
+  const int slot = slot_of(A, place);
+  const float s = FUSED ? few_scales[m % kFewRows] : A.row_scales[UP ? slot / A.top_k : place];
+  float v[EACH][4];
 #pragma unroll
-    for (int w = 0; w < EACH; ++w) {
-      v4i sum = *reinterpret_cast<const v4i*>(&sums[w][0][m * PITCH + (threadIdx.x & 7) * 4]);
+  for (int w = 0; w < EACH; ++w) {
+    v4i sum = *reinterpret_cast<const v4i*>(&sums[w][0][m * PITCH + (threadIdx.x & 7) * 4]);
 #pragma unroll
-      for (int o = 1; o < WAVES; ++o) sum += *reinterpret_cast<const v4i*>(&sums[w][o][m * PITCH + (threadIdx.x & 7) * 4]);
-      const float* of = A.scales + (static_cast<int64_t>(t.group) * EACH + w) * A.N;
+    for (int o = 1; o < WAVES; ++o) sum += *reinterpret_cast<const v4i*>(&sums[w][o][m * PITCH + (threadIdx.x & 7) * 4]);
+    const float* of = A.scales + (static_cast<int64_t>(t.group) * EACH + w) * A.N;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[w][j] = static_cast<float>(sum[j]) * (s * of[min(n0 + j, A.N - 1)]);
+    for (int j = 0; j < 4; ++j) v[w][j] = static_cast<float>(sum[j]) * (s * of[min(n0 + j, A.N - 1)]);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float y = v[0][j];
+    if constexpr (UP) {
+      y = activate(A.activation, y);
+      if constexpr (GATED) y = y * v[1][j];
+      if (n0 + j < A.N) store_output<OUT>(A.out, static_cast<int64_t>(place) * A.N + n0 + j, y);
+    } else {
+      if (n0 + j < A.N) static_cast<float*>(A.out)[static_cast<int64_t>(slot) * A.N + n0 + j] = y;
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float y = v[0][j];
-      if constexpr (UP) {
-        y = activate(A.activation, y);
-        if constexpr (GATED) y = y * v[1][j];
-        if (n0 + j < A.N) store_output<OUT>(A.out, static_cast<int64_t>(place) * A.N + n0 + j, y);
-      } else {
-        if (n0 + j < A.N) static_cast<float*>(A.out)[static_cast<int64_t>(slot) * A.N + n0 + j] = y;
-      }
-    }
-  });
+  }
 }
 
 // The way back of very few choices in one launch: a workgroup has a strip of 32 channels of every expert that is chosen.  Its
@@ -784,13 +770,13 @@ void launch_quantize(const void* x, int64_t stride, int64_t rows, int64_t K, con
   });
 }
 
-template <int OUT, bool GATED, int RT, int WAVES, int SOURCE>
+template <int OUT, bool GATED, int WAVES, int SOURCE>
 int launch_stream(ProductArgs A, hipStream_t st) {
   A.few = A.slots / A.top_k;  // (tokens: an expert has no more rows, unless a token names it twice, which is one more tile)
-  const int per_tile = SOURCE != 0 ? A.few : 32 * RT, lds = SOURCE != 0 ? A.few * A.pitch : 0;
+  const int per_tile = SOURCE != 0 ? A.few : 32, lds = SOURCE != 0 ? A.few * A.pitch : 0;
   constexpr int STATIC = (GATED ? 2 : 1) * WAVES * 32 * 36 * 4 + 1024;
   static unsigned long long configured;
-  const auto kernel = experts_stream_kernel<OUT, GATED, RT, WAVES, SOURCE>;
+  const auto kernel = experts_stream_kernel<OUT, GATED, WAVES, SOURCE>;
   if (STATIC + lds > 64 * 1024 && !device_bit(&configured, false)) {
     const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kFewBytes);
     if (err != hipSuccess) return hip_fail(err, "hipFuncSetAttribute(experts_stream_kernel)");
@@ -822,16 +808,20 @@ int launch_tiles(ProductArgs A, hipStream_t st) {
 }
 template <int OUT, bool GATED>
 int launch_products(const ProductArgs& A, hipStream_t st) {
-  const int64_t each = A.slots / A.experts;
+  // Tiles cost a workgroup about 10 us whatever they hold, and have to be enough of them; strips read an expert's weights again for every 32
+  // rows.  Measured, tiles : strips in us, 8 experts of 4096 x 4096, gated, at 16, 32, 64 rows each 67 : 57, 68 : 75, 75 : 130, not gated 49 : 44,
+  // 54 : 66, 66 : 99; 32 of 1408 x 2048, not gated, at 8, 16 30 : 29, 32 : 38; 4 of 14336 x 4096 (64 tiles) at 32, 64 134 : 101, 162 : 171;
+  // 8 of 1024 x 1024 (64 tiles) at 64, 128, 256 18 : 13, 24 : 21, 25 : 30.
+  constexpr int WIDTH = GATED ? 128 : 256;
+  const int64_t each = A.slots / A.experts, tiles = static_cast<int64_t>(A.experts) * ((A.N + WIDTH - 1) / WIDTH);
   const bool near = OUT == 0 || A.slots / A.top_k * static_cast<int64_t>(A.pitch) < (1LL << 32);  // up: codes in reach of 32 bits
-  if (each > 64 && A.chunks >= 2 * kTileSteps && near) {
+  if (each >= (GATED ? 24 : 12) && each * tiles >= (A.pitch >= 2048 ? 3072 : 8192) && A.chunks >= 2 * kTileSteps && near) {
     if (GATED && A.activation == ITEXHIP_ACT_SWISH) return launch_tiles<OUT, GATED, GATED, 256, 256>(A, st);
     return launch_tiles<OUT, GATED, false, 256, 256>(A, st);
   }
-  if (each > 16) return launch_stream<OUT, GATED, 2, 4, 0>(A, st);
   // few strips: more wavefronts for each, so that the device has enough on their way
   const int64_t strips = tiles_bound(A.slots, A.experts, 32, false) * A.strips;
-  return strips >= 1024 ? launch_stream<OUT, GATED, 1, 4, 0>(A, st) : launch_stream<OUT, GATED, 1, 8, 0>(A, st);
+  return strips >= 512 ? launch_stream<OUT, GATED, 4, 0>(A, st) : launch_stream<OUT, GATED, 8, 0>(A, st);
 }
 
 ProductArgs product_args(const itexhip_experts_params& p, bool up, const Layout& l, void* workspace, const int32_t* offsets, const int32_t* rows,
@@ -868,8 +858,8 @@ int run_up(const itexhip_experts_params& p, const void* x, const int32_t* offset
   A.x_vec = aligned(x, 16) && (p.x_stride * element_size(T)) % 16 == 0;
   if (few_up(A)) {
     const int64_t strips = tiles_bound(A.slots, A.experts, 32, false) * A.strips;
-    if (p.gated) return strips >= 1024 ? launch_stream<T, true, 1, 4, T>(A, st) : launch_stream<T, true, 1, 8, T>(A, st);
-    return strips >= 1024 ? launch_stream<T, false, 1, 4, T>(A, st) : launch_stream<T, false, 1, 8, T>(A, st);
+    if (p.gated) return strips >= 512 ? launch_stream<T, true, 4, T>(A, st) : launch_stream<T, true, 8, T>(A, st);
+    return strips >= 512 ? launch_stream<T, false, 4, T>(A, st) : launch_stream<T, false, 8, T>(A, st);
   }
   launch_quantize<T>(x, p.x_stride, p.tokens, p.hidden, A, st);
   return p.gated ? launch_products<T, true>(A, st) : launch_products<T, false>(A, st);
