@@ -266,14 +266,13 @@ __global__ __launch_bounds__(256, KS <= 2 ? 3 : 2) void expand_kernel(const Adap
     }
 
   for (int n = threadIdx.x; n < ROWS; n += 256) tokens[n] = token_of(A, t.begin + min(n, t.rows - 1));
-  __syncthreads();
   const int row = threadIdx.x >> 4, part = threadIdx.x & 15;  // 16 threads a row of operands
   constexpr int EACH = KS * 2;  // r that a thread has, in pairs from 2 part on
   struct Round {
     float v[EACH];
     Run<T, NT> base[4];  // of the lane's rows, 4 (lane / 16) .. + 3
   };
-  auto load = [&](int n, Round& q) {
+  auto load_middle = [&](int n, Round& q) {
     const float* from = A.middle + static_cast<int64_t>(t.begin + min(n * 16 + row, t.rows - 1)) * A.deep + slice * A.p.rank + part * 2;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -294,6 +293,8 @@ __global__ __launch_bounds__(256, KS <= 2 ? 3 : 2) void expand_kernel(const Adap
       q.v[2 * s] = sum.x;
       q.v[2 * s + 1] = s * 32 + part * 2 + 1 < rank ? sum.y : 0.0f;
     }
+  };
+  auto load_base = [&](int n, Round& q) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int m = n * 16 + (lane >> 4) * 4 + i;
@@ -305,7 +306,9 @@ __global__ __launch_bounds__(256, KS <= 2 ? 3 : 2) void expand_kernel(const Adap
   };
   const int rounds = (t.rows + 15) / 16;
   Round now, next;
-  load(0, now);
+  load_middle(0, now);
+  __syncthreads();
+  load_base(0, now);
   for (int n = 0; n < rounds; ++n) {
     const int parity = n & 1;
     float up = 1.0f, down = 1.0f;
@@ -333,7 +336,10 @@ __global__ __launch_bounds__(256, KS <= 2 ? 3 : 2) void expand_kernel(const Adap
       }
     }
     __syncthreads();  // (one a round: the next one's operands go to the other half)
-    if (n + 1 < rounds) load(n + 1, next);
+    if (n + 1 < rounds) {
+      load_middle(n + 1, next);
+      load_base(n + 1, next);
+    }
     v4f d[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) d[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
@@ -384,8 +390,8 @@ int check(const itexhip_adapters_params* p, const char* name) {
   return ITEXHIP_OK;
 }
 
-// Many places an adapter: tiles of 64 of them (16 where most would be empty), which read A a quarter as often
-bool long_tiles(int64_t tokens, int adapters) { return tokens > 32 * static_cast<int64_t>(adapters); }
+// Many places an adapter: tiles of 64 of them, which read A a quarter as often; 16 where most would be empty or tiles few
+bool long_tiles(int64_t tokens, int adapters) { return tokens > 32 * static_cast<int64_t>(adapters) && tiles_bound(tokens, adapters, 64, false) >= 64; }
 // Shares of K: enough workgroups for the device where tiles are few, of at least 256 k each
 constexpr int kEnoughTiles = 512;
 int splits_of(int64_t tokens, int adapters, int64_t parts, int64_t in) {
@@ -431,13 +437,20 @@ void launch_expand(AdapterArgs A, hipStream_t st) {
     expand_kernel<T, KS, NT, ROWS><<<count, 256, 0, st>>>(A);
   });
 }
-template <int T, int ROWS>
+template <int T, int KS, int NT>
+void launch_expand(const AdapterArgs& A, hipStream_t st) {
+  // 64 places a workgroup where that leaves enough of them
+  const int64_t blocks = (A.columns + 64 * NT - 1) / (64 * NT);
+  if (long_tiles(A.tokens, A.p.adapters) && tiles_bound(A.tokens, A.p.adapters, 64, true) * blocks >= kEnoughTiles) launch_expand<T, KS, NT, 64>(A, st);
+  else launch_expand<T, KS, NT, 16>(A, st);
+}
+template <int T>
 void launch_expand(const AdapterArgs& A, hipStream_t st) {
   constexpr int NT = T == ITEXHIP_FLOAT ? 4 : 8;  // 16 bytes of a lane's row; fewer where more would not fit the registers
-  if (A.p.rank <= 32) launch_expand<T, 1, NT, ROWS>(A, st);
-  else if (A.p.rank <= 64) launch_expand<T, 2, NT, ROWS>(A, st);
-  else if (A.p.rank <= 128) launch_expand<T, 4, 4, ROWS>(A, st);
-  else launch_expand<T, 8, T == ITEXHIP_FLOAT ? 2 : 4, ROWS>(A, st);
+  if (A.p.rank <= 32) launch_expand<T, 1, NT>(A, st);
+  else if (A.p.rank <= 64) launch_expand<T, 2, NT>(A, st);
+  else if (A.p.rank <= 128) launch_expand<T, 4, 4>(A, st);
+  else launch_expand<T, 8, T == ITEXHIP_FLOAT ? 2 : 4>(A, st);
 }
 
 template <int T>
@@ -449,8 +462,7 @@ void run_adapters(AdapterArgs A, hipStream_t st) {
   const bool wide = long_tiles(A.tokens, A.p.adapters);
   if (vec) wide ? launch_shrink<T, true, 4>(A, st) : launch_shrink<T, true, 1>(A, st);
   else wide ? launch_shrink<T, false, 4>(A, st) : launch_shrink<T, false, 1>(A, st);
-  if (wide) launch_expand<T, 64>(A, st);
-  else launch_expand<T, 16>(A, st);
+  launch_expand<T>(A, st);
 }
 
 }  // namespace

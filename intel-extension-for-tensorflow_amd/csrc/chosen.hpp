@@ -105,9 +105,9 @@ struct TileCount {
     int first = __builtin_amdgcn_readlane(begin, owner), count = __builtin_amdgcn_readlane(rows, owner);
     for (int g = owner * each;;) {
       const int tiles = tiles_of(count);
-      if (rank < tiles * units) return GroupUnit{g, first, count, tiles, rank};
+      if (rank >= 0 && rank < tiles * units) return GroupUnit{g, first, count, tiles, rank};
       rank -= tiles * units;
-      ++g;
+      if (++g >= groups + (REST ? 1 : 0)) return GroupUnit{-1, 0, 0, 0, 0};  // (offsets that are none, whose tiles do not add up)
       first = __builtin_amdgcn_readfirstlane(at(g));
       count = __builtin_amdgcn_readfirstlane(max(at(g + 1) - first, 0));
     }

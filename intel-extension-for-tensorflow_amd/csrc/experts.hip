@@ -284,13 +284,13 @@ constexpr int kFewPlaces = 16, kFewWaves = 16;
 template <int T>
 __global__ __launch_bounds__(64 * kFewWaves) void experts_few_down_kernel(const ProductArgs A, const FewArgs F) {
   constexpr int PITCH = 36;
-  __shared__ __align__(16) int sums[kFewWaves][kFewPlaces * PITCH];
+  __shared__ __align__(16) int sums[kFewWaves][kFewPlaces * PITCH];  // of a share: a place's own expert
   __shared__ float results[kFewPlaces][32];
   __shared__ float row_scales[kFewPlaces];
   __shared__ uint32_t most[kFewWaves];
   extern __shared__ __align__(16) int8_t few_codes[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), strip = blockIdx.x;
-  // the lane's place (all lanes hold them again from kFewPlaces on), its slot and expert, -1: none here
+  // the lane's place (the upper lanes hold them again), its slot and expert, -1: none here
   const int place = lane & (kFewPlaces - 1);
   const int slot = slot_of(A, min(place, A.slots - 1));
   int expert = F.experts[slot];
@@ -300,16 +300,15 @@ __global__ __launch_bounds__(64 * kFewWaves) void experts_few_down_kernel(const 
   for (int p = 0; p < A.slots; ++p) {
     const int e = __builtin_amdgcn_readlane(expert, p);
     if (e < 0) continue;
-    const unsigned long long same = __ballot(expert == e) & ((1ull << kFewPlaces) - 1);
+    const unsigned long long same = __ballot(expert == e);
     if (__builtin_ctzll(same) != p) continue;
     if (expert == e) order = number;
     ++number;
   }
   number = __builtin_amdgcn_readfirstlane(number);
-  if (number > 0) {  // (the same for all wavefronts: they all waited for the same values)
+  if (number > 0) {  // (the same for all wavefronts: they all saw the same values)
     const int shares = kFewWaves / number, mine = wave % number, share = wave / number;
-    const unsigned long long of_mine = __ballot(order == mine && lane < kFewPlaces);
-    const int e = __builtin_amdgcn_readlane(expert, __builtin_ctzll(of_mine));
+    const int e = __builtin_amdgcn_readlane(expert, __builtin_ctzll(__ballot(order == mine)));
     const int8_t* weights = A.packed + static_cast<int64_t>(e) * A.panel + static_cast<int64_t>(strip) * A.chunks * kChunkBytes + lane * 16;
     constexpr int AT_ONCE = 8;
     v4i now[AT_ONCE], next[AT_ONCE];
@@ -319,11 +318,11 @@ __global__ __launch_bounds__(64 * kFewWaves) void experts_few_down_kernel(const 
     };
     if (share < shares) load(share, now);
     quantize_few<T, kFewWaves>(A.x, A.x_vec, A.slots, A.K, A.pitch, few_codes, row_scales, most, [&](int r) { return r * A.x_stride; });
-    v16i acc;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[r] = 0;
-    const int8_t* source = few_codes + min(lane & 31, A.slots - 1) * A.pitch + (lane >> 5) * 16;
     if (share < shares) {
+      const int8_t* source = few_codes + min(lane & 31, A.slots - 1) * A.pitch + (lane >> 5) * 16;
+      v16i acc;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[r] = 0;
       for (int c = share; c < A.chunks; c += AT_ONCE * shares) {
         if (c + AT_ONCE * shares < A.chunks) load(c + AT_ONCE * shares, next);
 #pragma unroll
@@ -334,22 +333,20 @@ __global__ __launch_bounds__(64 * kFewWaves) void experts_few_down_kernel(const 
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u) now[u] = next[u];
       }
-    }
-    if ((lane & 31) < kFewPlaces) {
+      if ((lane & 31) == place && order == mine) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<v4i*>(&sums[wave][(lane & 31) * PITCH + g * 8 + (lane >> 5) * 4]) = v4i{acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<v4i*>(&sums[share][place * PITCH + g * 8 + (lane >> 5) * 4]) = v4i{acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
+      }
     }
     __syncthreads();
     // a thread for each place and channel
     const int p = threadIdx.x >> 5, n = threadIdx.x & 31;
-    if (p < kFewPlaces) {
-      const int to = __shfl(slot, p), which = __shfl(order, p), its = __shfl(expert, p);
-      if (p < A.slots && which >= 0) {
-        int sum = 0;
-        for (int o = 0; o < shares; ++o) sum += sums[which + o * number][p * PITCH + n];
-        results[to % kFewPlaces][n] = static_cast<float>(sum) * (row_scales[p] * A.scales[static_cast<int64_t>(its) * A.N + min(strip * 32 + n, A.N - 1)]);
-      }
+    const int to = __shfl(slot, p), which = __shfl(order, p), its = __shfl(expert, p);
+    if (p < A.slots && which >= 0) {
+      int sum = 0;
+      for (int o = 0; o < shares; ++o) sum += sums[o][p * PITCH + n];
+      results[to][n] = static_cast<float>(sum) * (row_scales[p] * A.scales[static_cast<int64_t>(its) * A.N + min(strip * 32 + n, A.N - 1)]);
     }
     __syncthreads();
   }
@@ -458,6 +455,8 @@ __global__ __launch_bounds__(256) void experts_tile_kernel(const ProductArgs A) 
     if (!w.there) return;
     const bool whole = local >= last_run;
     const GroupUnit u = whole ? full.find(columns, full_begin + local - last_run) : last.find(columns, last_begin + local);
+    w.there = u.group >= 0;
+    if (!w.there) return;
     int tile_m, tile_n;
     if (whole) {
       const int group = __builtin_amdgcn_readfirstlane(static_cast<int>(u.index / (kTileGroup * columns)));
@@ -483,13 +482,13 @@ __global__ __launch_bounds__(256) void experts_tile_kernel(const ProductArgs A) 
       const int ld = wave * B_PER_WAVE + static_cast<int>(c), strip = min((w.n_base + channel_of(ld >> 1)) >> 5, A.strips - 1);
       src.b[c] = weights + which_of(ld >> 1) * A.panel + (static_cast<int64_t>(strip) * A.chunks + (ld & 1)) * kChunkBytes;
     });
-    static_assert(BM == 256 && BN == 256, "a thread for each row and channel");
+    static_assert(BM == 256 && BN <= 256, "a thread for each row and channel");
     {
       const int place = w.begin + min(static_cast<int>(threadIdx.x), w.rows - 1), slot = slot_of(A, place);
       panel[BN + threadIdx.x] = A.row_scales[UP ? slot / A.top_k : place];
       reinterpret_cast<int*>(panel)[BN + BM + threadIdx.x] = slot;
-      const int c = threadIdx.x >> 5, n = min(w.n_base + channel_of(c) + static_cast<int>(threadIdx.x & 31), A.N - 1);
-      panel[threadIdx.x] = A.scales[(static_cast<int64_t>(u.group) * EACH + which_of(c)) * A.N + n];
+      const int c = threadIdx.x % BN >> 5, n = min(w.n_base + channel_of(c) + static_cast<int>(threadIdx.x & 31), A.N - 1);
+      if (threadIdx.x < BN) panel[threadIdx.x] = A.scales[(static_cast<int64_t>(u.group) * EACH + which_of(c)) * A.N + n];
     }
   };
   const uint32_t lane16 = lane * 16;
@@ -529,10 +528,10 @@ __global__ __launch_bounds__(256) void experts_tile_kernel(const ProductArgs A) 
   __syncthreads();
 
   int ring = 0;  // stage of the tile's first step
-  int number = blockIdx.x >> 3;
+  int64_t number = blockIdx.x >> 3;
   for (int slot = 0;; slot = slot == 2 ? 0 : slot + 1) {
     // (a third panel: a wavefront may be here while another one still is at the results of the tile before)
-    number += static_cast<int>(gridDim.x >> 3);
+    number += gridDim.x >> 3;
     find(number, next, next_src, panels + (slot == 2 ? 0 : slot + 1) * PANEL);
     const bool more = __builtin_amdgcn_readfirstlane(next.there);  // what is fetched behind the last tile is not used
     v16i acc[TN * TM];
@@ -748,13 +747,18 @@ Layout layout_of(const itexhip_experts_params& p, bool up) {
 }
 
 // Codes that a workgroup keeps in LDS
-constexpr int kFewBytes = 48 * 1024;
-// up: a workgroup makes the codes of its tokens itself, up to 32 elements a thread; beyond, a launch that makes them once is shorter
+constexpr int kFewBytes = 64 * 1024;
+// up: a workgroup makes the codes of its tokens itself where they are about 32 elements a thread; beyond, a launch that makes them once is shorter
 bool few_up(const ProductArgs& A) {
-  const int64_t tokens = A.slots / A.top_k;
-  return tokens <= kFewRows && tokens * A.pitch <= 8192;
+  const int64_t tokens = A.slots / A.top_k, each = A.slots > A.experts ? (A.slots + A.experts - 1) / A.experts : 1;
+  return tokens <= kFewRows && each * A.pitch <= 8192 && tokens * A.pitch <= kFewBytes / 2;
 }
-bool few_down(const ProductArgs& A) { return A.slots <= kFewPlaces && static_cast<int64_t>(A.slots) * A.pitch <= kFewBytes; }
+// down, one launch : three in us: 2 rows of 768 to 14336 7 : 12 to 32 : 34, 4 of 1536 and 4096 11 : 16 and 18 : 15, 8 of 768 and 1536 10 : 13 and 13 : 17,
+// where there are few channels 12 : 12, 16 of 768 13 : 13
+bool few_down(const ProductArgs& A) {
+  const int64_t bytes = static_cast<int64_t>(A.slots) * A.pitch;
+  return A.slots <= kFewPlaces && (A.slots <= 2 || bytes <= 8192) && bytes <= kFewBytes;
+}
 
 template <int T>
 void launch_quantize(const void* x, int64_t stride, int64_t rows, int64_t K, const ProductArgs& A, hipStream_t st) {
@@ -774,10 +778,9 @@ template <int OUT, bool GATED, int WAVES, int SOURCE>
 int launch_stream(ProductArgs A, hipStream_t st) {
   A.few = A.slots / A.top_k;  // (tokens: an expert has no more rows, unless a token names it twice, which is one more tile)
   const int per_tile = SOURCE != 0 ? A.few : 32, lds = SOURCE != 0 ? A.few * A.pitch : 0;
-  constexpr int STATIC = (GATED ? 2 : 1) * WAVES * 32 * 36 * 4 + 1024;
   static unsigned long long configured;
   const auto kernel = experts_stream_kernel<OUT, GATED, WAVES, SOURCE>;
-  if (STATIC + lds > 64 * 1024 && !device_bit(&configured, false)) {
+  if (SOURCE != 0 && !device_bit(&configured, false)) {
     const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kFewBytes);
     if (err != hipSuccess) return hip_fail(err, "hipFuncSetAttribute(experts_stream_kernel)");
     device_bit(&configured, true);
@@ -787,6 +790,11 @@ int launch_stream(ProductArgs A, hipStream_t st) {
     kernel<<<count, 64 * WAVES, lds, st>>>(A);
   });
   return ITEXHIP_OK;
+}
+// Few strips: eight wavefronts each instead of four, so that the device has enough on their way (896 strips of 4096: 46 -> 39 us), unless that
+// leaves a wavefront a handful of chunks (736 of 1024: 13 -> 15)
+bool few_strips(const ProductArgs& A) {
+  return tiles_bound(A.slots, A.experts, 32, false) * A.strips < (A.chunks >= 64 ? 1024 : 512);
 }
 constexpr int kWorkgroups = 256;  // one for each CU; they take the tiles in turns
 
@@ -816,12 +824,15 @@ int launch_products(const ProductArgs& A, hipStream_t st) {
   const int64_t each = A.slots / A.experts, tiles = static_cast<int64_t>(A.experts) * ((A.N + WIDTH - 1) / WIDTH);
   const bool near = OUT == 0 || A.slots / A.top_k * static_cast<int64_t>(A.pitch) < (1LL << 32);  // up: codes in reach of 32 bits
   if (each >= (GATED ? 24 : 12) && each * tiles >= (A.pitch >= 2048 ? 3072 : 8192) && A.chunks >= 2 * kTileSteps && near) {
-    if (GATED && A.activation == ITEXHIP_ACT_SWISH) return launch_tiles<OUT, GATED, GATED, 256, 256>(A, st);
+    constexpr bool SWISH = GATED;
+    if (tiles * ((each + 255) / 256) < kWorkgroups * 3 / 4) {  // half as many channels a tile where they are too few for the device
+      if (SWISH && A.activation == ITEXHIP_ACT_SWISH) return launch_tiles<OUT, GATED, SWISH, 256, 128>(A, st);
+      return launch_tiles<OUT, GATED, false, 256, 128>(A, st);
+    }
+    if (SWISH && A.activation == ITEXHIP_ACT_SWISH) return launch_tiles<OUT, GATED, SWISH, 256, 256>(A, st);
     return launch_tiles<OUT, GATED, false, 256, 256>(A, st);
   }
-  // few strips: more wavefronts for each, so that the device has enough on their way
-  const int64_t strips = tiles_bound(A.slots, A.experts, 32, false) * A.strips;
-  return strips >= 512 ? launch_stream<OUT, GATED, 4, 0>(A, st) : launch_stream<OUT, GATED, 8, 0>(A, st);
+  return few_strips(A) ? launch_stream<OUT, GATED, 8, 0>(A, st) : launch_stream<OUT, GATED, 4, 0>(A, st);
 }
 
 ProductArgs product_args(const itexhip_experts_params& p, bool up, const Layout& l, void* workspace, const int32_t* offsets, const int32_t* rows,
@@ -857,9 +868,8 @@ int run_up(const itexhip_experts_params& p, const void* x, const int32_t* offset
   A.x_stride = p.x_stride;
   A.x_vec = aligned(x, 16) && (p.x_stride * element_size(T)) % 16 == 0;
   if (few_up(A)) {
-    const int64_t strips = tiles_bound(A.slots, A.experts, 32, false) * A.strips;
-    if (p.gated) return strips >= 512 ? launch_stream<T, true, 4, T>(A, st) : launch_stream<T, true, 8, T>(A, st);
-    return strips >= 512 ? launch_stream<T, false, 4, T>(A, st) : launch_stream<T, false, 8, T>(A, st);
+    if (p.gated) return few_strips(A) ? launch_stream<T, true, 8, T>(A, st) : launch_stream<T, true, 4, T>(A, st);
+    return few_strips(A) ? launch_stream<T, false, 8, T>(A, st) : launch_stream<T, false, 4, T>(A, st);
   }
   launch_quantize<T>(x, p.x_stride, p.tokens, p.hidden, A, st);
   return p.gated ? launch_products<T, true>(A, st) : launch_products<T, false>(A, st);
@@ -935,6 +945,7 @@ extern "C" int itexhip_experts_down(const itexhip_experts_params* p, const void*
                       aligned(scales, 4) && aligned(weights, 4),
                   "itexhip_experts_down: buffers are aligned to their elements");
   ITEXHIP_REQUIRE(aligned(packed, 16) && aligned(workspace, 16), "itexhip_experts_down: packed weights and workspace are aligned to 16 bytes");
+  ITEXHIP_REQUIRE(addend != out || p->addend_stride == p->out_stride, "itexhip_experts_down: in place, addend_stride and out_stride are the same");
   hipStream_t st = as_stream(stream);
   const int status = p->type == ITEXHIP_FLOAT      ? run_down<ITEXHIP_FLOAT>(*p, h, experts, offsets, rows, packed, scales, weights, addend, out, workspace, st)
                      : p->type == ITEXHIP_BFLOAT16 ? run_down<ITEXHIP_BFLOAT16>(*p, h, experts, offsets, rows, packed, scales, weights, addend, out, workspace, st)

@@ -254,7 +254,9 @@ void launch_route(RouteArgs A, hipStream_t st) {
 }
 template <int T>
 void launch_route(const RouteArgs& A, hipStream_t st) {
+  // few tokens: more lanes each, whose instructions one after the other are what takes the time
   if (A.p.experts <= 64) launch_route<T, 16, 4>(A, st);
+  else if (A.p.experts <= 256 && A.tokens <= 1024) launch_route<T, 64, 4>(A, st);
   else if (A.p.experts <= 256) launch_route<T, 16, 16>(A, st);
   else launch_route<T, 64, 16>(A, st);
 }

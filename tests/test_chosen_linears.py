@@ -113,6 +113,9 @@ def test_experts_refuse(hip):
         args[at] = bad
         with pytest.raises(hip.ItexHipError, match="aligned"):
             hip.experts_down(p, *args)
+    other = hip.experts_params(hip.BFLOAT16, **{**{k: v for k, v in EXPERTS.items() if k != "type"}, "addend_stride": 80})
+    with pytest.raises(hip.ItexHipError, match="in place"):
+        hip.experts_down(other, *([64] * 10))
     empty = hip.experts_params(hip.HALF, **{k: v for k, v in {**EXPERTS, "tokens": 0}.items() if k != "type"})
     hip.experts_up(empty, *([None] * 7))
     hip.experts_down(empty, *([None] * 10))

@@ -50,7 +50,8 @@ def whole(shape, limit, g):
 SIZES = [  # tokens, adapters, rank, K, ends, ragged ranks
     (1, 1, 8, 8, [1], False), (1, 4, 16, 64, [64], False), (2, 2, 8, 40, [100], False), (7, 3, 24, 72, [64, 96, 131], True), (16, 1, 32, 256, [130], False),
     (17, 5, 64, 200, [33, 34, 97, 200], True), (64, 64, 16, 512, [256, 320, 384], True), (65, 2, 40, 1040, [70], False), (100, 1000, 8, 64, [48], False),
-    (300, 3, 128, 96, [300], True), (33, 2, 256, 64, [128], True), (1000, 5, 16, 160, [513], False), (5, 3, 16, 4104, [64], False), (2100, 4, 64, 320, [200], False)]
+    (300, 3, 128, 96, [300], True), (33, 2, 256, 64, [128], True), (1000, 5, 16, 160, [513], False), (5, 3, 16, 4104, [64], False), (2100, 4, 64, 320, [200], False),
+    (4500, 2, 16, 96, [4100], False), (4200, 3, 72, 72, [1030, 2070], True), (4200, 1, 256, 64, [2100], False)]
 
 
 @pytest.mark.parametrize("name", list(ref.TYPES))
@@ -205,7 +206,7 @@ def test_beside_a_quantized_linear_and_captured(hip, dev):
 def test_orders_that_are_none_stay_inside(hip, dev):
     t, n, rank, K, N = 9, 3, 8, 64, 64
     p = hip.adapters_params(hip.FLOAT, n, rank, t, K, [N])
-    for offsets in ([0, 5, 100, 9], [-4, 7, 3, 1 << 30], [9, 9, 9, 9]):
+    for offsets in ([0, 5, 100, 9], [-4, 7, 3, 1 << 30], [9, 9, 9, 9], [0, 9, 0, 9], [9, 0, 9, 0]):
         rows = torch.tensor([0, 8, 9, -1, 1 << 30, 3, 3, 3, 3], dtype=torch.int32, device=dev)
         out, size = torch.zeros(t + 1, N, device=dev), hip.adapters_workspace(p)
         work = torch.full((size + 64,), 0x5a, dtype=torch.uint8, device=dev)

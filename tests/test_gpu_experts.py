@@ -95,7 +95,9 @@ def whole(shape, limit, g, largest=None):
 
 SIZES = [  # tokens, top_k, experts, K, N, total experts
     (1, 2, 8, 64, 32, 8), (1, 1, 1, 1, 1, 1), (2, 2, 4, 33, 31, 4), (5, 3, 7, 100, 65, 14), (33, 4, 6, 200, 130, 6), (64, 6, 64, 256, 96, 64), (31, 1, 3, 1000, 40, 3),
-    (300, 2, 4, 128, 264, 8), (129, 8, 16, 72, 48, 16), (700, 2, 3, 64, 70, 3), (3, 32, 40, 64, 33, 80), (40, 1, 1024, 48, 32, 1024), (600, 1, 1, 192, 512, 1), (1100, 4, 5, 320, 136, 5)]
+    (300, 2, 4, 128, 264, 8), (129, 8, 16, 72, 48, 16), (700, 2, 3, 64, 70, 3), (3, 32, 40, 64, 33, 80), (40, 1, 1024, 48, 32, 1024), (600, 1, 1, 192, 512, 1), (1100, 4, 5, 320, 136, 5),
+    (1, 32, 40, 64, 33, 80), (2, 16, 20, 80, 40, 20), (4, 8, 64, 100, 64, 64), (16, 2, 5, 64, 100, 5), (8, 3, 3, 1000, 33, 6), (2, 1, 2, 8192, 40, 2), (13, 1, 1, 512, 96, 1),
+    (1500, 2, 3, 256, 600, 3), (3200, 2, 16, 200, 2100, 16), (1030, 2, 4, 449, 1100, 8), (4, 2, 2, 14336, 70, 2)]
 
 
 @pytest.mark.parametrize("name", list(ref.TYPES))
@@ -239,7 +241,7 @@ def test_orders_that_are_none_stay_inside(hip, dev):
     """Offsets and rows that are no order give no defined result, but nothing outside the outputs is read or written."""
     t, k, e, K, N = 9, 2, 3, 64, 64
     w = torch.ones(e, 1, N, K, dtype=torch.int8)
-    for offsets in ([0, 5, 100, 18], [-4, 7, 3, 1 << 30], [18, 18, 18, 18]):
+    for offsets in ([0, 5, 100, 18], [-4, 7, 3, 1 << 30], [18, 18, 18, 18], [0, 18, 0, 18], [18, 0, 18, 0]):
         offsets = torch.tensor(offsets, dtype=torch.int32)
         rows = torch.tensor([0, 17, 18, -1, 1 << 30] + [3] * 13, dtype=torch.int32)
         p = hip.experts_params(hip.FLOAT, e, k, t, K, N, activation=hip.ACT_NONE, gated=False)
@@ -251,6 +253,40 @@ def test_orders_that_are_none_stay_inside(hip, dev):
         hip.experts_down(p, torch.ones(t * k, K, device=dev), ids, offsets.to(dev), rows.to(dev), packed, ones, torch.ones(t, k, device=dev), None, out, work)
         torch.cuda.synchronize()
         assert bool((h[-1] == 0).all()) and bool((out[-1] == 0).all()) and bool((work[-256:] == 0x5a).all())
+
+
+def test_orders_that_are_none_stay_inside_tiles(hip, dev):
+    """The same for sizes whose rows go through tiles."""
+    t, k, e, K, N = 1500, 2, 3, 256, 600
+    n = t * k
+    w = torch.ones(e, 2, N, K, dtype=torch.int8)
+    packed, ones = pack(hip, dev, w), torch.ones(e, 2, N, device=dev)
+    p = hip.experts_params(hip.HALF, e, k, t, K, N, activation=hip.ACT_NONE)
+    for offsets in ([0, n, 0, n], [5, 7, 1 << 30, -3], [n, 0, n, 0]):
+        rows = torch.full((n,), -9, dtype=torch.int32)
+        rows[::3] = 1 << 30
+        h = torch.zeros(n + 1, N, dtype=torch.float16, device=dev)
+        size = hip.experts_workspace(p)
+        work = guarded(size, dev)
+        hip.experts_up(p, torch.ones(t, K, dtype=torch.float16, device=dev), torch.tensor(offsets, dtype=torch.int32, device=dev), rows.to(dev), packed, ones, h, work)
+        torch.cuda.synchronize()
+        assert bool((h[-1] == 0).all()) and bool((work[size:] == 0x5a).all())
+
+
+def test_a_token_that_names_an_expert_twice(hip, dev):
+    """Each choice is a row of its own, also where workgroups make the codes of as many rows as there are tokens."""
+    g = torch.Generator().manual_seed(8)
+    for t, k, e, K, N in ((1, 2, 4, 64, 40), (3, 4, 2, 100, 40), (5, 6, 3, 64, 64), (40, 2, 2, 64, 33)):
+        experts = torch.randint(0, e, (t, k), generator=g, dtype=torch.int32)
+        experts[0] = 1
+        offsets, rows = ref.order(experts, e)
+        x, w, scales = whole((t, K), 3, g, largest=127.0), whole((e, 1, N, K), 4, g).to(torch.int8), torch.full((e, 1, N), 0.5)
+        h = run_up(hip, dev, "float", x, offsets, rows, k, w, scales, "none", False)
+        assert torch.equal(h, ref.up(x, offsets, rows, k, w, scales, "none", False).float())
+        hh, w2, s2 = whole((t * k, N), 3, g, largest=127.0), whole((e, 1, K, N), 4, g).to(torch.int8), torch.full((e, 1, K), 0.5)
+        weights = torch.randint(0, 5, (t, k), generator=g).float()
+        out = run_down(hip, dev, "float", hh, experts, offsets, rows, w2, s2, weights, None)
+        assert torch.equal(out, ref.down(hh, experts, offsets, rows, w2, s2, weights, None)[0].float())
 
 
 def test_a_layer_from_router_to_sum(hip, dev):

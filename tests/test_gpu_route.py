@@ -44,7 +44,7 @@ def logits_of(t, e, dtype, seed, spread=1.5):
 
 
 @pytest.mark.parametrize("name", list(ref.TYPES))
-@pytest.mark.parametrize("t,e,k", [(1, 1, 1), (1, 8, 2), (3, 4, 4), (17, 60, 4), (33, 64, 6), (5, 65, 8), (65, 128, 8), (7, 255, 32), (130, 256, 8), (9, 257, 3), (6, 1000, 32), (5, 1024, 8)])
+@pytest.mark.parametrize("t,e,k", [(1, 1, 1), (1, 8, 2), (3, 4, 4), (17, 60, 4), (33, 64, 6), (5, 65, 8), (65, 128, 8), (7, 255, 32), (130, 256, 8), (9, 257, 3), (6, 1000, 32), (5, 1024, 8), (1030, 100, 8), (1500, 256, 5)])
 @pytest.mark.parametrize("score,biased,renormalise", [("softmax", False, True), ("sigmoid", True, True), ("softmax", True, False)])
 def test_route(hip, dev, name, t, e, k, score, biased, renormalise):
     x = logits_of(t, e, ref.TYPES[name], t * 1000 + e)
@@ -57,7 +57,12 @@ def test_route(hip, dev, name, t, e, k, score, biased, renormalise):
                                                        (510, 51, 7, 2, 9), (16, 1, 1, 1, 3), (63, 63, 63, 1, 32)])
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_groups(hip, dev, e, groups, top_groups, best, k, score):
-    x = logits_of(37, e, torch.float32, e + groups)
+    for t in (37, 1100):
+        groups_of_tokens(hip, dev, t, e, groups, top_groups, best, k, score)
+
+
+def groups_of_tokens(hip, dev, t, e, groups, top_groups, best, k, score):
+    x = logits_of(t, e, torch.float32, e + groups + t)
     bias = logits_of(1, e, torch.float32, 6, 0.3)[0]
     kw = dict(groups=groups, top_groups=top_groups, group_best=best, renormalise=True)
     check(route(hip, dev, x, bias, k, score, **kw), ref.route(x, bias, k, score, **kw))
