@@ -664,10 +664,10 @@ int itexhip_group_rows(int64_t n, int groups, const int32_t* group_of, int32_t* 
  *       order's places, and those behind offsets[experts] are left as they are.
  * down: out[t, n] = addend[t, n] + sum over j of weights[t, j] * v[n] of slot t * top_k + j, from the row of h in that slot's place; in fp32, j upwards,
  *       rounded to the type once; choices whose experts[t, j] is not in 0 .. experts - 1 are no part of it.  addend may be NULL
- *       (zero) or `out` itself.
- * packed: [experts][2 if gated, else 1][itexhip_qgemm_packed_bytes(K, N)] of itexhip_qgemm_prepack_b (16-byte aligned), gate first; K = hidden
- * and N = inner for up, the other way round for down.  scales: [experts][2 or 1][N], the weight that a code of 1 stands for.
- * activation: ITEXHIP_ACT_NONE, RELU, GELU_APPROX, GELU_EXACT or SWISH (for up). */
+ *       (zero) or `out` itself, with the same stride.
+ * packed: [experts][weights][itexhip_qgemm_packed_bytes(K, N)] of itexhip_qgemm_prepack_b (16-byte aligned); up has two weights if gated, the gate
+ * first, else one, with K = hidden and N = inner, down has one with K = inner and N = hidden.  scales: [experts][weights][N], what a code of 1 stands for.
+ * activation: ITEXHIP_ACT_NONE, RELU, GELU_APPROX, GELU_EXACT or SWISH (down reads neither it nor gated). */
 typedef struct {
   int type;           /* FLOAT | BFLOAT16 | HALF of x, h, addend and out */
   int experts;        /* 1 .. 1024 */

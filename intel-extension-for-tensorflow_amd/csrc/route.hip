@@ -9,7 +9,8 @@ namespace {
 // ------------------------------------------------------------------------------------------------
 // Router.  LPT lanes hold a token's ranks in 64 bits, PER consecutive experts each, so that LPT = 16 lets a wavefront choose for
 // four tokens at once.  What is chosen or left out becomes NaN, which neither a maximum nor an equality sees: top_k rounds of
-// one maximum over the lanes and the lowest expert that equals it.
+// one maximum over the lanes and the lowest expert that equals it.  8192 tokens, 8 of 256 experts in groups, logistic scores (fp32): 14 us for 8 MB, bound
+// by vector instructions, 1700 of a wavefront: 500 for the scores, 140 a round.
 // ------------------------------------------------------------------------------------------------
 struct RouteArgs {
   itexhip_route_params p;
@@ -265,7 +266,8 @@ void launch_route(const RouteArgs& A, hipStream_t st) {
 // Order of rows by group: a counting sort.  The rows are cut into runs, one a workgroup, whose wavefronts take consecutive shares.
 // A first launch counts each run's groups; in the second a wavefront knows where its rows of a group begin: behind all smaller
 // groups, the group's rows of earlier runs and those of the run's earlier wavefronts.  Rows of one group within 64 keep their
-// order by their number among the lanes.  One workgroup does both where there are few rows.
+// order by their number among the lanes.  One workgroup does both where there are few rows.  65536 rows in 256 groups: 4 us to count, 11 to order, round
+// trips for the runs' counts, the groups' sums and the rows one after the other; up to 1024 rows 2.5 to 4.
 // ------------------------------------------------------------------------------------------------
 constexpr int kOrderWaves = 4;
 constexpr int kRunRows = 1024, kMostRuns = 256;
