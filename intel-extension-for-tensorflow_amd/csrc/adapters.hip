@@ -374,6 +374,129 @@ __global__ __launch_bounds__(256, KS <= 2 ? 3 : 2) void expand_kernel(const Adap
   }
 }
 
+// Both products in one launch, for ranks up to 16: a workgroup makes x A^T of its 16 places and one slice for itself, 16 wavefronts a share of K each, and
+// goes on with 1024 columns, whose B and base travel meanwhile.  A is read once for every such block of columns, from L2 but for the first time.
+// One launch : two in us (runs differ by the host's pace), 1 token of 1024 to 4096 columns 6.6 : 7.7-9.4, of 2048 7.5 : 7.9-9.3, of 4096 9.5 : 8.4-9.7;
+// 64 of 1024 to 1024, an adapter each, 7.5 : 8.7-10.8; 1000 of 512 to 2048 8.4 : 9.3-11.6, 4000 of 512 to 1024 (4 MB of A read in all) 13.6-14.2 :
+// 13.2-14.0; 2000 of 1024 to 4096 (16 MB) 21 : 16.  fp32 and ranks of 32 do not fit the registers of 16 wavefronts.
+constexpr int kOnceWaves = 16;
+template <int T>
+__global__ __launch_bounds__(64 * kOnceWaves) void once_kernel(const AdapterArgs A) {
+  constexpr int NT = 4, PITCH = 32 * 2 + 16, SUMS = 16 + 4;
+  __shared__ __align__(16) float sums[kOnceWaves][16 * SUMS];
+  __shared__ __align__(16) uint8_t operands[2][16 * PITCH];
+  __shared__ float downs[16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int all = A.blocks[A.p.n_slices - 1];
+  const int64_t id = A.first + blockIdx.x;
+  const int index = static_cast<int>(id / all), block = static_cast<int>(id - static_cast<int64_t>(index) * all);
+  const RowTile t = find_tile<true>(A.offsets, A.p.adapters, A.tokens, 16, index);
+  if (t.group < 0) return;
+  const bool none = t.group == A.p.adapters;
+  if (none && A.out == A.base) return;
+  int slice = 0;
+  while (block >= A.blocks[slice]) ++slice;
+  const int slice_begin = slice == 0 ? 0 : static_cast<int>(A.p.slice_end[slice - 1]), slice_end = static_cast<int>(A.p.slice_end[slice]);
+  const int column0 = slice_begin + ((block - (slice == 0 ? 0 : A.blocks[slice - 1])) * kOnceWaves + wave) * (16 * NT);
+  const int column = column0 + (lane & 15) * NT;  // the lane's first
+  const int rank = none ? 0 : rank_of(A, t.group);
+  const float scale = none ? 0.0f : A.scales[t.group];
+  const bool vec = A.vec && column + NT <= slice_end;
+  const int place = lane & 15, k0 = (lane >> 4) * 8;
+  const int64_t x_row = static_cast<int64_t>(token_of(A, t.begin + min(place, t.rows - 1))) * A.p.x_stride;
+
+  // B and the base travel while x A^T is made
+  operand_t<T> b[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int64_t row = (static_cast<int64_t>(none ? 0 : t.group) * A.columns + min(column + j, slice_end - 1)) * A.p.rank;
+    b[j] = load_operand<T, true>(A.b, row, k0, (rank + 7) / 8 * 8);
+  }
+  Run<T, NT> base[4];
+  int64_t token[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int m = (lane >> 4) * 4 + i;
+    if (m >= t.rows || column >= slice_end) continue;
+    token[i] = token_of(A, t.begin + m);
+    const int64_t at = token[i] * A.p.base_stride + column;
+    if (vec) base[i].load(A.base, at);
+    else base[i].load_some(A.base, at, slice_end - column);
+  }
+  v4f d = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (!none) {
+    const int there = place < rank ? A.in : 0;  // rows behind the rank are not read
+    const int64_t a_row = (static_cast<int64_t>(t.group) * A.deep + slice * A.p.rank + min(place, A.p.rank - 1)) * A.in;
+    const int steps = (A.in + 31) / 32;
+    constexpr int AT_ONCE = 8;
+    for (int c = wave; c < steps; c += AT_ONCE * kOnceWaves) {  // (steps behind the last are of zeros)
+      operand_t<T> x[AT_ONCE], a[AT_ONCE];
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const int k = (c + u * kOnceWaves) * 32 + k0;
+        x[u] = load_operand<T, true>(A.x, x_row, k, A.in);
+        a[u] = load_operand<T, true>(A.a, a_row, k, there);
+      }
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) d = product<T>(a[u], x[u], d);
+    }
+  }
+  *reinterpret_cast<v4f*>(&sums[wave][place * SUMS + (lane >> 4) * 4]) = d;
+  __syncthreads();
+  {  // a wavefront for each place, its lanes for its values
+    float v = 0.0f;
+    if (lane < 16) {
+#pragma unroll
+      for (int w = 0; w < kOnceWaves; ++w) v += sums[w][wave * SUMS + lane];
+    }
+    float up = 1.0f, down = 1.0f;
+    if constexpr (T == ITEXHIP_HALF) {
+      uint32_t top = __float_as_uint(v) & 0x7fffffffu;
+#pragma unroll
+      for (int m = 1; m < 64; m *= 2) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), m)));
+      power_of(top, &up, &down);
+      if (lane == 0) downs[wave] = down;
+    }
+    if (lane < 32) {  // (zeros from 16 on)
+      const float a = v * up;
+      const uint32_t hi = f32_to_bits16<T>(a);
+      const float h = T == ITEXHIP_BFLOAT16 ? bf16_bits_to_f32(hi) : f16_bits_to_f32(hi);
+      *reinterpret_cast<uint16_t*>(operands[0] + wave * PITCH + lane * 2) = static_cast<uint16_t>(hi);
+      *reinterpret_cast<uint16_t*>(operands[1] + wave * PITCH + lane * 2) = static_cast<uint16_t>(f32_to_bits16<T>(a - h));
+    }
+  }
+  __syncthreads();
+  if (column0 >= slice_end) return;  // the whole wavefront
+  v4f y[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) y[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+    if (rank % 8 != 0) cut<T>(b[j], rank - k0);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    operand_t<T> o;
+    __builtin_memcpy(&o, operands[h] + place * PITCH + k0 * 2, sizeof(o));
+#pragma unroll
+    for (int j = 0; j < NT; ++j) y[j] = product<T>(o, b[j], y[j]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int m = (lane >> 4) * 4 + i;
+    if (m >= t.rows || column >= slice_end) continue;
+    const float factor = T == ITEXHIP_HALF ? downs[m] : 1.0f;
+    Run<T, NT> r = base[i];
+    if (!none) {
+#pragma unroll
+      for (int j = 0; j < NT; j += 2)
+        r.set(j, base[i].at(j) + scale * (y[j][i] * factor), base[i].at(j + 1) + scale * (y[j + 1][i] * factor));
+    }
+    const int64_t at = token[i] * A.p.out_stride + column;
+    if (vec) r.store(A.out, at);
+    else r.store_some(A.out, at, slice_end - column);
+  }
+}
+
 int check(const itexhip_adapters_params* p, const char* name) {
   ITEXHIP_REQUIRE(p != nullptr, "%s: null parameters", name);
   ITEXHIP_REQUIRE(is_chosen_type(p->type), "%s: the type is float, bfloat16 or half", name);
@@ -457,11 +580,34 @@ void launch_expand(const AdapterArgs& A, hipStream_t st) {
 }
 
 template <int T>
+void launch_once(AdapterArgs A, hipStream_t st) {
+  constexpr int COLUMNS = 64 * kOnceWaves;
+  int64_t begin = 0;
+  for (int i = 0, blocks = 0; i < A.p.n_slices; ++i) {
+    blocks += static_cast<int>((A.p.slice_end[i] - begin + COLUMNS - 1) / COLUMNS);
+    A.blocks[i] = blocks;
+    begin = A.p.slice_end[i];
+  }
+  launch_blocks(tiles_bound(A.tokens, A.p.adapters, 16, true) * A.blocks[A.p.n_slices - 1], [&](int64_t first, unsigned count) {
+    A.first = first;
+    once_kernel<T><<<count, 64 * kOnceWaves, 0, st>>>(A);
+  });
+}
+// One launch where a workgroup's part of x A^T is short and reading A again for every 1024 columns costs less than a second launch
+bool once(const AdapterArgs& A) {
+  const int64_t blocks = (A.columns + 1023) / 1024 + A.p.n_slices - 1;
+  return A.p.rank <= 16 && A.in <= 2048 && tiles_bound(A.tokens, A.p.adapters, 16, false) * blocks * A.p.rank * A.in * 2 <= (4 << 20);
+}
+
+template <int T>
 void run_adapters(AdapterArgs A, hipStream_t st) {
   const int64_t size = element_size(T);
   const bool vec = A.in % 8 == 0 && aligned(A.x, 16) && aligned(A.a, 16) && (A.p.x_stride * size) % 16 == 0;
   A.vec = aligned(A.base, 16) && aligned(A.out, 16) && (A.p.base_stride * size) % 16 == 0 && (A.p.out_stride * size) % 16 == 0;
   for (int i = 0; i + 1 < A.p.n_slices; ++i) A.vec = A.vec && (A.p.slice_end[i] * size) % 16 == 0;
+  if constexpr (T != ITEXHIP_FLOAT) {
+    if (vec && once(A)) return launch_once<T>(A, st);
+  }
   const bool wide = long_tiles(A.tokens, A.p.adapters);
   if (vec) wide ? launch_shrink<T, true, 4>(A, st) : launch_shrink<T, true, 1>(A, st);
   else wide ? launch_shrink<T, false, 4>(A, st) : launch_shrink<T, false, 1>(A, st);

@@ -51,7 +51,7 @@ SIZES = [  # tokens, adapters, rank, K, ends, ragged ranks
     (1, 1, 8, 8, [1], False), (1, 4, 16, 64, [64], False), (2, 2, 8, 40, [100], False), (7, 3, 24, 72, [64, 96, 131], True), (16, 1, 32, 256, [130], False),
     (17, 5, 64, 200, [33, 34, 97, 200], True), (64, 64, 16, 512, [256, 320, 384], True), (65, 2, 40, 1040, [70], False), (100, 1000, 8, 64, [48], False),
     (300, 3, 128, 96, [300], True), (33, 2, 256, 64, [128], True), (1000, 5, 16, 160, [513], False), (5, 3, 16, 4104, [64], False), (2100, 4, 64, 320, [200], False),
-    (4500, 2, 16, 96, [4100], False), (4200, 3, 72, 72, [1030, 2070], True), (4200, 1, 256, 64, [2100], False)]
+    (4500, 2, 16, 96, [4100], False), (4500, 2, 24, 96, [4100], True), (40, 3, 16, 2048, [1030, 2100], True), (20, 20, 8, 2056, [1024], False), (4200, 3, 72, 72, [1030, 2070], True), (4200, 1, 256, 64, [2100], False)]
 
 
 @pytest.mark.parametrize("name", list(ref.TYPES))
