@@ -91,10 +91,24 @@ template <int T, int N>
 struct Run {
   static constexpr int WORDS = N * (T == ITEXHIP_FLOAT ? 4 : 2) / 4;
   uint32_t w[WORDS];
+  // PASSING: past the caches' order of use, for tensors that do not stay in them
+  template <bool PASSING = false>
   __device__ __forceinline__ void load(const void* base, int64_t i) {
+    if constexpr (PASSING && WORDS == 4) {
+      const v4i v = __builtin_nontemporal_load(reinterpret_cast<const v4i*>(static_cast<const char*>(base) + i * (T == ITEXHIP_FLOAT ? 4 : 2)));
+      __builtin_memcpy(w, &v, 16);
+      return;
+    }
     __builtin_memcpy(w, __builtin_assume_aligned(static_cast<const char*>(base) + i * (T == ITEXHIP_FLOAT ? 4 : 2), run_alignment<T, N>()), 4 * WORDS);
   }
+  template <bool PASSING = false>
   __device__ __forceinline__ void store(void* base, int64_t i) const {
+    if constexpr (PASSING && WORDS == 4) {
+      v4i v;
+      __builtin_memcpy(&v, w, 16);
+      __builtin_nontemporal_store(v, reinterpret_cast<v4i*>(static_cast<char*>(base) + i * (T == ITEXHIP_FLOAT ? 4 : 2)));
+      return;
+    }
     __builtin_memcpy(__builtin_assume_aligned(static_cast<char*>(base) + i * (T == ITEXHIP_FLOAT ? 4 : 2), run_alignment<T, N>()), w, 4 * WORDS);
   }
   __device__ __forceinline__ float at(int j) const {
@@ -231,8 +245,9 @@ __device__ __forceinline__ void power_of(uint32_t bits, float* up, float* down) 
 // and goes through up to ROWS places of one adapter, 16 at a time.  A lane's column of the j-th tile is NT (lane % 16) + j of them, so that it ends
 // with NT neighbouring columns of four rows and 16 lanes with a run of 16 NT.  The workgroup adds up the shares of x A^T and holds them in LDS as operands: the
 // sum of two numbers of the type (one of bfloat16 alone would be off by 2^-9 of it); in half precision times a power of two that keeps a
-// row's largest in range.  Bound by memory: 8192 tokens of 14336 columns, rank 64, take 121 us for 470 MB, 3.9 TB/s, the next 16 rows' base on its way
-// while the last ones are multiplied (without that 241); 64 rows a workgroup 144 us with x A^T, 128 147, 256 162; three wavefronts a SIMD 147, two 162.
+// row's largest in range.  Bound by memory: 8192 tokens of 14336 columns, rank 64, take 113 us for 470 MB, 4.2 TB/s, the next 16 rows' base on its way
+// while the last ones are multiplied (without that 241).  With x A^T, 64 rows a workgroup 144 us, 128 147, 256 162; three wavefronts a SIMD 147, two 162;
+// stores past the caches' order of use 144 -> 136.
 template <int T, int KS, int NT, int ROWS>
 __global__ __launch_bounds__(256, KS <= 2 ? 3 : 2) void expand_kernel(const AdapterArgs A) {
   constexpr int SIZE = T == ITEXHIP_FLOAT ? 4 : 2, PARTS = T == ITEXHIP_FLOAT ? 1 : 2;
@@ -303,7 +318,7 @@ __global__ __launch_bounds__(256, KS <= 2 ? 3 : 2) void expand_kernel(const Adap
       const int m = n * 16 + (lane >> 4) * 4 + i;
       if (m >= t.rows || column >= slice_end) continue;
       const int64_t at = static_cast<int64_t>(tokens[m]) * A.p.base_stride + column;
-      if (vec) q.base[i].load(A.base, at);
+      if (vec) q.base[i].template load<(ROWS > 16)>(A.base, at);
       else q.base[i].load_some(A.base, at, slice_end - column);
     }
   };
@@ -367,7 +382,7 @@ __global__ __launch_bounds__(256, KS <= 2 ? 3 : 2) void expand_kernel(const Adap
           y.set(j, now.base[i].at(j) + scale * (d[j][i] * factor), now.base[i].at(j + 1) + scale * (d[j + 1][i] * factor));
       }
       const int64_t at = static_cast<int64_t>(tokens[m]) * A.p.out_stride + column;
-      if (vec) y.store(A.out, at);
+      if (vec) y.template store<(ROWS > 16)>(A.out, at);
       else y.store_some(A.out, at, slice_end - column);
     }
     now = next;
