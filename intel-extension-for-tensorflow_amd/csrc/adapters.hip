@@ -460,7 +460,7 @@ __global__ __launch_bounds__(64 * kOnceWaves) void once_kernel(const AdapterArgs
   __syncthreads();
   {  // a wavefront for each place, its lanes for its values
     float v = 0.0f;
-    if (lane < 16) {
+    if (lane < rank) {  // (behind the rank an x that is not finite has left zeros times it)
 #pragma unroll
       for (int w = 0; w < kOnceWaves; ++w) v += sums[w][wave * SUMS + lane];
     }

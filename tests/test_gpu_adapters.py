@@ -147,6 +147,20 @@ def test_what_is_not_read_and_what_is_not_finite(hip, dev):
         assert bool((~got[0].isfinite()).all()) and torch.equal(got[1:], want[1:].float().to(dtype)), name
 
 
+@pytest.mark.parametrize("rank,K", [(16, 64), (8, 40), (16, 4096), (32, 64)])
+def test_an_adapter_of_no_rank_adds_nothing(hip, dev, rank, K):
+    """whatever its tokens hold: x A^T has no columns then"""
+    t, ends = 5, [40, 90]
+    g = torch.Generator().manual_seed(6)
+    for name, dtype in ref.TYPES.items():
+        x, a, b = whole((t, K), 2, g).to(dtype), whole((2, 2 * rank, K), 2, g).to(dtype), whole((2, 90, rank), 2, g).to(dtype)
+        x[0, 3], x[2, 1] = math.nan, math.inf
+        base, ranks = whole((t, 90), 9, g).to(dtype), torch.tensor([0, 3], dtype=torch.int32)
+        offsets, rows = ref.order(torch.tensor([0, 1, 0, 1, 0]), 2)
+        got = run(hip, dev, name, x, offsets, rows, a, b, ranks, torch.ones(2), base, ends, rank)
+        assert torch.equal(got[[0, 2, 4]], base[[0, 2, 4]]), name
+
+
 def test_beside_a_quantized_linear_and_captured(hip, dev):
     """A quantized linear's output gets its adapters in place, eagerly on another stream and in a graph that is replayed with other tokens."""
     t, n, rank, K, N = 20, 4, 16, 256, 192
