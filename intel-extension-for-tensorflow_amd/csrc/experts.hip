@@ -24,7 +24,7 @@ __device__ __forceinline__ int code_of(float x, float s, float inv) {
   return static_cast<int>(n);
 }
 // Eight codes in two words.  The fma with 3 2^22 brings the nearest integer of x / s (1 + e), |e| <= 2^-24, into the low byte; it is that of the quotient
-// too where what is left over is 2^-16 or more away from a half, since the two are 127 2^-24 apart at most.  One element in 16000 is not and has
+// too where what is left over is 2^-15 or more away from a half, since the two are 127 2^-24 apart at most.  One element in 16000 is not and has
 // its wavefront go through the exact remainders.
 __device__ __forceinline__ uint2 codes_of(const float (&x)[8], float s, float inv) {
   constexpr float kMagic = 12582912.0f;
@@ -292,8 +292,8 @@ __global__ __launch_bounds__(64 * WAVES) void experts_stream_kernel(const Produc
 
 // The way back of very few choices in one launch: a workgroup has a strip of 32 channels of every expert that is chosen.  Its
 // wavefronts divide the experts and, within one, the chunks of K; every place of the order is a row of every product, and where the sums meet each place
-// takes its own expert's.  Then the strip's part of each token is all there.  One token's two experts of 14336 x 4096, 118 MB, take 30 us, of which the codes,
-// made by every workgroup for itself while its first chunks travel, are about 5; three launches took 48.
+// takes its own expert's.  Then the strip's part of each token is all there.  One token's two experts of 14336 x 4096, 118 MB, take 28 us, of which the codes,
+// made by every workgroup for itself while its first chunks travel, are about 3; three launches took 48.
 struct FewArgs {
   const int32_t* experts;
   const float* weights;
