@@ -843,14 +843,14 @@ int launch_tiles(ProductArgs A, hipStream_t st) {
 }
 template <int OUT, bool GATED>
 int launch_products(const ProductArgs& A, hipStream_t st) {
-  // Tiles cost a workgroup about 10 us whatever they hold, and have to be enough of them; strips read an expert's weights again for every 32
-  // rows.  Measured, tiles : strips in us, 8 experts of 4096 x 4096, gated, at 16, 32, 64 rows each 67 : 57, 68 : 75, 75 : 130, not gated 49 : 44,
+  // Tiles cost a workgroup about 10 us whatever they hold, and have to be enough of them (rows of tiles a workgroup); strips read
+  // an expert's weights again for every 32 rows.  Measured, tiles : strips in us, 8 experts of 4096 x 4096, gated, at 16, 32, 64 rows each 67 : 57, 68 : 75, 75 : 130, not gated 49 : 44,
   // 54 : 66, 66 : 99; 32 of 1408 x 2048, not gated, at 8, 16 30 : 29, 32 : 38; 4 of 14336 x 4096 (64 tiles) at 32, 64 134 : 101, 162 : 171;
   // 8 of 1024 x 1024 (64 tiles) at 64, 128, 256 18 : 13, 24 : 21, 25 : 30.
   constexpr int WIDTH = GATED ? 128 : 256;
   const int64_t each = A.slots / A.experts, tiles = static_cast<int64_t>(A.experts) * ((A.N + WIDTH - 1) / WIDTH);
   const bool near = OUT == 0 || A.slots / A.top_k * static_cast<int64_t>(A.pitch) < (1LL << 32);  // up: codes in reach of 32 bits
-  if (each >= (GATED ? 24 : 12) && each * tiles >= (A.pitch >= 2048 ? 3072 : 8192) && A.chunks >= 2 * kTileSteps && near) {
+  if (each >= (GATED ? 24 : 12) && each * tiles >= kWorkgroups * (A.pitch >= 2048 ? 12 : 32) && A.chunks >= 2 * kTileSteps && near) {
     constexpr bool SWISH = GATED;
     if (tiles * ((each + 255) / 256) < kWorkgroups * 3 / 4) {  // half as many channels a tile where they are too few for the device
       if (SWISH && A.activation == ITEXHIP_ACT_SWISH) return launch_tiles<OUT, GATED, SWISH, 256, 128>(A, st);
