@@ -52,6 +52,11 @@ def _has_untracked_asm(src):
     return os.path.basename(src).startswith("qgemm_tile_")
 
 
+def keeps_assembly(src):
+    """True for the translation units whose device assembly is checked: those, and the one whose direct loads to LDS are inline assembly."""
+    return _has_untracked_asm(src) or os.path.basename(src) == "experts.hip"
+
+
 def device_assembly_of(src):
     """Where the compile step leaves the device assembly of a translation unit with inline-assembly memory instructions."""
     stem = os.path.splitext(os.path.basename(src))[0]
@@ -60,7 +65,7 @@ def device_assembly_of(src):
 
 def _compile_hip(src):
     obj = os.path.join(OBJ, os.path.basename(src) + ".o")
-    keep = ["-save-temps=obj"] if _has_untracked_asm(src) else []
+    keep = ["-save-temps=obj"] if keeps_assembly(src) else []
     out = _run([HIPCC] + HIP_FLAGS + keep + ["-c", src, "-o", obj])
     if keep:   # only the device assembly is wanted from the intermediate files
         stem = os.path.splitext(os.path.basename(src))[0]
@@ -75,7 +80,7 @@ def _compile_hip(src):
 
 
 def check_inline_asm_hazards(asm_files, verbose=True):
-    """The compiler neither counts the inline-assembly loads of the tile kernels in its wait counts nor gives their
+    """The compiler neither counts the inline-assembly loads of the tile kernels in its wait counts nor gives them or their
     assembly stores hazard wait states; csrc/check_asm_hazards.py proves on the compiled device assembly that the
     hand-written waits cover every path.  A finding fails the build: the library is not linked."""
     import contextlib
@@ -114,7 +119,7 @@ def build(jobs=8, verbose=True):
     hip_srcs = sorted(glob.glob(os.path.join(CSRC, "*.hip")))
     with concurrent.futures.ThreadPoolExecutor(max_workers=jobs) as ex:
         objs = list(ex.map(_compile_hip, hip_srcs))
-    check_inline_asm_hazards([device_assembly_of(f) for f in hip_srcs if _has_untracked_asm(f)], verbose)
+    check_inline_asm_hazards([device_assembly_of(f) for f in hip_srcs if keeps_assembly(f)], verbose)
     libitexhip = os.path.join(LIB, "libitexhip.so")
     _run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", libitexhip] + objs)
     if verbose:

@@ -1,7 +1,7 @@
-"""Checks the device assembly of the tile kernels for the two hazards their inline assembly can create.
+"""Checks the device assembly of the tile kernels for the hazards their inline assembly can create.
 
 The compiler inserts wait counts and hazard wait states only for memory instructions it emitted itself; the ones
-written as inline assembly in qgemm_common.hpp / qgemm_tile.hpp are opaque text to it:
+written as inline assembly in qgemm_common.hpp / qgemm_tile.hpp / experts.hip are opaque text to it:
 
 1. The early channel-parameter loads (load_raw_channel_early) return their data some hundred cycles after issue.  Until
    an s_waitcnt vmcnt(n) with n <= (vector memory instructions issued since the load) no instruction may write the
@@ -13,8 +13,10 @@ written as inline assembly in qgemm_common.hpp / qgemm_tile.hpp are opaque text 
    overwrites it.
 2. A vector store of more than 8 bytes reads its data registers for two more cycles after issue.  Each write-through
    store in the epilogue must be followed by at least two wait states inside the same assembly statement.
+3. A load to LDS takes its destination from m0.  Between a scalar instruction that writes m0 and the load there must be
+   one wait state, along every path (for a load that it emits itself the compiler inserts an s_nop 0).
 
-Usage:  python check_asm_hazards.py            compiles every qgemm_tile_*.hip to assembly (minutes) and checks it
+Usage:  python check_asm_hazards.py            compiles the units that the build checks to assembly (minutes) and checks it
         python check_asm_hazards.py a.s b.s    checks assembly files made with the build's flags plus -S --offload-device-only
 Exit status 0 when nothing is flagged.
 """
@@ -28,6 +30,7 @@ import tempfile
 
 VMEM = re.compile(r"^(global_|buffer_|flat_|scratch_)(load|store|atomic)")
 EARLY = re.compile(r"global_load_(dword|ushort)\s+v(\d+),")
+LDS_LOAD = re.compile(r"(global|buffer)_load_lds_|buffer_load_\w+ .*\blds\b")
 BRANCH = re.compile(r"(s_branch|s_cbranch_\w+)\s+(\S+)")
 
 
@@ -49,6 +52,58 @@ def dead_high_half(ins, pc, reg):
     return True
 
 
+def writes(code):
+    """The scalar registers an instruction writes: numbers, and "m0"."""
+    ops = code.split(None, 1)
+    dst = ops[1].split(",")[0].strip() if len(ops) > 1 else ""
+    m = re.match(r"s\[(\d+):(\d+)\]$", dst)
+    if m:
+        return set(range(int(m.group(1)), int(m.group(2)) + 1))
+    m = re.match(r"s(\d+)$", dst)
+    return {int(m.group(1))} if m else {"m0"} if dst == "m0" else set()
+
+
+def states_before(ins, entries, at, reg, enough):
+    """The fewest wait states, along any path, between the last instruction that writes `reg` and ins[at], with that
+    instruction's index; None where there are `enough` of them.  entries: the branches to each index."""
+    best, seen, work = None, set(), [(at, 0)]
+    while work:
+        pc, states = work.pop()
+        if (pc, states) in seen:
+            continue
+        seen.add((pc, states))
+        before = entries.get(pc, [])
+        if pc > 0 and not re.match(r"s_branch|s_endpgm", ins[pc - 1][1]):
+            before = before + [pc - 1]
+        for q in before:
+            code = ins[q][1]
+            if reg in writes(code):
+                if best is None or states < best[0]:
+                    best = (states, q)
+                continue
+            m = re.match(r"s_nop\s+(\d+)", code)
+            past = states + (int(m.group(1)) + 1 if m else 1)
+            if past < enough:
+                work.append((q, past))
+    return best
+
+
+def check_lds_loads(ins, labels):
+    """Rule 3."""
+    findings, entries = set(), {}
+    for i, (_, code, _) in enumerate(ins):
+        mb = BRANCH.match(code)
+        if mb and mb.group(2) in labels:
+            entries.setdefault(labels[mb.group(2)], []).append(i)
+    for at, (ln, code, in_asm) in enumerate(ins):
+        if not (in_asm and LDS_LOAD.match(code)):
+            continue
+        near = states_before(ins, entries, at, "m0", 1)
+        if near:
+            findings.add((ln, "a load to LDS without a wait state after the write of m0: " + code))
+    return findings
+
+
 def check_function(ins, labels):
     """ins: [(line number, instruction text, inside an inline-assembly block)].  Returns (load sites, findings)."""
     sites = [i for i, (_, c, a) in enumerate(ins) if a and EARLY.match(c)]
@@ -60,6 +115,7 @@ def check_function(ins, labels):
             m = re.match(r"s_nop\s+(\d+)", nxt[1])
             if not (nxt[2] and m and int(m.group(1)) >= 1):
                 findings.add((ln, "assembly store without two wait states after it: " + code))
+    findings |= check_lds_loads(ins, labels)
     if not sites:
         return 0, findings
     last = sites[-1]
@@ -184,7 +240,7 @@ def compile_to_assembly(out_dir):
     here = os.path.dirname(os.path.abspath(__file__))
     sys.path.insert(0, os.path.dirname(here))
     import build as b
-    srcs = sorted(glob.glob(os.path.join(here, "qgemm_tile_*.hip")))
+    srcs = [f for f in sorted(glob.glob(os.path.join(here, "*.hip"))) if b.keeps_assembly(f)]
 
     def one(src):
         out = os.path.join(out_dir, os.path.basename(src) + ".s")

@@ -427,7 +427,7 @@ __device__ __forceinline__ const int8_t* uniform(const int8_t* p) {
 // lds_dma16 to OFFSET behind lds_addr, the sum formed in m0
 template <int OFFSET>
 __device__ __forceinline__ void lds_dma16_at(const void* base, uint32_t lane_offset, uint32_t lds_addr) {
-  asm volatile("s_add_u32 m0, %2, %3\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(lane_offset), "s"(base), "s"(lds_addr), "i"(OFFSET) : "memory", "m0", "scc");
+  asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(lane_offset), "s"(base), "s"(lds_addr), "i"(OFFSET) : "memory", "m0", "scc");
 }
 
 // SWISH: the activation, known when compiled; with the others beside it this one's code would be fetched around them

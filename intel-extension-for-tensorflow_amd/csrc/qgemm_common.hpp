@@ -406,13 +406,14 @@ __device__ __forceinline__ void static_for(F&& f) {
 // Direct global -> LDS loads (global_load_lds_dwordx4): each lane's 16 bytes land at LDS base + 16 * lane, no VGPRs
 // and no ds_write on the way.  They count in vmcnt like any other vector memory load and return in order with them.
 __device__ __forceinline__ void lds_dma16(const void* gptr, uint32_t lds_addr) {
-  // m0 = LDS byte address of lane 0's destination; the instruction adds 16 * lane
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(gptr), "s"(lds_addr) : "memory", "m0");
+  // m0 = LDS byte address of lane 0's destination; the instruction adds 16 * lane.  A load to LDS needs a wait state after a
+  // scalar write of m0, which the compiler does not insert into assembly.
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(gptr), "s"(lds_addr) : "memory", "m0");
 }
 // same with a wavefront-uniform 64-bit base (SGPR pair) and a 32-bit per-lane byte offset: no vector
 // address arithmetic per load
 __device__ __forceinline__ void lds_dma16(const void* sbase, uint32_t lane_off, uint32_t lds_addr) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(lane_off), "s"(sbase), "s"(lds_addr) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(lane_off), "s"(sbase), "s"(lds_addr) : "memory", "m0");
 }
 
 template <int N>
