@@ -15,6 +15,8 @@ written as inline assembly in qgemm_common.hpp / qgemm_tile.hpp / experts.hip ar
    store in the epilogue must be followed by at least two wait states inside the same assembly statement.
 3. A load to LDS takes its destination from m0.  Between a scalar instruction that writes m0 and the load there must be
    one wait state, along every path (for a load that it emits itself the compiler inserts an s_nop 0).
+4. A memory instruction that reads a scalar register, such as the base of its address, needs five wait states after a
+   vector instruction (v_readfirstlane, a comparison) has written it (s_nop 4 in the compiler's own code).
 
 Usage:  python check_asm_hazards.py            compiles the units that the build checks to assembly (minutes) and checks it
         python check_asm_hazards.py a.s b.s    checks assembly files made with the build's flags plus -S --offload-device-only
@@ -54,18 +56,27 @@ def dead_high_half(ins, pc, reg):
 
 def writes(code):
     """The scalar registers an instruction writes: numbers, and "m0"."""
-    ops = code.split(None, 1)
-    dst = ops[1].split(",")[0].strip() if len(ops) > 1 else ""
-    m = re.match(r"s\[(\d+):(\d+)\]$", dst)
+    name, _, rest = code.partition(" ")
+    ops = rest.split(",")
+    regs = sregs(ops[0])
+    if len(ops) > 1 and re.match(r"v_\w*_co_|v_mad_[ui]64_[ui]32|v_div_scale", name):   # a carry or condition beside the result
+        regs |= sregs(ops[1])
+    return regs
+
+
+def sregs(operand):
+    operand = operand.strip().split(" ")[0]
+    m = re.match(r"s\[(\d+):(\d+)\]$", operand)
     if m:
         return set(range(int(m.group(1)), int(m.group(2)) + 1))
-    m = re.match(r"s(\d+)$", dst)
-    return {int(m.group(1))} if m else {"m0"} if dst == "m0" else set()
+    m = re.match(r"s(\d+)$", operand)
+    return {int(m.group(1))} if m else {operand} if operand in ("m0", "vcc") else set()
 
 
-def states_before(ins, entries, at, reg, enough):
-    """The fewest wait states, along any path, between the last instruction that writes `reg` and ins[at], with that
-    instruction's index; None where there are `enough` of them.  entries: the branches to each index."""
+def states_before(ins, entries, at, reg, enough, writer=""):
+    """The fewest wait states, along any path, between ins[at] and the last instruction before it that writes `reg`, if that is
+    one whose name begins with `writer`, with that instruction's index; None where there are `enough` of them.  entries: the
+    branches to each index."""
     best, seen, work = None, set(), [(at, 0)]
     while work:
         pc, states = work.pop()
@@ -78,7 +89,7 @@ def states_before(ins, entries, at, reg, enough):
         for q in before:
             code = ins[q][1]
             if reg in writes(code):
-                if best is None or states < best[0]:
+                if code.startswith(writer) and (best is None or states < best[0]):
                     best = (states, q)
                 continue
             m = re.match(r"s_nop\s+(\d+)", code)
@@ -88,19 +99,22 @@ def states_before(ins, entries, at, reg, enough):
     return best
 
 
-def check_lds_loads(ins, labels):
-    """Rule 3."""
+def check_scalar_operands(ins, labels):
+    """Rules 3 and 4."""
     findings, entries = set(), {}
     for i, (_, code, _) in enumerate(ins):
         mb = BRANCH.match(code)
         if mb and mb.group(2) in labels:
             entries.setdefault(labels[mb.group(2)], []).append(i)
     for at, (ln, code, in_asm) in enumerate(ins):
-        if not (in_asm and LDS_LOAD.match(code)):
+        if not (in_asm and VMEM.match(code)):
             continue
-        near = states_before(ins, entries, at, "m0", 1)
-        if near:
+        if LDS_LOAD.match(code) and states_before(ins, entries, at, "m0", 1):
             findings.add((ln, "a load to LDS without a wait state after the write of m0: " + code))
+        for reg in sorted(set().union(*(sregs(o) for o in code.partition(" ")[2].split(","))), key=str):
+            near = states_before(ins, entries, at, reg, 5, "v_")
+            if near:
+                findings.add((ln, "%d wait state(s) between %s (line %d) and %s" % (near[0], ins[near[1]][1], ins[near[1]][0], code)))
     return findings
 
 
@@ -115,7 +129,7 @@ def check_function(ins, labels):
             m = re.match(r"s_nop\s+(\d+)", nxt[1])
             if not (nxt[2] and m and int(m.group(1)) >= 1):
                 findings.add((ln, "assembly store without two wait states after it: " + code))
-    findings |= check_lds_loads(ins, labels)
+    findings |= check_scalar_operands(ins, labels)
     if not sites:
         return 0, findings
     last = sites[-1]

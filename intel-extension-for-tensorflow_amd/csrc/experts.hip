@@ -417,11 +417,14 @@ __device__ __forceinline__ void activate16(int activation, float (&y)[16]) {
 #undef ITEXHIP_EACH
 }
 
-// A pointer that all lanes have, in scalar registers
+// A pointer that all lanes have, in scalar registers, for loads written as assembly: a memory instruction reads them five wait states after the
+// vector instructions that wrote them at the earliest, and the compiler counts those for its own loads only
 __device__ __forceinline__ const int8_t* uniform(const int8_t* p) {
   const uint64_t v = reinterpret_cast<uint64_t>(p);
   const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int>(v)), hi = __builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32));
-  return reinterpret_cast<const int8_t*>(static_cast<uint64_t>(hi) << 32 | lo);
+  uint64_t q = static_cast<uint64_t>(hi) << 32 | lo;
+  asm volatile("s_nop 4" : "+s"(q));
+  return reinterpret_cast<const int8_t*>(q);
 }
 
 // lds_dma16 to OFFSET behind lds_addr, the sum formed in m0

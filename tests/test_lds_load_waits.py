@@ -55,8 +55,20 @@ def test_m0_written_where_a_branch_comes_from(chk, tmp_path, capsys):
     assert n == 0, out
 
 
+@pytest.mark.parametrize("before,bad", [
+    (["v_readfirstlane_b32 s4, v3", "s_add_i32 s9, s9, 1", "s_mov_b32 m0, s3", "s_nop 0"], 1), (["v_readfirstlane_b32 s4, v3", "s_nop 3"], 1),
+    (["v_readfirstlane_b32 s4, v3", "s_nop 4"], 0), (["v_readfirstlane_b32 s4, v3", "s_nop 1", "v_mov_b32_e32 v9, 0", "s_nop 1"], 0),
+    (["v_readfirstlane_b32 s6, v3", "s_mov_b32 s4, s6"], 0), (["v_cmp_lt_u32_e64 s[4:5], v3, v4"], 1), (["v_add_co_u32_e64 v7, s[4:5], v3, v4"], 1),
+    (["v_readfirstlane_b32 s5, v3", ".LBB0_1:", "s_nop 3"], 1), (["s_cbranch_scc1 .LBB0_3", "s_nop 4", ".LBB0_3:"], 0),
+    (["v_readlane_b32 s5, v3, 4", "s_cbranch_scc1 .LBB0_3", "s_nop 4", ".LBB0_3:"], 1)])
+def test_five_wait_states_after_a_vector_instruction_wrote_the_base(chk, tmp_path, capsys, before, bad):
+    n, out = flagged(chk, tmp_path, capsys, before + [";;#ASMSTART", LOAD, ";;#ASMEND", "s_endpgm"])
+    assert n == bad, out
+    assert ("wait state(s) between v_" in out) == bool(bad)
+
+
 def test_the_compiler_s_own_loads_are_not_looked_at(chk, tmp_path, capsys):
-    assert flagged(chk, tmp_path, capsys, ["s_mov_b32 m0, s3", LOAD, "s_endpgm"])[0] == 0
+    assert flagged(chk, tmp_path, capsys, ["s_mov_b32 m0, s3", LOAD, "v_readfirstlane_b32 s4, v3", LOAD, "s_endpgm"])[0] == 0
 
 
 def test_every_unit_with_such_a_load_is_checked(build):
