@@ -132,7 +132,7 @@ struct ProductArgs {
 
 __device__ __forceinline__ float activate(int activation, float x) {
   switch (activation) {
-    case ITEXHIP_ACT_RELU: return fmaxf(x, 0.0f);
+    case ITEXHIP_ACT_RELU: return x <= 0.0f ? 0.0f : x;  // (NaN stays, which a maximum would drop)
     case ITEXHIP_ACT_GELU_APPROX: return apply_eltwise(itexhip_eltwise{ITEXHIP_ELT_GELU_TANH, 0.0f, 0.0f}, x);
     case ITEXHIP_ACT_GELU_EXACT: return apply_eltwise(itexhip_eltwise{ITEXHIP_ELT_GELU_ERF, 0.0f, 0.0f}, x);
     case ITEXHIP_ACT_SWISH: return apply_eltwise(itexhip_eltwise{ITEXHIP_ELT_SWISH, 1.0f, 0.0f}, x);
