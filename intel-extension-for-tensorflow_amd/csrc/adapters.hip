@@ -11,8 +11,6 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
-constexpr int kMaxSplits = 6;
-
 struct AdapterArgs {
   itexhip_adapters_params p;
   const void *x, *a, *b, *base;
@@ -531,22 +529,6 @@ int check(const itexhip_adapters_params* p, const char* name) {
   return ITEXHIP_OK;
 }
 
-// Many places an adapter: tiles of 64 of them, which read A a quarter as often; 16 where most would be empty or tiles few
-bool long_tiles(int64_t tokens, int adapters) { return tokens > 32 * static_cast<int64_t>(adapters) && tiles_bound(tokens, adapters, 64, false) >= 64; }
-// Shares of K: enough workgroups for the device where tiles are few, of at least 256 k each
-constexpr int kEnoughTiles = 512;
-int splits_of(int64_t tokens, int adapters, int64_t parts, int64_t in) {
-  const int64_t tiles = tiles_bound(tokens, adapters, long_tiles(tokens, adapters) ? 64 : 16, false) * parts;
-  int64_t n = tiles == 0 ? 1 : (kEnoughTiles + tiles - 1) / tiles;
-  n = n < (in + 255) / 256 ? n : (in + 255) / 256;
-  return static_cast<int>(n < kMaxSplits ? n : kMaxSplits);
-}
-// Rows of the middle that any call of up to this many tokens needs: a share's tiles hold at most 64 tokens each
-int64_t middle_rows(int64_t tokens) {
-  const int64_t most = kMaxSplits * tokens, few = 64 * 2 * kEnoughTiles;
-  return most < few ? most : few > tokens ? few : tokens;
-}
-
 template <int T, bool VEC, int RT, int CT>
 void launch_shrink(AdapterArgs A, hipStream_t st) {
   const int64_t parts = static_cast<int64_t>((A.p.rank + 16 * CT - 1) / (16 * CT)) * A.p.n_slices;
@@ -563,7 +545,6 @@ void launch_shrink(const AdapterArgs& A, hipStream_t st) {
   else if (A.p.rank <= 32) launch_shrink<T, VEC, RT, 2>(A, st);
   else launch_shrink<T, VEC, RT, 4>(A, st);
 }
-int shrink_parts(int rank) { return rank <= 64 ? 1 : (rank + 63) / 64; }
 
 template <int T, int KS, int NT, int ROWS>
 void launch_expand(AdapterArgs A, hipStream_t st) {
@@ -580,9 +561,7 @@ void launch_expand(AdapterArgs A, hipStream_t st) {
 }
 template <int T, int KS, int NT>
 void launch_expand(const AdapterArgs& A, hipStream_t st) {
-  // 64 places a workgroup where that leaves enough of them
-  const int64_t blocks = (A.columns + 64 * NT - 1) / (64 * NT);
-  if (long_tiles(A.tokens, A.p.adapters) && tiles_bound(A.tokens, A.p.adapters, 64, true) * blocks >= kEnoughTiles) launch_expand<T, KS, NT, 64>(A, st);
+  if (long_expand(A.tokens, A.p.adapters, A.columns, 64 * NT)) launch_expand<T, KS, NT, 64>(A, st);
   else launch_expand<T, KS, NT, 16>(A, st);
 }
 template <int T>
@@ -608,12 +587,6 @@ void launch_once(AdapterArgs A, hipStream_t st) {
     once_kernel<T><<<count, 64 * kOnceWaves, 0, st>>>(A);
   });
 }
-// One launch where a workgroup's part of x A^T is short and reading A again for every 1024 columns costs less than a second launch
-bool once(const AdapterArgs& A) {
-  const int64_t blocks = (A.columns + 1023) / 1024 + A.p.n_slices - 1;
-  return A.p.rank <= 16 && A.in <= 2048 && tiles_bound(A.tokens, A.p.adapters, 16, false) * blocks * A.p.rank * A.in * 2 <= (4 << 20);
-}
-
 template <int T>
 void run_adapters(AdapterArgs A, hipStream_t st) {
   const int64_t size = element_size(T);
@@ -621,7 +594,7 @@ void run_adapters(AdapterArgs A, hipStream_t st) {
   A.vec = aligned(A.base, 16) && aligned(A.out, 16) && (A.p.base_stride * size) % 16 == 0 && (A.p.out_stride * size) % 16 == 0;
   for (int i = 0; i + 1 < A.p.n_slices; ++i) A.vec = A.vec && (A.p.slice_end[i] * size) % 16 == 0;
   if constexpr (T != ITEXHIP_FLOAT) {
-    if (vec && once(A)) return launch_once<T>(A, st);
+    if (vec && one_launch(A.tokens, A.p.adapters, A.p.rank, A.p.n_slices, A.in, A.columns)) return launch_once<T>(A, st);
   }
   const bool wide = long_tiles(A.tokens, A.p.adapters);
   if (vec) wide ? launch_shrink<T, true, 4>(A, st) : launch_shrink<T, true, 1>(A, st);

@@ -3,6 +3,7 @@
 #ifndef ITEXHIP_CHOSEN_HPP_
 #define ITEXHIP_CHOSEN_HPP_
 
+#include "chosen_rules.hpp"
 #include "common.hpp"
 
 namespace itexhip {
@@ -45,14 +46,7 @@ inline void launch_blocks(int64_t blocks, F&& f) {
   in_pieces(0, blocks, [&](int64_t begin, int64_t end) { f(begin, static_cast<unsigned>(end - begin)); }, 1LL << 23);
 }
 
-// Tiles of up to `per_tile` places of the order, group by group; with REST the rows of no group are a group of their own behind the
-// others.  How many there are is known on the device only: a launch has room for tiles_bound of them, and those beyond the
-// last find group = -1.
-inline int64_t tiles_bound(int64_t n, int groups, int per_tile, bool rest) {
-  const int64_t parts = groups + (rest ? 1 : 0);
-  const int64_t open = n < parts ? n : parts;  // groups that can have a tile that is not full
-  return open + (n - open) / per_tile;
-}
+// The tiles that tiles_bound counts
 struct RowTile {
   int group;       // groups: the rows of no group
   int begin, rows; // places

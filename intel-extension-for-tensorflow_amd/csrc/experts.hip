@@ -145,7 +145,6 @@ __device__ __forceinline__ int slot_of(const ProductArgs& A, int place) { return
 
 // Codes and scales of a few rows in LDS, by all wavefronts of a workgroup: each has a share of one row.  `at` gives a row's first element.
 // All of them wait twice.
-constexpr int kFewRows = 16;
 template <int T, int WAVES, class F>
 __device__ __forceinline__ void quantize_few(const void* x, bool vec, int rows, int K, int pitch, int8_t* codes, float* scales, uint32_t (&most)[WAVES], F&& at) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -301,7 +300,7 @@ struct FewArgs {
   int64_t addend_stride, out_stride;
   int tokens;
 };
-constexpr int kFewPlaces = 16, kFewWaves = 16;
+constexpr int kFewWaves = 16;
 template <int T>
 __global__ __launch_bounds__(64 * kFewWaves) void experts_few_down_kernel(const ProductArgs A, const FewArgs F) {
   constexpr int PITCH = 36;
@@ -400,7 +399,6 @@ __global__ __launch_bounds__(64 * kFewWaves) void experts_few_down_kernel(const 
 // its products that registers allow.  Bases in scalar registers and one offset for all weights' loads of a step brought 1049 to 1015 us.
 // ------------------------------------------------------------------------------------------------
 constexpr int kTileGroup = 8;  // tiles of rows that share a column
-constexpr int kTileSteps = 4;  // K steps that a tile has to have
 // MFMA tiles of results that go through a wavefront's piece of LDS at a time: 128 bytes of a row
 constexpr int tile_pair(int element, int out_tn) { return element == 2 && out_tn >= 2 ? 2 : 1; }
 constexpr int tile_lds(int element, int out_tn, int bm, int bn) {
@@ -776,19 +774,7 @@ Layout layout_of(const itexhip_experts_params& p, bool up) {
   return l;
 }
 
-// Codes that a workgroup keeps in LDS
-constexpr int kFewBytes = 64 * 1024;
-// up: a workgroup makes the codes of its tokens itself where they are about 32 elements a thread; beyond, a launch that makes them once is shorter
-bool few_up(const ProductArgs& A) {
-  const int64_t tokens = A.slots / A.top_k, each = A.slots > A.experts ? (A.slots + A.experts - 1) / A.experts : 1;
-  return tokens <= kFewRows && each * A.pitch <= 8192 && tokens * A.pitch <= kFewBytes / 2;
-}
-// down, one launch : three in us: 2 rows of 768 to 14336 7 : 12 to 32 : 34, 4 of 1536 and 4096 11 : 16 and 18 : 15, 8 of 768 and 1536 10 : 13 and 13 : 17,
-// where there are few channels 12 : 12, 16 of 768 13 : 13
-bool few_down(const ProductArgs& A) {
-  const int64_t bytes = static_cast<int64_t>(A.slots) * A.pitch;
-  return A.slots <= kFewPlaces && (A.slots <= 2 || bytes <= 8192) && bytes <= kFewBytes;
-}
+ProductSizes sizes_of(const ProductArgs& A, bool up, bool gated) { return ProductSizes{A.slots, A.top_k, A.experts, A.pitch, A.N, up, gated}; }
 
 template <int T>
 void launch_quantize(const void* x, int64_t stride, int64_t rows, int64_t K, const ProductArgs& A, hipStream_t st) {
@@ -821,13 +807,6 @@ int launch_stream(ProductArgs A, hipStream_t st) {
   });
   return ITEXHIP_OK;
 }
-// Few strips: eight wavefronts each instead of four, so that the device has enough on their way (896 strips of 4096: 46 -> 39 us), unless that
-// leaves a wavefront a handful of chunks (736 of 1024: 13 -> 15)
-bool few_strips(const ProductArgs& A) {
-  return tiles_bound(A.slots, A.experts, 32, false) * A.strips < (A.chunks >= 64 ? 1024 : 512);
-}
-constexpr int kWorkgroups = 256;  // one for each CU; they take the tiles in turns
-
 template <int OUT, bool GATED, bool SWISH, int BM, int BN>
 int launch_tiles(ProductArgs A, hipStream_t st) {
   constexpr int WIDTH = GATED ? BN / 2 : BN, LDS = tile_lds(OUT == ITEXHIP_BFLOAT16 || OUT == ITEXHIP_HALF ? 2 : 4, WIDTH / 64, BM, BN);
@@ -846,23 +825,14 @@ int launch_tiles(ProductArgs A, hipStream_t st) {
 }
 template <int OUT, bool GATED>
 int launch_products(const ProductArgs& A, hipStream_t st) {
-  // Tiles cost a workgroup about 10 us whatever they hold, and have to be enough of them (rows of tiles a workgroup); strips read
-  // an expert's weights again for every 32 rows.  Measured, tiles : strips in us, 8 experts of 4096 x 4096, gated, at 16, 32, 64 rows each 67 : 57, 68 : 75, 75 : 130, not gated 49 : 44,
-  // 54 : 66, 66 : 99; 32 of 1408 x 2048, not gated, at 8, 16 30 : 29, 32 : 38; 4 of 14336 x 4096 (64 tiles) at 32, 64 134 : 101, 162 : 171;
-  // 8 of 1024 x 1024 (64 tiles) at 64, 128, 256 18 : 13, 24 : 21, 25 : 30.
-  constexpr int WIDTH = GATED ? 128 : 256;
-  const int64_t each = A.slots / A.experts, tiles = static_cast<int64_t>(A.experts) * ((A.N + WIDTH - 1) / WIDTH);
-  const bool near = OUT == 0 || A.slots / A.top_k * static_cast<int64_t>(A.pitch) < (1LL << 32);  // up: codes in reach of 32 bits
-  if (each >= (GATED ? 24 : 12) && each * tiles >= kWorkgroups * (A.pitch >= 2048 ? 12 : 32) && A.chunks >= 2 * kTileSteps && near) {
-    constexpr bool SWISH = GATED;
-    if (tiles * ((each + 255) / 256) < kWorkgroups * 3 / 4) {  // half as many channels a tile where they are too few for the device
-      if (SWISH && A.activation == ITEXHIP_ACT_SWISH) return launch_tiles<OUT, GATED, SWISH, 256, 128>(A, st);
-      return launch_tiles<OUT, GATED, false, 256, 128>(A, st);
-    }
-    if (SWISH && A.activation == ITEXHIP_ACT_SWISH) return launch_tiles<OUT, GATED, SWISH, 256, 256>(A, st);
-    return launch_tiles<OUT, GATED, false, 256, 256>(A, st);
+  constexpr bool SWISH = GATED;
+  const bool swish = SWISH && A.activation == ITEXHIP_ACT_SWISH;
+  switch (product_kernel(sizes_of(A, OUT != 0, GATED))) {
+    case kTiles128: return swish ? launch_tiles<OUT, GATED, SWISH, 256, 128>(A, st) : launch_tiles<OUT, GATED, false, 256, 128>(A, st);
+    case kTiles256: return swish ? launch_tiles<OUT, GATED, SWISH, 256, 256>(A, st) : launch_tiles<OUT, GATED, false, 256, 256>(A, st);
+    case kStrips8: return launch_stream<OUT, GATED, 8, 0>(A, st);
+    default: return launch_stream<OUT, GATED, 4, 0>(A, st);
   }
-  return few_strips(A) ? launch_stream<OUT, GATED, 8, 0>(A, st) : launch_stream<OUT, GATED, 4, 0>(A, st);
 }
 
 ProductArgs product_args(const itexhip_experts_params& p, bool up, const Layout& l, void* workspace, const int32_t* offsets, const int32_t* rows,
@@ -897,9 +867,10 @@ int run_up(const itexhip_experts_params& p, const void* x, const int32_t* offset
   A.x = x;
   A.x_stride = p.x_stride;
   A.x_vec = aligned(x, 16) && (p.x_stride * element_size(T)) % 16 == 0;
-  if (few_up(A)) {
-    if (p.gated) return few_strips(A) ? launch_stream<T, true, 8, T>(A, st) : launch_stream<T, true, 4, T>(A, st);
-    return few_strips(A) ? launch_stream<T, false, 8, T>(A, st) : launch_stream<T, false, 4, T>(A, st);
+  const ProductSizes sizes = sizes_of(A, true, p.gated != 0);
+  if (few_up(sizes)) {
+    if (p.gated) return few_strips(sizes) ? launch_stream<T, true, 8, T>(A, st) : launch_stream<T, true, 4, T>(A, st);
+    return few_strips(sizes) ? launch_stream<T, false, 8, T>(A, st) : launch_stream<T, false, 4, T>(A, st);
   }
   launch_quantize<T>(x, p.x_stride, p.tokens, p.hidden, A, st);
   return p.gated ? launch_products<T, true>(A, st) : launch_products<T, false>(A, st);
@@ -914,7 +885,7 @@ int run_down(const itexhip_experts_params& p, const void* h, const int32_t* expe
   A.x = h;
   A.x_stride = p.inner;
   A.x_vec = aligned(h, 16) && (p.inner * element_size(T)) % 16 == 0;
-  if (few_down(A)) {
+  if (few_down(sizes_of(A, false, false))) {
     static unsigned long long configured;
     const auto kernel = experts_few_down_kernel<T>;
     if (!device_bit(&configured, false)) {

@@ -16,7 +16,8 @@ pytestmark = pytest.mark.gpu
 
 # kernel: tokens, top_k, experts, K, N
 SIZES = {
-    "fused strips": (6, 2, 5, 530, 150),
+    "fused strips of 8": (6, 2, 5, 530, 150),
+    "fused strips of 4": (16, 2, 64, 64, 1100),
     "strips": (40, 2, 5, 530, 150),
     "tiles of 128": (900, 2, 5, 530, 1100),
     "tiles of 128, long rows": (400, 2, 4, 2000, 1100),
