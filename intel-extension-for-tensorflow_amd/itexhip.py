@@ -734,7 +734,8 @@ def adapters_params(type, adapters, rank, tokens, in_dim, slice_ends, x_stride=N
     """slice_ends: the column behind each slice, the last one the width of the output; strides (between tokens) in elements, dense where not given."""
     ends = [int(n) for n in slice_ends]
     x = int(in_dim if x_stride is None else x_stride)
-    base, out = (int(ends[-1] if s is None else s) for s in (base_stride, out_stride))
+    columns = ends[-1] if ends else 0   # (no slice: refused by the calls)
+    base, out = (int(columns if s is None else s) for s in (base_stride, out_stride))
     return AdaptersParams(type, int(adapters), int(rank), len(ends), int(tokens), int(in_dim), (C.c_int64 * 4)(*ends[:4]), x, base, out)
 
 
