@@ -658,7 +658,7 @@ int itexhip_group_rows(int64_t n, int groups, const int32_t* group_of, int32_t* 
  * slots by expert (itexhip_group_rows of the chosen experts; ids outside 0 .. experts - 1 belong to another device and are
  * left out).  A row of activations becomes int8 codes by its own largest absolute value:
  *   s = max(fp32(absmax / 127), 2^-100), code = rne(x / s)  (the quotient itself, not a rounded one); a row that holds an infinity
- *   or NaN has s = NaN.
+ *   or NaN has s = NaN, and all its results are NaN, through every activation.
  * up:   h[place, n] = act(v0[n]) * v1[n] if gated, else act(v0[n]);  v = fp32(sum of codes) * (s * scales[e, which, n]) with the codes of the
  *       token of slot rows[place] and e's weights, the products summed exactly; h has top_k * tokens rows of `inner`, in the
  *       order's places, and those behind offsets[experts] are left as they are.

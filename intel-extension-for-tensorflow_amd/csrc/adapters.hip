@@ -154,8 +154,8 @@ __device__ __forceinline__ void cut(operand_t<T>& o, int count) {
 
 // x A^T.  A workgroup has 16 RT places of one adapter, up to 16 CT of one slice's rows of A and a share of K.  Its wavefronts take the
 // share's steps of 32 in turns, so that together they read 256 consecutive bytes of a row, and add up in LDS.  Operands go straight from
-// memory to registers: x is read once, A stays in L2.  8192 tokens of 4096, rank 64 (bfloat16): 24 us, 2.8 TB/s of x, with A four times as many
-// bytes from L2 again.  One token: 3.5 us, a launch and two round trips to memory.
+// memory to registers: x is read once, A stays in L2.  8192 tokens of 4096, rank 64 (bfloat16): 21 to 23 us, 2.9 to 3.2 TB/s of x, with A four times as many
+// bytes from L2 again.  One token: 4 us, a launch and two round trips to memory.
 template <int T, bool VEC, int RT, int CT>
 __global__ __launch_bounds__(256) void shrink_kernel(const AdapterArgs A) {
   constexpr int PITCH = 16 * CT + 4;
@@ -243,8 +243,8 @@ __device__ __forceinline__ void power_of(uint32_t bits, float* up, float* down) 
 // and goes through up to ROWS places of one adapter, 16 at a time.  A lane's column of the j-th tile is NT (lane % 16) + j of them, so that it ends
 // with NT neighbouring columns of four rows and 16 lanes with a run of 16 NT.  The workgroup adds up the shares of x A^T and holds them in LDS as operands: the
 // sum of two numbers of the type (one of bfloat16 alone would be off by 2^-9 of it); in half precision times a power of two that keeps a
-// row's largest in range.  Bound by memory: 8192 tokens of 14336 columns, rank 64, take 113 us for 470 MB, 4.2 TB/s, the next 16 rows' base on its way
-// while the last ones are multiplied (without that 241).  With x A^T, 64 rows a workgroup 144 us, 128 147, 256 162; three wavefronts a SIMD 147, two 162;
+// row's largest in range.  Bound by memory: 8192 tokens of 14336 columns, rank 64, take 118 to 123 us for 470 MB, 3.8 to 4.0 TB/s, the next 16 rows' base on its way
+// while the last ones are multiplied (without that 241).  With x A^T, a pass of 64 rows a workgroup took 144 us, 128 147, 256 162; three wavefronts a SIMD 147, two 162;
 // stores past the caches' order of use 144 -> 136.
 template <int T, int KS, int NT, int ROWS>
 __global__ __launch_bounds__(256, KS <= 2 ? 3 : 2) void expand_kernel(const AdapterArgs A) {

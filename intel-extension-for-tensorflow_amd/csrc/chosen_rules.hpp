@@ -37,7 +37,7 @@ inline bool few_up(const ProductSizes& s) {
   return tokens <= kFewRows && each * s.pitch <= 8192 && tokens * s.pitch <= kFewBytes / 2;
 }
 // down, one launch : three in us: 2 rows of 768 to 14336 7 : 12 to 32 : 34, 4 of 1536 and 4096 11 : 16 and 18 : 15, 8 of 768 and 1536 10 : 13 and 13 : 17,
-// where there are few channels 12 : 12, 16 of 768 13 : 13
+// where there are few channels 12 : 12, 16 of 768 13 : 13.  8 of 1536 are 12288 bytes: the rule leaves them to the three launches, 17 for 13; 3 rows were not measured
 inline bool few_down(const ProductSizes& s) {
   const int64_t bytes = s.slots * s.pitch;
   return s.slots <= kFewPlaces && (s.slots <= 2 || bytes <= 8192) && bytes <= kFewBytes;
@@ -52,7 +52,9 @@ inline bool few_strips(const ProductSizes& s) {
 // Tiles cost a workgroup about 10 us whatever they hold, and have to be enough of them (rows of tiles a workgroup); strips read
 // an expert's weights again for every 32 rows.  Measured, tiles : strips in us, 8 experts of 4096 x 4096, gated, at 16, 32, 64 rows each 67 : 57, 68 : 75, 75 : 130, not gated 49 : 44,
 // 54 : 66, 66 : 99; 32 of 1408 x 2048, not gated, at 8, 16 30 : 29, 32 : 38; 4 of 14336 x 4096 (64 tiles) at 32, 64 134 : 101, 162 : 171;
-// 8 of 1024 x 1024 (64 tiles) at 64, 128, 256 18 : 13, 24 : 21, 25 : 30.
+// 8 of 1024 x 1024, gated (64 tiles), at 64, 128, 256 18 : 13, 24 : 21, 25 : 30, not gated (32 tiles) at 256, 512 33 : 31, 39 : 50.  At three of the 70 sizes that were
+// measured the rule takes the longer one: 24 for 21 and 33 for 31 of the last, 38 for 32 of 1408 x 2048 at 16.  Rows are counted by slots: with
+// experts on other devices an expert here has fewer than the rule takes it to have.
 enum ProductKernel { kStrips4, kStrips8, kTiles128, kTiles256 };
 inline ProductKernel product_kernel(const ProductSizes& s) {
   const int64_t width = s.gated ? 128 : 256, each = s.slots / s.experts, tiles = s.experts * ((s.N + width - 1) / width);

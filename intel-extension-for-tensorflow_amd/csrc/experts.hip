@@ -10,7 +10,7 @@ namespace {
 // next to it, and the remainder x - n s, which is a multiple of ulp(s) / 2 below 2 s and therefore exact in one fma, tells
 // whether the nearest integer is n or a neighbour, and where it is halfway.
 // Rows of codes are `pitch` bytes (K rounded up to 64), zeros behind K: the packed weights' K steps.
-// A workgroup has a row and keeps it between the two passes.  8192 rows of 14336 (bfloat16) take 72 us, 4.9 TB/s read and written (85 with every
+// A workgroup has a row and keeps it between the two passes.  8192 rows of 14336 (bfloat16) take 68 us, 5.2 TB/s read and written (85 with every
 // element through its remainder).
 // ------------------------------------------------------------------------------------------------
 constexpr float kLeastScale = 0x1p-100f;
@@ -51,7 +51,7 @@ __device__ __forceinline__ float scale_of(uint32_t absmax_bits) {
   return fmaxf(__uint_as_float(absmax_bits) / 127.0f, kLeastScale);
 }
 
-// HELD: runs of 8 elements that a thread keeps between the two passes (0: it reads them again)
+// HELD: runs of 8 elements that a thread keeps between the two passes, up to 7 (14336 elements a row; 8 and more were not measured); 0: it reads them again
 template <int T, bool VEC, int HELD>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const void* __restrict__ x, int64_t stride, int K, int pitch, int8_t* __restrict__ codes,
                                                             float* __restrict__ scales, int64_t first) {
@@ -196,7 +196,7 @@ __device__ __forceinline__ v4i load_once(const int8_t* p) { return __builtin_non
 // their way while the last ones are multiplied; the shares' sums meet in LDS.  The rows' codes come from the caches, or (SOURCE: the
 // type of x) the workgroup makes them itself, which saves a launch where rows are very few.
 // Bound by memory: one token's two experts of 4096 x 14336, gate and up, 235 MB, take 40 us (5.8 TB/s), 64 tokens through 64 experts of
-// 2048 x 1408, 369 MB, 55 to 57 (6.5 TB/s).  With each batch of chunks waited for before the next is asked for the latter took 70.
+// 2048 x 1408, 369 MB, 55 to 57 with the codes' launch (6.5 TB/s; the profiler has 59 for this one alone, 54 at best).  With each batch of chunks waited for before the next is asked for the latter took 70.
 // OUT: type of h (up), or 0: fp32 by slot (down).
 template <int OUT, bool GATED, int WAVES, int SOURCE>
 __global__ __launch_bounds__(64 * WAVES) void experts_stream_kernel(const ProductArgs A) {
@@ -393,8 +393,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void experts_few_down_kernel(const 
 // a contiguous run of the experts' last tiles, which are not full, and then of the others: its 32 workgroups share a few columns of weights and up to 8 tiles of rows in their L2.  A workgroup
 // stays for all its tiles: the last steps of one fetch the first ones of the next, which then travel while results are written.
 //
-// 4096 tokens, 2 of 8 experts of 4096 x 14336, gate and up (1.92 TOP): 0.99 ms, 1.9 POP/s; the way back 0.54 ms, 1.8.  The board's power bounds it: the matrix
-// cores are busy half of the cycles at 1.74 GHz, so what costs energy costs time.  Steps alone take 0.87 ms, as long as this library's MatMul of as many
+// 4096 tokens, 2 of 8 experts of 4096 x 14336, gate and up (1.92 TOP): launches apart from one another 1.07 ms, 1.01 at best, 1.8 to 1.9 POP/s; the way back 0.56, 0.55 at best, 1.7 to 1.8.  The board's power bounds it: the matrix
+// cores are busy 50 % of the cycles at 1.74 GHz (the way back 43 % at 1.93), so what costs energy costs time.  Steps alone took 0.87 ms of 1.02, as long as this library's MatMul of as many
 // rows of one weight; the results' arithmetic, which no matrix instruction covers, makes the difference.  A tile of 256 x 256 has the fewest operand bytes for
 // its products that registers allow.  Bases in scalar registers and one offset for all weights' loads of a step brought 1049 to 1015 us.
 // ------------------------------------------------------------------------------------------------
